@@ -26,38 +26,13 @@
 //     accumulator) over the wave's tokens; the waves are merged through LDS in wave order.
 // The result is a fixed function of (request data, seq_len, num_splits, seg): no
 // atomics, no dependence on batch composition or scheduling.
-#include "common.h"
+#include "decode_split.h"
 
 #include <cstdlib>
 #include <mutex>
 
 namespace sid {
 namespace {
-
-constexpr int HEAD_DIM = 128;
-constexpr int HKV = 8;              // kv heads (a lane group per head)
-constexpr int QPK = 2;              // query heads per kv head
-constexpr int HQ = HKV * QPK;
-constexpr bool kNonTemporal = true;  // K/V rows are streamed once: +9% HBM throughput
-constexpr int HEUR_TILE = 32;       // granularity of the heuristic split size
-constexpr float NEG_BIG = -1e30f;   // finite "minus infinity" for running maxima
-constexpr int kOrderSlotBits = 12;  // wg_order entries: request << 12 | slot
-constexpr int kOrderEmpty = 1 << 30;  // wg_order entry flag: the item holds no tokens
-
-__host__ __device__ __forceinline__ int kv_per_split(int seq_len, int n_splits, int fixed_split) {
-  if (fixed_split > 0) return fixed_split;
-  return ceil_div(ceil_div(seq_len, n_splits), HEUR_TILE) * HEUR_TILE;
-}
-
-// The split count of a request when the caller passes no num_splits array: the reference's
-// policies restated on the device (sid/kernels/decode_attention.py:65-85): fixed-size splits
-// cover the sequence, the heuristic takes one split per 32 tokens up to the grid's split
-// count. A request without tokens gets 0 (its output is zeros).
-__device__ __forceinline__ int derived_splits(int seq_len, int max_splits, int fixed_split) {
-  if (seq_len <= 0) return 0;
-  if (fixed_split > 0) return ceil_div(seq_len, fixed_split);
-  return min(ceil_div(seq_len, HEUR_TILE), max_splits);
-}
 
 __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, a),
@@ -78,14 +53,6 @@ __device__ __forceinline__ float dot16(const u32x4_v (&qa)[2], const u32x4_v (&k
   return s;
 }
 
-// Sum over the 8 lanes of a token group; all 8 lanes get identical bits.
-__device__ __forceinline__ float group8_sum(float v) {
-  v += dpp<DPP_QUAD_XOR1>(v);
-  v += dpp<DPP_QUAD_XOR2>(v);
-  v += dpp<DPP_HALF_MIRROR>(v);
-  return v;
-}
-
 __device__ __forceinline__ void unpack16(const u32x4_v (&va)[2], float (&out)[16]) {
   const uint32_t w[8] = {va[0].x, va[0].y, va[0].z, va[0].w, va[1].x, va[1].y, va[1].z, va[1].w};
 #pragma unroll
@@ -100,45 +67,6 @@ template <int TPL>
 struct TileRegs {
   u32x4_v k[TPL][2];
   u32x4_v v[TPL][2];
-};
-
-template <bool NT>
-__device__ __forceinline__ u32x4_v ld16(const u32x4_v* p) {
-  if constexpr (NT) {
-    return __builtin_nontemporal_load(p);
-  } else {
-    return *p;
-  }
-}
-
-// Token range [start, end) of partial slot y of a request, or false if the slot is empty.
-// Slot y is segment j = y % sps of split s = y / sps, with sps = ceil(chunk / seg).
-__host__ __device__ __forceinline__ bool segment_range(int seq_len, int n_splits, int fixed_split,
-                                                       int seg, int y, int& start, int& end) {
-  const int chunk = kv_per_split(seq_len, n_splits, fixed_split);
-  const int sl = seg > 0 ? min(seg, chunk) : chunk;
-  const int sps = ceil_div(chunk, sl);
-  const int s = y / sps;
-  if (s >= n_splits) return false;
-  const int split_start = s * chunk;
-  const int split_end = min(split_start + chunk, seq_len);
-  start = split_start + (y % sps) * sl;
-  end = min(start + sl, split_end);
-  return start < end;
-}
-
-// LDS of one stage-1 workgroup: the waves' softmax states, then the merge's scales. The
-// accumulators come first and the struct is 16-byte aligned, so their stores and the merge's
-// reads are whole 16-byte LDS accesses (with a 4-byte-aligned struct the compiler splits
-// them into 4-byte pairs: one request of 1024 tokens took 9.3 -> 10.0 us).
-template <int NW>
-struct alignas(16) Stage1Lds {
-  float acc[NW][HQ][HEAD_DIM];
-  float m[NW][HQ];
-  float l[NW][HQ];
-  float sc[NW][HQ];
-  float den[HQ];
-  float mx[HQ];
 };
 
 // The partial attention of request b over partial slot y (a segment of one split), by one
@@ -304,54 +232,7 @@ __device__ __forceinline__ void stage1_item(
   }
   __syncthreads();
 
-  // Merge the waves in increasing wave order. A wave that saw no token of the segment has
-  // m = NEG_BIG and l = 0 and drops out (its scale underflows). One thread per query head
-  // takes the max over the waves, every wave's scale and the denominator once; then each
-  // thread folds 4 consecutive dims of one head (128-bit LDS reads), with the same
-  // per-output operations in the same order as folding every dim on its own.
-  auto& s_sc = sh.sc;
-  auto& s_den = sh.den;
-  auto& s_mx = sh.mx;
-  if (tid < HQ) {
-    float mx = s_m[0][tid];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_m[w][tid]);
-    float den = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float sc = __expf(s_m[w][tid] - mx);
-      s_sc[w][tid] = sc;
-      den += s_l[w][tid] * sc;
-    }
-    s_den[tid] = den;
-    s_mx[tid] = mx;
-  }
-  __syncthreads();
-  constexpr int Q4 = HEAD_DIM / 4;
-  for (int i = tid; i < HQ * Q4; i += NW * 64) {
-    const int h = i / Q4;
-    const int d0 = (i % Q4) * 4;
-    float num[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float sc = s_sc[w][h];
-      const float4 a = *reinterpret_cast<const float4*>(&s_acc[w][h][d0]);
-      num[0] += a.x * sc;
-      num[1] += a.y * sc;
-      num[2] += a.z * sc;
-      num[3] += a.w * sc;
-    }
-    const float den = s_den[h];
-    const float4 out = make_float4(num[0] / den, num[1] / den, num[2] / den, num[3] / den);
-    if (o_direct != nullptr) {
-      *reinterpret_cast<uint2*>(&o_direct[(out_row + h) * HEAD_DIM + d0]) =
-          make_uint2(pack_bf16x2(out.x, out.y), pack_bf16x2(out.z, out.w));
-    } else {
-      const int64_t prow = (out_row + h) * part_stride + y;
-      *reinterpret_cast<float4*>(&part_o[prow * HEAD_DIM + d0]) = out;
-      if (d0 == 0) part_lse[prow] = s_mx[h] + __logf(den);
-    }
-  }
+  stage1_merge<NW>(sh, tid, out_row, y, part_stride, part_o, part_lse, o_direct);
 }
 
 
@@ -433,8 +314,6 @@ __global__ void __launch_bounds__(NW * 64) decode_stage1_worker_kernel(
 // with segments in place of splits. A request with no used slot gets zeros
 // (flash_decode.cu:246-249). The partial loads of different slots are independent, so they
 // overlap.
-constexpr int kMaxGridSlots = 1024;
-
 __global__ void __launch_bounds__(HEAD_DIM) decode_stage2_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_lse, int grid_slots,
     int part_stride, bf16_t* __restrict__ o) {
@@ -610,8 +489,15 @@ int launch_decode(const void* q, const void* k_cache, const void* v_cache,
       default: worker(decode_stage1_worker_kernel<4, 4>, 4); break;
     }
   }
-  int rc = check_launch("flash_decode_fwd stage1");
+  const int rc = check_launch("flash_decode_fwd stage1");
   if (rc != SID_OK || direct) return rc;
+  return launch_decode_stage2(batch, grid_slots, part_o, part_lse, part_stride, o, s);
+}
+
+}  // namespace
+
+int launch_decode_stage2(int batch, int grid_slots, const float* part_o, const float* part_lse,
+                         int part_stride, void* o, hipStream_t s) {
   if (batch <= kLatencyBatch) {
     hipLaunchKernelGGL(decode_stage2_latency_kernel, dim3(HQ, batch), dim3(HEAD_DIM), 0, s,
                        part_o, part_lse, grid_slots, part_stride, (bf16_t*)o);
@@ -633,27 +519,44 @@ int launch_decode(const void* q, const void* k_cache, const void* v_cache,
   return check_launch("flash_decode_fwd stage2");
 }
 
-int check_decode_args(const void* q, const void* k_cache, const void* v_cache,
-                      const int32_t* kv_indptr, const int32_t* kv_indices,
-                      const int32_t* num_splits, void* o, int batch, int num_q_heads,
-                      int num_kv_heads, int head_dim, int64_t num_slots, int max_splits,
-                      int fixed_split_size) {
-  SID_REQUIRE(q && k_cache && v_cache && kv_indptr && kv_indices && o,
-              "flash_decode_fwd: null pointer");
-  SID_REQUIRE(head_dim == HEAD_DIM, "flash_decode_fwd: head_dim must be %d, got %d", HEAD_DIM,
-              head_dim);
+int check_decode_args(const char* name, const void* q, const void* k_cache, const void* v_cache,
+                      const int32_t* kv_indptr, const int32_t* kv_indices, void* o, int batch,
+                      int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
+                      int max_splits, int fixed_split_size) {
+  SID_REQUIRE(q && k_cache && v_cache && kv_indptr && kv_indices && o, "%s: null pointer", name);
+  SID_REQUIRE(head_dim == HEAD_DIM, "%s: head_dim must be %d, got %d", name, HEAD_DIM, head_dim);
   SID_REQUIRE(num_kv_heads == HKV && num_q_heads == HQ,
-              "flash_decode_fwd: expected %d q heads and %d kv heads (got %d q, %d kv)", HQ, HKV,
+              "%s: expected %d q heads and %d kv heads (got %d q, %d kv)", name, HQ, HKV,
               num_q_heads, num_kv_heads);
-  SID_REQUIRE(num_slots > 0, "flash_decode_fwd: empty KV pool");
+  SID_REQUIRE(num_slots > 0, "%s: empty KV pool", name);
   SID_REQUIRE(max_splits >= 1 && max_splits <= kMaxGridSlots,
-              "flash_decode_fwd: max_splits %d out of range [1, %d]", max_splits, kMaxGridSlots);
-  SID_REQUIRE(fixed_split_size >= 0, "flash_decode_fwd: negative fixed_split_size");
-  SID_REQUIRE(batch <= (1 << 30), "flash_decode_fwd: batch %d too large", batch);
+              "%s: max_splits %d out of range [1, %d]", name, max_splits, kMaxGridSlots);
+  SID_REQUIRE(fixed_split_size >= 0, "%s: negative fixed_split_size", name);
+  SID_REQUIRE(batch <= (1 << 30), "%s: batch %d too large", name, batch);
   return SID_OK;
 }
 
-}  // namespace
+int check_decode_plan(const char* name, int batch, int segment_size, int grid_slots,
+                      const int32_t* wg_order, int workers, const float* part_o,
+                      const float* part_lse, int part_batch, int part_stride) {
+  SID_REQUIRE(segment_size >= 0, "%s: negative segment_size", name);
+  SID_REQUIRE(grid_slots >= 1 && grid_slots <= kMaxGridSlots,
+              "%s: grid_slots %d out of range [1, %d]", name, grid_slots, kMaxGridSlots);
+  SID_REQUIRE(batch < (1 << (30 - kOrderSlotBits)) && kMaxGridSlots <= (1 << kOrderSlotBits),
+              "%s: batch %d too large for the workgroup order", name, batch);
+  SID_REQUIRE(workers >= 0 && workers <= (1 << 20), "%s: workers %d out of range", name, workers);
+  SID_REQUIRE(workers == 0 || wg_order != nullptr,
+              "%s: a worker launch needs the item order (wg_order)", name);
+  if (grid_slots > 1) {
+    SID_REQUIRE(part_o && part_lse, "%s: null workspace", name);
+    SID_REQUIRE(part_batch >= batch && part_stride >= grid_slots,
+                "%s: part_o workspace too small / wrong shape "
+                "(part_batch %d, part_stride %d, batch %d, grid_slots %d)",
+                name, part_batch, part_stride, batch, grid_slots);
+  }
+  return SID_OK;
+}
+
 }  // namespace sid
 
 using namespace sid;
@@ -669,26 +572,14 @@ extern "C" int sid_flash_decode_workers_fwd(
   SID_REQUIRE(variant >= 0 && variant < kNumVariants, "flash_decode_fwd: unknown variant %d",
               variant);
   if (batch == 0) return SID_OK;
-  int rc = check_decode_args(q, k_cache, v_cache, kv_indptr, kv_indices, num_splits, o, batch,
+  const char* name = "flash_decode_fwd";
+  int rc = check_decode_args(name, q, k_cache, v_cache, kv_indptr, kv_indices, o, batch,
                              num_q_heads, num_kv_heads, head_dim, num_slots, max_splits,
                              fixed_split_size);
   if (rc != SID_OK) return rc;
-  SID_REQUIRE(segment_size >= 0, "flash_decode_fwd: negative segment_size");
-  SID_REQUIRE(grid_slots >= 1 && grid_slots <= kMaxGridSlots,
-              "flash_decode_fwd: grid_slots %d out of range [1, %d]", grid_slots, kMaxGridSlots);
-  SID_REQUIRE(batch < (1 << (30 - kOrderSlotBits)) && kMaxGridSlots <= (1 << kOrderSlotBits),
-              "flash_decode_fwd: batch %d too large for the workgroup order", batch);
-  SID_REQUIRE(workers >= 0 && workers <= (1 << 20), "flash_decode_fwd: workers %d out of range",
-              workers);
-  SID_REQUIRE(workers == 0 || wg_order != nullptr,
-              "flash_decode_fwd: a worker launch needs the item order (wg_order)");
-  if (grid_slots > 1) {
-    SID_REQUIRE(part_o && part_lse, "flash_decode_fwd: null workspace");
-    SID_REQUIRE(part_batch >= batch && part_stride >= grid_slots,
-                "flash_decode_fwd: part_o workspace too small / wrong shape "
-                "(part_batch %d, part_stride %d, batch %d, grid_slots %d)",
-                part_batch, part_stride, batch, grid_slots);
-  }
+  rc = check_decode_plan(name, batch, segment_size, grid_slots, wg_order, workers, part_o,
+                         part_lse, part_batch, part_stride);
+  if (rc != SID_OK) return rc;
   return launch_decode(q, k_cache, v_cache, kv_indptr, kv_indices, num_splits, max_splits, batch,
                        num_slots, fixed_split_size, segment_size, grid_slots, sm_scale, part_o, part_lse,
                        part_stride, o, variant, wg_order, workers,
@@ -777,7 +668,8 @@ extern "C" int sid_flash_decode_segments_fwd_noalloc(
   SID_REQUIRE(variant >= 0 && variant < kNumVariants,
               "flash_decode_fwd_noalloc: unknown variant %d", variant);
   if (batch == 0) return SID_OK;
-  int rc = check_decode_args(q, k_cache, v_cache, kv_indptr, kv_indices, num_splits, o, batch,
+  int rc = check_decode_args("flash_decode_fwd_noalloc", q, k_cache, v_cache, kv_indptr,
+                             kv_indices, o, batch,
                              num_q_heads, num_kv_heads, head_dim, num_slots, max_splits,
                              fixed_split_size);
   if (rc != SID_OK) return rc;

@@ -29,7 +29,7 @@
 // numbered so they land on the same XCD (workgroups are dealt round-robin over the 8 XCDs
 // in id order) and share its L2.
 #include "common.h"
-#include "rowmath.h"
+#include "kv_fp8.h"
 
 namespace sid {
 namespace {
@@ -410,15 +410,17 @@ __global__ void __launch_bounds__(2 * PL * (NB / NBW) * 64) norm_silu_kernel(
 constexpr int QD = 128;
 
 // MBS = 2: 32-row workgroups (each weight fragment used for two row blocks), for batches
-// whose 16-row grid would not fit the CUs in one round.
-template <int PL, bool F32, int MBS>
+// whose 16-row grid would not fit the CUs in one round. FP8: 8-bit pools (kv_fp8.h), k and v
+// quantised from the same bf16 values.
+template <int PL, bool F32, int MBS, bool FP8>
 __global__ void __launch_bounds__(512) norm_qkv_kernel(
     const void* __restrict__ src, const uint4* __restrict__ norm_w, float eps,
     const bf16_t* __restrict__ w, int M, int num_q_heads, int num_kv_heads, int R,
     const uint4* __restrict__ q_norm, const uint4* __restrict__ k_norm,
     const int64_t* __restrict__ positions, const float* __restrict__ cos_sin,
     int64_t max_positions, const int64_t* __restrict__ slots, uint4* __restrict__ q_out,
-    uint4* __restrict__ k_cache, uint4* __restrict__ v_cache, int64_t num_slots) {
+    void* __restrict__ k_cache, void* __restrict__ v_cache, uint8_t* __restrict__ kv_scales,
+    int64_t num_slots) {
   constexpr int NCH = 2 * PL;
   constexpr int H = 512 * PL;
   constexpr int YS = QD + 4;
@@ -494,15 +496,24 @@ __global__ void __launch_bounds__(512) norm_qkv_kernel(
   const bool slot_ok = valid && slot >= 0 && slot < num_slots;
   const int kv_row = 16 * num_kv_heads;  // uint4 per pool row
   if (is_v) {
-    if (slot_ok) v_cache[slot * kv_row + (head - num_q_heads - num_kv_heads) * 16 + j] = store8(y);
+    const int h = head - num_q_heads - num_kv_heads;
+    if constexpr (FP8) {
+      fp8_store_vector(y, j, slot_ok, static_cast<uint2*>(v_cache), kv_scales,
+                       slot * num_kv_heads + h, 1);
+    } else if (slot_ok) {
+      static_cast<uint4*>(v_cache)[slot * kv_row + h * 16 + j] = store8(y);
+    }
     return;
   }
   float o[8];
   qk_head_norm_rope(y, j, in, eps, o);
   if (is_q) {
     if (valid) q_out[(t * num_q_heads + head) * 16 + j] = store8(o);
+  } else if constexpr (FP8) {
+    fp8_store_vector(o, j, slot_ok, static_cast<uint2*>(k_cache), kv_scales,
+                     slot * num_kv_heads + head - num_q_heads, 0);
   } else if (slot_ok) {
-    k_cache[slot * kv_row + (head - num_q_heads) * 16 + j] = store8(o);
+    static_cast<uint4*>(k_cache)[slot * kv_row + (head - num_q_heads) * 16 + j] = store8(o);
   }
 }
 
@@ -648,6 +659,53 @@ extern "C" int sid_rmsnorm_linear_silu_mul(const void* src, int src_fp32, const 
   return check_launch("rmsnorm_linear_silu_mul");
 }
 
+// sid_rmsnorm_qkv_post (kv_scales NULL: bf16 pools) and sid_rmsnorm_qkv_post_fp8.
+static int launch_norm_qkv(const char* name, const void* src, int src_fp32, const void* norm_w,
+                           float eps, const void* w_qkv, int64_t m, int64_t hidden,
+                           int num_q_heads, int num_kv_heads, int head_dim, const void* q_norm,
+                           const void* k_norm, const int64_t* positions, const float* cos_sin,
+                           int64_t max_positions, const int64_t* slots, void* q_out,
+                           void* k_cache, void* v_cache, void* kv_scales, int64_t num_slots,
+                           void* stream) {
+  SID_REQUIRE(src && norm_w && w_qkv && q_norm && k_norm && positions && cos_sin && slots &&
+                  q_out && k_cache && v_cache,
+              "%s: null pointer", name);
+  SID_REQUIRE(head_dim == QD, "%s: head_dim must be %d, got %d", name, QD, head_dim);
+  SID_REQUIRE(num_q_heads > 0 && num_kv_heads > 0, "%s: bad head counts", name);
+  SID_REQUIRE(hidden == 512 || hidden == 1024,
+              "%s: hidden %lld must be 512 or 1024", name, (long long)hidden);
+  SID_REQUIRE(num_slots > 0, "%s: empty KV pool", name);
+  SID_REQUIRE(aligned16(src) && aligned16(norm_w) && aligned16(w_qkv) && aligned16(q_out) &&
+                  aligned16(k_cache) && aligned16(v_cache),
+              "%s: operands must be 16-byte aligned", name);
+  // 32-row workgroups once 16-row ones would take more than one round of the CUs.
+  const int mbs = m > kQkvWideAboveRows ? 2 : 1;
+  const int64_t R = (m + 16 * mbs - 1) / (16 * mbs);
+  const int heads = num_q_heads + 2 * num_kv_heads;
+  SID_REQUIRE(R * heads < (1ll << 31), "%s: too large", name);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(R * heads));
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, dim3(512), 0, s, src, (const uint4*)norm_w, eps,
+                       (const bf16_t*)w_qkv, (int)m, num_q_heads, num_kv_heads, (int)R,
+                       (const uint4*)q_norm, (const uint4*)k_norm, positions, cos_sin,
+                       max_positions, slots, (uint4*)q_out, k_cache, v_cache,
+                       (uint8_t*)kv_scales, num_slots);
+  };
+#define SID_NQ(PL, F)                                                                         \
+  (kv_scales ? (mbs == 1 ? go(norm_qkv_kernel<PL, F, 1, true>)                                \
+                         : go(norm_qkv_kernel<PL, F, 2, true>))                               \
+             : (mbs == 1 ? go(norm_qkv_kernel<PL, F, 1, false>)                               \
+                         : go(norm_qkv_kernel<PL, F, 2, false>)))
+  if (hidden == 512) {
+    if (src_fp32) SID_NQ(1, true); else SID_NQ(1, false);
+  } else {
+    if (src_fp32) SID_NQ(2, true); else SID_NQ(2, false);
+  }
+#undef SID_NQ
+  return check_launch(name);
+}
+
 extern "C" int sid_rmsnorm_qkv_post(const void* src, int src_fp32, const void* norm_w, float eps,
                                     const void* w_qkv, int64_t m, int64_t hidden,
                                     int num_q_heads, int num_kv_heads, int head_dim,
@@ -658,40 +716,26 @@ extern "C" int sid_rmsnorm_qkv_post(const void* src, int src_fp32, const void* n
                                     void* stream) {
   SID_REQUIRE(m >= 0 && hidden >= 0, "rmsnorm_qkv_post: negative size");
   if (m == 0) return SID_OK;
-  SID_REQUIRE(src && norm_w && w_qkv && q_norm && k_norm && positions && cos_sin && slots &&
-                  q_out && k_cache && v_cache,
-              "rmsnorm_qkv_post: null pointer");
-  SID_REQUIRE(head_dim == QD, "rmsnorm_qkv_post: head_dim must be %d, got %d", QD, head_dim);
-  SID_REQUIRE(num_q_heads > 0 && num_kv_heads > 0, "rmsnorm_qkv_post: bad head counts");
-  SID_REQUIRE(hidden == 512 || hidden == 1024,
-              "rmsnorm_qkv_post: hidden %lld must be 512 or 1024", (long long)hidden);
-  SID_REQUIRE(num_slots > 0, "rmsnorm_qkv_post: empty KV pool");
-  SID_REQUIRE(aligned16(src) && aligned16(norm_w) && aligned16(w_qkv) && aligned16(q_out) &&
-                  aligned16(k_cache) && aligned16(v_cache),
-              "rmsnorm_qkv_post: operands must be 16-byte aligned");
-  // 32-row workgroups once 16-row ones would take more than one round of the CUs.
-  const int mbs = m > kQkvWideAboveRows ? 2 : 1;
-  const int64_t R = (m + 16 * mbs - 1) / (16 * mbs);
-  const int heads = num_q_heads + 2 * num_kv_heads;
-  SID_REQUIRE(R * heads < (1ll << 31), "rmsnorm_qkv_post: too large");
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(R * heads));
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(512), 0, s, src, (const uint4*)norm_w, eps,
-                       (const bf16_t*)w_qkv, (int)m, num_q_heads, num_kv_heads, (int)R,
-                       (const uint4*)q_norm, (const uint4*)k_norm, positions, cos_sin,
-                       max_positions, slots, (uint4*)q_out, (uint4*)k_cache, (uint4*)v_cache,
-                       num_slots);
-  };
-#define SID_NQ(PL, F) \
-  (mbs == 1 ? go(norm_qkv_kernel<PL, F, 1>) : go(norm_qkv_kernel<PL, F, 2>))
-  if (hidden == 512) {
-    if (src_fp32) SID_NQ(1, true); else SID_NQ(1, false);
-  } else {
-    if (src_fp32) SID_NQ(2, true); else SID_NQ(2, false);
-  }
-#undef SID_NQ
-  return check_launch("rmsnorm_qkv_post");
+  return launch_norm_qkv("rmsnorm_qkv_post", src, src_fp32, norm_w, eps, w_qkv, m, hidden,
+                         num_q_heads, num_kv_heads, head_dim, q_norm, k_norm, positions, cos_sin,
+                         max_positions, slots, q_out, k_cache, v_cache, nullptr, num_slots, stream);
+}
+
+extern "C" int sid_rmsnorm_qkv_post_fp8(const void* src, int src_fp32, const void* norm_w, float eps,
+                                    const void* w_qkv, int64_t m, int64_t hidden,
+                                    int num_q_heads, int num_kv_heads, int head_dim,
+                                    const void* q_norm, const void* k_norm,
+                                    const int64_t* positions, const float* cos_sin,
+                                    int64_t max_positions, const int64_t* slots, void* q_out,
+                                    void* k_cache, void* v_cache, void* kv_scales,
+                                        int64_t num_slots,
+                                    void* stream) {
+  SID_REQUIRE(m >= 0 && hidden >= 0, "rmsnorm_qkv_post_fp8: negative size");
+  if (m == 0) return SID_OK;
+  SID_REQUIRE(kv_scales != nullptr, "rmsnorm_qkv_post_fp8: null pointer");
+  return launch_norm_qkv("rmsnorm_qkv_post_fp8", src, src_fp32, norm_w, eps, w_qkv, m, hidden,
+                         num_q_heads, num_kv_heads, head_dim, q_norm, k_norm, positions, cos_sin,
+                         max_positions, slots, q_out, k_cache, v_cache, kv_scales, num_slots, stream);
 }
 
 extern "C" int sid_pack_decode_weight(const void* w, void* packed, int64_t n, int64_t k,

@@ -35,124 +35,24 @@
 //   O^T += V^T P^T: 8 dim blocks x 2 k-steps, A = V^T from a transposed LDS
 //                   copy of the V tile, B = bf16(P) (P is rounded to bf16
 //                   before the PV product, as sid/kernels/extend_attention.py:106).
-#include "common.h"
+#include "extend_tile.h"
 
 #include <type_traits>
 
 namespace sid {
 namespace {
 
-constexpr int D = 128;
-constexpr int BN = 64;          // keys per tile
-constexpr int BQ = 32;          // query positions per workgroup (x 2 heads = 64 rows)
-constexpr int KSPLIT = 256;     // keys per split (4 tiles), anchored at position 0
 // LDS row strides (bf16) of the K and V tiles: 304 bytes each. Layout only (bit-identical);
 // of 136-152 x 136-160 this measured best on the verify fan-out (~4% over 272 / 288 bytes)
 // and equal on prefill.
 constexpr int KS_STRIDE = D + 24;
 constexpr int VS_STRIDE = D + 24;
-constexpr float NEG_BIG = -1e30f;
-constexpr float LOG2E = 1.4426950408889634f;
-// Slack of the lazy softmax maximum, in log2 units: scores up to 2^LAZY_T above the row's
-// reference maximum are taken without moving it.
-constexpr float LAZY_T = 8.0f;
-
-// 2^x by the hardware instruction (v_exp_f32): the argument is at most LAZY_T, and results
-// that would be denormal may flush to zero.
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Reductions over lanes l and l ^ 16 (l ^ 32): v_permlane16/32_swap hand each lane the
-// values of both lanes of its pair as (lower lane's, upper lane's), so both lanes compute
-// the same expression on the same operands (identical bits) without an LDS round trip.
-__device__ __forceinline__ float pair16_max(float v) {
-  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float pair32_max(float v) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float pair16_sum(float v) {
-  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-__device__ __forceinline__ float pair32_sum(float v) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-
-typedef short s16x4_v __attribute__((ext_vector_type(4)));
-typedef short s16x8_v __attribute__((ext_vector_type(8)));
-
-typedef __attribute__((address_space(3))) char* lds_char_t;
-
 // 4 bf16 of a V^T fragment through the LDS transpose read: within each 16-lane group,
 // lane L receives element L % 4 of the 8-byte values addressed by lanes L / 4 + 4j
 // (j = 0..3) of its group.
 __device__ __forceinline__ s16x4_v ld_tr16(const bf16_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (__attribute__((address_space(3))) s16x4_v*)(p));
-}
-
-// acc / l (l > 0), shared by every path that divides: y = 1 / l rounded, q = acc y, then one
-// correction (Markstein: the quotient correctly rounded), 5 operations for each of a row's
-// dims instead of a division's 12. An infinite or NaN q stays.
-__device__ __forceinline__ float div_row(float acc, float l, float y) {
-  const float q = acc * y;
-  const float c = __builtin_fmaf(__builtin_fmaf(-q, l, acc), y, q);
-  return __builtin_fabsf(q) < INFINITY ? c : q;
-}
-
-// Per-lane softmax state of one query row (the lane's 32 output dims).
-struct RowState {
-  float m;
-  float l;
-  f32x4_v acc[8];
-};
-
-__device__ __forceinline__ void fresh(RowState& s) {
-  s.m = NEG_BIG;
-  s.l = 0.0f;
-#pragma unroll
-  for (int db = 0; db < 8; ++db) s.acc[db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
-}
-
-// run <- fold(run, part): the one merge used by every path.
-// The fold's per-row scalars and its elementwise step, shared by every path that folds.
-struct FoldScale {
-  float mn, alpha, beta;
-};
-__device__ __forceinline__ FoldScale fold_scale(float run_m, float m) {
-  const float mn = fmaxf(run_m, m);
-  return {mn, exp2_fast(run_m - mn), exp2_fast(m - mn)};
-}
-// Written as one explicit fma over a separately rounded product, so the compiler has no
-// contraction choice to make differently in different kernels.
-__device__ __forceinline__ float fold_elem(float run, float part, const FoldScale& f) {
-  return __builtin_fmaf(run, f.alpha, part * f.beta);
-}
-
-__device__ __forceinline__ void fold(RowState& run, float m, float l, const f32x4_v (&a)[8]) {
-  const FoldScale f = fold_scale(run.m, m);
-  run.l = fold_elem(run.l, l, f);
-#pragma unroll
-  for (int db = 0; db < 8; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) run.acc[db][i] = fold_elem(run.acc[db][i], a[db][i], f);
-  run.m = f.mn;
-}
-
-// The row's output: acc / l rounded to bf16 (this lane: dims 16 db + 4 g .. +3).
-__device__ __forceinline__ void store_row(bf16_t* op, const RowState& run, int g) {
-  const float y = 1.0f / run.l;
-#pragma unroll
-  for (int db = 0; db < 8; ++db) {
-    const f32x4_v a = run.acc[db];
-    uint2 u;
-    u.x = pack_bf16x2(div_row(a[0], run.l, y), div_row(a[1], run.l, y));
-    u.y = pack_bf16x2(div_row(a[2], run.l, y), div_row(a[3], run.l, y));
-    *reinterpret_cast<uint2*>(op + 16 * db + 4 * g) = u;
-  }
 }
 
 struct Ctx {
@@ -213,76 +113,6 @@ __device__ __forceinline__ void store_tile(const TileRegs& r, const Ctx& c, bf16
     const int v = c.tid + 256 * i;
     *reinterpret_cast<u32x4_v*>(&sK[(v >> 4) * KS_STRIDE + (v & 15) * 8]) = r.k[i];
     *reinterpret_cast<u32x4_v*>(&sV[(v >> 4) * VS_STRIDE + (v & 15) * 8]) = r.v[i];
-  }
-}
-
-// Softmax of one tile's scores s (in place: s becomes p), in the exp2 domain:
-// p = 2^(s * sc2 - m) with sc2 = sm_scale * log2(e) and m the row's reference maximum in
-// the same units. The reference maximum is lazy: it moves to the tile's maximum only when
-// that exceeds it by more than LAZY_T, so p <= 2^LAZY_T and most tiles leave it (and the
-// accumulator) alone. Every decision is per row (per lane group), so a row's bits depend
-// on its own scores only. MASK: apply causality and row validity (keys beyond the row's
-// position give p = 0). Returns the accumulator's rescale factor (exactly 1 when the
-// reference maximum stays).
-template <bool MASK>
-__device__ __forceinline__ float softmax_tile(float (&s)[16], RowState& st, const Ctx& c, int t0,
-                                              float sc2) {
-  bool vis[16];
-  float tmax = NEG_BIG;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (MASK) {
-      const int key = t0 + 32 * (i >> 3) + 8 * c.g + (i & 7);
-      vis[i] = (key <= c.q_abs) & c.row_ok;
-      tmax = fmaxf(tmax, vis[i] ? s[i] : NEG_BIG);
-    } else {
-      tmax = fmaxf(tmax, s[i]);
-    }
-  }
-  tmax = pair16_max(tmax);
-  tmax = pair32_max(tmax);
-  const float mc = tmax * sc2;
-  const float m_used = mc > st.m + LAZY_T ? mc : st.m;
-  const float rescale = exp2_fast(st.m - m_used);
-  float psum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float p = exp2_fast(__builtin_fmaf(s[i], sc2, -m_used));
-    if constexpr (MASK) s[i] = vis[i] ? p : 0.0f;
-    else s[i] = p;
-    psum += s[i];
-  }
-  psum = pair16_sum(psum);
-  psum = pair32_sum(psum);
-  st.l = __builtin_fmaf(st.l, rescale, psum);
-  st.m = m_used;
-  return rescale;
-}
-
-// p of a tile as the PV product's B operand (p is finite: exp of a finite difference, or 0).
-__device__ __forceinline__ void pack_p(bf16x8_v (&pf)[2], const float (&s)[16]) {
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb) {
-    uint4 u;
-    u.x = pack_bf16x2(s[8 * kb + 0], s[8 * kb + 1]);
-    u.y = pack_bf16x2(s[8 * kb + 2], s[8 * kb + 3]);
-    u.z = pack_bf16x2(s[8 * kb + 4], s[8 * kb + 5]);
-    u.w = pack_bf16x2(s[8 * kb + 6], s[8 * kb + 7]);
-    pf[kb] = __builtin_bit_cast(bf16x8_v, u);
-  }
-}
-
-// x * 1 == x: the rescale is skipped (same bits) unless some row of the wave moved its
-// reference maximum.
-__device__ __forceinline__ void apply_rescale(RowState& st, float rescale) {
-  if (__builtin_amdgcn_ballot_w64(rescale != 1.0f) != 0) {
-#pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      st.acc[db][0] *= rescale;
-      st.acc[db][1] *= rescale;
-      st.acc[db][2] *= rescale;
-      st.acc[db][3] *= rescale;
-    }
   }
 }
 
@@ -461,11 +291,6 @@ __global__ void __launch_bounds__(256) extend_fanout_kernel(
 // 1 x 2048 55 -> 50, 8420 ragged tokens 174 -> 154 / 138, 200 decode rows 168 -> 153.
 // Measured and not taken: softmax interleaved with the next tile's S MFMAs over four-deep
 // rings (141), two row blocks per wave (122, but 90 for 1 x 2048), six waves (173).
-//
-// LDS tiles are 64 rows of 256 bytes; 16-byte piece p of key's row sits at p ^ swz(key): over
-// the 16 keys of a fragment or transpose read swz takes 16 values.
-__device__ __forceinline__ int swz(int key) { return (key & 3) | (((key >> 3) & 3) << 2); }
-
 // Lane l's 16 bytes at its address -> LDS byte lds + 16 l.
 __device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
@@ -476,8 +301,6 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
                "s"(base), "s"(lds)
                : "memory", "m0");
 }
-
-constexpr int kTileBytes = BN * D * 2;  // one K or V tile
 
 // OFF32: the pool is smaller than 4 GiB, so 32-bit offsets address it.
 template <int NW, bool OFF32>
@@ -700,7 +523,10 @@ constexpr int kFanoutBelowWg = 512;
 // 45, 5000 + 3000 229 vs 204.
 constexpr int64_t kWideWg = 672;
 constexpr int kWideMinLen = 1024;
-int prefill_rows(int batch, int64_t total_q, int num_kv_heads, int max_extend_len) {
+
+}  // namespace
+
+int extend_prefill_rows(int batch, int64_t total_q, int num_kv_heads, int max_extend_len) {
   const bool uniform = 2 * total_q >= static_cast<int64_t>(batch) * max_extend_len;
   return max_extend_len >= kWideMinLen && uniform &&
                  num_kv_heads * ((total_q + 63) / 64) >= kWideWg
@@ -708,14 +534,70 @@ int prefill_rows(int batch, int64_t total_q, int num_kv_heads, int max_extend_le
              : 32;
 }
 
-}  // namespace
+ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, const void* v_cache,
+                       const int32_t* qo_indptr, const int32_t* kv_indptr,
+                       const int32_t* kv_indices, const void* o, int batch, int64_t total_q,
+                       int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
+                       int max_extend_len, int max_kv_len, void* workspace,
+                       int64_t workspace_bytes) {
+  ExtendPlan p{};
+  auto check = [&]() -> int {
+    SID_REQUIRE(batch >= 0 && total_q >= 0, "%s: negative size", name);
+    p.empty = batch == 0 || total_q == 0 || max_extend_len <= 0;
+    if (p.empty) return SID_OK;
+    SID_REQUIRE(q && k_cache && v_cache && qo_indptr && kv_indptr && kv_indices && o,
+                "%s: null pointer", name);
+    SID_REQUIRE(head_dim == D, "%s: head_dim must be %d, got %d", name, D, head_dim);
+    SID_REQUIRE(num_kv_heads > 0 && num_q_heads == 2 * num_kv_heads,
+                "%s: expected 2 q heads per kv head (got %d q, %d kv)", name, num_q_heads,
+                num_kv_heads);
+    SID_REQUIRE(num_slots > 0, "%s: empty KV pool", name);
+    SID_REQUIRE(batch <= 65535 && num_kv_heads <= 65535, "%s: grid too large", name);
+    const int64_t need = sid_extend_attention_workspace_bytes(batch, total_q, num_q_heads,
+                                                             num_kv_heads, max_extend_len,
+                                                             max_kv_len);
+    p.fanout = need > 0 && workspace != nullptr && workspace_bytes >= need;
+    p.items = total_q * num_q_heads;
+    const int mtiles = ceil_div(max_extend_len, BQ);
+    if (p.fanout) {
+      p.rows = BQ;
+      p.mtiles = mtiles;
+      p.splits = ceil_div(max_kv_len, KSPLIT);
+      SID_REQUIRE(static_cast<int64_t>(mtiles) * p.splits <= 65535, "%s: grid too large", name);
+      SID_REQUIRE((p.items + 3) / 4 < (1ll << 31), "%s: too many rows for the merge", name);
+      p.part_a = static_cast<float*>(workspace);
+      p.part_ml = p.part_a + static_cast<int64_t>(p.splits) * p.items * D;
+      p.part_n = reinterpret_cast<int32_t*>(p.part_ml + static_cast<int64_t>(p.splits) * p.items * 2);
+      return SID_OK;
+    }
+    SID_REQUIRE(mtiles <= 65535, "%s: grid too large", name);
+    p.rows = extend_prefill_rows(batch, total_q, num_kv_heads, max_extend_len);
+    p.mtiles = ceil_div(max_extend_len, p.rows);
+    // Request b's workgroups are `batch` ids apart. Where only some requests reach the late tiles
+    // an even distance puts a long request's on few XCDs and CUs, so the grid then has an odd
+    // one (2048 + 15 x 16 445 -> 54 us, 31 x 1 + 4000 3160 -> 126, 5000 + 3000 268 -> 209; full
+    // batches keep theirs: 12 x 512 36 vs 38 padded, 8 x 1024 69 vs 72).
+    const bool ragged = 8 * total_q < 7 * static_cast<int64_t>(batch) * max_extend_len;
+    p.grid_x = static_cast<unsigned>(ragged ? batch | 1 : batch);
+    return SID_OK;
+  };
+  p.rc = check();
+  return p;
+}
+
+int extend_merge(const char* name, const ExtendPlan& p, void* o, hipStream_t s) {
+  hipLaunchKernelGGL(extend_merge_kernel, dim3((unsigned)((p.items + 3) / 4)), dim3(256), 0, s,
+                     p.items, p.splits, p.part_a, p.part_ml, p.part_n, (bf16_t*)o);
+  return check_launch(name);
+}
+
 }  // namespace sid
 
 using namespace sid;
 
 extern "C" int sid_extend_attention_query_rows(int batch, int64_t total_q, int num_kv_heads,
                                                int max_extend_len) {
-  return prefill_rows(batch, total_q, num_kv_heads, max_extend_len);
+  return extend_prefill_rows(batch, total_q, num_kv_heads, max_extend_len);
 }
 
 extern "C" int64_t sid_extend_attention_workspace_bytes(int batch, int64_t total_q,
@@ -736,59 +618,32 @@ extern "C" int sid_extend_attention_fwd(const void* q, const void* k_cache, cons
                                         int64_t num_slots, int max_extend_len, int max_kv_len,
                                         float sm_scale, void* workspace, int64_t workspace_bytes,
                                         void* o, void* stream) {
-  SID_REQUIRE(batch >= 0 && total_q >= 0, "extend_attention: negative size");
-  if (batch == 0 || total_q == 0 || max_extend_len <= 0) return SID_OK;
-  SID_REQUIRE(q && k_cache && v_cache && qo_indptr && kv_indptr && kv_indices && o,
-              "extend_attention: null pointer");
-  SID_REQUIRE(head_dim == D, "extend_attention: head_dim must be %d, got %d", D, head_dim);
-  SID_REQUIRE(num_kv_heads > 0 && num_q_heads == 2 * num_kv_heads,
-              "extend_attention: expected 2 q heads per kv head (got %d q, %d kv)", num_q_heads,
-              num_kv_heads);
-  SID_REQUIRE(num_slots > 0, "extend_attention: empty KV pool");
-  SID_REQUIRE(batch <= 65535 && num_kv_heads <= 65535, "extend_attention: grid too large");
-  const int mtiles = ceil_div(max_extend_len, BQ);
+  const char* name = "extend_attention";
+  const ExtendPlan p = extend_plan(name, q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o,
+                                   batch, total_q, num_q_heads, num_kv_heads, head_dim, num_slots,
+                                   max_extend_len, max_kv_len, workspace, workspace_bytes);
+  if (p.rc != SID_OK || p.empty) return p.rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t need = sid_extend_attention_workspace_bytes(batch, total_q, num_q_heads,
-                                                           num_kv_heads, max_extend_len,
-                                                           max_kv_len);
-  const bool fanout = need > 0 && workspace != nullptr && workspace_bytes >= need;
-  if (fanout) {
-    const int splits = ceil_div(max_kv_len, KSPLIT);
-    SID_REQUIRE(static_cast<int64_t>(mtiles) * splits <= 65535, "extend_attention: grid too large");
-    const int64_t items = total_q * num_q_heads;
-    float* pa = static_cast<float*>(workspace);
-    float* pml = pa + static_cast<int64_t>(splits) * items * D;
-    int32_t* pn = reinterpret_cast<int32_t*>(pml + static_cast<int64_t>(splits) * items * 2);
-    hipLaunchKernelGGL(extend_fanout_kernel, dim3(batch, num_kv_heads, mtiles * splits),
+  if (p.fanout) {
+    hipLaunchKernelGGL(extend_fanout_kernel, dim3(batch, num_kv_heads, p.mtiles * p.splits),
                        dim3(256), 0, s, (const bf16_t*)q, (const bf16_t*)k_cache,
                        (const bf16_t*)v_cache, qo_indptr, kv_indptr, kv_indices, num_q_heads,
-                       num_kv_heads, num_slots, sm_scale, mtiles, total_q, pa, pml, pn);
-    int rc = check_launch("extend_attention");
-    if (rc != SID_OK) return rc;
-    const int64_t groups = (items + 3) / 4;
-    SID_REQUIRE(groups < (1ll << 31), "extend_attention: too many rows for the merge");
-    hipLaunchKernelGGL(extend_merge_kernel, dim3((unsigned)groups), dim3(256), 0, s, items,
-                       splits, pa, pml, pn, (bf16_t*)o);
-    return check_launch("extend_attention merge");
+                       num_kv_heads, num_slots, sm_scale, p.mtiles, total_q, p.part_a, p.part_ml,
+                       p.part_n);
+    const int rc = check_launch(name);
+    return rc != SID_OK ? rc : extend_merge(name, p, o, s);
   }
-  SID_REQUIRE(mtiles <= 65535, "extend_attention: grid too large");
-  // Request b's workgroups are `batch` ids apart. Where only some requests reach the late tiles
-  // an even distance puts a long request's on few XCDs and CUs, so the grid then has an odd
-  // one (2048 + 15 x 16 445 -> 54 us, 31 x 1 + 4000 3160 -> 126, 5000 + 3000 268 -> 209; full
-  // batches keep theirs: 12 x 512 36 vs 38 padded, 8 x 1024 69 vs 72).
-  const bool ragged = 8 * total_q < 7 * static_cast<int64_t>(batch) * max_extend_len;
   auto prefill = [&](auto kern, int nw) {
-    const int mt = ceil_div(max_extend_len, 8 * nw);
-    hipLaunchKernelGGL(kern, dim3(ragged ? batch | 1 : batch, num_kv_heads, mt), dim3(nw * 64),
+    hipLaunchKernelGGL(kern, dim3(p.grid_x, num_kv_heads, p.mtiles), dim3(nw * 64),
                        4 * kTileBytes, s, (const bf16_t*)q, (const bf16_t*)k_cache,
                        (const bf16_t*)v_cache, qo_indptr, kv_indptr, kv_indices, batch, num_q_heads,
-                       num_kv_heads, num_slots, sm_scale, mt, (bf16_t*)o);
+                       num_kv_heads, num_slots, sm_scale, p.mtiles, (bf16_t*)o);
   };
   const bool off32 = num_slots * num_kv_heads * D * 2 < (1ll << 32);
-  if (prefill_rows(batch, total_q, num_kv_heads, max_extend_len) == 64) {
+  if (p.rows == 64) {
     off32 ? prefill(extend_prefill_kernel<8, true>, 8) : prefill(extend_prefill_kernel<8, false>, 8);
   } else {
     off32 ? prefill(extend_prefill_kernel<4, true>, 4) : prefill(extend_prefill_kernel<4, false>, 4);
   }
-  return check_launch("extend_attention");
+  return check_launch(name);
 }

@@ -1,0 +1,216 @@
+// What the extend attention's kernels for the two pool formats (extend_attention.hip: bf16,
+// extend_attention_fp8.hip: e4m3 codes) share: the tile and split sizes, a row's softmax state
+// and its arithmetic, the fold of splits, the LDS swizzle and the host's size rules. Both compute
+// a tile by the same operations on the same bf16 values in the same order.
+#pragma once
+
+#include "common.h"
+
+namespace sid {
+
+constexpr int D = 128;
+constexpr int BN = 64;          // keys per tile
+constexpr int BQ = 32;          // query positions per workgroup (x 2 heads = 64 rows)
+constexpr int KSPLIT = 256;     // keys per split (4 tiles), anchored at position 0
+constexpr float NEG_BIG = -1e30f;
+constexpr float LOG2E = 1.4426950408889634f;
+// Slack of the lazy softmax maximum, in log2 units: scores up to 2^LAZY_T above the row's
+// reference maximum are taken without moving it.
+constexpr float LAZY_T = 8.0f;
+
+// 2^x by the hardware instruction (v_exp_f32): the argument is at most LAZY_T, and results
+// that would be denormal may flush to zero.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Reductions over lanes l and l ^ 16 (l ^ 32): v_permlane16/32_swap hand each lane the
+// values of both lanes of its pair as (lower lane's, upper lane's), so both lanes compute
+// the same expression on the same operands (identical bits) without an LDS round trip.
+__device__ __forceinline__ float pair16_max(float v) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float pair32_max(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float pair16_sum(float v) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float pair32_sum(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+typedef short s16x4_v __attribute__((ext_vector_type(4)));
+typedef short s16x8_v __attribute__((ext_vector_type(8)));
+
+typedef __attribute__((address_space(3))) char* lds_char_t;
+
+// acc / l (l > 0), shared by every path that divides: y = 1 / l rounded, q = acc y, then one
+// correction (Markstein: the quotient correctly rounded), 5 operations for each of a row's
+// dims instead of a division's 12. An infinite or NaN q stays.
+__device__ __forceinline__ float div_row(float acc, float l, float y) {
+  const float q = acc * y;
+  const float c = __builtin_fmaf(__builtin_fmaf(-q, l, acc), y, q);
+  return __builtin_fabsf(q) < INFINITY ? c : q;
+}
+
+// Per-lane softmax state of one query row (the lane's 32 output dims).
+struct RowState {
+  float m;
+  float l;
+  f32x4_v acc[8];
+};
+
+__device__ __forceinline__ void fresh(RowState& s) {
+  s.m = NEG_BIG;
+  s.l = 0.0f;
+#pragma unroll
+  for (int db = 0; db < 8; ++db) s.acc[db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// run <- fold(run, part): the one merge used by every path.
+// The fold's per-row scalars and its elementwise step, shared by every path that folds.
+struct FoldScale {
+  float mn, alpha, beta;
+};
+__device__ __forceinline__ FoldScale fold_scale(float run_m, float m) {
+  const float mn = fmaxf(run_m, m);
+  return {mn, exp2_fast(run_m - mn), exp2_fast(m - mn)};
+}
+// Written as one explicit fma over a separately rounded product, so the compiler has no
+// contraction choice to make differently in different kernels.
+__device__ __forceinline__ float fold_elem(float run, float part, const FoldScale& f) {
+  return __builtin_fmaf(run, f.alpha, part * f.beta);
+}
+
+__device__ __forceinline__ void fold(RowState& run, float m, float l, const f32x4_v (&a)[8]) {
+  const FoldScale f = fold_scale(run.m, m);
+  run.l = fold_elem(run.l, l, f);
+#pragma unroll
+  for (int db = 0; db < 8; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) run.acc[db][i] = fold_elem(run.acc[db][i], a[db][i], f);
+  run.m = f.mn;
+}
+
+// The row's output: acc / l rounded to bf16 (this lane: dims 16 db + 4 g .. +3).
+__device__ __forceinline__ void store_row(bf16_t* op, const RowState& run, int g) {
+  const float y = 1.0f / run.l;
+#pragma unroll
+  for (int db = 0; db < 8; ++db) {
+    const f32x4_v a = run.acc[db];
+    uint2 u;
+    u.x = pack_bf16x2(div_row(a[0], run.l, y), div_row(a[1], run.l, y));
+    u.y = pack_bf16x2(div_row(a[2], run.l, y), div_row(a[3], run.l, y));
+    *reinterpret_cast<uint2*>(op + 16 * db + 4 * g) = u;
+  }
+}
+
+// Softmax of one tile's scores s (in place: s becomes p), in the exp2 domain:
+// p = 2^(s * sc2 - m) with sc2 = sm_scale * log2(e) and m the row's reference maximum in
+// the same units. The reference maximum is lazy: it moves to the tile's maximum only when
+// that exceeds it by more than LAZY_T, so p <= 2^LAZY_T and most tiles leave it (and the
+// accumulator) alone. Every decision is per row (per lane group), so a row's bits depend
+// on its own scores only. MASK: apply causality and row validity (keys beyond the row's
+// position give p = 0). Returns the accumulator's rescale factor (exactly 1 when the
+// reference maximum stays).
+template <bool MASK, class C>
+__device__ __forceinline__ float softmax_tile(float (&s)[16], RowState& st, const C& c, int t0,
+                                              float sc2) {
+  bool vis[16];
+  float tmax = NEG_BIG;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (MASK) {
+      const int key = t0 + 32 * (i >> 3) + 8 * c.g + (i & 7);
+      vis[i] = (key <= c.q_abs) & c.row_ok;
+      tmax = fmaxf(tmax, vis[i] ? s[i] : NEG_BIG);
+    } else {
+      tmax = fmaxf(tmax, s[i]);
+    }
+  }
+  tmax = pair16_max(tmax);
+  tmax = pair32_max(tmax);
+  const float mc = tmax * sc2;
+  const float m_used = mc > st.m + LAZY_T ? mc : st.m;
+  const float rescale = exp2_fast(st.m - m_used);
+  float psum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float p = exp2_fast(__builtin_fmaf(s[i], sc2, -m_used));
+    if constexpr (MASK) s[i] = vis[i] ? p : 0.0f;
+    else s[i] = p;
+    psum += s[i];
+  }
+  psum = pair16_sum(psum);
+  psum = pair32_sum(psum);
+  st.l = __builtin_fmaf(st.l, rescale, psum);
+  st.m = m_used;
+  return rescale;
+}
+
+// p of a tile as the PV product's B operand (p is finite: exp of a finite difference, or 0).
+__device__ __forceinline__ void pack_p(bf16x8_v (&pf)[2], const float (&s)[16]) {
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    uint4 u;
+    u.x = pack_bf16x2(s[8 * kb + 0], s[8 * kb + 1]);
+    u.y = pack_bf16x2(s[8 * kb + 2], s[8 * kb + 3]);
+    u.z = pack_bf16x2(s[8 * kb + 4], s[8 * kb + 5]);
+    u.w = pack_bf16x2(s[8 * kb + 6], s[8 * kb + 7]);
+    pf[kb] = __builtin_bit_cast(bf16x8_v, u);
+  }
+}
+
+// x * 1 == x: the rescale is skipped (same bits) unless some row of the wave moved its
+// reference maximum.
+__device__ __forceinline__ void apply_rescale(RowState& st, float rescale) {
+  if (__builtin_amdgcn_ballot_w64(rescale != 1.0f) != 0) {
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      st.acc[db][0] *= rescale;
+      st.acc[db][1] *= rescale;
+      st.acc[db][2] *= rescale;
+      st.acc[db][3] *= rescale;
+    }
+  }
+}
+
+// LDS tiles are 64 rows of 256 bytes; 16-byte piece p of key's row sits at p ^ swz(key): over
+// the 16 keys of a fragment or transpose read swz takes 16 values.
+__device__ __forceinline__ int swz(int key) { return (key & 3) | (((key >> 3) & 3) << 2); }
+
+constexpr int kTileBytes = BN * D * 2;  // one K or V tile
+
+// ---- host side (extend_attention.hip) -----------------------------------------------------
+
+// Query positions (32 or 64) of a workgroup that walks all keys of its rows.
+int extend_prefill_rows(int batch, int64_t total_q, int num_kv_heads, int max_extend_len);
+
+// The launch of a call, worked out once for both formats: what is checked, whether the splits
+// fan out over workgroups (workspace given and the grid small), the grid.
+struct ExtendPlan {
+  int rc;             // SID_OK or the error
+  bool empty;         // nothing to do
+  bool fanout;
+  int rows;           // 32 or 64 query positions a workgroup (fan-out: 32)
+  int mtiles, splits;
+  unsigned grid_x;    // workgroups over the requests (padded for ragged batches)
+  int64_t items;      // (query row, head) pairs
+  float* part_a;
+  float* part_ml;
+  int32_t* part_n;
+};
+ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, const void* v_cache,
+                       const int32_t* qo_indptr, const int32_t* kv_indptr,
+                       const int32_t* kv_indices, const void* o, int batch, int64_t total_q,
+                       int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
+                       int max_extend_len, int max_kv_len, void* workspace,
+                       int64_t workspace_bytes);
+
+// The fan-out's second launch: the saved split states of every item folded in order.
+int extend_merge(const char* name, const ExtendPlan& p, void* o, hipStream_t s);
+
+}  // namespace sid

@@ -13,7 +13,7 @@
 // kernels share goes through the same helpers with explicit fmaf, so the
 // fused and unfused paths also agree bit for bit after the first rounding.
 #include "common.h"
-#include "rowmath.h"
+#include "kv_fp8.h"
 
 #include <cmath>
 
@@ -302,13 +302,16 @@ __global__ void __launch_bounds__(128) silu_mul_kernel(RowSrc gu, uint2* __restr
 // v heads: copied. q goes to q_out [T, HQ, 128]; k and v to the pools at slots[t].
 constexpr int QD = 128;
 
-template <int NCH>
+//
+// FP8: the pools hold codes and kv_scales their powers of two (kv_fp8.h); k and v are then
+// quantised from the same bf16 values.
+template <int NCH, bool FP8>
 __global__ void __launch_bounds__(128) qkv_post_kernel(
     RowSrc src, int num_q_heads, int num_kv_heads, const uint4* __restrict__ q_norm,
     const uint4* __restrict__ k_norm, float eps, const int64_t* __restrict__ positions,
     const float* __restrict__ cos_sin, int64_t max_positions, const int64_t* __restrict__ slots,
-    uint4* __restrict__ q_out, uint4* __restrict__ k_cache, uint4* __restrict__ v_cache,
-    int64_t num_slots) {
+    uint4* __restrict__ q_out, void* __restrict__ k_cache, void* __restrict__ v_cache,
+    uint8_t* __restrict__ kv_scales, int64_t num_slots) {
   const int64_t t = blockIdx.x;
   const int head = blockIdx.y * 8 + (threadIdx.x >> 4);
   const int j = threadIdx.x & 15;
@@ -325,8 +328,13 @@ __global__ void __launch_bounds__(128) qkv_post_kernel(
   const bool slot_ok = slot >= 0 && slot < num_slots;
   const int kv_row = 16 * num_kv_heads;  // uint4 per pool row
   if (is_v) {
-    if (valid && slot_ok)
-      v_cache[slot * kv_row + (hh - num_q_heads - num_kv_heads) * 16 + j] = store8(v);
+    const int h = hh - num_q_heads - num_kv_heads;
+    if constexpr (FP8) {
+      fp8_store_vector(v, j, valid && slot_ok, static_cast<uint2*>(v_cache), kv_scales,
+                       slot * num_kv_heads + h, 1);
+    } else if (valid && slot_ok) {
+      static_cast<uint4*>(v_cache)[slot * kv_row + h * 16 + j] = store8(v);
+    }
     return;  // v heads occupy whole blocks' tail groups; no cross-lane op follows for them
   }
   const bool is_q = hh < num_q_heads;
@@ -337,8 +345,11 @@ __global__ void __launch_bounds__(128) qkv_post_kernel(
   if (!valid) return;
   if (is_q) {
     q_out[(t * num_q_heads + hh) * 16 + j] = store8(o);
+  } else if constexpr (FP8) {
+    fp8_store_vector(o, j, slot_ok, static_cast<uint2*>(k_cache), kv_scales,
+                     slot * num_kv_heads + hh - num_q_heads, 0);
   } else if (slot_ok) {
-    k_cache[slot * kv_row + (hh - num_q_heads) * 16 + j] = store8(o);
+    static_cast<uint4*>(k_cache)[slot * kv_row + (hh - num_q_heads) * 16 + j] = store8(o);
   }
 }
 
@@ -463,6 +474,38 @@ extern "C" int sid_silu_mul_partials(const float* partials, int nchunks, void* o
                      stream, "silu_mul_partials");
 }
 
+// sid_qkv_post (kv_scales NULL: bf16 pools) and sid_qkv_post_fp8.
+static int launch_qkv_post(const char* name, const void* qkv, const float* partials, int nchunks,
+                           int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                           const void* q_norm, const void* k_norm, float eps,
+                           const int64_t* positions, const float* cos_sin, int64_t max_positions,
+                           const int64_t* slots, void* q_out, void* k_cache, void* v_cache,
+                           void* kv_scales, int64_t num_slots, void* stream) {
+  SID_REQUIRE((qkv != nullptr) != (partials != nullptr),
+              "%s: exactly one of qkv and partials must be given", name);
+  SID_REQUIRE(partials == nullptr || nchunks >= 1, "%s: nchunks must be >= 1", name);
+  SID_REQUIRE(head_dim == QD, "%s: head_dim must be %d, got %d", name, QD, head_dim);
+  SID_REQUIRE(num_q_heads > 0 && num_kv_heads > 0, "%s: bad head counts", name);
+  SID_REQUIRE(q_norm && k_norm && positions && cos_sin && slots && q_out && k_cache && v_cache,
+              "%s: null pointer", name);
+  SID_REQUIRE(num_slots > 0, "%s: empty KV pool", name);
+  SID_REQUIRE(num_tokens < (1ll << 31), "%s: too many tokens", name);
+  const int64_t ld = static_cast<int64_t>(num_q_heads + 2 * num_kv_heads) * QD;
+  const RowSrc src = partials ? part_src(partials, nchunks, num_tokens, ld) : bf_src(qkv, ld);
+  const int heads = num_q_heads + 2 * num_kv_heads;
+  const dim3 grid((unsigned)num_tokens, (unsigned)ceil_div(heads, 8));
+  dispatch_nch(src, [&]<int NCH>() {
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, grid, dim3(128), 0, static_cast<hipStream_t>(stream), src,
+                         num_q_heads, num_kv_heads, (const uint4*)q_norm, (const uint4*)k_norm,
+                         eps, positions, cos_sin, max_positions, slots, (uint4*)q_out, k_cache,
+                         v_cache, (uint8_t*)kv_scales, num_slots);
+    };
+    if (kv_scales) go(qkv_post_kernel<NCH, true>); else go(qkv_post_kernel<NCH, false>);
+  });
+  return check_launch(name);
+}
+
 extern "C" int sid_qkv_post(const void* qkv, const float* partials, int nchunks,
                             int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
                             const void* q_norm, const void* k_norm, float eps,
@@ -471,24 +514,24 @@ extern "C" int sid_qkv_post(const void* qkv, const float* partials, int nchunks,
                             void* k_cache, void* v_cache, int64_t num_slots, void* stream) {
   SID_REQUIRE(num_tokens >= 0, "qkv_post: negative token count");
   if (num_tokens == 0) return SID_OK;
-  SID_REQUIRE((qkv != nullptr) != (partials != nullptr),
-              "qkv_post: exactly one of qkv and partials must be given");
-  SID_REQUIRE(partials == nullptr || nchunks >= 1, "qkv_post: nchunks must be >= 1");
-  SID_REQUIRE(head_dim == QD, "qkv_post: head_dim must be %d, got %d", QD, head_dim);
-  SID_REQUIRE(num_q_heads > 0 && num_kv_heads > 0, "qkv_post: bad head counts");
-  SID_REQUIRE(q_norm && k_norm && positions && cos_sin && slots && q_out && k_cache && v_cache,
-              "qkv_post: null pointer");
-  SID_REQUIRE(num_slots > 0, "qkv_post: empty KV pool");
-  SID_REQUIRE(num_tokens < (1ll << 31), "qkv_post: too many tokens");
-  const int64_t ld = static_cast<int64_t>(num_q_heads + 2 * num_kv_heads) * QD;
-  const RowSrc src = partials ? part_src(partials, nchunks, num_tokens, ld) : bf_src(qkv, ld);
-  const int heads = num_q_heads + 2 * num_kv_heads;
-  const dim3 grid((unsigned)num_tokens, (unsigned)ceil_div(heads, 8));
-  dispatch_nch(src, [&]<int NCH>() {
-    hipLaunchKernelGGL(qkv_post_kernel<NCH>, grid, dim3(128), 0, static_cast<hipStream_t>(stream),
-                       src, num_q_heads, num_kv_heads, (const uint4*)q_norm, (const uint4*)k_norm,
-                       eps, positions, cos_sin, max_positions, slots, (uint4*)q_out,
-                       (uint4*)k_cache, (uint4*)v_cache, num_slots);
-  });
-  return check_launch("qkv_post");
+  return launch_qkv_post("qkv_post", qkv, partials, nchunks, num_tokens, num_q_heads,
+                         num_kv_heads, head_dim, q_norm, k_norm, eps, positions, cos_sin,
+                         max_positions, slots, q_out, k_cache, v_cache, nullptr, num_slots,
+                         stream);
+}
+
+extern "C" int sid_qkv_post_fp8(const void* qkv, const float* partials, int nchunks,
+                                int64_t num_tokens, int num_q_heads, int num_kv_heads,
+                                int head_dim, const void* q_norm, const void* k_norm, float eps,
+                                const int64_t* positions, const float* cos_sin,
+                                int64_t max_positions, const int64_t* slots, void* q_out,
+                                void* k_cache, void* v_cache, void* kv_scales, int64_t num_slots,
+                                void* stream) {
+  SID_REQUIRE(num_tokens >= 0, "qkv_post_fp8: negative token count");
+  if (num_tokens == 0) return SID_OK;
+  SID_REQUIRE(kv_scales != nullptr, "qkv_post_fp8: null pointer");
+  return launch_qkv_post("qkv_post_fp8", qkv, partials, nchunks, num_tokens, num_q_heads,
+                         num_kv_heads, head_dim, q_norm, k_norm, eps, positions, cos_sin,
+                         max_positions, slots, q_out, k_cache, v_cache, kv_scales, num_slots,
+                         stream);
 }

@@ -56,6 +56,18 @@ _SIGNATURES = {
                              _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp],
     "sid_rmsnorm_f32": [_vp, _vp, _vp, _i64, _i32, _f32, _vp],
     "sid_pack_decode_weight": [_vp, _vp, _i64, _i64, _i32, _vp],
+    "sid_reshape_and_cache_fp8": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32,
+                                  _i64, _vp],
+    "sid_gather_cache_fp8": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _vp],
+    "sid_qkv_post_fp8": [_vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _vp, _vp, _i64,
+                         _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "sid_rmsnorm_qkv_post_fp8": [_vp, _i32, _vp, _f32, _vp, _i64, _i64, _i32, _i32, _i32, _vp,
+                                 _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "sid_flash_decode_fp8_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64,
+                                 _i32, _i32, _i32, _i32, _i32, _vp, _f32, _vp, _vp, _i32, _i32,
+                                 _vp, _i32, _vp],
+    "sid_extend_attention_fp8_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
+                                     _i32, _i64, _i32, _i32, _f32, _vp, _i64, _vp, _vp],
 }
 EXPORTED = ("sid_last_error", "sid_abi_version", "sid_extend_attention_workspace_bytes",
             "sid_linear_argmax_workspace_bytes", "sid_sample_workspace_bytes",
@@ -80,6 +92,27 @@ def _gpu(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> None:
         raise RuntimeError(f"{name} must be contiguous")
     if dtype is not None and t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _pool8(k_cache, v_cache, kv_scales, head_dim: int, device) -> tuple:
+    """Checks an 8-bit KV pool (codes and their scales) on `device`; its shape [S, HKV, D]."""
+    _gpu(k_cache, "k_cache", torch.float8_e4m3fn)
+    _gpu(v_cache, "v_cache", torch.float8_e4m3fn)
+    _gpu(kv_scales, "kv_scales", torch.float8_e8m0fnu)
+    ks = k_cache.shape
+    if len(ks) != 3 or ks[2] != head_dim or v_cache.shape != ks:
+        raise RuntimeError(f"k_cache and v_cache must both be [S, HKV, {head_dim}]")
+    if tuple(kv_scales.shape) != (ks[0], ks[1], 2):
+        raise RuntimeError(f"kv_scales must be [S, HKV, 2] = [{ks[0]}, {ks[1]}, 2], got "
+                           f"{list(kv_scales.shape)}")
+    _same_device(device, k_cache, v_cache, kv_scales)
+    return ks
+
+
+def _same_device(device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"operands on {t.device} and {device}: all must be on one device")
 
 
 def _ptr(t) -> int:
@@ -128,28 +161,43 @@ class NativeLib:
         if rc != 0:
             raise RuntimeError(f"{name}: {self.lib.sid_last_error().decode(errors='replace')}")
 
+    def _launch(self, t: torch.Tensor, name: str, *args) -> None:
+        """_call with t's current stream, t's device made current if it is not (the null stream
+        belongs to the current device)."""
+        if t.get_device() == torch._C._cuda_getDevice():
+            self._call(name, *args, _stream(t))
+        else:
+            with torch.cuda.device(t.device):
+                self._call(name, *args, _stream(t))
+
     # ---- reference module `sid_flash_decode` (sid/csrc/flash_decode.cu:408-413) ----------
 
     def flash_decode_fwd(self, q, k_cache, v_cache, kv_indptr, kv_indices, num_splits,
                          max_splits: int, fixed_split_size: int, sm_scale: float,
                          part_o, part_lse, o, segment_size: int = 0,
                          grid_slots: int | None = None, variant: int = 0,
-                         wg_order=None, workers: int = 0) -> None:
+                         wg_order=None, workers: int = 0, kv_scales=None) -> None:
         """segment_size / grid_slots / variant / wg_order: see sid_flash_decode_segments_fwd
         (defaults: one segment per split, grid of max_splits slots = the reference's
         partition, the default workgroup shape, the grid's own order); workers > 0: stage 1
         by that many workgroups over the items of wg_order (sid_flash_decode_workers_fwd; entries
-        flagged ORDER_EMPTY hold no tokens)."""
+        flagged ORDER_EMPTY hold no tokens); kv_scales: the caches are an 8-bit pool
+        (sid_flash_decode_fp8_fwd)."""
         _gpu(q, "q", torch.bfloat16)
         _check(q.dim() == 3, "q must be [B, HQ, D]")
         b, hq, d = qs = q.shape  # (each .shape builds a new object: taken once)
-        _gpu(k_cache, "k_cache", torch.bfloat16)
-        _gpu(v_cache, "v_cache", torch.bfloat16)
-        ks, vs = k_cache.shape, v_cache.shape
-        for name, sh in (("k_cache", ks), ("v_cache", vs)):
-            if not (len(sh) == 3 and sh[2] == d):
-                raise RuntimeError(f"{name} must be [slots, HKV, {d}]")
-        _check(ks == vs, "k_cache and v_cache shapes differ")
+        if kv_scales is not None:
+            ks = _pool8(k_cache, v_cache, kv_scales, d, q.device)
+            _same_device(q.device, kv_indptr, kv_indices, num_splits, part_o, part_lse, o,
+                         wg_order)
+        else:
+            _gpu(k_cache, "k_cache", torch.bfloat16)
+            _gpu(v_cache, "v_cache", torch.bfloat16)
+            ks, vs = k_cache.shape, v_cache.shape
+            for name, sh in (("k_cache", ks), ("v_cache", vs)):
+                if not (len(sh) == 3 and sh[2] == d):
+                    raise RuntimeError(f"{name} must be [slots, HKV, {d}]")
+            _check(ks == vs, "k_cache and v_cache shapes differ")
         num_slots, hkv, _ = ks
         _gpu(kv_indptr, "kv_indptr", torch.int32)
         _check(kv_indptr.numel() == b + 1, "kv_indptr must have B+1 entries")
@@ -169,13 +217,16 @@ class NativeLib:
         slots = int(max_splits) if grid_slots is None else int(grid_slots)
         order = self._order_ptr(wg_order, b * slots)
         _check(workers == 0 or wg_order is not None, "a worker launch needs wg_order")
+        plan = (kv_indptr.data_ptr(), kv_indices.data_ptr(), _ptr(num_splits), b, hq, hkv, d,
+                num_slots, int(max_splits), int(fixed_split_size), int(segment_size), slots,
+                int(variant), order, float(sm_scale), part_o.data_ptr(), part_lse.data_ptr(),
+                po[0], po[2], o.data_ptr(), int(workers))
+        if kv_scales is not None:
+            self._launch(q, "sid_flash_decode_fp8_fwd", q.data_ptr(), k_cache.data_ptr(),
+                         v_cache.data_ptr(), kv_scales.data_ptr(), *plan)
+            return
         self._call("sid_flash_decode_workers_fwd", q.data_ptr(), k_cache.data_ptr(),
-                   v_cache.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
-                   _ptr(num_splits), b, hq, hkv, d, num_slots, int(max_splits),
-                   int(fixed_split_size), int(segment_size), slots, int(variant), order,
-                   float(sm_scale),
-                   part_o.data_ptr(), part_lse.data_ptr(), po[0], po[2],
-                   o.data_ptr(), int(workers), _stream(q))
+                   v_cache.data_ptr(), *plan, _stream(q))
 
     def flash_decode_fwd_noalloc(self, q, k_cache, v_cache, kv_indptr, kv_indices, num_splits,
                                  max_splits: int, fixed_split_size: int, sm_scale: float, o,
@@ -232,6 +283,48 @@ class NativeLib:
                    v_cache.data_ptr(), slot_mapping.data_ptr(), ks[0], cs[1], cs[2],
                    cs[0], _stream(k))
 
+    # ---- 8-bit pool ----------------------------------------------------------------------
+
+    def reshape_and_cache_fp8(self, k, v, k_cache, v_cache, kv_scales, slot_mapping) -> None:
+        for name, x in (("k", k), ("v", v)):
+            if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.bfloat16):
+                raise RuntimeError(f"{name} must be a bf16 GPU tensor")
+            if x.dim() != 3:
+                raise RuntimeError(f"{name} must be [T, HKV, D]")
+        xs = k.shape
+        _check(v.shape == xs, "v must have k's shape")
+        cs = _pool8(k_cache, v_cache, kv_scales, xs[2], k.device)
+        _check(xs[1] == cs[1], "k must be [T, HKV, D] matching the cache")
+        _gpu(slot_mapping, "slot_mapping", torch.int64)
+        _check(slot_mapping.numel() == xs[0], "slot_mapping must have T entries")
+        _same_device(k.device, v, slot_mapping)
+        if xs[0] == 0:
+            return
+        row = xs[1] * xs[2]
+        ld = []
+        for name, x in (("k", k), ("v", v)):  # heads and dims dense, any token stride
+            if (x.stride(2) != 1 and xs[2] > 1) or (x.stride(1) != xs[2] and xs[1] > 1):
+                raise RuntimeError(f"{name}'s heads and dims must be contiguous")
+            ld.append(x.stride(0) if xs[0] > 1 else row)
+        self._launch(k, "sid_reshape_and_cache_fp8", k.data_ptr(), ld[0], v.data_ptr(), ld[1],
+                     k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
+                     slot_mapping.data_ptr(), xs[0], cs[1], cs[2], cs[0])
+
+    def gather_cache_fp8(self, k_cache, v_cache, kv_scales, slots, k, v) -> None:
+        _gpu(slots, "slots", torch.int64)
+        _gpu(k, "k", torch.bfloat16)
+        _gpu(v, "v", torch.bfloat16)
+        n = slots.numel()
+        _check(k.dim() == 3 and v.shape == k.shape, "k and v must both be [N, HKV, D]")
+        cs = _pool8(k_cache, v_cache, kv_scales, k.shape[2], slots.device)
+        _check(k.shape[0] == n and k.shape[1] == cs[1], "k must be [N, HKV, D] matching the cache")
+        _same_device(slots.device, k, v)
+        if n == 0:
+            return
+        self._launch(k, "sid_gather_cache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
+                     kv_scales.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), n, cs[1],
+                     cs[2], cs[0])
+
     # ---- the rest of the decode path ----------------------------------------------------
 
     def extend_attention_workspace_bytes(self, batch, total_q, hq, hkv, max_extend_len,
@@ -241,13 +334,18 @@ class NativeLib:
 
     def extend_attention_fwd(self, q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices,
                              max_extend_len: int, sm_scale: float, o, max_kv_len: int,
-                             workspace=None) -> None:
+                             workspace=None, kv_scales=None) -> None:
+        """kv_scales: the buffers are an 8-bit pool (sid_extend_attention_fp8_fwd)."""
         _gpu(q, "q_extend", torch.bfloat16)
         _check(q.dim() == 3, "q_extend must be [Text, HQ, D]")
-        _gpu(k_buffer, "k_buffer", torch.bfloat16)
-        _gpu(v_buffer, "v_buffer", torch.bfloat16)
-        _check(k_buffer.shape == v_buffer.shape and k_buffer.dim() == 3
-               and k_buffer.shape[2] == q.shape[2], "bad KV buffer shapes")
+        if kv_scales is not None:
+            _pool8(k_buffer, v_buffer, kv_scales, q.shape[2], q.device)
+            _same_device(q.device, qo_indptr, kv_indptr, kv_indices, o, workspace)
+        else:
+            _gpu(k_buffer, "k_buffer", torch.bfloat16)
+            _gpu(v_buffer, "v_buffer", torch.bfloat16)
+            _check(k_buffer.shape == v_buffer.shape and k_buffer.dim() == 3
+                   and k_buffer.shape[2] == q.shape[2], "bad KV buffer shapes")
         _gpu(qo_indptr, "qo_indptr", torch.int32)
         _gpu(kv_indptr, "kv_indptr", torch.int32)
         _gpu(kv_indices, "kv_indices", torch.int32)
@@ -258,11 +356,16 @@ class NativeLib:
         if workspace is not None:
             _gpu(workspace, "workspace", torch.uint8)
             ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
+        rest = (qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
+                qo_indptr.numel() - 1, q.shape[0], q.shape[1], k_buffer.shape[1], q.shape[2],
+                k_buffer.shape[0], int(max_extend_len), int(max_kv_len), float(sm_scale), ws_ptr,
+                ws_bytes, o.data_ptr())
+        if kv_scales is not None:
+            self._launch(q, "sid_extend_attention_fp8_fwd", q.data_ptr(), k_buffer.data_ptr(),
+                         v_buffer.data_ptr(), kv_scales.data_ptr(), *rest)
+            return
         self._call("sid_extend_attention_fwd", q.data_ptr(), k_buffer.data_ptr(),
-                   v_buffer.data_ptr(), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
-                   kv_indices.data_ptr(), qo_indptr.numel() - 1, q.shape[0], q.shape[1],
-                   k_buffer.shape[1], q.shape[2], k_buffer.shape[0], int(max_extend_len),
-                   int(max_kv_len), float(sm_scale), ws_ptr, ws_bytes, o.data_ptr(), _stream(q))
+                   v_buffer.data_ptr(), *rest, _stream(q))
 
     def rmsnorm(self, x, w, out, eps: float) -> None:
         _gpu(x, "x", torch.bfloat16)
@@ -384,7 +487,8 @@ class NativeLib:
                    two_i // 2, _stream(out))
 
     def qkv_post(self, qkv, partials, q_norm, k_norm, eps: float, positions, cos_sin, slots,
-                 q_out, k_cache, v_cache) -> None:
+                 q_out, k_cache, v_cache, kv_scales=None) -> None:
+        """kv_scales: the caches are an 8-bit pool (sid_qkv_post_fp8)."""
         _check((qkv is None) != (partials is None), "give exactly one of qkv and partials")
         if qkv is not None:
             _gpu(qkv, "qkv", torch.bfloat16)
@@ -395,9 +499,7 @@ class NativeLib:
         _gpu(q_out, "q_out", torch.bfloat16)
         _check(q_out.dim() == 3 and q_out.shape[0] == t, "q_out must be [T, HQ, D]")
         hq, d = q_out.shape[1], q_out.shape[2]
-        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            _gpu(c, name, torch.bfloat16)
-            _check(c.dim() == 3 and c.shape[2] == d, f"{name} must be [S, HKV, D]")
+        self._cache_operands(k_cache, v_cache, kv_scales, d, q_out.device)
         hkv = k_cache.shape[1]
         _check(width == (hq + 2 * hkv) * d, "projection width != (HQ + 2*HKV) * D")
         _gpu(q_norm, "q_norm", torch.bfloat16)
@@ -406,11 +508,24 @@ class NativeLib:
         _gpu(slots, "slots", torch.int64)
         _gpu(cos_sin, "cos_sin", torch.float32)
         _check(positions.numel() == t and slots.numel() == t, "positions/slots must have T entries")
-        self._call("sid_qkv_post", qkv.data_ptr() if qkv is not None else None,
-                   partials.data_ptr() if partials is not None else None, nch, t, hq, hkv, d,
-                   q_norm.data_ptr(), k_norm.data_ptr(), float(eps), positions.data_ptr(),
-                   cos_sin.data_ptr(), cos_sin.shape[0], slots.data_ptr(), q_out.data_ptr(),
-                   k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], _stream(q_out))
+        args = (_ptr(qkv), _ptr(partials), nch, t, hq, hkv, d, q_norm.data_ptr(),
+                k_norm.data_ptr(), float(eps), positions.data_ptr(), cos_sin.data_ptr(),
+                cos_sin.shape[0], slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+                v_cache.data_ptr())
+        if kv_scales is not None:
+            _same_device(q_out.device, qkv, partials, q_norm, k_norm, positions, cos_sin, slots)
+            self._launch(q_out, "sid_qkv_post_fp8", *args, kv_scales.data_ptr(), k_cache.shape[0])
+            return
+        self._call("sid_qkv_post", *args, k_cache.shape[0], _stream(q_out))
+
+    @staticmethod
+    def _cache_operands(k_cache, v_cache, kv_scales, d: int, device) -> None:
+        if kv_scales is not None:
+            _pool8(k_cache, v_cache, kv_scales, d, device)
+            return
+        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+            _gpu(c, name, torch.bfloat16)
+            _check(c.dim() == 3 and c.shape[2] == d, f"{name} must be [S, HKV, D]")
 
     def linear_residual(self, x, w, residual, r32) -> None:
         """residual, r32 <- r = residual + bf16(x @ w^T) (fp32 r; residual = bf16(r))."""
@@ -444,8 +559,9 @@ class NativeLib:
                    float(eps), w.data_ptr(), out.data_ptr(), m, hidden, inter, _stream(out))
 
     def rmsnorm_qkv_post(self, src, norm_w, eps: float, w, q_norm, k_norm, positions, cos_sin,
-                         slots, q_out, k_cache, v_cache) -> None:
-        """qkv_post over bf16(rmsnorm(src) * norm_w) @ w^T (one launch)."""
+                         slots, q_out, k_cache, v_cache, kv_scales=None) -> None:
+        """qkv_post over bf16(rmsnorm(src) * norm_w) @ w^T (one launch); kv_scales: the caches
+        are an 8-bit pool (sid_rmsnorm_qkv_post_fp8)."""
         f32 = self._norm_src(src)
         m, hidden = src.shape
         _gpu(norm_w, "norm weight", torch.bfloat16)
@@ -453,9 +569,7 @@ class NativeLib:
         _gpu(q_out, "q_out", torch.bfloat16)
         _check(q_out.dim() == 3 and q_out.shape[0] == m, "q_out must be [M, HQ, D]")
         hq, d = q_out.shape[1], q_out.shape[2]
-        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            _gpu(c, name, torch.bfloat16)
-            _check(c.dim() == 3 and c.shape[2] == d, f"{name} must be [S, HKV, D]")
+        self._cache_operands(k_cache, v_cache, kv_scales, d, q_out.device)
         hkv = k_cache.shape[1]
         _check(w.dim() == 2 and w.shape[0] == (hq + 2 * hkv) * d and w.shape[1] == hidden
                and norm_w.numel() == hidden, "qkv weight must be [(HQ + 2*HKV) * D, hidden]")
@@ -465,11 +579,16 @@ class NativeLib:
         _gpu(slots, "slots", torch.int64)
         _gpu(cos_sin, "cos_sin", torch.float32)
         _check(positions.numel() == m and slots.numel() == m, "positions/slots must have M entries")
-        self._call("sid_rmsnorm_qkv_post", src.data_ptr(), f32, norm_w.data_ptr(), float(eps),
-                   w.data_ptr(), m, hidden, hq, hkv, d, q_norm.data_ptr(), k_norm.data_ptr(),
-                   positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], slots.data_ptr(),
-                   q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
-                   _stream(q_out))
+        args = (src.data_ptr(), f32, norm_w.data_ptr(), float(eps), w.data_ptr(), m, hidden, hq,
+                hkv, d, q_norm.data_ptr(), k_norm.data_ptr(), positions.data_ptr(),
+                cos_sin.data_ptr(), cos_sin.shape[0], slots.data_ptr(), q_out.data_ptr(),
+                k_cache.data_ptr(), v_cache.data_ptr())
+        if kv_scales is not None:
+            _same_device(q_out.device, src, norm_w, w, q_norm, k_norm, positions, cos_sin, slots)
+            self._launch(q_out, "sid_rmsnorm_qkv_post_fp8", *args, kv_scales.data_ptr(),
+                         k_cache.shape[0])
+            return
+        self._call("sid_rmsnorm_qkv_post", *args, k_cache.shape[0], _stream(q_out))
 
     def pack_decode_weight(self, w, packed, gate_up: bool) -> None:
         """packed <- w [N, K] in the fragment-packed order of the decode-chain kernels."""

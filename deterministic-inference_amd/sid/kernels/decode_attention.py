@@ -385,12 +385,33 @@ class DecodeAttention:
         splits, seg, slots = geometry
         return None, splits, 0, seg, slots
 
+    def step_plan(self, lengths, kv_fp8: bool = False, max_len: int | None = None) -> dict:
+        """The nondet/dvr plan of a decode step over requests of these lengths (host-side), as
+        forward's arguments: geometry and workgroup shape (plan_variant) and the placement of
+        the workgroups (workgroup_order, worker_order). One plan serves the step's layers. Its
+        order is copied to the device here: make it outside a graph capture. max_len: the bound
+        that forward is called with, if it is not the longest length; kv_fp8: 8-bit pool."""
+        lens = [int(n) for n in lengths]
+        bound = max(max(lens, default=1) if max_len is None else int(max_len), 1)
+        cu = self.cu_count()
+        geom, variant = plan_variant(lens, bound, self.num_kv_heads, cu, self.max_kv_splits,
+                                     invariant=False)
+        tokens = segment_tokens(lens, len(lens), geom[0], 0, geom[1], geom[2])
+        nonempty = int(np.count_nonzero(tokens))
+        workers = stage1_workers(nonempty, variant, geom[2], cu)
+        order = None
+        if workers or nonempty >= cu:
+            host = worker_order(tokens, workers) if workers else workgroup_order(tokens, cu)
+            order = torch.from_numpy(host).to(self.device)
+        return dict(variant=variant, geometry=geom, wg_order=order, workers=workers)
+
     def forward(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 kv_indptr: torch.Tensor, kv_indices: torch.Tensor, seq_lens: torch.Tensor,
                 max_seq_len: int, sm_scale: float, invariant: bool,
                 policy_batch: int | None = None, variant: int | None = None,
                 geometry: tuple | None = None,
-                wg_order: torch.Tensor | None = None, workers: int = 0) -> torch.Tensor:
+                wg_order: torch.Tensor | None = None, workers: int = 0,
+                kv_scales: torch.Tensor | None = None) -> torch.Tensor:
         """q: [B, HQ, D] bf16 -> o: [B, HQ, D] bf16 (max_seq_len is host-side, no sync).
         policy_batch: real requests among the B rows (the rest are empty padding); variant:
         the stage-1 workgroup shape (stage1_variant; None: INVARIANT_VARIANT in batch_invariant
@@ -399,7 +420,7 @@ class DecodeAttention:
         max_seq_len alone); wg_order: workgroup_order of this plan, on the device (None: the
         grid's own order); workers > 0: stage 1 by that many workgroups, each computing the
         items of wg_order dealt to it (then a permutation of every (request, slot) item; see
-        worker_order)."""
+        worker_order); kv_scales: the caches are an 8-bit pool (sid.kernels.kv_fp8)."""
         if variant is None:
             variant = INVARIANT_VARIANT if invariant else 0
         assert not invariant or variant == INVARIANT_VARIANT, \
@@ -419,5 +440,5 @@ class DecodeAttention:
         self.ext.flash_decode_fwd(q, k_cache, v_cache, kv_indptr, kv_indices, num_splits,
                                   grid_splits, fixed, sm_scale, self.part_o, self.part_lse, o,
                                   segment_size=seg, grid_slots=slots, variant=variant,
-                                  wg_order=wg_order, workers=workers)
+                                  wg_order=wg_order, workers=workers, kv_scales=kv_scales)
         return o

@@ -19,9 +19,11 @@ from sid.kernels.jit import load_ext
 def extend_attention_fwd(q_extend: torch.Tensor, k_buffer: torch.Tensor, v_buffer: torch.Tensor,
                          qo_indptr: torch.Tensor, kv_indptr: torch.Tensor,
                          kv_indices: torch.Tensor, max_extend_len: int,
-                         sm_scale: float, max_kv_len: int | None = None) -> torch.Tensor:
+                         sm_scale: float, max_kv_len: int | None = None,
+                         kv_scales: torch.Tensor | None = None) -> torch.Tensor:
     """max_kv_len (an extension of the reference signature): an upper bound of every
-    request's kv length; defaults to kv_indices.numel(), which needs no device sync."""
+    request's kv length; defaults to kv_indices.numel(), which needs no device sync.
+    kv_scales: the buffers are an 8-bit pool and these its scales (sid.kernels.kv_fp8)."""
     assert q_extend.is_contiguous()
     assert k_buffer.is_contiguous() and v_buffer.is_contiguous()
     ext = load_ext()
@@ -33,5 +35,5 @@ def extend_attention_fwd(q_extend: torch.Tensor, k_buffer: torch.Tensor, v_buffe
                                                 max_extend_len, max_kv_len)
     ws = torch.empty(need, dtype=torch.uint8, device=q_extend.device) if need else None
     ext.extend_attention_fwd(q_extend, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices,
-                             max_extend_len, sm_scale, o_extend, max_kv_len, ws)
+                             max_extend_len, sm_scale, o_extend, max_kv_len, ws, kv_scales=kv_scales)
     return o_extend

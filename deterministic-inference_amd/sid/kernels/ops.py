@@ -64,15 +64,18 @@ def fused_add_rmsnorm_partials(partials: torch.Tensor, residual: torch.Tensor,
 
 def qkv_post(qkv_or_partials: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
              positions: torch.Tensor, cos_sin: torch.Tensor, slots: torch.Tensor,
-             k_cache: torch.Tensor, v_cache: torch.Tensor, num_q_heads: int) -> torch.Tensor:
+             k_cache: torch.Tensor, v_cache: torch.Tensor, num_q_heads: int,
+             kv_scales: torch.Tensor | None = None) -> torch.Tensor:
     """Fused q/k-norm + RoPE + KV-cache write of a QKV projection (bf16 [T, W] or chunk
-    partials [C, T, W]); returns q [T, HQ, D]."""
+    partials [C, T, W]); returns q [T, HQ, D]. kv_scales: the caches are an 8-bit pool, which
+    gets what reshape_and_cache_fp8 of the same rows would store (sid.kernels.kv_fp8)."""
     partial = qkv_or_partials.dtype == torch.float32
     t = qkv_or_partials.shape[1] if partial else qkv_or_partials.shape[0]
     d = k_cache.shape[2]
     q = torch.empty(t, num_q_heads, d, dtype=torch.bfloat16, device=k_cache.device)
     load_ext().qkv_post(None if partial else qkv_or_partials, qkv_or_partials if partial else None,
-                        q_norm, k_norm, eps, positions, cos_sin, slots, q, k_cache, v_cache)
+                        q_norm, k_norm, eps, positions, cos_sin, slots, q, k_cache, v_cache,
+                        kv_scales=kv_scales)
     return q
 
 
@@ -116,13 +119,14 @@ def rmsnorm_linear_silu_mul(src: torch.Tensor, norm_w: torch.Tensor, eps: float,
 def rmsnorm_qkv_post(src: torch.Tensor, norm_w: torch.Tensor, eps: float, weight: torch.Tensor,
                      q_norm: torch.Tensor, k_norm: torch.Tensor, positions: torch.Tensor,
                      cos_sin: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
-                     v_cache: torch.Tensor, num_q_heads: int) -> torch.Tensor:
+                     v_cache: torch.Tensor, num_q_heads: int,
+                     kv_scales: torch.Tensor | None = None) -> torch.Tensor:
     """qkv_post of the qkv projection of bf16(rmsnorm(src) * norm_w); returns q [T, HQ, D].
-    weight = pack_decode_weight(qkv)."""
+    weight = pack_decode_weight(qkv); kv_scales as in qkv_post."""
     d = k_cache.shape[2]
     q = torch.empty(src.shape[0], num_q_heads, d, dtype=torch.bfloat16, device=src.device)
     load_ext().rmsnorm_qkv_post(src, norm_w, eps, weight, q_norm, k_norm, positions, cos_sin,
-                                slots, q, k_cache, v_cache)
+                                slots, q, k_cache, v_cache, kv_scales=kv_scales)
     return q
 
 

@@ -568,6 +568,83 @@ int sid_build_paged_decode_indices(int32_t* block_tables, int64_t max_pages, int
                                    const int32_t* kv_indptr, int32_t* kv_indices, int batch,
                                    void* stream);
 
+/*
+ * ---- 8-bit KV pool -------------------------------------------------------------------
+ *
+ * k_cache, v_cache: e4m3 codes [S, HKV, 128] (1 byte each); kv_scales: E8M0 bytes
+ * [S, HKV, 2], K's then V's. A vector x of 128 elements (one slot's head) is stored as
+ * codes c and 2^e with the smallest e for which max |x| <= 448 2^e, clamped to
+ * [-117, 119]; c = e4m3(x 2^-e), round to nearest even, saturating; byte e + 127. c 2^e is
+ * exact in bf16. A vector that holds an infinity or a NaN is NaN as a whole (codes 0x7f, byte
+ * 255). The reference has a bf16 pool only (sid/engine/kv_cache.py:33-40); these entry points
+ * are the 8-bit forms of the ones that replace its kernels, with the same arguments and
+ * semantics otherwise. All operands 16-byte aligned; head_dim 128.
+ *
+ * sid_reshape_and_cache_fp8: k, v bf16 [T, HKV, 128] with token strides ldk, ldv (elements,
+ * multiples of 8, at least HKV * 128: K and V may be columns of a projection) quantised into
+ * the pool at slot_mapping[t]; slots outside [0, S) are skipped. A slot may be named once
+ * only (two rows for one slot leave unspecified contents there).
+ */
+int sid_reshape_and_cache_fp8(const void* k, int64_t ldk, const void* v, int64_t ldv,
+                              void* k_cache, void* v_cache, void* kv_scales,
+                              const int64_t* slot_mapping, int64_t num_tokens, int num_kv_heads,
+                              int head_dim, int64_t num_slots, void* stream);
+
+/*
+ * k, v bf16 [N, HKV, 128] = the pool's rows slots[i] (int64 [N]), exactly what the codes stand
+ * for; slots outside [0, S) give rows of zeros.
+ */
+int sid_gather_cache_fp8(const void* k_cache, const void* v_cache, const void* kv_scales,
+                         const int64_t* slots, void* k, void* v, int64_t n, int num_kv_heads,
+                         int head_dim, int64_t num_slots, void* stream);
+
+/*
+ * sid_qkv_post / sid_rmsnorm_qkv_post into an 8-bit pool: k and v are rounded to bf16 and
+ * quantised from there, so the pool gets what sid_reshape_and_cache_fp8 of the unfused
+ * sequence's rows would put there, bit for bit; q is the same.
+ */
+int sid_qkv_post_fp8(const void* qkv, const float* partials, int nchunks, int64_t num_tokens,
+                     int num_q_heads, int num_kv_heads, int head_dim, const void* q_norm,
+                     const void* k_norm, float eps, const int64_t* positions,
+                     const float* cos_sin, int64_t max_positions, const int64_t* slots,
+                     void* q_out, void* k_cache, void* v_cache, void* kv_scales,
+                     int64_t num_slots, void* stream);
+int sid_rmsnorm_qkv_post_fp8(const void* src, int src_fp32, const void* norm_w, float eps,
+                             const void* w_qkv, int64_t m, int64_t hidden, int num_q_heads,
+                             int num_kv_heads, int head_dim, const void* q_norm,
+                             const void* k_norm, const int64_t* positions, const float* cos_sin,
+                             int64_t max_positions, const int64_t* slots, void* q_out,
+                             void* k_cache, void* v_cache, void* kv_scales, int64_t num_slots,
+                             void* stream);
+
+/*
+ * sid_flash_decode_workers_fwd over an 8-bit pool: the same splits, segments, orders and merge.
+ * The workgroup shapes that `variant` picks are this kernel's own (part of the reduction order,
+ * as there): 0 = 4 waves x 8 tokens per wave iteration, 1 = 4 x 2, 2 = 8 x 4, 3 = 4 x 4.
+ */
+int sid_flash_decode_fp8_fwd(const void* q, const void* k_cache, const void* v_cache,
+                             const void* kv_scales, const int32_t* kv_indptr,
+                             const int32_t* kv_indices, const int32_t* num_splits, int batch,
+                             int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
+                             int max_splits, int fixed_split_size, int segment_size,
+                             int grid_slots, int variant, const int32_t* wg_order,
+                             float sm_scale, float* part_o, float* part_lse, int part_batch,
+                             int part_stride, void* o, int workers, void* stream);
+
+/*
+ * sid_extend_attention_fwd over an 8-bit pool, with its workspace
+ * (sid_extend_attention_workspace_bytes) and its invariances: a query's result depends only on
+ * its position and its sequence's keys. A NaN vector reaches the queries that see its key and
+ * no others.
+ */
+int sid_extend_attention_fp8_fwd(const void* q, const void* k_cache, const void* v_cache,
+                                 const void* kv_scales, const int32_t* qo_indptr,
+                                 const int32_t* kv_indptr, const int32_t* kv_indices, int batch,
+                                 int64_t total_q, int num_q_heads, int num_kv_heads,
+                                 int head_dim, int64_t num_slots, int max_extend_len,
+                                 int max_kv_len, float sm_scale, void* workspace,
+                                 int64_t workspace_bytes, void* o, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
