@@ -149,9 +149,10 @@ extern "C" int64_t sid_qwen3_extend_workspace_bytes(const sid_qwen3_model* m,
   return plan(m, b, nullptr).total;
 }
 
-extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
-                                        void* workspace, int64_t workspace_bytes, float* logits,
-                                        int64_t* greedy_tokens, void* stream) {
+// kv_scales NULL: the layers' pools are bf16; else their scales' addresses, layer by layer.
+static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
+                          void* const* kv_scales, void* workspace, int64_t workspace_bytes,
+                          float* logits, int64_t* greedy_tokens, void* stream) {
   SID_REQUIRE(m && b, "qwen3_extend_forward: null descriptor");
   SID_REQUIRE(b->num_tokens >= 0 && b->batch >= 0, "qwen3_extend_forward: negative size");
   if (b->num_tokens == 0) return SID_OK;
@@ -184,6 +185,44 @@ extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_exte
   float* part = static_cast<float*>(l.proj);
   const int kvmax = static_cast<int>(b->max_kv_len > 0 ? b->max_kv_len : b->num_kv_indices);
 
+  auto scales = [&](int i) { return kv_scales ? kv_scales[i] : nullptr; };
+  auto norm_qkv_post = [&](int i, const void* src, int f32) {
+    const sid_qwen3_layer& lw = m->layers[i];
+    if (scales(i)) {
+      return sid_rmsnorm_qkv_post_fp8(src, f32, lw.input_ln, eps, lw.qkv_packed, t, h, hq, hkv, d,
+                                      lw.q_norm, lw.k_norm, b->positions, m->cos_sin,
+                                      m->max_positions, b->out_slots, l.q, lw.k_cache, lw.v_cache,
+                                      scales(i), m->num_slots, stream);
+    }
+    return sid_rmsnorm_qkv_post(src, f32, lw.input_ln, eps, lw.qkv_packed, t, h, hq, hkv, d,
+                                lw.q_norm, lw.k_norm, b->positions, m->cos_sin, m->max_positions,
+                                b->out_slots, l.q, lw.k_cache, lw.v_cache, m->num_slots, stream);
+  };
+  auto qkv_post = [&](int i, const void* qkv, const float* partials, int nch) {
+    const sid_qwen3_layer& lw = m->layers[i];
+    if (scales(i)) {
+      return sid_qkv_post_fp8(qkv, partials, nch, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps,
+                              b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q,
+                              lw.k_cache, lw.v_cache, scales(i), m->num_slots, stream);
+    }
+    return sid_qkv_post(qkv, partials, nch, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps,
+                        b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q, lw.k_cache,
+                        lw.v_cache, m->num_slots, stream);
+  };
+  auto attention = [&](int i) {
+    const sid_qwen3_layer& lw = m->layers[i];
+    const int longest = std::max(b->max_extend_len, 1);
+    if (scales(i)) {
+      return sid_extend_attention_fp8_fwd(l.q, lw.k_cache, lw.v_cache, scales(i), b->qo_indptr,
+                                          b->kv_indptr, b->kv_indices, b->batch, t, hq, hkv, d,
+                                          m->num_slots, longest, kvmax, m->sm_scale, l.ext_ws,
+                                          l.ext_ws_bytes, l.attn, stream);
+    }
+    return sid_extend_attention_fwd(l.q, lw.k_cache, lw.v_cache, b->qo_indptr, b->kv_indptr,
+                                    b->kv_indices, b->batch, t, hq, hkv, d, m->num_slots, longest,
+                                    kvmax, m->sm_scale, l.ext_ws, l.ext_ws_bytes, l.attn, stream);
+  };
+
   // residual = embed[ids]; x = rmsnorm(residual, input_ln of layer 0)
   SID_TRY(sid_gather_rows(m->embed, b->input_ids, l.resid, t, h, m->vocab, stream));
   if (use_chain(m, t)) {
@@ -191,15 +230,8 @@ extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_exte
     for (int i = 0; i < m->num_layers; ++i) {
       const sid_qwen3_layer& lw = m->layers[i];
       const bool first = i == 0;  // layer 0 normalises the embedding rows themselves
-      SID_TRY(sid_rmsnorm_qkv_post(first ? l.resid : static_cast<const void*>(l.r32), !first,
-                                   lw.input_ln, eps, lw.qkv_packed, t, h, hq, hkv, d,
-                                   lw.q_norm, lw.k_norm, b->positions, m->cos_sin,
-                                   m->max_positions, b->out_slots, l.q, lw.k_cache, lw.v_cache,
-                                   m->num_slots, stream));
-      SID_TRY(sid_extend_attention_fwd(l.q, lw.k_cache, lw.v_cache, b->qo_indptr, b->kv_indptr,
-                                       b->kv_indices, b->batch, t, hq, hkv, d, m->num_slots,
-                                       std::max(b->max_extend_len, 1), kvmax, m->sm_scale,
-                                       l.ext_ws, l.ext_ws_bytes, l.attn, stream));
+      SID_TRY(norm_qkv_post(i, first ? l.resid : static_cast<const void*>(l.r32), !first));
+      SID_TRY(attention(i));
       SID_TRY(sid_linear_residual(l.attn, ao, lw.o_packed, l.resid, l.r32, t, h, ao, stream));
       SID_TRY(sid_rmsnorm_linear_silu_mul(l.r32, 1, lw.post_ln, eps, lw.gate_up_packed, l.act,
                                           t, h, inter, stream));
@@ -215,19 +247,12 @@ extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_exte
     // qkv projection -> q/k-norm, RoPE, KV-cache write
     if (split_qkv) {
       SID_TRY(sid_linear_partials(l.x, h, lw.qkv, part, t, wq, h, stream));
-      SID_TRY(sid_qkv_post(nullptr, part, h / 256, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps,
-                           b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q,
-                           lw.k_cache, lw.v_cache, m->num_slots, stream));
+      SID_TRY(qkv_post(i, nullptr, part, h / 256));
     } else {
       SID_TRY(sid_linear(l.x, h, lw.qkv, nullptr, l.proj, t, wq, h, 0, stream));
-      SID_TRY(sid_qkv_post(l.proj, nullptr, 0, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps,
-                           b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q,
-                           lw.k_cache, lw.v_cache, m->num_slots, stream));
+      SID_TRY(qkv_post(i, l.proj, nullptr, 0));
     }
-    SID_TRY(sid_extend_attention_fwd(l.q, lw.k_cache, lw.v_cache, b->qo_indptr, b->kv_indptr,
-                                     b->kv_indices, b->batch, t, hq, hkv, d, m->num_slots,
-                                     std::max(b->max_extend_len, 1), kvmax, m->sm_scale,
-                                     l.ext_ws, l.ext_ws_bytes, l.attn, stream));
+    SID_TRY(attention(i));
     // o projection; residual += o; x = rmsnorm(residual, post_ln)
     if (split_o) {
       SID_TRY(sid_linear_partials(l.attn, ao, lw.o, part, t, h, ao, stream));
@@ -260,4 +285,20 @@ extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_exte
     }
   }
   return lm_head(m, b, l, logits, greedy_tokens, stream);
+}
+
+extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
+                                        void* workspace, int64_t workspace_bytes, float* logits,
+                                        int64_t* greedy_tokens, void* stream) {
+  return extend_forward(m, b, nullptr, workspace, workspace_bytes, logits, greedy_tokens, stream);
+}
+
+extern "C" int sid_qwen3_extend_forward_fp8(const sid_qwen3_model* m, const sid_extend_batch* b,
+                                            void* const* kv_scales, void* workspace,
+                                            int64_t workspace_bytes, float* logits,
+                                            int64_t* greedy_tokens, void* stream) {
+  SID_REQUIRE(m && kv_scales, "qwen3_extend_forward_fp8: null descriptor");
+  for (int i = 0; i < m->num_layers; ++i)
+    SID_REQUIRE(kv_scales[i] != nullptr, "qwen3_extend_forward_fp8: layer %d has no scales", i);
+  return extend_forward(m, b, kv_scales, workspace, workspace_bytes, logits, greedy_tokens, stream);
 }

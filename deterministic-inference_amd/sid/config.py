@@ -61,6 +61,12 @@ class EngineConfig:
     dtype: str = "bfloat16"
 
     kv_pool_tokens: int = 256 * 1024
+    # "bfloat16" (the reference's) or "fp8_e4m3": an 8-bit KV pool, e4m3 codes with a power-of-two
+    # scale for each token's head (sid.kernels.kv_fp8). It holds a token in 2064 bytes a layer
+    # instead of 4096 (Qwen3-0.6B), so twice the tokens fit, and decode attention reads half as
+    # much. Tokens differ from a bf16 pool's (each K/V value is rounded to 4 significant bits);
+    # the modes' guarantees are the same, since every path reads the same stored values.
+    kv_cache_dtype: str = "bfloat16"
     # KV pages: a request holds whole pages of this many consecutive pool slots (a power of
     # two; 1 = the reference's token-granular pool). Slot numbering, and so every kernel's
     # view of the pool, is the same for any page size.
@@ -118,6 +124,9 @@ class EngineConfig:
     def __post_init__(self):
         self.mode = Mode(self.mode)
         self.decode_backend = decode_backend_kind(self.decode_backend)
+        if self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"unknown kv_cache_dtype {self.kv_cache_dtype!r}: use one of "
+                             f"{', '.join(KV_CACHE_DTYPES)}")
         # Prefill batches (at most max_decode_batch sequences) and verify passes (G x W
         # rows) draw their untruncated rows inside the lm_head with one fixed grouping,
         # which takes up to MAX_SAMPLED_ROWS rows per pass; larger passes would switch those
@@ -133,6 +142,8 @@ class EngineConfig:
 
 # Rows one lm_head-fused sampling pass takes with 128-column tiles (sid_linear_sample).
 MAX_SAMPLED_ROWS = 4096
+
+KV_CACHE_DTYPES = ("bfloat16", "fp8_e4m3")
 
 _DECODE_BACKENDS = {"cuda": "hip", "hip": "hip", "triton": "extend", "extend": "extend"}
 

@@ -3,7 +3,8 @@
 Replaces sid/engine/kv_cache.py of the reference, whose pool is token-granular (a GPU free
 stack of single slots and an int32 request -> token table [max_reqs, max_seq_len]). Here:
 
-  * pools: per layer, K and V bf16 [num_pages * page_size, HKV, D]. Slot numbering is
+  * pools: per layer, K and V bf16 [num_pages * page_size, HKV, D] (kv_cache_dtype "fp8_e4m3":
+    codes of that shape, and their scales; sid.kernels.kv_fp8). Slot numbering is
     unchanged (slot = page * page_size + offset), so every kernel that takes slots
     (reshape_and_cache, attention through kv_indices) sees the reference's pool format;
   * block tables: int32 [max_reqs, max_pages] page ids per request row. The host copy is
@@ -29,6 +30,8 @@ import torch
 
 from sid.config import EngineConfig, ModelConfig
 from sid.kernels.jit import load_ext
+from sid.kernels.kv_fp8 import HEAD_DIM, alloc_cache_fp8, gather_cache_fp8
+from sid.kernels.ops import gather_rows
 
 
 def _pages(n_tokens, page_size: int):
@@ -51,11 +54,19 @@ class KVCache:
         self.max_pages = _pages(cfg.max_seq_len, ps) + 1
         self.device = device
         self.ext = load_ext()
-        shape = (self.num_slots, mcfg.num_kv_heads, mcfg.head_dim)
-        self.k_pools = [torch.zeros(shape, dtype=torch.bfloat16, device=device)
-                        for _ in range(mcfg.num_layers)]
-        self.v_pools = [torch.zeros(shape, dtype=torch.bfloat16, device=device)
-                        for _ in range(mcfg.num_layers)]
+        self.kv_scales = None
+        if cfg.kv_cache_dtype == "fp8_e4m3":
+            if mcfg.head_dim != HEAD_DIM:
+                raise ValueError(f"an 8-bit KV pool needs head_dim {HEAD_DIM}, got {mcfg.head_dim}")
+            layers = [alloc_cache_fp8(self.num_slots, mcfg.num_kv_heads, device)
+                      for _ in range(mcfg.num_layers)]
+            self.k_pools, self.v_pools, self.kv_scales = (list(x) for x in zip(*layers))
+        else:
+            shape = (self.num_slots, mcfg.num_kv_heads, mcfg.head_dim)
+            self.k_pools = [torch.zeros(shape, dtype=torch.bfloat16, device=device)
+                            for _ in range(mcfg.num_layers)]
+            self.v_pools = [torch.zeros(shape, dtype=torch.bfloat16, device=device)
+                            for _ in range(mcfg.num_layers)]
 
         # free pages: stack[:top] (the top of the stack is handed out first)
         self._stack = np.arange(self.num_pages - 1, 0, -1, dtype=np.int32)
@@ -72,6 +83,20 @@ class KVCache:
 
     def layer(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
         return self.k_pools[i], self.v_pools[i]
+
+    def scales(self, i: int):
+        """The scales of layer i's 8-bit pools (sid.kernels.kv_fp8); None for bf16 pools."""
+        return None if self.kv_scales is None else self.kv_scales[i]
+
+    def read(self, i: int, row: int, start: int, end: int) -> tuple:
+        """K and V (bf16 [end - start, HKV, D]) of positions start .. end-1 of a row in layer i,
+        whatever the pool's type: what a caller that moves or inspects a request's cache reads."""
+        slots = torch.from_numpy(self.slot_range(row, start, end)).to(self.device)
+        k, v = self.layer(i)
+        if self.kv_scales is not None:
+            return gather_cache_fp8(k, v, self.kv_scales[i], slots)
+        return tuple(gather_rows(x.view(self.num_slots, -1), slots).view(-1, *x.shape[1:])
+                     for x in (k, v))
 
     @property
     def free_pages(self) -> int:

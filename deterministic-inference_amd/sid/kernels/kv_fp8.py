@@ -23,6 +23,12 @@ from sid.kernels.jit import load_ext
 HEAD_DIM = 128
 
 
+def layer_scales(kv_cache, layer: int):
+    """The scales of a KV cache's layer; None where its pools are bf16."""
+    scales = getattr(kv_cache, "scales", None)
+    return None if scales is None else scales(layer)
+
+
 def alloc_cache_fp8(num_slots: int, num_kv_heads: int, device) -> tuple:
     """(k_cache, v_cache, kv_scales) of an empty pool: every vector zero."""
     shape = (num_slots, num_kv_heads, HEAD_DIM)

@@ -12,6 +12,7 @@ from typing import Optional
 import torch
 
 from sid.kernels.jit import load_ext
+from sid.kernels.kv_fp8 import layer_scales
 
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
@@ -51,6 +52,9 @@ def _bind(lib) -> None:
     lib.sid_qwen3_extend_forward.restype = _i32
     lib.sid_qwen3_extend_forward.argtypes = [ctypes.POINTER(Model), ctypes.POINTER(Batch), _vp,
                                              _i64, _vp, _vp, _vp]
+    lib.sid_qwen3_extend_forward_fp8.restype = _i32
+    lib.sid_qwen3_extend_forward_fp8.argtypes = [ctypes.POINTER(Model), ctypes.POINTER(Batch),
+                                                 ctypes.POINTER(_vp), _vp, _i64, _vp, _vp, _vp]
     lib._sid_native_forward_bound = True
 
 
@@ -76,6 +80,10 @@ class NativeQwen3:
                                    lw["o"].data_ptr(), lw["post_ln"].data_ptr(),
                                    lw["gate_up"].data_ptr(), lw["down"].data_ptr(),
                                    kp.data_ptr(), vp.data_ptr(), *pw)
+        # 8-bit pools: their scales' addresses, layer by layer
+        scales = [layer_scales(kv_cache, i) for i in range(cfg.num_layers)]
+        self.kv_scales = None if scales[0] is None else (_vp * cfg.num_layers)(
+            *(s.data_ptr() for s in scales))
         kp0, _ = kv_cache.layer(0)
         self.model = Model(cfg.num_layers, cfg.hidden_size, cfg.num_q_heads, cfg.num_kv_heads,
                            cfg.head_dim, cfg.intermediate_size, cfg.vocab_size,
@@ -113,11 +121,14 @@ class NativeQwen3:
             tokens = torch.empty(r, dtype=torch.int64, device=dev)
         if not (greedy or sample) or with_logits:
             logits = torch.empty(r, self.vocab, dtype=torch.float32, device=dev)
-        rc = lib.sid_qwen3_extend_forward(
-            ctypes.byref(self.model), ctypes.byref(b), ws.data_ptr(), ws.numel(),
-            logits.data_ptr() if logits is not None else None,
-            tokens.data_ptr() if tokens is not None else None,
-            torch.cuda.current_stream(dev).cuda_stream)
+        out = (ws.data_ptr(), ws.numel(), logits.data_ptr() if logits is not None else None,
+               tokens.data_ptr() if tokens is not None else None,
+               torch.cuda.current_stream(dev).cuda_stream)
+        if self.kv_scales is None:
+            rc = lib.sid_qwen3_extend_forward(ctypes.byref(self.model), ctypes.byref(b), *out)
+        else:
+            rc = lib.sid_qwen3_extend_forward_fp8(ctypes.byref(self.model), ctypes.byref(b),
+                                                  self.kv_scales, *out)
         if rc != 0:
             raise RuntimeError(f"sid_qwen3_extend_forward: {lib.sid_last_error().decode()}")
         if tokens is None:

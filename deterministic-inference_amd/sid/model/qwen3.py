@@ -15,6 +15,7 @@ import torch
 from sid.config import ModelConfig, decode_backend_kind
 from sid.engine.batch import ForwardBatch, ForwardMode
 from sid.kernels.extend_attention import extend_attention_fwd
+from sid.kernels.kv_fp8 import layer_scales
 from sid.kernels.matmul_persistent import (linear, linear_argmax, linear_argmax_supported,
                                             linear_partials, linear_sample, linear_silu_mul,
                                             linear_silu_mul_preferred)
@@ -81,7 +82,8 @@ class Qwen3Model:
         k_pool, v_pool = kv_cache.layer(layer_idx)
         proj = linear_partials(x, lw["qkv"]) if split else linear(x, lw["qkv"])
         q = qkv_post(proj, lw["q_norm"], lw["k_norm"], cfg.rms_norm_eps, fb.positions,
-                     self.rope.cos_sin, fb.out_slots, k_pool, v_pool, cfg.num_q_heads)
+                     self.rope.cos_sin, fb.out_slots, k_pool, v_pool, cfg.num_q_heads,
+                     kv_scales=layer_scales(kv_cache, layer_idx))
         return self._attend(layer_idx, q, fb, kv_cache, decode_attn, decode_backend)
 
     def _attend(self, layer_idx: int, q: torch.Tensor, fb: ForwardBatch, kv_cache, decode_attn,
@@ -90,19 +92,21 @@ class Qwen3Model:
         cfg = self.cfg
         t = q.shape[0]
         k_pool, v_pool = kv_cache.layer(layer_idx)
+        scales = layer_scales(kv_cache, layer_idx)
         if fb.mode == ForwardMode.DECODE and decode_backend == "hip":
             o = decode_attn.forward(q, k_pool, v_pool, fb.kv_indptr, fb.kv_indices, fb.seq_lens,
                                     fb.max_seq_len, self.sm_scale, invariant=fb.invariant,
                                     policy_batch=fb.real_rows, variant=fb.decode_variant,
                                     geometry=fb.decode_geometry, wg_order=fb.decode_wg_order,
-                                    workers=fb.decode_workers)
+                                    workers=fb.decode_workers, kv_scales=scales)
         else:
             qo = fb.qo_indptr
             if qo is None:  # decode through the extend kernel: one query per request
                 qo = torch.arange(t + 1, dtype=torch.int32, device=q.device)
             o = extend_attention_fwd(q, k_pool, v_pool, qo, fb.kv_indptr, fb.kv_indices,
                                      max(fb.max_extend_len, 1), self.sm_scale,
-                                     max_kv_len=fb.max_kv_len or fb.max_seq_len or None)
+                                     max_kv_len=fb.max_kv_len or fb.max_seq_len or None,
+                                     kv_scales=scales)
         return o.view(t, cfg.q_size)
 
     def _packed_weights(self) -> list:
@@ -133,7 +137,7 @@ class Qwen3Model:
             k_pool, v_pool = kv_cache.layer(i)
             q = rmsnorm_qkv_post(src, lw["input_ln"], eps, pw["qkv"], lw["q_norm"], lw["k_norm"],
                                  fb.positions, self.rope.cos_sin, fb.out_slots, k_pool, v_pool,
-                                 cfg.num_q_heads)
+                                 cfg.num_q_heads, kv_scales=layer_scales(kv_cache, i))
             o = self._attend(i, q, fb, kv_cache, decode_attn, decode_backend)
             linear_residual(o, pw["o"], residual, r32)
             act = rmsnorm_linear_silu_mul(r32, lw["post_ln"], eps, pw["gate_up"])
@@ -222,7 +226,8 @@ class Qwen3Model:
     def _native_forward(self, fb: ForwardBatch, kv_cache, greedy: bool, sample: bool = False,
                         with_logits: bool = False):
         from sid.model.native import NativeQwen3
-        key = (id(kv_cache), tuple(kv_cache.layer(0)[0].shape), self.decode_chain)
+        pool = kv_cache.layer(0)[0]
+        key = (id(kv_cache), tuple(pool.shape), pool.dtype, self.decode_chain)
         if self._native is None or self._native.key != key:
             self._native = NativeQwen3(self, kv_cache, SPLIT_K_MAX_TOKENS,
                                        DECODE_CHAIN_MAX_ROWS if self.decode_chain else 0)

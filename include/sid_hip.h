@@ -645,6 +645,15 @@ int sid_extend_attention_fp8_fwd(const void* q, const void* k_cache, const void*
                                  int max_kv_len, float sm_scale, void* workspace,
                                  int64_t workspace_bytes, void* o, void* stream);
 
+/*
+ * sid_qwen3_extend_forward with 8-bit pools: every layer's k_cache / v_cache hold codes, and
+ * kv_scales (a host array of m->num_layers device pointers) their scales. Same workspace.
+ */
+int sid_qwen3_extend_forward_fp8(const sid_qwen3_model* m, const sid_extend_batch* b,
+                                 void* const* kv_scales, void* workspace,
+                                 int64_t workspace_bytes, float* logits, int64_t* tokens,
+                                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -134,6 +134,34 @@ def test_no_work_is_a_success(lib):
     assert lib.sid_extend_attention_fp8_fwd(*{**EXTEND, "t": 0}.values(), z) == 0
 
 
+def test_engine_config_and_pool():
+    from sid.config import EngineConfig, ModelConfig
+    from sid.engine.kv_cache import KVCache
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        EngineConfig(kv_cache_dtype="int3")
+    cfg = EngineConfig(kv_pool_tokens=64, max_reqs=2, max_seq_len=64, kv_cache_dtype="fp8_e4m3")
+    kv = KVCache(cfg, ModelConfig(num_layers=2), "cpu")
+    assert kv.layer(1)[0].dtype == torch.float8_e4m3fn and kv.scales(1).shape == (64, 8, 2)
+    with pytest.raises(ValueError, match="head_dim"):
+        KVCache(cfg, ModelConfig(num_layers=2, head_dim=64), "cpu")
+    plain = KVCache(EngineConfig(kv_pool_tokens=64, max_reqs=2, max_seq_len=64),
+                    ModelConfig(num_layers=2), "cpu")
+    assert plain.layer(1)[0].dtype == torch.bfloat16 and plain.scales(1) is None
+
+
+def test_native_forward_refuses_missing_scales(lib):
+    from sid.model.native import Batch, Model, _bind
+    _bind(lib)
+    m, b = Model(), Batch()
+    m.num_layers = 2
+    none = (ctypes.c_void_p * 2)(16, None)
+    assert lib.sid_qwen3_extend_forward_fp8(ctypes.byref(m), ctypes.byref(b), None, None, 0, None,
+                                            None, None) == 1
+    assert lib.sid_qwen3_extend_forward_fp8(ctypes.byref(m), ctypes.byref(b), none, None, 0, None,
+                                            None, None) == 1
+    assert "layer 1" in _err(lib)
+
+
 def test_ops_reject_cpu_tensors():
     from sid.kernels.kv_fp8 import alloc_cache_fp8, gather_cache_fp8, reshape_and_cache_fp8
     k, v, s = alloc_cache_fp8(4, 8, "cpu")
