@@ -1,9 +1,9 @@
 // Varlen causal "extend" attention over the 8-bit pool (format: kv_fp8.h), gfx950 MFMA.
 //
 // The contract, the splits, the tile arithmetic and the fan-out are extend_attention.hip's
-// (extend_tile.h). Codes become bf16 values on their way into the LDS tiles, exactly, so a
-// result has the bits that the bf16 kernels give on the pool read back: independent of the
-// window, the batch and the launch's form.
+// (extend_tile.h): a query's result depends only on its position and its sequence's keys. What
+// differs is how the products get their operands: K's codes lie in the LDS as they are and S = K
+// Q^T is taken on them, with q as two e4m3 vectors; V's become bf16 on their way into the LDS.
 #include "extend_tile.h"
 #include "kv_fp8.h"
 
@@ -12,31 +12,78 @@
 namespace sid {
 namespace {
 
-// ---- staging -------------------------------------------------------------------------------
+// ---- LDS ---------------------------------------------------------------------------------
 //
-// A tile's K (and V) is 512 pieces of 16 codes: piece p is key p / 8, dims 16 (p % 8) .. +15. A
-// thread holds PER pieces of each between the global loads, issued a whole tile ahead, and the
-// LDS, where they are two 16-byte pieces of bf16.
-template <int PER>
-struct Raw {
-  u32x4_v k[PER];
-  u32x4_v v[PER];
-  uint32_t s[PER];  // the key's scale bytes, K | V << 8
+// A tile is 64 keys. K stays in codes, 128 bytes a key: 16-byte unit u of a key's row holds piece
+// u ^ swk(key), so that the 16 rows of a fragment read fall on all 64 banks. V is bf16, as in
+// extend_attention.hip's tiles (piece p at p ^ swz(key)). Beside them K's scale bytes as the
+// matrix instruction takes them: word r holds the bytes of row r of the tile's four key blocks.
+constexpr int kKTile = BN * D;
+constexpr int kVAt = 2 * kKTile;                 // [2] K tiles, [2] V tiles, [2] K scale words
+constexpr int kScalesAt = kVAt + 2 * kTileBytes;
+constexpr int kLdsBytes = kScalesAt + 2 * 64;
+
+__device__ __forceinline__ int swk(int key) { return ((key >> 1) & 1) | (((key >> 3) & 3) << 1); }
+
+// Lane l's 16 bytes at its address -> LDS byte lds + 16 l.
+__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
+               : "memory", "m0");
+}
+
+typedef int i32x8_v __attribute__((ext_vector_type(8)));
+
+// A query row as two e4m3 vectors: q = 2^e (hi + lo / 16), with q's own e of the pool's rule.
+// hi keeps 4 significant bits and lo the other 4 of a bf16 value, so the sum is q exactly down to
+// 2^-13 of 2^e (less than 2^-20 of the row's largest element): two fp8 products give q . k to
+// fp32 accuracy, at the matrix rate of one bf16 product and half its operand reads, and the
+// codes need no conversion. A lane holds dims 16 g .. +15 and 64 + 16 g .. +15 of row r.
+struct QRow {
+  i32x8_v hi, lo;
+  int scale;  // E8M0 bytes: hi's in byte 0, lo's in byte 1
 };
 
-// A NaN vector must reach the queries that see its key and no others, but a hidden key's value
-// is multiplied by p = 0, which leaves a NaN. So a key whose K or V is NaN gets NaN scores (a
-// hidden key's scores are never used) and values 0, and a key past the sequence's end (which
-// every query hides) values 0. Both are rare: one test finds that a wave has none.
-template <int PER>
-__device__ __forceinline__ void guard(Raw<PER>& r, int i, bool exists) {
-  const bool nan = (r.s[i] & 255u) == kScaleNaN || r.s[i] >> 8 == kScaleNaN;
-  if (__builtin_amdgcn_ballot_w64(nan || !exists) == 0) return;
-  if (nan) {
-    r.k[i] = u32x4_v{kCodesNaN, kCodesNaN, kCodesNaN, kCodesNaN};
-    r.s[i] = 127u | 127u << 8;
+__device__ __forceinline__ QRow split_q(const bf16_t* qp, bool row_ok, int g) {
+  uint32_t amax = 0;
+  float x[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 u = *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 16 * g + 8 * (i & 1));
+    load8(row_ok ? u : make_uint4(0, 0, 0, 0), x[i]);
+    amax = max(amax, absmax8(x[i]));
   }
-  if (nan || !exists) r.v[i] = u32x4_v{0, 0, 0, 0};
+  {
+    const auto p = __builtin_amdgcn_permlane16_swap(amax, amax, false, false);
+    amax = max(p[0], p[1]);
+    const auto p2 = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
+    amax = max(p2[0], p2[1]);
+  }
+  const int byte = fp8_scale_byte(amax);
+  const bool nan = byte == kScaleNaN;  // an infinity or a NaN in q: the row's scores are NaN
+  const float inv = __uint_as_float(static_cast<uint32_t>(nan ? 127 : 254 - byte) << 23);
+  QRow q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint2 h = fp8_encode8(x[i], byte);
+    float r[8];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const uint32_t c = w == 0 ? h.x : h.y;
+      const f32x2_cvt a = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
+      const f32x2_cvt b = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+      r[4 * w] = (x[i][4 * w] * inv - a.x) * 16.0f;
+      r[4 * w + 1] = (x[i][4 * w + 1] * inv - a.y) * 16.0f;
+      r[4 * w + 2] = (x[i][4 * w + 2] * inv - b.x) * 16.0f;
+      r[4 * w + 3] = (x[i][4 * w + 3] * inv - b.y) * 16.0f;
+    }
+    const uint2 l = nan ? h : fp8_encode8(r, 127);
+    q.hi[2 * i] = h.x;
+    q.hi[2 * i + 1] = h.y;
+    q.lo[2 * i] = l.x;
+    q.lo[2 * i + 1] = l.y;
+  }
+  q.scale = nan ? 127 | 127 << 8 : byte | (byte - 4) << 8;
+  return q;
 }
 
 // 16 codes times 2^e as two 16-byte pieces of bf16.
@@ -49,26 +96,33 @@ __device__ __forceinline__ void unpack16(u32x4_v c, uint32_t byte, u32x4_v (&out
   }
 }
 
+// The other buffer of a pair (an immediate where this one is).
+__device__ __forceinline__ int other(int buf) { return 1 - buf; }
+template <int B>
+__device__ __forceinline__ std::integral_constant<int, 1 - B> other(std::integral_constant<int, B>) {
+  return {};
+}
+
 struct RowCtx {  // what softmax_tile reads
   int g;
   int q_abs;
   bool row_ok;
 };
 
-// Workgroup = (request, kv head, 8 NW query positions), NW waves; wave w: head w / (NW / 2), one
-// block of 16 query rows. FANOUT (NW = 4): the workgroup computes one split and saves its state
-// for the fold; else it walks the splits in order.
-template <int NW, bool FANOUT>
-__global__ void __launch_bounds__(NW * 64, NW / 2) extend_fp8_kernel(
+// Workgroup = (request, kv head, 8 NW HPW query positions), NW waves. HPW = 2: a wave takes 16
+// positions of both query heads, which share every fragment it reads; HPW = 1: of one head
+// (wave w: head w / (NW / 2)). FANOUT: the workgroup computes one split and saves its state for
+// the fold; else it walks the splits in order.
+template <int NW, int HPW, bool FANOUT>
+__global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ k_cache,
     const uint8_t* __restrict__ v_cache, const uint16_t* __restrict__ kv_scales,
     const int32_t* __restrict__ qo_indptr, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, int batch, int num_q_heads, int num_kv_heads,
     int64_t num_slots, float sm_scale, int mtiles, int64_t items, bf16_t* __restrict__ o,
     float* __restrict__ part_a, float* __restrict__ part_ml, int32_t* __restrict__ part_n) {
-  extern __shared__ __align__(1024) char lds[];  // [2][K tile, V tile], bf16
-  constexpr int ROWS = 8 * NW;
-  constexpr int PER = 8 / NW;
+  extern __shared__ __align__(1024) char lds[];
+  constexpr int ROWS = 8 * NW * HPW;
   const int b = min(static_cast<int>(blockIdx.x), batch - 1);
   const int h_kv = blockIdx.y;
   // Late query tiles walk the most keys: dispatch them first.
@@ -86,11 +140,12 @@ __global__ void __launch_bounds__(NW * 64, NW / 2) extend_fp8_kernel(
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
-  const int hq = h_kv * 2 + wave / (NW / 2);
-  const int w_row = mtile * ROWS + 16 * (wave % (NW / 2));  // the wave's first query row
+  constexpr int BLOCKS = NW * HPW / 2;  // 16-position blocks of the workgroup
+  const int hq0 = h_kv * 2 + (HPW == 2 ? 0 : wave / BLOCKS);
+  const int w_row = mtile * ROWS + 16 * (wave % BLOCKS);  // the wave's first query row
   const int qr = w_row + (lane & 15);
   const bool row_ok = qr < extend_len;
-  const int64_t prow = static_cast<int64_t>(q_start + (row_ok ? qr : 0)) * num_q_heads + hq;
+  const int64_t prow = static_cast<int64_t>(q_start + (row_ok ? qr : 0)) * num_q_heads + hq0;
   const float sc2 = sm_scale * LOG2E;
   const int last_row = min(extend_len, (mtile + 1) * ROWS) - 1;
   const int visible_end = min(kv_len, prefix + last_row + 1);
@@ -103,141 +158,252 @@ __global__ void __launch_bounds__(NW * 64, NW / 2) extend_fp8_kernel(
   const int w_first = prefix + w_row;  // the wave's first and last positions
   const int w_last = prefix + min(extend_len, w_row + 16) - 1;
 
-  bf16x8_v qf[4];
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    qf[ks] = *reinterpret_cast<const bf16x8_v*>(q + prow * D + 32 * ks + 8 * (lane >> 4));
-    if (!row_ok) qf[ks] = bf16x8_v{};
-  }
-
+  // ---- staging. Thread t's pieces i of 16 codes: key t / 8 + 8 NW i, piece t % 8. K's go to the
+  // LDS by DMA; V's through registers, where they become bf16 with their scale (once for all
+  // waves: converted at every fragment read instead, 64 more conversions and 32 products a wave
+  // and tile). V is loaded two tiles ahead, K one, the slots another. No branch guards a load (past
+  // the sequence's end its last key is read again): a load in a branch is waited for where the
+  // branch ends, and the tile's DMA with it.
+  constexpr int KP = 8 / NW;
   const int32_t* idx = kv_indices + kv_start;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char_t)lds));
   const uint32_t max_slots = static_cast<uint32_t>(min<int64_t>(num_slots, 0x7fffffff));
-  const uint8_t* kb = k_cache + h_kv * D + 16 * (tid & 7);
-  const uint8_t* vb = v_cache + h_kv * D + 16 * (tid & 7);
+  const uint8_t* kb = k_cache + h_kv * D;
+  const uint8_t* vb = v_cache + h_kv * D;
   const uint16_t* sb = kv_scales + h_kv;
   struct Slots {
-    uint32_t s[PER];
+    uint32_t s[KP];
   };
   auto load_slots = [&](int tile) {
     Slots v;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int key = tile * BN + ((tid + 64 * NW * i) >> 3);
-      v.s[i] = key < kv_len ? idx[key] : 0;
+    for (int i = 0; i < KP; ++i) {
+      v.s[i] = idx[min(tile * BN + (tid >> 3) + 8 * NW * i, kv_len - 1)];
+      v.s[i] = v.s[i] < max_slots ? v.s[i] : 0;  // (out of range: slot 0)
     }
     return v;
   };
-  Raw<PER> raw;
-  auto load_raw = [&](const Slots& v) {
+  const uint32_t row_bytes = static_cast<uint32_t>(num_kv_heads) * D;
+  const uint8_t* ksrc[KP];  // (a thread's pieces differ in their swizzle)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int64_t slot = v.s[i] < max_slots ? v.s[i] : 0u;  // (out of range: slot 0)
-      raw.k[i] = *reinterpret_cast<const u32x4_v*>(kb + slot * num_kv_heads * D);
-      raw.v[i] = *reinterpret_cast<const u32x4_v*>(vb + slot * num_kv_heads * D);
-      raw.s[i] = sb[slot * num_kv_heads];
+  for (int i = 0; i < KP; ++i) ksrc[i] = kb + 16 * ((tid & 7) ^ swk((tid >> 3) + 8 * NW * i));
+  const uint8_t* vsrc = vb + 16 * (tid & 7);
+  auto load_k = [&](const Slots& v, int buf) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      dma16(ksrc[i] + static_cast<uint64_t>(v.s[i]) * row_bytes,
+            lds0 + buf * kKTile + 1024u * (wave + NW * i));
+  };
+  u32x4_v raw[KP];
+  uint32_t raw_s[KP];  // the keys' scale bytes, K | V << 8
+  auto load_v = [&](const Slots& v) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      raw[i] = *reinterpret_cast<const u32x4_v*>(vsrc + static_cast<uint64_t>(v.s[i]) * row_bytes);
+      raw_s[i] = sb[static_cast<uint64_t>(v.s[i]) * static_cast<uint32_t>(num_kv_heads)];
     }
   };
-  auto store_raw = [&](int tile) {
+  // A NaN vector must reach the queries that see its key and no others, but a hidden key's value
+  // is multiplied by p = 0, which leaves a NaN. So a key whose K or V is NaN gets a NaN scale for K
+  // (E8M0's 255: NaN scores, and a hidden key's scores are never used) and values 0; a key past the
+  // sequence's end, which every query hides, values 0 too. One test finds that a wave has neither.
+  // (A thread's key of piece i is 8 NW i after its first: the swizzle of a multiple of 32 keys is the
+  // same, of 64 threads' 32-key step always.)
+  uint32_t vdst = lds0 + kVAt + 256 * (tid >> 3) + 16 * ((2 * (tid & 7)) ^ swz(tid >> 3));
+  asm volatile("" : "+v"(vdst));
+  auto store_v = [&](int tile, auto buf) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int key = (tid + 64 * NW * i) >> 3;
-      guard(raw, i, tile * BN + key < kv_len);
-      u32x4_v k[2], v[2];
-      unpack16(raw.k[i], raw.s[i] & 255u, k);
-      unpack16(raw.v[i], raw.s[i] >> 8, v);
-      char* dst = lds + (tile & 1) * 2 * kTileBytes + 256 * key;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int at = 16 * ((2 * (tid & 7) + e) ^ swz(key));
-        *reinterpret_cast<u32x4_v*>(dst + at) = k[e];
-        *reinterpret_cast<u32x4_v*>(dst + kTileBytes + at) = v[e];
+    for (int i = 0; i < KP; ++i) {
+      const int key = (tid >> 3) + 8 * NW * i;
+      uint32_t ks = raw_s[i] & 255u, vs = raw_s[i] >> 8;
+      const bool nan = vs == kScaleNaN || ks == kScaleNaN;
+      const bool gone = nan || tile * BN + key >= kv_len;
+      if (__builtin_amdgcn_ballot_w64(gone) != 0) {
+        ks = nan ? kScaleNaN : ks;
+        vs = gone ? 127 : vs;
+        raw[i] = gone ? u32x4_v{0, 0, 0, 0} : raw[i];
+      }
+      u32x4_v v[2];
+      unpack16(raw[i], vs, v);
+      typedef __attribute__((address_space(3))) u32x4_v* lds_w_t;
+      *(lds_w_t)(vdst + buf * kTileBytes + 256 * 8 * NW * i) = v[0];
+      *(lds_w_t)((vdst ^ 16u) + buf * kTileBytes + 256 * 8 * NW * i) = v[1];
+      if ((tid & 7) == 0) {
+        const int m = 4 * ((key >> 3) & 3) + (key & 3), j = 2 * (key >> 5) + ((key >> 2) & 1);
+        reinterpret_cast<uint8_t*>(lds + kScalesAt + buf * 64)[4 * m + j] = static_cast<uint8_t>(ks);
       }
     }
   };
 
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char_t)lds));
-  RowState run, st;
-  fresh(run);
-  fresh(st);
-  // One tile's math out of LDS buffer `buf`. MASK: some key is hidden from some row.
-  auto tile_math = [&](auto mask, int t0, int buf) {
-    int l = lane;  // opaque: per-lane constants are not kept in registers between tiles
-    asm volatile("" : "+v"(l));
-    const int r = l & 15, g = l >> 4;
-    const int key_a0 = 8 * (r >> 2) + (r & 3);
-    const uint32_t ka = lds0 + buf * 2 * kTileBytes + key_a0 * 256 + 16 * (g ^ swz(key_a0));
-    f32x4_v s4[4];
+  QRow qf[HPW];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {  // key block j, k-step ks
-      const int j = i & 3, ks = i >> 2;
-      const bf16x8_v kf = *(__attribute__((address_space(3))) const bf16x8_v*)(
-          (ka ^ (64u * ks)) + 256 * (32 * (j >> 1) + 4 * (j & 1)));
-      s4[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          kf, qf[ks], ks == 0 ? f32x4_v{0.0f, 0.0f, 0.0f, 0.0f} : s4[j], 0, 0, 0);
+  for (int h = 0; h < HPW; ++h) qf[h] = split_q(q + (prow + h) * D, row_ok, lane >> 4);
+
+  RowState run[HPW], st[HPW];
+#pragma unroll
+  for (int h = 0; h < HPW; ++h) {
+    fresh(run[h]);
+    fresh(st[h]);
+  }
+  // LDS addresses of a lane's fragments in buffer 0, kept in registers.
+  const int r = lane & 15, g = lane >> 4;
+  // S^T = K Q^T: row m of key block j is key 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4, so a lane
+  // ends with the scores of keys 8 g .. +7 and 32 + 8 g .. +7 of its query.
+  const int key_a0 = 8 * (r >> 2) + (r & 3);
+  uint32_t ka[2], va[8], sa = lds0 + kScalesAt + 4 * r;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) ka[e] = lds0 + key_a0 * D + 16 * ((g + 4 * e) ^ swk(key_a0));
+  const int key_v = 8 * g + (r >> 2);
+#pragma unroll
+  for (int db = 0; db < 8; ++db)
+    va[db] = (lds0 + kVAt + key_v * 256 + 16 * (((r & 3) >> 1) ^ swz(key_v)) + 8 * (r & 1)) ^ (32u * db);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(va[i]));
+  asm volatile("" : "+v"(ka[0]), "+v"(ka[1]), "+v"(sa));
+  // One tile's math out of LDS buffer `buf`. MASK: some key is hidden from some row.
+  auto tile_math = [&](auto mask, int t0, auto buf) {
+    typedef __attribute__((address_space(3))) const u32x4_v* lds_u4_t;
+    const int ks = *(__attribute__((address_space(3))) const int*)(sa + 64 * buf);
+    f32x4_v s4[HPW][4];
+    i32x8_v kf[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = buf * kKTile + (32 * (j >> 1) + 4 * (j & 1)) * D;  // (swk is the same for all j)
+      const u32x4_v k0 = *(lds_u4_t)(ka[0] + at);
+      const u32x4_v k1 = *(lds_u4_t)(ka[1] + at);
+      kf[j] = i32x8_v{(int)k0.x, (int)k0.y, (int)k0.z, (int)k0.w,
+                      (int)k1.x, (int)k1.y, (int)k1.z, (int)k1.w};
     }
     __builtin_amdgcn_sched_barrier(0);
-    const RowCtx c{g, w_first + r, row_ok};
-    float s[16];
+    // (the scale operands' byte is an immediate: key block j of ks, part P of the row's scale)
+#define SID_QK(J, P, PART, C)                                                                   \
+  _Pragma("unroll") for (int h = 0; h < HPW; ++h)                                               \
+      s4[h][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[J], qf[h].PART, C, 0, 0, J, \
+                                                                  ks, P, qf[h].scale)
+    const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    SID_QK(0, 0, hi, zero); SID_QK(1, 0, hi, zero); SID_QK(2, 0, hi, zero); SID_QK(3, 0, hi, zero);
+    SID_QK(0, 1, lo, s4[h][0]); SID_QK(1, 1, lo, s4[h][1]); SID_QK(2, 1, lo, s4[h][2]);
+    SID_QK(3, 1, lo, s4[h][3]);
+#undef SID_QK
+    // V fragments: A = V^T rows 16 db + r (dims), columns 32 kb + 8 g .. +7 (keys), by two
+    // transpose reads (extend_attention.hip). They go out in groups of 4, each before the products
+    // of the one before it, the first before the softmax.
+    typedef __attribute__((address_space(3))) s16x4_v* tr_ptr_t;
+    s16x4_v vw[2][4][2];
+    auto read_v = [&](int n) {  // group n: key half n / 2, dim blocks 4 (n % 2) .. +3
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = s4[i >> 2][i & 3];
-    const float rescale = softmax_tile<decltype(mask)::value>(s, st, c, t0, sc2);
-    bf16x8_v pf[2];
-    pack_p(pf, s);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t p = va[4 * (n & 1) + i] + buf * kTileBytes + 8192 * (n >> 1);
+        vw[n & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)p);
+        vw[n & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(p + 1024));
+      }
+    };
+    read_v(0);
     __builtin_amdgcn_sched_barrier(0);
-    apply_rescale(st, rescale);
-    const int key_v = 8 * g + (r >> 2);
-    const uint32_t va = lds0 + (buf * 2 + 1) * kTileBytes + key_v * 256 +
-                        16 * (((r & 3) >> 1) ^ swz(key_v)) + 8 * (r & 1);
+    const RowCtx c{g, w_first + r, row_ok};
+    bf16x8_v pf[HPW][2];
+    float rescale[HPW];
+    bool moved = false;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {  // dim block db, key half kb
-      const int db = i & 7, kb2 = i >> 3;
-      typedef __attribute__((address_space(3))) s16x4_v* tr_ptr_t;
-      const uint32_t p = (va ^ (32u * db)) + 8192 * kb2;
-      const s16x4_v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)p);
-      const s16x4_v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(p + 1024));
-      const bf16x8_v vf = __builtin_bit_cast(
-          bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)));
-      st.acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[kb2], st.acc[db], 0, 0, 0);
+    for (int h = 0; h < HPW; ++h) {  // (no branch between the heads: their chains interleave)
+      float s[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = s4[h][i >> 2][i & 3];
+      rescale[h] = softmax_tile<decltype(mask)::value>(s, st[h], c, t0, sc2);
+      moved |= rescale[h] != 1.0f;
+      pack_p(pf[h], s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // x * 1 == x: skipped (same bits) unless some row of the wave moved its reference maximum.
+    if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+      for (int h = 0; h < HPW; ++h)
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[h].acc[db][i] *= rescale[h];
+    }
+    // O^T += V^T P^T
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (n < 3) read_v(n + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int db = 4 * (n & 1) + i;
+        const bf16x8_v vf = __builtin_bit_cast(
+            bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(
+                          vw[n & 1][i][0], vw[n & 1][i][1], 0, 1, 2, 3, 4, 5, 6, 7)));
+#pragma unroll
+        for (int h = 0; h < HPW; ++h)
+          st[h].acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[h][n >> 1], st[h].acc[db], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  load_raw(load_slots(t_begin));
-  Slots next = load_slots(t_begin + 1);
-  store_raw(t_begin);
-  load_raw(next);
-  next = load_slots(t_begin + 2);
-  for (int t = t_begin; t < t_end; ++t) {
-    __syncthreads();  // tile t is stored and every wave is done with the other buffer
+  Slots s1 = load_slots(t_begin), s2 = load_slots(t_begin + 1);
+  load_k(s1, 0);
+  load_v(s1);
+  store_v(t_begin, 0);  // (t_begin is a split's first tile: even)
+  load_v(s2);
+  s1 = s2;
+  s2 = load_slots(t_begin + 2);
+  auto step = [&](auto mask, int t, auto buf) {  // buf: t & 1
+    // Tile t has landed and every wave is done with the other buffers.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     if (t + 1 < t_end) {
-      store_raw(t + 1);
-      load_raw(next);
-      next = load_slots(t + 3);
+      load_k(s1, 1 - buf);
+      store_v(t + 1, other(buf));
+      load_v(s2);
+      s1 = s2;
+      s2 = load_slots(t + 3);
     }
-    const int t0 = t * BN;
-    if (t0 + BN - 1 <= w_first && w_row < extend_len) {
-      tile_math(std::false_type{}, t0, t & 1);
-    } else if (t0 <= w_last && w_row < extend_len) {
-      tile_math(std::true_type{}, t0, t & 1);
+    if constexpr (decltype(mask)::value) {
+      // A tile past the wave's last row is left out.
+      if (t * BN > w_last || w_row >= extend_len) return;
     }
-    if (!FANOUT && ((t & 3) == 3 || t + 1 == t_end)) {  // the split's end
-      fold(run, st.m, st.l, st.acc);
-      fresh(st);
+    tile_math(mask, t * BN, buf);
+  };
+  // Tiles that every row of the workgroup sees whole, in pairs (their buffers' addresses are
+  // immediates), then the others with the mask: one loop each, split by split (a branch between
+  // the kinds in one loop, or the fold in it, costs a copy of the accumulators each turn).
+  const int t_full = (prefix + mtile * ROWS + 1) / BN;
+  for (int s0 = t_begin; s0 < t_end; s0 += KSPLIT / BN) {
+    const int s_end = min(s0 + KSPLIT / BN, t_end);
+    int t = s0;
+    for (const int e = min(s_end, t_full); t + 1 < e; t += 2) {
+      step(std::false_type{}, t, std::integral_constant<int, 0>{});
+      step(std::false_type{}, t + 1, std::integral_constant<int, 1>{});
+    }
+    for (; t < s_end; ++t) step(std::true_type{}, t, t & 1);
+    if constexpr (!FANOUT) {
+#pragma unroll
+      for (int h = 0; h < HPW; ++h) {
+        fold(run[h], st[h].m, st[h].l, st[h].acc);
+        fresh(st[h]);
+      }
     }
   }
   if (!row_ok) return;
-  if constexpr (FANOUT) {
-    const int64_t pr = split * items + prow;
-    const int g = lane >> 4;
 #pragma unroll
-    for (int db = 0; db < 8; ++db)
-      *reinterpret_cast<f32x4_v*>(part_a + pr * D + 16 * db + 4 * g) = st.acc[db];
-    if (g == 0) {
-      part_ml[2 * pr] = st.m;
-      part_ml[2 * pr + 1] = st.l;
-      if (split == 0) part_n[prow] = nsplits;
+  for (int h = 0; h < HPW; ++h) {
+    if constexpr (FANOUT) {
+      const int64_t pr = split * items + prow + h;
+      const int g = lane >> 4;
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+        *reinterpret_cast<f32x4_v*>(part_a + pr * D + 16 * db + 4 * g) = st[h].acc[db];
+      if (g == 0) {
+        part_ml[2 * pr] = st[h].m;
+        part_ml[2 * pr + 1] = st[h].l;
+        if (split == 0) part_n[prow + h] = nsplits;
+      }
+    } else {
+      store_row(o + (prow + h) * D, run[h], lane >> 4);
     }
-  } else {
-    store_row(o + prow * D, run, lane >> 4);
   }
 }
 
@@ -264,7 +430,7 @@ extern "C" int sid_extend_attention_fp8_fwd(
               "%s: operands must be 16-byte aligned", name);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto kern, int nw, dim3 grid) {
-    hipLaunchKernelGGL(kern, grid, dim3(nw * 64), 4 * kTileBytes, s, (const bf16_t*)q,
+    hipLaunchKernelGGL(kern, grid, dim3(nw * 64), kLdsBytes, s, (const bf16_t*)q,
                        (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint16_t*)kv_scales, qo_indptr, kv_indptr, kv_indices, batch,
                        num_q_heads, num_kv_heads, num_slots, sm_scale, p.mtiles, p.items,
@@ -272,11 +438,11 @@ extern "C" int sid_extend_attention_fp8_fwd(
     return check_launch(name);
   };
   if (p.fanout) {
-    const int rc = launch(extend_fp8_kernel<4, true>, 4,
+    const int rc = launch(extend_fp8_kernel<4, 1, true>, 4,
                           dim3(batch, num_kv_heads, p.mtiles * p.splits));
     return rc != SID_OK ? rc : extend_merge(name, p, o, s);
   }
   const dim3 grid(p.grid_x, num_kv_heads, p.mtiles);
-  return p.rows == 64 ? launch(extend_fp8_kernel<8, false>, 8, grid)
-                      : launch(extend_fp8_kernel<4, false>, 4, grid);
+  return p.rows == 64 ? launch(extend_fp8_kernel<8, 1, false>, 8, grid)
+                      : launch(extend_fp8_kernel<4, 1, false>, 4, grid);
 }

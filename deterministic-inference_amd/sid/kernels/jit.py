@@ -39,6 +39,7 @@ _ext = None
 # softmax rescales them with VALU ops, which cannot read AGPRs).
 SOURCE_FLAGS = {
     "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "extend_attention_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -50,7 +50,11 @@ def gather_cache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: to
                      slots: torch.Tensor) -> tuple:
     """The pool's rows of `slots` (int64) as bf16 k, v [N, HKV, 128], exactly; rows of slots
     outside the pool are zeros."""
-    n, hkv, d = slots.numel(), k_cache.shape[1], k_cache.shape[2]
-    k, v = (torch.empty(n, hkv, d, dtype=torch.bfloat16, device=slots.device) for _ in range(2))
+    shape = k_cache.shape
+    if len(shape) != 3:
+        raise RuntimeError("k_cache must be [S, HKV, D]")
+    n, hkv, d = slots.numel(), shape[1], shape[2]
+    # one allocation for both (an eager call of a few rows is bound by the host)
+    k, v = torch.empty((2, n, hkv, d), dtype=torch.bfloat16, device=slots.device).unbind(0)
     load_ext().gather_cache_fp8(k_cache, v_cache, kv_scales, slots.reshape(-1), k, v)
     return k, v
