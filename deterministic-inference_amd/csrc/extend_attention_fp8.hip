@@ -179,10 +179,11 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
 #pragma unroll
     for (int i = 0; i < KP; ++i) {
       v.s[i] = idx[min(tile * BN + (tid >> 3) + 8 * NW * i, kv_len - 1)];
-      v.s[i] = v.s[i] < max_slots ? v.s[i] : 0;  // (out of range: slot 0)
     }
     return v;
   };
+  // Out of range: slot 0. (Looked at where a slot is used: at its load, it would be waited for.)
+  auto checked = [&](uint32_t slot) { return static_cast<uint64_t>(slot < max_slots ? slot : 0); };
   const uint32_t row_bytes = static_cast<uint32_t>(num_kv_heads) * D;
   const uint8_t* ksrc[KP];  // (a thread's pieces differ in their swizzle)
 #pragma unroll
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   auto load_k = [&](const Slots& v, int buf) {
 #pragma unroll
     for (int i = 0; i < KP; ++i)
-      dma16(ksrc[i] + static_cast<uint64_t>(v.s[i]) * row_bytes,
+      dma16(ksrc[i] + checked(v.s[i]) * row_bytes,
             lds0 + buf * kKTile + 1024u * (wave + NW * i));
   };
   u32x4_v raw[KP];
@@ -199,8 +200,8 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   auto load_v = [&](const Slots& v) {
 #pragma unroll
     for (int i = 0; i < KP; ++i) {
-      raw[i] = *reinterpret_cast<const u32x4_v*>(vsrc + static_cast<uint64_t>(v.s[i]) * row_bytes);
-      raw_s[i] = sb[static_cast<uint64_t>(v.s[i]) * static_cast<uint32_t>(num_kv_heads)];
+      raw[i] = *reinterpret_cast<const u32x4_v*>(vsrc + checked(v.s[i]) * row_bytes);
+      raw_s[i] = sb[checked(v.s[i]) * static_cast<uint32_t>(num_kv_heads)];
     }
   };
   // A NaN vector must reach the queries that see its key and no others, but a hidden key's value
@@ -344,22 +345,30 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
 
   Slots s1 = load_slots(t_begin), s2 = load_slots(t_begin + 1);
   load_k(s1, 0);
+  __builtin_amdgcn_sched_barrier(0);
   load_v(s1);
   store_v(t_begin, 0);  // (t_begin is a split's first tile: even)
   load_v(s2);
   s1 = s2;
   s2 = load_slots(t_begin + 2);
   auto step = [&](auto mask, int t, auto buf) {  // buf: t & 1
-    // Tile t has landed and every wave is done with the other buffers.
+    // Every load has landed (they had a whole tile's time) and every wave is done with the other
+    // buffers.
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     if (t + 1 < t_end) {
-      load_k(s1, 1 - buf);
+#pragma unroll
+      for (int i = 0; i < KP; ++i)  // (not converted ahead of the barrier)
+        asm volatile("" : "+v"(raw[i]), "+v"(raw_s[i]));
       store_v(t + 1, other(buf));
-      load_v(s2);
+      const Slots k_at = s1;
       s1 = s2;
+      load_v(s2);
       s2 = load_slots(t + 3);
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(k_at, 1 - buf);  // last: a wait for an earlier load would include the DMA
+      __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (decltype(mask)::value) {
       // A tile past the wave's last row is left out.
@@ -429,20 +438,21 @@ extern "C" int sid_extend_attention_fp8_fwd(
                   !misaligned(kv_scales) && !misaligned(o) && !misaligned(workspace),
               "%s: operands must be 16-byte aligned", name);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto kern, int nw, dim3 grid) {
+  auto launch = [&](auto kern, int nw, dim3 grid, int mtiles) {
     hipLaunchKernelGGL(kern, grid, dim3(nw * 64), kLdsBytes, s, (const bf16_t*)q,
                        (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint16_t*)kv_scales, qo_indptr, kv_indptr, kv_indices, batch,
-                       num_q_heads, num_kv_heads, num_slots, sm_scale, p.mtiles, p.items,
+                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, p.items,
                        (bf16_t*)o, p.part_a, p.part_ml, p.part_n);
     return check_launch(name);
   };
   if (p.fanout) {
     const int rc = launch(extend_fp8_kernel<4, 1, true>, 4,
-                          dim3(batch, num_kv_heads, p.mtiles * p.splits));
+                          dim3(batch, num_kv_heads, p.mtiles * p.splits), p.mtiles);
     return rc != SID_OK ? rc : extend_merge(name, p, o, s);
   }
-  const dim3 grid(p.grid_x, num_kv_heads, p.mtiles);
-  return p.rows == 64 ? launch(extend_fp8_kernel<8, 1, false>, 8, grid)
-                      : launch(extend_fp8_kernel<4, 1, false>, 4, grid);
+  const int mtiles = ceil_div(max_extend_len, p.rows);
+  const dim3 grid(p.grid_x, num_kv_heads, mtiles);
+  return p.rows == 64 ? launch(extend_fp8_kernel<8, 1, false>, 8, grid, mtiles)
+                      : launch(extend_fp8_kernel<4, 1, false>, 4, grid, mtiles);
 }
