@@ -109,6 +109,9 @@ __device__ __forceinline__ float seeded_gumbel(uint32_t row_hash, int col) {
 void set_error(const char* fmt, ...);
 int check_launch(const char* what);
 
+// Compute units of the current device.
+int cu_count();
+
 }  // namespace sid
 
 #define SID_REQUIRE(cond, ...)                 \

@@ -538,8 +538,8 @@ ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, con
                        const int32_t* qo_indptr, const int32_t* kv_indptr,
                        const int32_t* kv_indices, const void* o, int batch, int64_t total_q,
                        int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
-                       int max_extend_len, int max_kv_len, void* workspace,
-                       int64_t workspace_bytes) {
+                       int max_extend_len, int max_kv_len, int split_keys, int64_t need,
+                       void* workspace, int64_t workspace_bytes) {
   ExtendPlan p{};
   auto check = [&]() -> int {
     SID_REQUIRE(batch >= 0 && total_q >= 0, "%s: negative size", name);
@@ -553,16 +553,13 @@ ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, con
                 num_kv_heads);
     SID_REQUIRE(num_slots > 0, "%s: empty KV pool", name);
     SID_REQUIRE(batch <= 65535 && num_kv_heads <= 65535, "%s: grid too large", name);
-    const int64_t need = sid_extend_attention_workspace_bytes(batch, total_q, num_q_heads,
-                                                             num_kv_heads, max_extend_len,
-                                                             max_kv_len);
     p.fanout = need > 0 && workspace != nullptr && workspace_bytes >= need;
     p.items = total_q * num_q_heads;
     const int mtiles = ceil_div(max_extend_len, BQ);
     if (p.fanout) {
       p.rows = BQ;
       p.mtiles = mtiles;
-      p.splits = ceil_div(max_kv_len, KSPLIT);
+      p.splits = ceil_div(max_kv_len, split_keys);
       SID_REQUIRE(static_cast<int64_t>(mtiles) * p.splits <= 65535, "%s: grid too large", name);
       SID_REQUIRE((p.items + 3) / 4 < (1ll << 31), "%s: too many rows for the merge", name);
       p.part_a = static_cast<float*>(workspace);
@@ -621,7 +618,11 @@ extern "C" int sid_extend_attention_fwd(const void* q, const void* k_cache, cons
   const char* name = "extend_attention";
   const ExtendPlan p = extend_plan(name, q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o,
                                    batch, total_q, num_q_heads, num_kv_heads, head_dim, num_slots,
-                                   max_extend_len, max_kv_len, workspace, workspace_bytes);
+                                   max_extend_len, max_kv_len, KSPLIT,
+                                   sid_extend_attention_workspace_bytes(batch, total_q, num_q_heads,
+                                                                        num_kv_heads, max_extend_len,
+                                                                        max_kv_len),
+                                   workspace, workspace_bytes);
   if (p.rc != SID_OK || p.empty) return p.rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.fanout) {

@@ -12,6 +12,11 @@
 namespace sid {
 namespace {
 
+// Keys per split: the unit in which a row's state is folded, and in which a small grid fans out. (256,
+// as for bf16 pools: 16 windows of 32 over 2048 keys 47 us against 38, 700 tokens over 4000 99
+// against 78; 4 windows 21.1 against 22.5.)
+constexpr int kSplit = 512;
+
 // ---- LDS ---------------------------------------------------------------------------------
 //
 // A tile is 64 keys. K stays in codes, 128 bytes a key: 16-byte unit u of a key's row holds piece
@@ -43,13 +48,23 @@ struct QRow {
   int scale;  // E8M0 bytes: hi's in byte 0, lo's in byte 1
 };
 
-__device__ __forceinline__ QRow split_q(const bf16_t* qp, bool row_ok, int g) {
+struct QRaw {
+  uint4 u[4];
+};
+__device__ __forceinline__ QRaw load_q(const bf16_t* qp, int g) {
+  QRaw q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q.u[i] = *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 16 * g + 8 * (i & 1));
+  return q;
+}
+
+__device__ __forceinline__ QRow split_q(const QRaw& raw, bool row_ok) {
   uint32_t amax = 0;
   float x[4][8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 u = *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 16 * g + 8 * (i & 1));
-    load8(row_ok ? u : make_uint4(0, 0, 0, 0), x[i]);
+    load8(row_ok ? raw.u[i] : make_uint4(0, 0, 0, 0), x[i]);
     amax = max(amax, absmax8(x[i]));
   }
   {
@@ -109,6 +124,94 @@ struct RowCtx {  // what softmax_tile reads
   bool row_ok;
 };
 
+// ---- placement ------------------------------------------------------------------------------
+//
+// The query tiles of a ragged batch walk from one key tile to a whole long context, and a grid ends
+// with its last workgroup. So there (`ordered`) the workgroups take the tiles by their keys, most
+// first: index i gives the i-th of them, ties by request. That follows from the lengths alone: tile
+// m of a request's mt stands at pre + m + 1, pre its prefix in tiles. A wave holds the batch, 64
+// requests a step, and finds the i-th place bit by bit. (5 chunks of 90-701 tokens over prefixes of
+// 333-5001: 139 -> 125 us; on a uniform batch the search only costs its time in every workgroup,
+// 16 x 512 52 -> 57.) Where two workgroups share a CU they are a round of `per_round`
+// indices apart, and every other round runs backwards: the longest beside the shortest (125 -> 117).
+// Placement only: no result depends on it.
+constexpr int kOrderSteps = 4;  // batches up to 256 are ordered
+
+struct Item {
+  int b, mtile;  // mtile < 0: there is no such tile
+};
+
+// Sum (or, with kMax, maximum) over the wave, in every lane.
+template <bool kMax>
+__device__ __forceinline__ int wave_reduce(int v) {
+  auto op = [](int a, int b) { return kMax ? max(a, b) : a + b; };
+  auto step = [](int a, auto ctrl) {
+    return __builtin_amdgcn_mov_dpp(a, decltype(ctrl)::value, 0xF, 0xF, false);
+  };
+  v = op(v, step(v, std::integral_constant<int, DPP_QUAD_XOR1>{}));
+  v = op(v, step(v, std::integral_constant<int, DPP_QUAD_XOR2>{}));
+  v = op(v, step(v, std::integral_constant<int, DPP_HALF_MIRROR>{}));
+  v = op(v, step(v, std::integral_constant<int, DPP_ROW_ROR8>{}));
+  return op(op(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+            op(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+template <int ROWS>
+__device__ __forceinline__ Item pick_item(int i, bool ordered, int per_round, int batch,
+                                          int mtiles, const int32_t* __restrict__ qo_indptr,
+                                          const int32_t* __restrict__ kv_indptr) {
+  const int round = per_round > 0 ? i / per_round : 0;
+  if ((round & 1) != 0 && (round + 1) * per_round <= batch * mtiles)
+    i = round * per_round + per_round - 1 - i % per_round;
+  if (!ordered) return {i % batch, mtiles - 1 - i / batch};
+  const int lane = __lane_id();
+  const int steps = ceil_div(batch, 64);
+  int pre[kOrderSteps], mt[kOrderSteps], top = 0, total = 0;
+#pragma unroll
+  for (int s = 0; s < kOrderSteps; ++s) {
+    pre[s] = mt[s] = 0;
+    if (s >= steps) continue;
+    const int b = min(64 * s + lane, batch - 1);
+    const int len = qo_indptr[b + 1] - qo_indptr[b];
+    const int prefix = kv_indptr[b + 1] - kv_indptr[b] - len;
+    pre[s] = max(prefix, 0) / ROWS;
+    mt[s] = 64 * s + lane < batch && len > 0 && prefix >= 0 ? ceil_div(len, ROWS) : 0;
+    total += mt[s];
+    top = max(top, mt[s] > 0 ? pre[s] + mt[s] : 0);
+  }
+  if (i >= wave_reduce<false>(total)) return {0, -1};
+  top = wave_reduce<true>(top);
+  auto above = [&](int x) {  // tiles at x or more
+    int n = 0;
+#pragma unroll
+    for (int s = 0; s < kOrderSteps; ++s) {
+      if (s >= steps) continue;
+      n += max(0, mt[s] - max(0, x - 1 - pre[s]));
+    }
+    return wave_reduce<false>(n);
+  };
+  int place = 0;  // the largest x with more than i tiles at x or more
+  for (int bit = 31 - __builtin_clz(top | 1); bit >= 0; --bit) {
+    const int x = place | 1 << bit;
+    if (x <= top && above(x) > i) place = x;
+  }
+  int left = i - above(place + 1);  // which of the tiles at this place
+#pragma unroll
+  for (int s = 0; s < kOrderSteps; ++s) {
+    if (s >= steps) continue;
+    const int m = place - 1 - pre[s];
+    uint64_t who = __builtin_amdgcn_ballot_w64(m >= 0 && m < mt[s]);
+    const int n = __builtin_popcountll(who);
+    if (left >= 0 && left < n) {
+      for (; left > 0; --left) who &= who - 1;
+      const int at = __builtin_ctzll(who);
+      return {64 * s + at, __builtin_amdgcn_readlane(m, at)};
+    }
+    left -= n;
+  }
+  return {0, -1};
+}
+
 // Workgroup = (request, kv head, 8 NW HPW query positions), NW waves. HPW = 2: a wave takes 16
 // positions of both query heads, which share every fragment it reads; HPW = 1: of one head
 // (wave w: head w / (NW / 2)). FANOUT: the workgroup computes one split and saves its state for
@@ -119,19 +222,29 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     const uint8_t* __restrict__ v_cache, const uint16_t* __restrict__ kv_scales,
     const int32_t* __restrict__ qo_indptr, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, int batch, int num_q_heads, int num_kv_heads,
-    int64_t num_slots, float sm_scale, int mtiles, int64_t items, bf16_t* __restrict__ o,
+    int64_t num_slots, float sm_scale, int mtiles, int per_round, int ordered, int64_t items,
+    bf16_t* __restrict__ o,
     float* __restrict__ part_a, float* __restrict__ part_ml, int32_t* __restrict__ part_n) {
   extern __shared__ __align__(1024) char lds[];
   constexpr int ROWS = 8 * NW * HPW;
-  const int b = min(static_cast<int>(blockIdx.x), batch - 1);
-  const int h_kv = blockIdx.y;
-  // Late query tiles walk the most keys: dispatch them first.
-  const int mtile = FANOUT ? static_cast<int>(blockIdx.z) % mtiles
-                           : mtiles - 1 - static_cast<int>(blockIdx.z);
-  const int split = FANOUT ? static_cast<int>(blockIdx.z) / mtiles : 0;
+  int b, h_kv, mtile, split = 0;
+  if constexpr (FANOUT) {
+    b = blockIdx.x;
+    h_kv = blockIdx.y;
+    mtile = static_cast<int>(blockIdx.z) % mtiles;
+    split = static_cast<int>(blockIdx.z) / mtiles;
+  } else {
+    // Heads fastest: with 8 of them a head's workgroups, which share its keys, are on one XCD.
+    h_kv = blockIdx.x % num_kv_heads;
+    const Item it = pick_item<ROWS>(blockIdx.x / num_kv_heads, ordered != 0, per_round, batch,
+                                    mtiles, qo_indptr, kv_indptr);
+    if (it.mtile < 0) return;
+    b = it.b;
+    mtile = it.mtile;
+  }
   const int q_start = qo_indptr[b];
   const int extend_len = qo_indptr[b + 1] - q_start;
-  if (mtile * ROWS >= extend_len || static_cast<int>(blockIdx.x) >= batch) return;
+  if (mtile * ROWS >= extend_len) return;
   const int kv_start = kv_indptr[b];
   const int kv_len = kv_indptr[b + 1] - kv_start;
   const int prefix = kv_len - extend_len;
@@ -149,11 +262,11 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   const float sc2 = sm_scale * LOG2E;
   const int last_row = min(extend_len, (mtile + 1) * ROWS) - 1;
   const int visible_end = min(kv_len, prefix + last_row + 1);
-  const int nsplits = ceil_div(visible_end, KSPLIT);
+  const int nsplits = ceil_div(visible_end, kSplit);
   if (FANOUT && split >= nsplits) return;  // the merge never reads this split
   // Tiles [t_begin, t_end) of the sequence.
-  const int t_begin = split * (KSPLIT / BN);
-  const int t_end = FANOUT ? min(ceil_div(visible_end, BN), t_begin + KSPLIT / BN)
+  const int t_begin = split * (kSplit / BN);
+  const int t_end = FANOUT ? min(ceil_div(visible_end, BN), t_begin + kSplit / BN)
                            : ceil_div(visible_end, BN);
   const int w_first = prefix + w_row;  // the wave's first and last positions
   const int w_last = prefix + min(extend_len, w_row + 16) - 1;
@@ -236,9 +349,26 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     }
   };
 
+  // The first loads, in the order of their latencies: slots and q, then what the slots name; q is
+  // split while those are under way.
+  Slots s1 = load_slots(t_begin), s2 = load_slots(t_begin + 1);
+  QRaw q_raw[HPW];
+#pragma unroll
+  for (int h = 0; h < HPW; ++h) q_raw[h] = load_q(q + (prow + h) * D, lane >> 4);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(s1);
+  __builtin_amdgcn_sched_barrier(0);
+  load_k(s1, 0);  // (t_begin is a split's first tile: even)
+  __builtin_amdgcn_sched_barrier(0);
   QRow qf[HPW];
 #pragma unroll
-  for (int h = 0; h < HPW; ++h) qf[h] = split_q(q + (prow + h) * D, row_ok, lane >> 4);
+  for (int h = 0; h < HPW; ++h) qf[h] = split_q(q_raw[h], row_ok);
+  __builtin_amdgcn_sched_barrier(0);
+  store_v(t_begin, 0);
+  load_v(s2);
+  s1 = s2;
+  s2 = load_slots(t_begin + 2);
+  __builtin_amdgcn_sched_barrier(0);
 
   RowState run[HPW], st[HPW];
 #pragma unroll
@@ -343,14 +473,6 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     }
   };
 
-  Slots s1 = load_slots(t_begin), s2 = load_slots(t_begin + 1);
-  load_k(s1, 0);
-  __builtin_amdgcn_sched_barrier(0);
-  load_v(s1);
-  store_v(t_begin, 0);  // (t_begin is a split's first tile: even)
-  load_v(s2);
-  s1 = s2;
-  s2 = load_slots(t_begin + 2);
   auto step = [&](auto mask, int t, auto buf) {  // buf: t & 1
     // Every load has landed (they had a whole tile's time) and every wave is done with the other
     // buffers.
@@ -380,8 +502,8 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   // immediates), then the others with the mask: one loop each, split by split (a branch between
   // the kinds in one loop, or the fold in it, costs a copy of the accumulators each turn).
   const int t_full = (prefix + mtile * ROWS + 1) / BN;
-  for (int s0 = t_begin; s0 < t_end; s0 += KSPLIT / BN) {
-    const int s_end = min(s0 + KSPLIT / BN, t_end);
+  for (int s0 = t_begin; s0 < t_end; s0 += kSplit / BN) {
+    const int s_end = min(s0 + kSplit / BN, t_end);
     int t = s0;
     for (const int e = min(s_end, t_full); t + 1 < e; t += 2) {
       step(std::false_type{}, t, std::integral_constant<int, 0>{});
@@ -416,10 +538,32 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   }
 }
 
+// Whether a grid of fewer than 512 workgroups fans out. Walking its keys in one workgroup takes about
+// 6 + 1.1 us a tile; fanned out, the launches take 18 us and the saved states of total_q rows in
+// every split 8.5 us a thousand. Walked and fanned out, us: 1 x 512 tokens 14 and 24, 1 x 1024 23 and
+// 40, 2 x 500 over 2000 49 and 69, 4 x 200 over 1000 28 and 36, 1 x 700 over 4000 82 and 78, 16 x 32
+// over 2048 42 and 38, 8 x 64 over 3000 57 and 44, 4 x 32 over 2048 40 and 22, 1 x 256 over 8000 138
+// and 56.
+bool fans_out(int batch, int64_t total_q, int num_kv_heads, int max_extend_len, int max_kv_len) {
+  const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * ceil_div(max_extend_len, BQ);
+  const int64_t states = total_q * ceil_div(max_kv_len, kSplit);
+  return groups < 512 && 110 * static_cast<int64_t>(ceil_div(max_kv_len, BN)) > 1200 + states * 85 / 100;
+}
+
 }  // namespace
 }  // namespace sid
 
 using namespace sid;
+
+extern "C" int64_t sid_extend_attention_fp8_workspace_bytes(int batch, int64_t total_q,
+                                                            int num_q_heads, int num_kv_heads,
+                                                            int max_extend_len, int max_kv_len) {
+  if (batch <= 0 || total_q <= 0 || max_extend_len <= 0 || max_kv_len <= 0) return 0;
+  if (!fans_out(batch, total_q, num_kv_heads, max_extend_len, max_kv_len)) return 0;
+  // per (split, row, head): 128 accumulator floats + (m, l); per (row, head): split count
+  const int64_t splits = ceil_div(max_kv_len, kSplit);
+  return (splits * (D + 2) + 1) * total_q * num_q_heads * static_cast<int64_t>(sizeof(float));
+}
 
 extern "C" int sid_extend_attention_fp8_fwd(
     const void* q, const void* k_cache, const void* v_cache, const void* kv_scales,
@@ -430,7 +574,11 @@ extern "C" int sid_extend_attention_fp8_fwd(
   const char* name = "extend_attention_fp8";
   const ExtendPlan p = extend_plan(name, q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o,
                                    batch, total_q, num_q_heads, num_kv_heads, head_dim, num_slots,
-                                   max_extend_len, max_kv_len, workspace, workspace_bytes);
+                                   max_extend_len, max_kv_len, kSplit,
+                                   sid_extend_attention_fp8_workspace_bytes(
+                                       batch, total_q, num_q_heads, num_kv_heads, max_extend_len,
+                                       max_kv_len),
+                                   workspace, workspace_bytes);
   if (p.rc != SID_OK || p.empty) return p.rc;
   SID_REQUIRE(kv_scales != nullptr, "%s: null pointer", name);
   auto misaligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) != 0; };
@@ -438,11 +586,17 @@ extern "C" int sid_extend_attention_fp8_fwd(
                   !misaligned(kv_scales) && !misaligned(o) && !misaligned(workspace),
               "%s: operands must be 16-byte aligned", name);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  // Tiles may differ in their keys: by the lengths, or by prefixes (of which only the longest key
+  // list says something here).
+  const int ordered = batch > 1 && batch <= 64 * kOrderSteps &&
+                      (8 * total_q < 7 * static_cast<int64_t>(batch) * max_extend_len ||
+                       max_kv_len > max_extend_len);
+  const int per_round = p.rows == 32 ? max(1, cu_count() / num_kv_heads) : 0;
   auto launch = [&](auto kern, int nw, dim3 grid, int mtiles) {
     hipLaunchKernelGGL(kern, grid, dim3(nw * 64), kLdsBytes, s, (const bf16_t*)q,
                        (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint16_t*)kv_scales, qo_indptr, kv_indptr, kv_indices, batch,
-                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, p.items,
+                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, per_round, ordered, p.items,
                        (bf16_t*)o, p.part_a, p.part_ml, p.part_n);
     return check_launch(name);
   };
@@ -452,7 +606,8 @@ extern "C" int sid_extend_attention_fp8_fwd(
     return rc != SID_OK ? rc : extend_merge(name, p, o, s);
   }
   const int mtiles = ceil_div(max_extend_len, p.rows);
-  const dim3 grid(p.grid_x, num_kv_heads, mtiles);
-  return p.rows == 64 ? launch(extend_fp8_kernel<8, 1, false>, 8, grid, mtiles)
-                      : launch(extend_fp8_kernel<4, 1, false>, 4, grid, mtiles);
+  const int64_t groups = static_cast<int64_t>(batch) * mtiles * num_kv_heads;
+  SID_REQUIRE(groups < (1ll << 31) / (64 * 8), "%s: grid too large", name);
+  return p.rows == 64 ? launch(extend_fp8_kernel<8, 1, false>, 8, dim3(groups), mtiles)
+                      : launch(extend_fp8_kernel<4, 1, false>, 4, dim3(groups), mtiles);
 }

@@ -189,8 +189,9 @@ constexpr int kTileBytes = BN * D * 2;  // one K or V tile
 // Query positions (32 or 64) of a workgroup that walks all keys of its rows.
 int extend_prefill_rows(int batch, int64_t total_q, int num_kv_heads, int max_extend_len);
 
-// The launch of a call, worked out once for both formats: what is checked, whether the splits
-// fan out over workgroups (workspace given and the grid small), the grid.
+// The launch of a call, worked out once for both formats: what is checked, whether the splits fan
+// out over workgroups (the caller's rule asks for `need` bytes and the workspace has them), the
+// grid.
 struct ExtendPlan {
   int rc;             // SID_OK or the error
   bool empty;         // nothing to do
@@ -207,8 +208,8 @@ ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, con
                        const int32_t* qo_indptr, const int32_t* kv_indptr,
                        const int32_t* kv_indices, const void* o, int batch, int64_t total_q,
                        int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
-                       int max_extend_len, int max_kv_len, void* workspace,
-                       int64_t workspace_bytes);
+                       int max_extend_len, int max_kv_len, int split_keys, int64_t need,
+                       void* workspace, int64_t workspace_bytes);
 
 // The fan-out's second launch: the saved split states of every item folded in order.
 int extend_merge(const char* name, const ExtendPlan& p, void* o, hipStream_t s);

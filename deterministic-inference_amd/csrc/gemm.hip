@@ -891,20 +891,6 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) linear_tile_kernel(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// Compute units of the current device.
-int cu_count() {
-  static int count[64] = {0};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (count[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-      n = 256;
-    count[dev] = n;
-  }
-  return count[dev];
-}
-
 template <int WM, int WN, int MB, int NB, int ST, int OCC, int PER_CU, int EPI>
 void launch_tile(const void* x, int64_t ldx, const void* w, int64_t m, int64_t n, int64_t k,
                  const TileOut& out, hipStream_t s) {

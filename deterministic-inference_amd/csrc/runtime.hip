@@ -23,6 +23,19 @@ int check_launch(const char* what) {
   return SID_OK;
 }
 
+int cu_count() {
+  static int count[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (count[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+      n = 256;
+    count[dev] = n;
+  }
+  return count[dev];
+}
+
 }  // namespace sid
 
 extern "C" const char* sid_last_error(void) { return sid::g_last_error; }

@@ -72,7 +72,7 @@ _SIGNATURES = {
 EXPORTED = ("sid_last_error", "sid_abi_version", "sid_extend_attention_workspace_bytes",
             "sid_linear_argmax_workspace_bytes", "sid_sample_workspace_bytes",
             "sid_qwen3_extend_workspace_bytes", "sid_qwen3_extend_forward",
-            "sid_qwen3_extend_forward_fp8",
+            "sid_qwen3_extend_forward_fp8", "sid_extend_attention_fp8_workspace_bytes",
             "sid_flash_decode_noalloc_scratch_bytes", "sid_linear_sample_workspace_bytes",
             "sid_extend_attention_query_rows", "sid_linear_tile", *_SIGNATURES)
 ABI_VERSION = 22
@@ -153,6 +153,9 @@ class NativeLib:
         self.lib.sid_abi_version.argtypes = []
         self.lib.sid_extend_attention_workspace_bytes.restype = ctypes.c_int64
         self.lib.sid_extend_attention_workspace_bytes.argtypes = [_i32, _i64, _i32, _i32, _i32, _i32]
+        self.lib.sid_extend_attention_fp8_workspace_bytes.restype = ctypes.c_int64
+        self.lib.sid_extend_attention_fp8_workspace_bytes.argtypes = [_i32, _i64, _i32, _i32, _i32,
+                                                                      _i32]
         self.lib.sid_extend_attention_query_rows.restype = ctypes.c_int
         self.lib.sid_extend_attention_query_rows.argtypes = [_i32, _i64, _i32, _i32]
         self.lib.sid_linear_tile.restype = ctypes.c_int
@@ -350,9 +353,10 @@ class NativeLib:
     # ---- the rest of the decode path ----------------------------------------------------
 
     def extend_attention_workspace_bytes(self, batch, total_q, hq, hkv, max_extend_len,
-                                         max_kv_len) -> int:
-        return int(self.lib.sid_extend_attention_workspace_bytes(
-            batch, total_q, hq, hkv, max_extend_len, max_kv_len))
+                                         max_kv_len, fp8: bool = False) -> int:
+        fn = (self.lib.sid_extend_attention_fp8_workspace_bytes if fp8
+              else self.lib.sid_extend_attention_workspace_bytes)
+        return int(fn(batch, total_q, hq, hkv, max_extend_len, max_kv_len))
 
     def extend_attention_fwd(self, q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices,
                              max_extend_len: int, sm_scale: float, o, max_kv_len: int,

@@ -32,7 +32,8 @@ def extend_attention_fwd(q_extend: torch.Tensor, k_buffer: torch.Tensor, v_buffe
     o_extend = torch.empty_like(q_extend)
     need = ext.extend_attention_workspace_bytes(qo_indptr.numel() - 1, q_extend.shape[0],
                                                 q_extend.shape[1], k_buffer.shape[1],
-                                                max_extend_len, max_kv_len)
+                                                max_extend_len, max_kv_len,
+                                                fp8=kv_scales is not None)
     ws = torch.empty(need, dtype=torch.uint8, device=q_extend.device) if need else None
     ext.extend_attention_fwd(q_extend, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices,
                              max_extend_len, sm_scale, o_extend, max_kv_len, ws, kv_scales=kv_scales)

@@ -632,11 +632,15 @@ int sid_flash_decode_fp8_fwd(const void* q, const void* k_cache, const void* v_c
                              int part_stride, void* o, int workers, void* stream);
 
 /*
- * sid_extend_attention_fwd over an 8-bit pool, with its workspace
- * (sid_extend_attention_workspace_bytes) and its invariances: a query's result depends only on
- * its position and its sequence's keys. A NaN vector reaches the queries that see its key and
- * no others.
+ * sid_extend_attention_fwd over an 8-bit pool, with its invariances: a query's result depends
+ * only on its position and its sequence's keys (reduced in 512-position splits here). A NaN
+ * vector reaches the queries that see its key and no others. workspace as there, of
+ * sid_extend_attention_fp8_workspace_bytes(...) bytes (never more than
+ * sid_extend_attention_workspace_bytes of the same arguments; 0 = no fan-out).
  */
+int64_t sid_extend_attention_fp8_workspace_bytes(int batch, int64_t total_q, int num_q_heads,
+                                                 int num_kv_heads, int max_extend_len,
+                                                 int max_kv_len);
 int sid_extend_attention_fp8_fwd(const void* q, const void* k_cache, const void* v_cache,
                                  const void* kv_scales, const int32_t* qo_indptr,
                                  const int32_t* kv_indptr, const int32_t* kv_indices, int batch,

@@ -488,6 +488,28 @@ def test_chunk_fanout_and_batch_keep_bits():
             assert torch.equal(part, o[a + lo:a + hi])
 
 
+@pytest.mark.parametrize("batch,lo,hi,pre", [(2, 900, 2100, 700), (17, 1, 400, 900),
+                                             (63, 1, 50, 300), (64, 1, 40, 100), (65, 20, 40, 5),
+                                             (200, 1, 30, 60), (256, 0, 9, 40), (257, 1, 9, 40),
+                                             (300, 1, 3, 20)])
+def test_chunk_placement_covers_every_tile(batch, lo, hi, pre):
+    """Ragged batches whose grid is placed by key count (up to 256 requests) or plainly: every
+    row is there, with the bits that its request alone gives (fanned out)."""
+    _say("placement", batch)
+    rng = np.random.default_rng(batch)
+    specs = [(int(rng.integers(0, pre + 1)), int(rng.integers(lo, hi + 1))) for _ in range(batch)]
+    specs[batch // 2] = (pre, hi)
+    q, pool, qo, ptr, idx, at, qoh = _chunk_batch(specs, seed=batch)
+    o = _chunk(q, pool, qo, ptr, idx, specs, workspace=False)
+    assert not o.isnan().any()
+    for i in sorted({0, 1, batch // 2, batch - 1, *rng.integers(0, batch, 6).tolist()}):
+        p, e = specs[i]
+        if e:
+            one = _chunk(q[int(qoh[i]):int(qoh[i + 1])].contiguous(), pool, _i32([0, e]),
+                         _i32([0, p + e]), _i32(at[i].tolist()), [(p, e)])
+            assert torch.equal(one, o[int(qoh[i]):int(qoh[i + 1])]), i
+
+
 @pytest.mark.parametrize("which", [0, 1], ids=["nan_k", "nan_v"])
 @pytest.mark.parametrize("specs", [[(100, 70)], [(5, 1200)] * 4], ids=["fanout", "grid"])
 def test_chunk_nan_reaches_only_rows_that_see_it(specs, which):

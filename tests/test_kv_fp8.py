@@ -118,6 +118,19 @@ def test_extend_refusals(lib, change, text):
     assert text in _err(lib)
 
 
+@pytest.mark.parametrize("batch,total,me,mk,fan", [
+    (4, 128, 32, 2080, True), (16, 512, 32, 2080, True), (1, 256, 256, 8256, True),
+    (8, 300, 64, 3064, True), (1, 1, 1, 4000, True), (1, 512, 512, 512, False),
+    (1, 1024, 1024, 1024, False), (2, 1000, 500, 2500, False), (4, 8192, 2048, 2048, False),
+    (64, 64, 1, 9000, False),
+], ids=str)
+def test_fan_out_rule(lib, batch, total, me, mk, fan):
+    need = lib.sid_extend_attention_fp8_workspace_bytes(batch, total, 16, 8, me, mk)
+    assert (need > 0) == fan
+    assert need <= lib.sid_extend_attention_workspace_bytes(batch, total, 16, 8, me, mk)
+    assert not fan or need == (-(-mk // 512) * 130 + 1) * total * 16 * 4
+
+
 def test_fused_writers_refuse(lib):
     post = [16, None, 0, 4, 16, 8, 128, 16, 16, F, 16, 16, 100, 16, 16, 16, 16, None, 10, None]
     assert lib.sid_qkv_post_fp8(*post) == 1 and "null" in _err(lib)
