@@ -7,6 +7,16 @@
 //     the two scales of (token, head) come as one 2-byte load, 16 bytes a token;
 //   * codes are converted without their scale (exact), the powers of two enter where a token
 //     has one value a head: s = (q . c_k) (2^e_k sm_scale) and o += (p 2^e_v) c_v.
+//
+// Bound: the pool's rows, 2064 bytes a token. A wave asks for 4 tokens' rows (8 KiB), then
+// computes on the 4 before: its conversions and dot products take about half as long as the rows
+// take to come, and with loads and math in turn neither hides the other (128 requests of 4096
+// keys 173.2 -> 169.3 us with the rows a step ahead, 64 of 2048 48.9 -> 47.0, 32 ragged ones of
+// 128-4096 31.6 -> 29.2). 4 tokens an iteration: with 8 the wave holds 209 registers and one
+// workgroup fits a CU, with 2 too little is in flight (128 x 4096: 172 us with two workgroups a
+// CU, 203 with a plan of one). 128 x 4096 keys: 171 us, 6.3 TB/s, where a plain read of the
+// same size reaches 6.0-6.5; 1 x 1024: 10.4 us, the chain of launch, slots, rows, merge and
+// stage 2's launch.
 #include "decode_split.h"
 #include "kv_fp8.h"
 
@@ -18,7 +28,8 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
                                          __builtin_bit_cast(bf16x2_v, b), c, false);
 }
 
-template <int TPL>
+constexpr int TPL = 4;  // tokens per wave iteration
+
 struct TileRegs {
   u32x4_v k[TPL];
   u32x4_v v[TPL];
@@ -27,9 +38,8 @@ struct TileRegs {
 
 // The partial attention of request b over partial slot y (a segment of one split), by one
 // workgroup of NW waves taking TPL tokens per wave iteration. Every exit is
-// workgroup-uniform. The next iteration's slot indices load while this one's rows are in
-// flight.
-template <int NW, int TPL>
+// workgroup-uniform.
+template <int NW>
 __device__ __forceinline__ void stage1_item(
     Stage1Lds<NW>& sh, int b, int y, const bf16_t* __restrict__ q,
     const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
@@ -88,7 +98,7 @@ __device__ __forceinline__ void stage1_item(
     for (int t = 0; t < TPL; ++t) raw[t] = idx[min(t0 + t, end - 1)];
   };
   // Positions past the segment's end load its last token again and get weight 0.
-  auto load_tile = [&](int t0, const int32_t (&raw)[TPL], bool (&ok)[TPL], TileRegs<TPL>& r) {
+  auto load_tile = [&](int t0, const int32_t (&raw)[TPL], bool (&ok)[TPL], TileRegs& r) {
 #pragma unroll
     for (int t = 0; t < TPL; ++t) {
       int64_t sv = static_cast<int64_t>(raw[t]);
@@ -100,7 +110,7 @@ __device__ __forceinline__ void stage1_item(
     }
     __builtin_amdgcn_sched_barrier(0);  // (as in decode_attention.hip: all loads go out first)
   };
-  auto compute = [&](const bool (&ok)[TPL], const TileRegs<TPL>& r) {
+  auto compute = [&](const bool (&ok)[TPL], const TileRegs& r) {
     float sc[QPK][TPL];
 #pragma unroll
     for (int t = 0; t < TPL; ++t) {
@@ -160,15 +170,25 @@ __device__ __forceinline__ void stage1_item(
     }
   };
 
+  // Rows are loaded one iteration ahead of their math, their slots two.
   int32_t raw[TPL];
-  load_idx(start + wave * TPL, raw);
-  for (int t0 = start + wave * TPL; t0 < end; t0 += IT) {
-    bool ok[TPL];
-    TileRegs<TPL> r;
-    load_tile(t0, raw, ok, r);
-    load_idx(t0 + IT, raw);
+  TileRegs r;
+  bool ok[TPL];
+  int t0 = start + wave * TPL;
+  load_idx(t0, raw);
+  load_tile(t0, raw, ok, r);
+  load_idx(t0 + IT, raw);
+  for (; t0 + IT < end; t0 += IT) {
+    TileRegs next;
+    bool next_ok[TPL];
+    load_tile(t0 + IT, raw, next_ok, next);
+    load_idx(t0 + 2 * IT, raw);
     compute(ok, r);
+    r = next;
+#pragma unroll
+    for (int t = 0; t < TPL; ++t) ok[t] = next_ok[t];
   }
+  if (t0 < end) compute(ok, r);
 
 #pragma unroll
   for (int h = 0; h < QPK; ++h) {
@@ -189,7 +209,7 @@ __device__ __forceinline__ void stage1_item(
 // Grid form and worker form, as in decode_attention.hip: workgroup (b, y), or the entry of
 // wg_order at its linear id; or the items that wg_order deals to each of `gridDim.x` workers
 // (order entries i, i + workers, ...; from the first one flagged empty on, all are).
-template <int NW, int TPL, bool WORKER>
+template <int NW, bool WORKER>
 __global__ void __launch_bounds__(NW * 64) decode_fp8_stage1_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ k_cache,
     const uint8_t* __restrict__ v_cache, const uint16_t* __restrict__ kv_scales,
@@ -200,7 +220,7 @@ __global__ void __launch_bounds__(NW * 64) decode_fp8_stage1_kernel(
     const int32_t* __restrict__ wg_order, int batch, int grid_slots) {
   __shared__ Stage1Lds<NW> sh;
   auto item = [&](int b, int y) {
-    stage1_item<NW, TPL>(sh, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices,
+    stage1_item<NW>(sh, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices,
                          num_splits, max_splits, fixed_split, seg, sm_scale, num_slots,
                          part_stride, part_o, part_lse, o_direct);
   };
@@ -278,16 +298,13 @@ extern "C" int sid_flash_decode_fp8_fwd(
                        fixed_split_size, segment_size, sm_scale, num_slots, part_stride, part_o,
                        part_lse, direct ? (bf16_t*)o : nullptr, wg_order, batch, grid_slots);
   };
-#define SID_SHAPE(NW, TPL)                                      \
-  (worker ? stage1(decode_fp8_stage1_kernel<NW, TPL, true>, NW) \
-          : stage1(decode_fp8_stage1_kernel<NW, TPL, false>, NW))
-  switch (variant) {
-    case 1: SID_SHAPE(4, 2); break;
-    case 2: SID_SHAPE(8, 4); break;
-    case 3: SID_SHAPE(4, 4); break;
-    default: SID_SHAPE(4, 8); break;
+  if (variant == 2) {
+    worker ? stage1(decode_fp8_stage1_kernel<8, true>, 8)
+           : stage1(decode_fp8_stage1_kernel<8, false>, 8);
+  } else {
+    worker ? stage1(decode_fp8_stage1_kernel<4, true>, 4)
+           : stage1(decode_fp8_stage1_kernel<4, false>, 4);
   }
-#undef SID_SHAPE
   rc = check_launch("flash_decode_fp8_fwd stage1");
   if (rc != SID_OK || direct) return rc;
   return launch_decode_stage2(batch, grid_slots, part_o, part_lse, part_stride, o, s);

@@ -21,8 +21,8 @@ from sid.engine.batch import (DecodeStatic, ForwardBatch, ForwardMode, batch_buc
 from sid.engine.kv_cache import KVCache
 from sid.engine.sampler import sample as _sample
 from sid.kernels.decode_attention import (INVARIANT_VARIANT, DecodeAttention, length_bucket,
-                                          plan_variant, segment_tokens, stage1_workers,
-                                          worker_order, workgroup_order)
+                                          plan_variant, plan_variant_fp8, segment_tokens,
+                                          stage1_workers, worker_order, workgroup_order)
 from sid.kernels.matmul_persistent import linear_sample_supported
 from sid.model.loader import build_model_config, load_weights, random_weights
 from sid.model.qwen3 import Qwen3Model
@@ -242,10 +242,13 @@ class ModelRunner:
     def _pick_variant(self, fb: ForwardBatch, bs: int, max_len: int) -> tuple:
         """The nondet plan's geometry and its stage-1 workgroup shape (fb.decode_variant),
         from the requests' host-known lengths."""
-        geom, fb.decode_variant = plan_variant(fb.seq_lens_host, max_len,
-                                               self.mcfg.num_kv_heads,
-                                               self.decode_attn.cu_count(),
-                                               self.cfg.max_kv_splits, invariant=False)
+        cu, splits = self.decode_attn.cu_count(), self.cfg.max_kv_splits
+        if self.kv_cache.kv_scales is not None:
+            geom, fb.decode_variant = plan_variant_fp8(fb.seq_lens_host, max_len, cu, splits)
+        else:
+            geom, fb.decode_variant = plan_variant(fb.seq_lens_host, max_len,
+                                                   self.mcfg.num_kv_heads, cu, splits,
+                                                   invariant=False)
         fb.decode_geometry = geom
         return geom
 

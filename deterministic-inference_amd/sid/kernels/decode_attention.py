@@ -153,19 +153,26 @@ WIDE_TOKENS_PER_LONGEST = 170  # the longest workgroup holds <= 1/170 of the bat
 WIDE_MAX_IMBALANCE = 1.3     # busiest CU / mean CU load, once they cover every CU
 
 
-def _cu_imbalance(sizes: np.ndarray, cu_count: int) -> float:
-    """Busiest CU's tokens over the mean when `sizes` (workgroup tokens) are dealt
-    heaviest first, every other round reversed, as workgroup_order deals them."""
+def _busiest_cu(sizes: np.ndarray, cu_count: int) -> int:
+    """The busiest CU's tokens when `sizes` (workgroup tokens) are dealt heaviest first, every
+    other round reversed, as workgroup_order deals them."""
     w = np.sort(sizes[sizes > 0])[::-1]
     if w.size == 0:
-        return 1.0
+        return 0
     rounds = _cdiv(w.size, cu_count)
     m = np.zeros(rounds * cu_count, dtype=np.int64)
     m[:w.size] = w
     m = m.reshape(rounds, cu_count)
     m[1::2] = m[1::2, ::-1]
-    loads = m.sum(axis=0)
-    return float(loads.max()) / max(float(loads.mean()), 1.0)
+    return int(m.sum(axis=0).max())
+
+
+def _cu_imbalance(sizes: np.ndarray, cu_count: int) -> float:
+    """The busiest CU's tokens (_busiest_cu) over the mean."""
+    total = int(sizes.sum())
+    if total == 0:
+        return 1.0
+    return _busiest_cu(sizes, cu_count) / max(total / cu_count, 1.0)
 
 
 def _wide_plan(lens: np.ndarray, cu_count: int):
@@ -235,6 +242,53 @@ def plan_variant(lengths, max_len: int, num_kv_heads: int, cu_count: int, max_kv
             chunk_max = max(32, _cdiv(_cdiv(max_len, splits), 32) * 32)
             return (splits, pick[0], splits * max(1, _cdiv(chunk_max, pick[0]))), pick[1]
     return geom, stage1_variant(nonempty_workgroups(lens, splits, seg), cu_count, invariant=False)
+
+
+# Plans over the 8-bit pool (sid_flash_decode_fp8_fwd). A wave loads the next iteration's rows
+# before it computes on this one's, so one 8 x 4 or 4 x 4 workgroup of a CU asks for more than
+# the CU's share of the memory's rate, and what decides is how evenly the tokens lie on the CUs
+# and how many workgroups start behind another. With a token's time at that share (2 KiB at a
+# 256th of 6.4 TB/s, 80 ns) as the unit, stage 1 takes about
+#     mean + a (max - mean) + r max(workgroups / CUs - 1, 0) + slots
+# mean and max being a CU's tokens when they are dealt heaviest first: a CU left with tokens
+# when the others are done runs them at 0.57 (8 x 4) or 0.64 (4 x 4) of that time each; an 8 x 4
+# workgroup fills its CU, and the next one's start costs 70 tokens, where 4 x 4 ones start next
+# to each other and cost 30; a partial slot adds a token's time to the merge. Fitted to 24 batches
+# (B = 1-256, uniform and ragged, lengths 20-8192; every segment size and both shapes, graph
+# timed with rotated pools): the plan of least estimate is 1.5% from the fastest of a batch on
+# average, 5% at worst, where the 2-byte pool's rules are 9% and up to 26% from it (128
+# requests of 4096 190.8 -> 171.2 us, 64 of 128-4096 73.4 -> 69.2, 8 of 100-8000 31.1 -> 24.7,
+# 256 of 20-300 30.2 -> 24.7).
+FP8_SEGMENTS = (2048, 1024, 512, 256, 128, 64, 32)
+FP8_SHAPES = ((2, 0.57, 70, 1), (3, 0.64, 30, 0))  # variant, a, r, cost of its own merge
+FP8_MAX_PER_CU = 6  # more workgroups than this a CU are never the fastest
+
+
+def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int) -> tuple:
+    """plan_variant's nondet plan for an 8-bit pool: ((1, segment size, grid slots), stage-1
+    variant). Every request is one split cut into segments, so its policy batch does not enter;
+    slots stay within what the workspace holds for any plan (workspace_slots)."""
+    lens = np.asarray(lengths, dtype=np.int64)
+    lens = lens[lens > 0]
+    max_len = max(int(max_len), 1)
+    most = min(max_len // SEGMENT_SIZES[-1] + max_kv_splits, MAX_GRID_SLOTS)
+    mean = float(lens.sum()) / cu_count
+    best = None
+    for seg in FP8_SEGMENTS:
+        slots = _cdiv(max_len, seg)
+        if best is not None and slots > most:
+            break
+        full, tail = lens // seg, lens % seg
+        sizes = np.concatenate([np.full(int(full.sum()), seg, dtype=np.int64), tail[tail > 0]])
+        if best is not None and sizes.size > FP8_MAX_PER_CU * cu_count:
+            break
+        longest = _busiest_cu(sizes, cu_count)
+        late = max(sizes.size / cu_count - 1.0, 0.0)
+        for variant, a, r, own in FP8_SHAPES:
+            cost = mean + a * (longest - mean) + r * late + slots + own
+            if best is None or cost < best[0]:
+                best = (cost, (1, seg, slots), variant)
+    return best[1], best[2]
 
 
 ORDER_SLOT_BITS = 12  # sid_flash_decode_segments_fwd wg_order entries: request << 12 | slot
@@ -387,15 +441,19 @@ class DecodeAttention:
 
     def step_plan(self, lengths, kv_fp8: bool = False, max_len: int | None = None) -> dict:
         """The nondet/dvr plan of a decode step over requests of these lengths (host-side), as
-        forward's arguments: geometry and workgroup shape (plan_variant) and the placement of
-        the workgroups (workgroup_order, worker_order). One plan serves the step's layers. Its
-        order is copied to the device here: make it outside a graph capture. max_len: the bound
-        that forward is called with, if it is not the longest length; kv_fp8: 8-bit pool."""
+        forward's arguments: geometry and workgroup shape (plan_variant; plan_variant_fp8 for
+        an 8-bit pool, kv_fp8) and the placement of the workgroups (workgroup_order,
+        worker_order). One plan serves the step's layers. Its order is copied to the device
+        here: make it outside a graph capture. max_len: the bound that forward is called with,
+        if it is not the longest length."""
         lens = [int(n) for n in lengths]
         bound = max(max(lens, default=1) if max_len is None else int(max_len), 1)
         cu = self.cu_count()
-        geom, variant = plan_variant(lens, bound, self.num_kv_heads, cu, self.max_kv_splits,
-                                     invariant=False)
+        if kv_fp8:
+            geom, variant = plan_variant_fp8(lens, bound, cu, self.max_kv_splits)
+        else:
+            geom, variant = plan_variant(lens, bound, self.num_kv_heads, cu, self.max_kv_splits,
+                                         invariant=False)
         tokens = segment_tokens(lens, len(lens), geom[0], 0, geom[1], geom[2])
         nonempty = int(np.count_nonzero(tokens))
         workers = stage1_workers(nonempty, variant, geom[2], cu)

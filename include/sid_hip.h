@@ -620,7 +620,7 @@ int sid_rmsnorm_qkv_post_fp8(const void* src, int src_fp32, const void* norm_w, 
 /*
  * sid_flash_decode_workers_fwd over an 8-bit pool: the same splits, segments, orders and merge.
  * The workgroup shapes that `variant` picks are this kernel's own (part of the reduction order,
- * as there): 0 = 4 waves x 8 tokens per wave iteration, 1 = 4 x 2, 2 = 8 x 4, 3 = 4 x 4.
+ * as there): 2 = 8 waves x 4 tokens per wave iteration, 0, 1 and 3 = 4 x 4.
  */
 int sid_flash_decode_fp8_fwd(const void* q, const void* k_cache, const void* v_cache,
                              const void* kv_scales, const int32_t* kv_indptr,

@@ -186,3 +186,35 @@ def test_ops_reject_cpu_tensors():
         reshape_and_cache_fp8(x, x, k, v, s, at)
     with pytest.raises(RuntimeError, match="GPU tensor"):
         gather_cache_fp8(k, v, s, at)
+
+
+# ---------------------------------------------------------------- decode plans (host)
+
+PLAN_BATCHES = [[1], [1024], [300] * 4, [500] * 3, [8192], [2048] * 8, [512] * 16,
+                list(range(128, 4097, 128)), [2048] * 64, [4096] * 128, [3000] * 160,
+                [1024] * 256, list(range(20, 301)), [100000, 1, 1, 1], [1] * 300, [2_000_000]]
+
+
+@pytest.mark.parametrize("lens", PLAN_BATCHES, ids=lambda x: f"{len(x)}x{max(x)}")
+@pytest.mark.parametrize("bucketed", [False, True])
+def test_decode_plan_covers_every_token(lens, bucketed):
+    from sid.kernels.decode_attention import (length_bucket, plan_variant_fp8, segment_tokens,
+                                              workspace_slots)
+    bound = length_bucket(max(lens)) if bucketed else max(lens)
+    (splits, seg, slots), variant = plan_variant_fp8(lens, bound, 256, 32)
+    assert splits == 1 and variant in (2, 3) and seg % 32 == 0
+    assert slots * seg >= bound and slots <= min(workspace_slots(bound, 32, 256), 1024)
+    tokens = segment_tokens(lens, len(lens), splits, 0, seg, slots)
+    assert tokens.sum(axis=0).tolist() == list(lens)
+    if sum(lens) >= 256 * 512 and max(lens) <= 4096:
+        # plenty of work: no CU is left more than a third above the mean
+        from sid.kernels.decode_attention import _busiest_cu
+        assert _busiest_cu(tokens.reshape(-1), 256) <= 1.34 * sum(lens) / 256
+
+
+def test_decode_plan_of_small_and_empty_batches():
+    from sid.kernels.decode_attention import plan_variant_fp8
+    assert plan_variant_fp8([1024], 1024, 256, 32) == ((1, 32, 32), 2)  # spread out
+    assert plan_variant_fp8([], 1, 256, 32)[0] == (1, 2048, 1)
+    assert plan_variant_fp8([0, 0, 5], 5, 256, 32)[0][0] == 1
+    assert plan_variant_fp8([0, 1024], 1024, 256, 32) == plan_variant_fp8([1024], 1024, 256, 32)
