@@ -4,6 +4,14 @@
 // (extend_tile.h): a query's result depends only on its position and its sequence's keys. What
 // differs is how the products get their operands: K's codes lie in the LDS as they are and S = K
 // Q^T is taken on them, with q as two e4m3 vectors; V's become bf16 on their way into the LDS.
+//
+// Bound: 4 operations for each of a query's keys and dims. 1 x 8192 tokens 330 us, 0.83 PFLOP/s;
+// 4 x 2048 114 us, 0.60, a third of which is the workgroups' first loads and last stores (one of 8
+// waves fills a CU); the 2-byte pool's kernel 420 and 133 us. The matrix products are 1024 of a
+// tile's 2900 cycles on a SIMD (two waves, 24 products each); the rest is a wave's own chain, V's
+// conversion, the softmax and the loads' addresses, which two waves that start a tile at the same
+// barrier overlap only in part. It is not the LDS (896 cycles a tile of 8 waves, no bank
+// conflicts) nor the count of vector operations (a third fewer: 2%).
 #include "extend_tile.h"
 #include "kv_fp8.h"
 
@@ -16,19 +24,29 @@ namespace {
 // as for bf16 pools: 16 windows of 32 over 2048 keys 47 us against 38, 700 tokens over 4000 99
 // against 78; 4 windows 21.1 against 22.5.)
 constexpr int kSplit = 512;
+constexpr int kSplitTiles = kSplit / BN;
 
 // ---- LDS ---------------------------------------------------------------------------------
 //
 // A tile is 64 keys. K stays in codes, 128 bytes a key: 16-byte unit u of a key's row holds piece
-// u ^ swk(key), so that the 16 rows of a fragment read fall on all 64 banks. V is bf16, as in
-// extend_attention.hip's tiles (piece p at p ^ swz(key)). Beside them K's scale bytes as the
-// matrix instruction takes them: word r holds the bytes of row r of the tile's four key blocks.
+// u ^ swk(key), so that the 16 rows of a fragment read fall on all 64 banks. V is bf16, 256
+// bytes a key, piece p at p ^ swv(key): half a wave's transpose read takes 32 bytes of 8 keys, which
+// swv puts on all banks. Beside them K's scale bytes as the matrix instruction takes them: word r
+// holds the bytes of row r of the tile's four key blocks.
 constexpr int kKTile = BN * D;
 constexpr int kVAt = 2 * kKTile;                 // [2] K tiles, [2] V tiles, [2] K scale words
 constexpr int kScalesAt = kVAt + 2 * kTileBytes;
-constexpr int kLdsBytes = kScalesAt + 2 * 64;
+constexpr int kParkedAt = kScalesAt + 2 * 64;
+// A lane's folded state stays in the LDS between two folds, 8 tiles apart: 7 of its 8
+// accumulator vectors (the registers hold the state of the split in work; with all 8, two 4-wave
+// workgroups would not fit a CU).
+constexpr int kParked = 7;
+constexpr int lds_bytes(int waves, bool fanout) {
+  return kParkedAt + (fanout ? 0 : kParked * waves * 1024);
+}
 
 __device__ __forceinline__ int swk(int key) { return ((key >> 1) & 1) | (((key >> 3) & 3) << 1); }
+__device__ __forceinline__ int swv(int key) { return 2 * (key & 3) | ((key >> 3) & 1) << 3; }
 
 // Lane l's 16 bytes at its address -> LDS byte lds + 16 l.
 __device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
@@ -118,12 +136,6 @@ __device__ __forceinline__ std::integral_constant<int, 1 - B> other(std::integra
   return {};
 }
 
-struct RowCtx {  // what softmax_tile reads
-  int g;
-  int q_abs;
-  bool row_ok;
-};
-
 // ---- placement ------------------------------------------------------------------------------
 //
 // The query tiles of a ragged batch walk from one key tile to a whole long context, and a grid ends
@@ -212,21 +224,20 @@ __device__ __forceinline__ Item pick_item(int i, bool ordered, int per_round, in
   return {0, -1};
 }
 
-// Workgroup = (request, kv head, 8 NW HPW query positions), NW waves. HPW = 2: a wave takes 16
-// positions of both query heads, which share every fragment it reads; HPW = 1: of one head
-// (wave w: head w / (NW / 2)). FANOUT: the workgroup computes one split and saves its state for
-// the fold; else it walks the splits in order.
-template <int NW, int HPW, bool FANOUT>
+// Workgroup = (request, kv head, 8 NW query positions), NW waves; wave w: 16 positions of query head
+// w / (NW / 2). FANOUT: the workgroup computes one split and saves its state for the fold; else it
+// walks the splits in order.
+template <int NW, bool FANOUT>
 __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ k_cache,
     const uint8_t* __restrict__ v_cache, const uint16_t* __restrict__ kv_scales,
     const int32_t* __restrict__ qo_indptr, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, int batch, int num_q_heads, int num_kv_heads,
     int64_t num_slots, float sm_scale, int mtiles, int per_round, int ordered, int64_t items,
-    bf16_t* __restrict__ o,
-    float* __restrict__ part_a, float* __restrict__ part_ml, int32_t* __restrict__ part_n) {
-  extern __shared__ __align__(1024) char lds[];
-  constexpr int ROWS = 8 * NW * HPW;
+    bf16_t* __restrict__ o, float* __restrict__ part_a, float* __restrict__ part_ml,
+    int32_t* __restrict__ part_n) {
+  __shared__ __align__(1024) char lds[lds_bytes(NW, FANOUT)];
+  constexpr int ROWS = 8 * NW;
   int b, h_kv, mtile, split = 0;
   if constexpr (FANOUT) {
     b = blockIdx.x;
@@ -253,30 +264,32 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
-  constexpr int BLOCKS = NW * HPW / 2;  // 16-position blocks of the workgroup
-  const int hq0 = h_kv * 2 + (HPW == 2 ? 0 : wave / BLOCKS);
-  const int w_row = mtile * ROWS + 16 * (wave % BLOCKS);  // the wave's first query row
-  const int qr = w_row + (lane & 15);
-  const bool row_ok = qr < extend_len;
-  const int64_t prow = static_cast<int64_t>(q_start + (row_ok ? qr : 0)) * num_q_heads + hq0;
+  const int hq = h_kv * 2 + wave / (NW / 2);
+  const int w_row = mtile * ROWS + 16 * (wave % (NW / 2));  // the wave's first query row
+  const int r = lane & 15, g = lane >> 4;
+  const bool row_ok = w_row + r < extend_len;
+  const int64_t prow = static_cast<int64_t>(q_start + (row_ok ? w_row + r : 0)) * num_q_heads + hq;
   const float sc2 = sm_scale * LOG2E;
   const int last_row = min(extend_len, (mtile + 1) * ROWS) - 1;
   const int visible_end = min(kv_len, prefix + last_row + 1);
   const int nsplits = ceil_div(visible_end, kSplit);
   if (FANOUT && split >= nsplits) return;  // the merge never reads this split
   // Tiles [t_begin, t_end) of the sequence.
-  const int t_begin = split * (kSplit / BN);
-  const int t_end = FANOUT ? min(ceil_div(visible_end, BN), t_begin + kSplit / BN)
+  const int t_begin = split * kSplitTiles;
+  const int t_end = FANOUT ? min(ceil_div(visible_end, BN), t_begin + kSplitTiles)
                            : ceil_div(visible_end, BN);
-  const int w_first = prefix + w_row;  // the wave's first and last positions
-  const int w_last = prefix + min(extend_len, w_row + 16) - 1;
+  const int q_abs = prefix + w_row + r;  // the lane's position
+  // The wave's tiles: no row of it sees a key of tile w_tiles or a later one.
+  const int w_tiles =
+      w_row < extend_len ? (prefix + min(extend_len, w_row + 16) - 1) / BN + 1 : 0;
 
   // ---- staging. Thread t's pieces i of 16 codes: key t / 8 + 8 NW i, piece t % 8. K's go to the
   // LDS by DMA; V's through registers, where they become bf16 with their scale (once for all
   // waves: converted at every fragment read instead, 64 more conversions and 32 products a wave
-  // and tile). V is loaded two tiles ahead, K one, the slots another. No branch guards a load (past
-  // the sequence's end its last key is read again): a load in a branch is waited for where the
-  // branch ends, and the tile's DMA with it.
+  // and tile). During tile t's step K of t + 2 and V of t + 1 load, the scales of t + 3 and the
+  // slots of t + 4. No branch guards a load with a register result (past the sequence's end its
+  // last key is read again): such a load is waited for where the branch ends, and the tile's DMA
+  // with it.
   constexpr int KP = 8 / NW;
   const int32_t* idx = kv_indices + kv_start;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char_t)lds));
@@ -284,100 +297,103 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   const uint8_t* kb = k_cache + h_kv * D;
   const uint8_t* vb = v_cache + h_kv * D;
   const uint16_t* sb = kv_scales + h_kv;
-  struct Slots {
-    uint32_t s[KP];
+  struct PerKey {
+    uint32_t x[KP];
   };
   auto load_slots = [&](int tile) {
-    Slots v;
-#pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      v.s[i] = idx[min(tile * BN + (tid >> 3) + 8 * NW * i, kv_len - 1)];
-    }
-    return v;
-  };
-  // Out of range: slot 0. (Looked at where a slot is used: at its load, it would be waited for.)
-  auto checked = [&](uint32_t slot) { return static_cast<uint64_t>(slot < max_slots ? slot : 0); };
-  const uint32_t row_bytes = static_cast<uint32_t>(num_kv_heads) * D;
-  const uint8_t* ksrc[KP];  // (a thread's pieces differ in their swizzle)
-#pragma unroll
-  for (int i = 0; i < KP; ++i) ksrc[i] = kb + 16 * ((tid & 7) ^ swk((tid >> 3) + 8 * NW * i));
-  const uint8_t* vsrc = vb + 16 * (tid & 7);
-  auto load_k = [&](const Slots& v, int buf) {
+    PerKey v;
 #pragma unroll
     for (int i = 0; i < KP; ++i)
-      dma16(ksrc[i] + checked(v.s[i]) * row_bytes,
+      v.x[i] = idx[min(tile * BN + (tid >> 3) + 8 * NW * i, kv_len - 1)];
+    return v;
+  };
+  // Out of range: slot 0. (Looked at where a slot is used first: at its load, it would be waited
+  // for.)
+  auto check = [&](PerKey& slot) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) slot.x[i] = slot.x[i] < max_slots ? slot.x[i] : 0;
+  };
+  const uint32_t row_bytes = static_cast<uint32_t>(num_kv_heads) * D;
+  // (A thread's key of piece i is 8 NW i after its first, a multiple of 32: the swizzles are the same.)
+  const uint8_t* ksrc = kb + 16 * ((tid & 7) ^ swk(tid >> 3));
+  const uint8_t* vsrc = vb + 16 * (tid & 7);
+  auto load_k = [&](const PerKey& slot, int buf) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      dma16(ksrc + static_cast<uint64_t>(slot.x[i]) * row_bytes,
             lds0 + buf * kKTile + 1024u * (wave + NW * i));
   };
   u32x4_v raw[KP];
-  uint32_t raw_s[KP];  // the keys' scale bytes, K | V << 8
-  auto load_v = [&](const Slots& v) {
+  auto load_v = [&](const PerKey& slot) {
 #pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      raw[i] = *reinterpret_cast<const u32x4_v*>(vsrc + checked(v.s[i]) * row_bytes);
-      raw_s[i] = sb[checked(v.s[i]) * static_cast<uint32_t>(num_kv_heads)];
-    }
+    for (int i = 0; i < KP; ++i)
+      raw[i] = *reinterpret_cast<const u32x4_v*>(vsrc + static_cast<uint64_t>(slot.x[i]) * row_bytes);
+  };
+  auto load_scales = [&](const PerKey& slot) {  // K | V << 8
+    PerKey v;
+#pragma unroll
+    for (int i = 0; i < KP; ++i) 
+      v.x[i] = sb[static_cast<uint64_t>(slot.x[i]) * static_cast<uint32_t>(num_kv_heads)];
+    return v;
   };
   // A NaN vector must reach the queries that see its key and no others, but a hidden key's value
   // is multiplied by p = 0, which leaves a NaN. So a key whose K or V is NaN gets a NaN scale for K
-  // (E8M0's 255: NaN scores, and a hidden key's scores are never used) and values 0; a key past the
-  // sequence's end, which every query hides, values 0 too. One test finds that a wave has neither.
-  // (A thread's key of piece i is 8 NW i after its first: the swizzle of a multiple of 32 keys is the
-  // same, of 64 threads' 32-key step always.)
-  uint32_t vdst = lds0 + kVAt + 256 * (tid >> 3) + 16 * ((2 * (tid & 7)) ^ swz(tid >> 3));
-  asm volatile("" : "+v"(vdst));
-  auto store_v = [&](int tile, auto buf) {
+  // (E8M0's 255: NaN scores, and a hidden key's scores are never used) and values 0. (Branches
+  // would cost more than they skip.)
+  auto store_scales = [&](PerKey& sc, auto buf) {
 #pragma unroll
     for (int i = 0; i < KP; ++i) {
+      sc.x[i] = sc.x[i] >= kScaleNaN << 8 ? 127 << 8 | kScaleNaN : sc.x[i];
       const int key = (tid >> 3) + 8 * NW * i;
-      uint32_t ks = raw_s[i] & 255u, vs = raw_s[i] >> 8;
-      const bool nan = vs == kScaleNaN || ks == kScaleNaN;
-      const bool gone = nan || tile * BN + key >= kv_len;
-      if (__builtin_amdgcn_ballot_w64(gone) != 0) {
-        ks = nan ? kScaleNaN : ks;
-        vs = gone ? 127 : vs;
-        raw[i] = gone ? u32x4_v{0, 0, 0, 0} : raw[i];
-      }
+      const int m = 4 * ((key >> 3) & 3) + (key & 3), j = 2 * (key >> 5) + ((key >> 2) & 1);
+      reinterpret_cast<uint8_t*>(lds + kScalesAt + buf * 64)[4 * m + j] =
+          static_cast<uint8_t>(sc.x[i]);
+    }
+  };
+  // Of a key's 8 threads the last 4 write their second piece first: 8 threads write 128 bytes a
+  // cycle, which have to lie on different banks.
+  const int v_swap = (tid >> 2) & 1;
+  uint32_t vdst = lds0 + kVAt + 256 * (tid >> 3) + 16 * ((2 * (tid & 7) + v_swap) ^ swv(tid >> 3));
+  asm volatile("" : "+v"(vdst));
+  auto store_v = [&](const PerKey& sc, auto buf) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      const bool nan = (sc.x[i] & 255u) == kScaleNaN;
+      u32x4_v c = v_swap ? u32x4_v{raw[i].z, raw[i].w, raw[i].x, raw[i].y} : raw[i];
+      c = nan ? u32x4_v{0, 0, 0, 0} : c;
       u32x4_v v[2];
-      unpack16(raw[i], vs, v);
+      unpack16(c, sc.x[i] >> 8, v);
       typedef __attribute__((address_space(3))) u32x4_v* lds_w_t;
       *(lds_w_t)(vdst + buf * kTileBytes + 256 * 8 * NW * i) = v[0];
       *(lds_w_t)((vdst ^ 16u) + buf * kTileBytes + 256 * 8 * NW * i) = v[1];
-      if ((tid & 7) == 0) {
-        const int m = 4 * ((key >> 3) & 3) + (key & 3), j = 2 * (key >> 5) + ((key >> 2) & 1);
-        reinterpret_cast<uint8_t*>(lds + kScalesAt + buf * 64)[4 * m + j] = static_cast<uint8_t>(ks);
-      }
     }
   };
 
   // The first loads, in the order of their latencies: slots and q, then what the slots name; q is
   // split while those are under way.
-  Slots s1 = load_slots(t_begin), s2 = load_slots(t_begin + 1);
-  QRaw q_raw[HPW];
-#pragma unroll
-  for (int h = 0; h < HPW; ++h) q_raw[h] = load_q(q + (prow + h) * D, lane >> 4);
+  PerKey sl1 = load_slots(t_begin), sl2 = load_slots(t_begin + 1), sl3 = load_slots(t_begin + 2),
+         sl4 = load_slots(t_begin + 3);
+  const QRaw q_raw = load_q(q + prow * D, g);
   __builtin_amdgcn_sched_barrier(0);
-  load_v(s1);
+  check(sl1);
+  check(sl2);
+  check(sl3);
+  PerKey sc0 = load_scales(sl1), sc1 = load_scales(sl2), scales_in = load_scales(sl3);
+  load_v(sl1);
   __builtin_amdgcn_sched_barrier(0);
-  load_k(s1, 0);  // (t_begin is a split's first tile: even)
+  load_k(sl1, 0);  // (t_begin is a split's first tile: even)
+  load_k(sl2, 1);
   __builtin_amdgcn_sched_barrier(0);
-  QRow qf[HPW];
-#pragma unroll
-  for (int h = 0; h < HPW; ++h) qf[h] = split_q(q_raw[h], row_ok);
+  const QRow qf = split_q(q_raw, row_ok);
   __builtin_amdgcn_sched_barrier(0);
-  store_v(t_begin, 0);
-  load_v(s2);
-  s1 = s2;
-  s2 = load_slots(t_begin + 2);
+  store_scales(sc0, 0);
+  store_scales(sc1, 1);
+  sl1 = sl2;
+  sl2 = sl3;
+  sl3 = sl4;
   __builtin_amdgcn_sched_barrier(0);
 
-  RowState run[HPW], st[HPW];
-#pragma unroll
-  for (int h = 0; h < HPW; ++h) {
-    fresh(run[h]);
-    fresh(st[h]);
-  }
   // LDS addresses of a lane's fragments in buffer 0, kept in registers.
-  const int r = lane & 15, g = lane >> 4;
   // S^T = K Q^T: row m of key block j is key 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4, so a lane
   // ends with the scores of keys 8 g .. +7 and 32 + 8 g .. +7 of its query.
   const int key_a0 = 8 * (r >> 2) + (r & 3);
@@ -387,163 +403,287 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   const int key_v = 8 * g + (r >> 2);
 #pragma unroll
   for (int db = 0; db < 8; ++db)
-    va[db] = (lds0 + kVAt + key_v * 256 + 16 * (((r & 3) >> 1) ^ swz(key_v)) + 8 * (r & 1)) ^ (32u * db);
+    va[db] = (lds0 + kVAt + key_v * 256 + 16 * (((r & 3) >> 1) ^ swv(key_v)) + 8 * (r & 1)) ^ (32u * db);
 #pragma unroll
   for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(va[i]));
   asm volatile("" : "+v"(ka[0]), "+v"(ka[1]), "+v"(sa));
-  // One tile's math out of LDS buffer `buf`. MASK: some key is hidden from some row.
-  auto tile_math = [&](auto mask, int t0, auto buf) {
-    typedef __attribute__((address_space(3))) const u32x4_v* lds_u4_t;
-    const int ks = *(__attribute__((address_space(3))) const int*)(sa + 64 * buf);
-    f32x4_v s4[HPW][4];
-    i32x8_v kf[4];
+
+  // A step takes the softmax of its tile t between the products of two others: S of tile t + 1 (qk)
+  // and the output of tile t - 1 (pv), so that no product waits for this tile's exponentials nor
+  // they for it. The softmax is dealt over 8 slices of 2 elements; with them go qk n: key block
+  // n / 2, q's hi part, then its lo part (two in each of the first 4 slices: their results are the
+  // first that the next step needs), and pv n: key half n / 4, dim blocks 2 (n % 4) and the next.
+  // (Products and softmax of one tile in turn: 4 windows of 32 over 2048 keys 22.9 us instead of
+  // 20.5, 1 x 8192 tokens 349 instead of 330.)
+  typedef __attribute__((address_space(3))) const u32x4_v* lds_u4_t;
+  typedef __attribute__((address_space(3))) s16x4_v* tr_ptr_t;
+  i32x8_v kf[2];
+  s16x4_v vw[2][4][2];
+  f32x4_v next[4];  // S of the next tile
+  float s[16];      // S of this one: key 8 g + i, or 32 + 8 g + i - 8
+  uint4 pn[2];      // P of this tile, and of the one before
+  bf16x8_v pf[2];
+  float m = NEG_BIG, l = 0.0f;  // (l: this lane's 16 keys of every tile)
+  f32x4_v acc[8];
+  float run_m = NEG_BIG, run_l = 0.0f;
+  f32x4_v run_top = {0.0f, 0.0f, 0.0f, 0.0f};
+  typedef __attribute__((address_space(3))) f32x4_v* park_t;
+  const park_t parked = (park_t)(lds0 + kParkedAt + 16 * tid);  // vector i: + 64 NW i
+  if constexpr (!FANOUT) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t at = buf * kKTile + (32 * (j >> 1) + 4 * (j & 1)) * D;  // (swk is the same for all j)
-      const u32x4_v k0 = *(lds_u4_t)(ka[0] + at);
-      const u32x4_v k1 = *(lds_u4_t)(ka[1] + at);
-      kf[j] = i32x8_v{(int)k0.x, (int)k0.y, (int)k0.z, (int)k0.w,
-                      (int)k1.x, (int)k1.y, (int)k1.z, (int)k1.w};
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    // (the scale operands' byte is an immediate: key block j of ks, part P of the row's scale)
-#define SID_QK(J, P, PART, C)                                                                   \
-  _Pragma("unroll") for (int h = 0; h < HPW; ++h)                                               \
-      s4[h][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[J], qf[h].PART, C, 0, 0, J, \
-                                                                  ks, P, qf[h].scale)
-    const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    SID_QK(0, 0, hi, zero); SID_QK(1, 0, hi, zero); SID_QK(2, 0, hi, zero); SID_QK(3, 0, hi, zero);
-    SID_QK(0, 1, lo, s4[h][0]); SID_QK(1, 1, lo, s4[h][1]); SID_QK(2, 1, lo, s4[h][2]);
-    SID_QK(3, 1, lo, s4[h][3]);
-#undef SID_QK
-    // V fragments: A = V^T rows 16 db + r (dims), columns 32 kb + 8 g .. +7 (keys), by two
-    // transpose reads (extend_attention.hip). They go out in groups of 4, each before the products
-    // of the one before it, the first before the softmax.
-    typedef __attribute__((address_space(3))) s16x4_v* tr_ptr_t;
-    s16x4_v vw[2][4][2];
-    auto read_v = [&](int n) {  // group n: key half n / 2, dim blocks 4 (n % 2) .. +3
+    for (int i = 0; i < kParked; ++i) parked[64 * NW * i] = run_top;
+  }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t p = va[4 * (n & 1) + i] + buf * kTileBytes + 8192 * (n >> 1);
-        vw[n & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)p);
-        vw[n & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(p + 1024));
-      }
-    };
-    read_v(0);
-    __builtin_amdgcn_sched_barrier(0);
-    const RowCtx c{g, w_first + r, row_ok};
-    bf16x8_v pf[HPW][2];
-    float rescale[HPW];
-    bool moved = false;
+  for (int db = 0; db < 8; ++db) acc[db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
+  pf[0] = pf[1] = bf16x8_v{};
+  auto read_k = [&](auto j_, auto buf) {
+    constexpr int j = decltype(j_)::value;
+    const uint32_t at = buf * kKTile + (32 * (j >> 1) + 4 * (j & 1)) * D;  // (swk is the same for all j)
+    const u32x4_v k0 = *(lds_u4_t)(ka[0] + at);
+    const u32x4_v k1 = *(lds_u4_t)(ka[1] + at);
+    kf[j & 1] = i32x8_v{(int)k0.x, (int)k0.y, (int)k0.z, (int)k0.w,
+                    (int)k1.x, (int)k1.y, (int)k1.z, (int)k1.w};
+  };
+  // V fragments: A = V^T rows 16 db + r (dims), columns 32 kb + 8 g .. +7 (keys), by two
+  // transpose reads (extend_attention.hip). They go out in groups of 4, each before the products
+  // of the one before it.
+  auto read_v = [&](auto n_, auto buf) {  // group n: key half n / 2, dim blocks 4 (n % 2) .. +3
+    constexpr int n = decltype(n_)::value;
 #pragma unroll
-    for (int h = 0; h < HPW; ++h) {  // (no branch between the heads: their chains interleave)
-      float s[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = s4[h][i >> 2][i & 3];
-      rescale[h] = softmax_tile<decltype(mask)::value>(s, st[h], c, t0, sc2);
-      moved |= rescale[h] != 1.0f;
-      pack_p(pf[h], s);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    // x * 1 == x: skipped (same bits) unless some row of the wave moved its reference maximum.
-    if (__builtin_amdgcn_ballot_w64(moved) != 0) {
-#pragma unroll
-      for (int h = 0; h < HPW; ++h)
-#pragma unroll
-        for (int db = 0; db < 8; ++db)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st[h].acc[db][i] *= rescale[h];
-    }
-    // O^T += V^T P^T
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      if (n < 3) read_v(n + 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int db = 4 * (n & 1) + i;
-        const bf16x8_v vf = __builtin_bit_cast(
-            bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(
-                          vw[n & 1][i][0], vw[n & 1][i][1], 0, 1, 2, 3, 4, 5, 6, 7)));
-#pragma unroll
-        for (int h = 0; h < HPW; ++h)
-          st[h].acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[h][n >> 1], st[h].acc[db], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = va[4 * (n & 1) + i] + buf * kTileBytes + 8192 * (n >> 1);
+      vw[n & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
+      vw[n & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 1024));
     }
   };
-
-  auto step = [&](auto mask, int t, auto buf) {  // buf: t & 1
-    // Every load has landed (they had a whole tile's time) and every wave is done with the other
-    // buffers.
+  auto qk = [&](auto n_, int ks) {
+    constexpr int n = decltype(n_)::value, j = n >> 1;
+    constexpr bool lo = (n & 1) != 0;
+    // (the scale operands' byte is an immediate: key block j of ks, hi or lo of the row's scale)
+    if constexpr (lo)
+      next[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[j & 1], qf.lo, next[j], 0, 0, j, ks, 1, qf.scale);
+    else
+      next[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          kf[j & 1], qf.hi, f32x4_v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, j, ks, 0, qf.scale);
+  };
+  auto pv = [&](auto n_) {
+    constexpr int n = decltype(n_)::value;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int w = 2 * (n & 1) + i;
+      const bf16x8_v vf = __builtin_bit_cast(
+          bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(
+                        vw[(n >> 1) & 1][w][0], vw[(n >> 1) & 1][w][1], 0, 1, 2, 3, 4, 5, 6, 7)));
+      f32x4_v& a = acc[2 * (n & 3) + i];
+      a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n >> 2], a, 0, 0, 0);
+    }
+  };
+  auto take_scores = [&] {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = next[i >> 2][i & 3];
+  };
+  auto each = [](auto f) {  // f(0) .. f(7), as constants
+    f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{});
+    f(std::integral_constant<int, 2>{}); f(std::integral_constant<int, 3>{});
+    f(std::integral_constant<int, 4>{}); f(std::integral_constant<int, 5>{});
+    f(std::integral_constant<int, 6>{}); f(std::integral_constant<int, 7>{});
+  };
+  typedef std::integral_constant<int, 0> c0;
+  typedef std::integral_constant<int, 1> c1;
+  typedef std::integral_constant<int, 2> c2;
+  typedef std::integral_constant<int, 3> c3;
+  auto barrier = [&] {
+    // Every load has landed (they had a whole tile's time) and every wave is done with the buffers
+    // that are written next.
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 < t_end) {
-#pragma unroll
-      for (int i = 0; i < KP; ++i)  // (not converted ahead of the barrier)
-        asm volatile("" : "+v"(raw[i]), "+v"(raw_s[i]));
-      store_v(t + 1, other(buf));
-      const Slots k_at = s1;
-      s1 = s2;
-      load_v(s2);
-      s2 = load_slots(t + 3);
-      __builtin_amdgcn_sched_barrier(0);
-      load_k(k_at, 1 - buf);  // last: a wait for an earlier load would include the DMA
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (decltype(mask)::value) {
-      // A tile past the wave's last row is left out.
-      if (t * BN > w_last || w_row >= extend_len) return;
-    }
-    tile_math(mask, t * BN, buf);
   };
+  auto fold_split = [&](float om, float ol) {  // the state of a split that is complete
+    const FoldScale f = fold_scale(run_m, om);
+    run_l = fold_elem(run_l, pair32_sum(pair16_sum(ol)), f);
+    run_m = f.mn;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      f32x4_v a = db < kParked ? parked[64 * NW * db] : run_top;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = fold_elem(a[i], acc[db][i], f);
+      if (db < kParked) parked[64 * NW * db] = a;
+      else run_top = a;
+    }
+  };
+
+  // Tile t's step; buf: t & 1. MASK: some key of it may be hidden from some row. FIRST: of a split.
+  auto step = [&](auto mask, auto first, int t, auto buf) {
+    constexpr bool kMask = decltype(mask)::value, kFirst = decltype(first)::value;
+    barrier();
+    const bool mine = !kMask || t <= w_tiles;  // (at w_tiles the tile before is still to be added)
+    int ks = 0;
+    if (mine) {
+      ks = *(__attribute__((address_space(3))) const int*)(sa + 64 * other(buf));
+      read_v(c0{}, other(buf));
+      read_k(c0{}, other(buf));
+      read_k(c1{}, other(buf));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < KP; ++i)  // (not converted ahead of the barrier)
+      asm volatile("" : "+v"(raw[i]), "+v"(sc0.x[i]), "+v"(scales_in.x[i]));
+    store_v(sc0, buf);
+    store_scales(scales_in, buf);
+    sc0 = sc1;
+    sc1 = scales_in;
+    load_v(sl1);
+    check(sl3);
+    scales_in = load_scales(sl3);
+    const PerKey k_at = sl2;
+    sl1 = sl2;
+    sl2 = sl3;
+    sl3 = load_slots(t + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 2 < t_end) load_k(k_at, buf);  // last: a wait for an earlier load would include the DMA
+    __builtin_amdgcn_sched_barrier(0);
+    if (!mine) return;
+    const float om = m, ol = l;
+    if constexpr (kFirst) {
+      m = NEG_BIG;
+      l = 0.0f;
+    }
+    bool vis[16];
+    float tmax = NEG_BIG;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (kMask) {
+        vis[i] = (t * BN + 32 * (i >> 3) + 8 * g + (i & 7) <= q_abs) & row_ok;
+        tmax = fmaxf(tmax, vis[i] ? s[i] : NEG_BIG);
+      } else {
+        tmax = fmaxf(tmax, s[i]);
+      }
+    }
+    // Each lane looks at its own 16 scores: only where one of them is LAZY_T above its row's
+    // reference maximum (seldom, but for a split's first tile) is the row's maximum taken.
+    const bool moved = kFirst || __builtin_amdgcn_ballot_w64(tmax * sc2 > m + LAZY_T) != 0;
+    float rescale = 1.0f;
+    if (moved) {
+      const float mc = pair32_max(pair16_max(tmax)) * sc2;
+      const float m_used = mc > m + LAZY_T ? mc : m;
+      rescale = exp2_fast(m - m_used);
+      m = m_used;
+      if constexpr (!kFirst) l *= rescale;
+    }
+    each([&](auto n_) {
+      constexpr int n = decltype(n_)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n < 4) qk(std::integral_constant<int, 2 * (n & 3)>{}, ks);
+      if constexpr (n == 0) read_v(c1{}, other(buf));
+      if constexpr (n == 1) read_k(c2{}, other(buf));
+      if constexpr (n == 2) read_k(c3{}, other(buf));
+      if constexpr (n == 2) read_v(c2{}, other(buf));
+      if constexpr (n == 4) read_v(c3{}, other(buf));
+      float p[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        p[i] = exp2_fast(__builtin_fmaf(s[2 * n + i], sc2, -m));
+        if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
+        l += p[i];
+      }
+      reinterpret_cast<uint32_t*>(&pn[n >> 2])[n & 3] = pack_bf16x2(p[0], p[1]);
+      pv(n_);
+      if constexpr (n < 4) qk(std::integral_constant<int, 2 * (n & 3) + 1>{}, ks);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    // (here, not where the next step uses them: past the branches below they would move there)
+    asm volatile("" : "+v"(next[0]), "+v"(next[1]), "+v"(next[2]), "+v"(next[3]));
+    asm volatile("" : "+v"(l), "+v"(pn[0].x), "+v"(pn[0].y), "+v"(pn[0].z), "+v"(pn[0].w),
+                 "+v"(pn[1].x), "+v"(pn[1].y), "+v"(pn[1].z), "+v"(pn[1].w));
+    if constexpr (kFirst) {
+      // (before the first split: nothing, times what lay in the LDS)
+      if (!FANOUT && t > t_begin) fold_split(om, ol);
+#pragma unroll
+      for (int db = 0; db < 8; ++db) acc[db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
+    } else if (moved) {  // (x * 1 == x for the rows that did not)
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[db][i] *= rescale;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pf[i] = __builtin_bit_cast(bf16x8_v, pn[i]);
+    take_scores();
+  };
+
+  // S of the first tile.
+  barrier();
+  {
+    const int ks = *(__attribute__((address_space(3))) const int*)sa;
+    read_k(c0{}, c0{});
+    each([&](auto n_) {
+      constexpr int n = decltype(n_)::value;
+      if constexpr (n < 6 && n % 2 == 0) read_k(std::integral_constant<int, n / 2 + 1>{}, c0{});
+      qk(n_, ks);
+    });
+    take_scores();
+  }
   // Tiles that every row of the workgroup sees whole, in pairs (their buffers' addresses are
   // immediates), then the others with the mask: one loop each, split by split (a branch between
   // the kinds in one loop, or the fold in it, costs a copy of the accumulators each turn).
   const int t_full = (prefix + mtile * ROWS + 1) / BN;
-  for (int s0 = t_begin; s0 < t_end; s0 += kSplit / BN) {
-    const int s_end = min(s0 + kSplit / BN, t_end);
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  for (int s0 = t_begin; s0 < t_end; s0 += kSplitTiles) {
+    const int s_end = min(s0 + kSplitTiles, t_end), e = min(s_end, t_full);
     int t = s0;
-    for (const int e = min(s_end, t_full); t + 1 < e; t += 2) {
-      step(std::false_type{}, t, std::integral_constant<int, 0>{});
-      step(std::false_type{}, t + 1, std::integral_constant<int, 1>{});
+    if (t < e) step(no, yes, t, c0{});
+    else step(yes, yes, t, c0{});
+    ++t;
+    for (; t + 1 < e; t += 2) {
+      step(no, no, t, c1{});
+      step(no, no, t + 1, c0{});
     }
-    for (; t < s_end; ++t) step(std::true_type{}, t, t & 1);
-    if constexpr (!FANOUT) {
-#pragma unroll
-      for (int h = 0; h < HPW; ++h) {
-        fold(run[h], st[h].m, st[h].l, st[h].acc);
-        fresh(st[h]);
-      }
-    }
+    if (t < e) step(no, no, t++, c1{});
+    for (; t < s_end; ++t) step(yes, no, t, t & 1);
   }
-  if (!row_ok) return;
+  // The last tile's output. (Its wave skips no P: a wave without that tile has P = 0.)
+  barrier();
+  {
+    const int buf = (t_end - 1) & 1;
+    read_v(c0{}, buf);
+    each([&](auto n_) {
+      constexpr int n = decltype(n_)::value;
+      if constexpr (n == 0) read_v(c1{}, buf);
+      if constexpr (n == 2) read_v(c2{}, buf);
+      if constexpr (n == 4) read_v(c3{}, buf);
+      __builtin_amdgcn_sched_barrier(0);
+      pv(n_);
+    });
+  }
+  if constexpr (FANOUT) {
+    l = pair32_sum(pair16_sum(l));
+    if (!row_ok) return;
+    const int64_t pr = split * items + prow;
 #pragma unroll
-  for (int h = 0; h < HPW; ++h) {
-    if constexpr (FANOUT) {
-      const int64_t pr = split * items + prow + h;
-      const int g = lane >> 4;
-#pragma unroll
-      for (int db = 0; db < 8; ++db)
-        *reinterpret_cast<f32x4_v*>(part_a + pr * D + 16 * db + 4 * g) = st[h].acc[db];
-      if (g == 0) {
-        part_ml[2 * pr] = st[h].m;
-        part_ml[2 * pr + 1] = st[h].l;
-        if (split == 0) part_n[prow + h] = nsplits;
-      }
-    } else {
-      store_row(o + (prow + h) * D, run[h], lane >> 4);
+    for (int db = 0; db < 8; ++db)
+      *reinterpret_cast<f32x4_v*>(part_a + pr * D + 16 * db + 4 * g) = acc[db];
+    if (g == 0) {
+      part_ml[2 * pr] = m;
+      part_ml[2 * pr + 1] = l;
+      if (split == 0) part_n[prow] = nsplits;
     }
+  } else {
+    fold_split(m, l);
+    RowState run{run_m, run_l, {}};
+#pragma unroll
+    for (int db = 0; db < 8; ++db) run.acc[db] = db < kParked ? parked[64 * NW * db] : run_top;
+    if (row_ok) store_row(o + prow * D, run, g);
   }
 }
 
 // Whether a grid of fewer than 512 workgroups fans out. Walking its keys in one workgroup takes about
 // 6 + 1.1 us a tile; fanned out, the launches take 18 us and the saved states of total_q rows in
-// every split 8.5 us a thousand. Walked and fanned out, us: 1 x 512 tokens 14 and 24, 1 x 1024 23 and
-// 40, 2 x 500 over 2000 49 and 69, 4 x 200 over 1000 28 and 36, 1 x 700 over 4000 82 and 78, 16 x 32
-// over 2048 42 and 38, 8 x 64 over 3000 57 and 44, 4 x 32 over 2048 40 and 22, 1 x 256 over 8000 138
-// and 56.
+// every split 8.5 us a thousand. Walked and fanned out, us: 1 x 512 tokens 14 and 23, 1 x 1024 23 and
+// 38, 2 x 500 over 2000 48 and 66, 4 x 200 over 1000 27 and 35, 1 x 700 over 4000 76 and 78, 16 x 32
+// over 2048 40 and 35, 8 x 64 over 3000 53 and 40, 4 x 32 over 2048 39 and 20, 1 x 256 over 8000 126
+// and 55.
 bool fans_out(int batch, int64_t total_q, int num_kv_heads, int max_extend_len, int max_kv_len) {
   const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * ceil_div(max_extend_len, BQ);
   const int64_t states = total_q * ceil_div(max_kv_len, kSplit);
@@ -593,7 +733,7 @@ extern "C" int sid_extend_attention_fp8_fwd(
                        max_kv_len > max_extend_len);
   const int per_round = p.rows == 32 ? max(1, cu_count() / num_kv_heads) : 0;
   auto launch = [&](auto kern, int nw, dim3 grid, int mtiles) {
-    hipLaunchKernelGGL(kern, grid, dim3(nw * 64), kLdsBytes, s, (const bf16_t*)q,
+    hipLaunchKernelGGL(kern, grid, dim3(nw * 64), 0, s, (const bf16_t*)q,
                        (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint16_t*)kv_scales, qo_indptr, kv_indptr, kv_indices, batch,
                        num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, per_round, ordered, p.items,
@@ -601,13 +741,13 @@ extern "C" int sid_extend_attention_fp8_fwd(
     return check_launch(name);
   };
   if (p.fanout) {
-    const int rc = launch(extend_fp8_kernel<4, 1, true>, 4,
+    const int rc = launch(extend_fp8_kernel<4, true>, 4,
                           dim3(batch, num_kv_heads, p.mtiles * p.splits), p.mtiles);
     return rc != SID_OK ? rc : extend_merge(name, p, o, s);
   }
   const int mtiles = ceil_div(max_extend_len, p.rows);
   const int64_t groups = static_cast<int64_t>(batch) * mtiles * num_kv_heads;
   SID_REQUIRE(groups < (1ll << 31) / (64 * 8), "%s: grid too large", name);
-  return p.rows == 64 ? launch(extend_fp8_kernel<8, 1, false>, 8, dim3(groups), mtiles)
-                      : launch(extend_fp8_kernel<4, 1, false>, 4, dim3(groups), mtiles);
+  return p.rows == 64 ? launch(extend_fp8_kernel<8, false>, 8, dim3(groups), mtiles)
+                      : launch(extend_fp8_kernel<4, false>, 4, dim3(groups), mtiles);
 }
