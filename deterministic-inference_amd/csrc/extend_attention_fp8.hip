@@ -5,10 +5,10 @@
 // differs is how the products get their operands: K's codes lie in the LDS as they are and S = K
 // Q^T is taken on them, with q as two e4m3 vectors; V's become bf16 on their way into the LDS.
 //
-// Bound: 4 operations for each of a query's keys and dims. 1 x 8192 tokens 330 us, 0.83 PFLOP/s;
-// 4 x 2048 114 us, 0.60, a third of which is the workgroups' first loads and last stores (one of 8
+// Bound: 4 operations for each of a query's keys and dims. 1 x 8192 tokens 323 us, 0.85 PFLOP/s;
+// 4 x 2048 111 us, 0.62, a third of which is the workgroups' first loads and last stores (one of 8
 // waves fills a CU); the 2-byte pool's kernel 420 and 133 us. The matrix products are 1024 of a
-// tile's 2900 cycles on a SIMD (two waves, 24 products each); the rest is a wave's own chain, V's
+// tile's 2800 cycles on a SIMD (two waves, 24 products each); the rest is a wave's own chain, V's
 // conversion, the softmax and the loads' addresses, which two waves that start a tile at the same
 // barrier overlap only in part. It is not the LDS (896 cycles a tile of 8 waves, no bank
 // conflicts) nor the count of vector operations (a third fewer: 2%).
@@ -571,6 +571,10 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
       m = m_used;
       if constexpr (!kFirst) l *= rescale;
     }
+    // (A wave with products to issue goes first: of two waves on a SIMD one is ahead, and its products
+    // run beside the other's conversions and loads. 5 ragged chunks 108 -> 101 us, 1 x 8192 tokens
+    // 330 -> 323.)
+    __builtin_amdgcn_s_setprio(1);
     each([&](auto n_) {
       constexpr int n = decltype(n_)::value;
       __builtin_amdgcn_sched_barrier(0);
@@ -592,6 +596,7 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
       if constexpr (n < 4) qk(std::integral_constant<int, 2 * (n & 3) + 1>{}, ks);
     });
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     // (here, not where the next step uses them: past the branches below they would move there)
     asm volatile("" : "+v"(next[0]), "+v"(next[1]), "+v"(next[2]), "+v"(next[3]));
     asm volatile("" : "+v"(l), "+v"(pn[0].x), "+v"(pn[0].y), "+v"(pn[0].z), "+v"(pn[0].w),
