@@ -255,10 +255,10 @@ def plan_variant(lengths, max_len: int, num_kv_heads: int, cu_count: int, max_kv
 # workgroup fills its CU, and the next one's start costs 70 tokens, where 4 x 4 ones start next
 # to each other and cost 30; a partial slot adds a token's time to the merge. Fitted to 24 batches
 # (B = 1-256, uniform and ragged, lengths 20-8192; every segment size and both shapes, graph
-# timed with rotated pools): the plan of least estimate is 1.5% from the fastest of a batch on
-# average, 5% at worst, where the 2-byte pool's rules are 9% and up to 26% from it (128
-# requests of 4096 190.8 -> 171.2 us, 64 of 128-4096 73.4 -> 69.2, 8 of 100-8000 31.1 -> 24.7,
-# 256 of 20-300 30.2 -> 24.7).
+# timed with rotated pools), where the plan of least estimate is 1.5% from the fastest of a
+# batch on average and 5% at worst, and checked on 16 others: 3% and 13%. The 2-byte pool's rules
+# are 8% and up to 26% from the fastest of the 24 (128 requests of 4096 190.8 -> 171.2 us, 64 of
+# 128-4096 73.4 -> 69.2, 8 of 100-8000 31.1 -> 24.7, 256 of 20-300 30.2 -> 24.7).
 FP8_SEGMENTS = (2048, 1024, 512, 256, 128, 64, 32)
 FP8_SHAPES = ((2, 0.57, 70, 1), (3, 0.64, 30, 0))  # variant, a, r, cost of its own merge
 FP8_MAX_PER_CU = 6  # more workgroups than this a CU are never the fastest

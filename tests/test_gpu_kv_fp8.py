@@ -333,7 +333,8 @@ def test_decode_against_oracle(lens, variant, plan):
 
 
 @pytest.mark.parametrize("lens", [[1], [1024], [300] * 5 + [1], [2000, 64, 7, 900] * 8,
-                                  [700 + i for i in range(96)], [40] * 256], ids=lambda s: f"b{len(s)}")
+                                  [700 + i for i in range(96)], [40] * 256,
+                                  [128 + 63 * i for i in range(64)]], ids=lambda s: f"b{len(s)}")
 def test_decode_step_plan(lens):
     """The plan that a serving loop makes (shape, geometry, order, workers) over paged slots."""
     from sid.kernels.decode_attention import DecodeAttention
@@ -523,6 +524,72 @@ def test_chunk_nan_reaches_only_rows_that_see_it(specs, which):
     hit[37:int(qoh[1]), 2 * head:2 * head + 2] = True
     assert o[hit].isnan().all()
     assert torch.equal(o[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("which", [0, 1], ids=["nan_k", "nan_v"])
+@pytest.mark.parametrize("specs,key", [([(100, 70)], 169), ([(100, 70)], 128), ([(5, 1200)] * 4, 1204),
+                                       ([(5, 1200)] * 4, 512)],
+                         ids=["fanout_last", "fanout_tile", "grid_last", "grid_split"])
+def test_chunk_nan_in_the_last_key_and_at_edges(specs, key, which):
+    """The last key, which stands in for the keys past the sequence's end, and a tile's and a
+    split's first."""
+    q, pool, qo, ptr, idx, at, qoh = _chunk_batch(specs, seed=21)
+    clean = _chunk(q, pool, qo, ptr, idx, specs)
+    pool[which].view(torch.uint8)[int(at[0][key]), 3] = 0x7f
+    pool[2].view(torch.uint8)[int(at[0][key]), 3, which] = 255
+    o = _chunk(q, pool, qo, ptr, idx, specs)
+    hit = torch.zeros(o.shape, dtype=torch.bool, device="cuda")
+    hit[max(0, key - specs[0][0]):int(qoh[1]), 6:8] = True
+    assert o[hit].isnan().all()
+    assert torch.equal(o[~hit], clean[~hit])
+
+
+def _ramp(lens, seed, up):
+    """A pool whose scores rise (or fall) by about 12 octaves of exp every 64 positions, and
+    queries for it: every tile moves its rows' maxima (or none but the first does)."""
+    g = torch.Generator().manual_seed(seed)
+    _, ptr, idx, at = _batch(lens, seed=seed, page=16)
+    size = int(idx.max()) + 17
+    w = torch.randn(HKV, D, generator=g)
+    x = torch.randn(2, size, HKV, D, generator=g)
+    for a in at:
+        pos = torch.arange(len(a), dtype=torch.float32)
+        x[0, torch.from_numpy(a)] += (pos if up else -pos)[:, None, None] * w / 87.0
+    pool, vals, bytes_ = [], [], []
+    for s in (0, 1):
+        codes, b = store_ref(x[s].to(torch.bfloat16).double().numpy())
+        pool.append(torch.from_numpy(codes).cuda().view(FP8))
+        bytes_.append(b)
+        vals.append(load_ref(codes, b))
+    scales = torch.from_numpy(np.stack(bytes_, -1)).cuda().view(E8M0)
+
+    def queries(n):
+        q = torch.randn(n, HQ, D, generator=g) * 0.3 + w.repeat_interleave(2, 0)
+        return q.to(torch.bfloat16).cuda()
+    return (pool[0], pool[1], scales, *vals), ptr, idx, at, queries
+
+
+@pytest.mark.parametrize("up", [True, False], ids=["rising", "falling"])
+@pytest.mark.parametrize("workspace", [True, False])
+def test_chunk_scores_that_move_every_tile(up, workspace):
+    specs = [(0, 130), (700, 50), (1000, 40)]
+    pool, ptr, idx, at, queries = _ramp([p + e for p, e in specs], 5, up)
+    qoh = np.concatenate([[0], np.cumsum([e for _, e in specs])])
+    q = queries(int(qoh[-1]))
+    o = _chunk(q, pool, _i32(qoh.tolist()), ptr, idx, specs, workspace)
+    for i, (p, e) in enumerate(specs):
+        a, b = int(qoh[i]), int(qoh[i + 1])
+        _bounded(o[a:b], q[a:b], pool[3][at[i]], pool[4][at[i]], first=p, chunk=True)
+
+
+@pytest.mark.parametrize("up", [True, False], ids=["rising", "falling"])
+@pytest.mark.parametrize("variant", [2, 3])
+def test_decode_scores_that_move_every_tile(up, variant):
+    lens = [1, 70, 500, 1300]
+    pool, ptr, idx, at, queries = _ramp(lens, 6, up)
+    q = queries(len(lens))
+    for args in ((1, 0, 0, 1), (1, 0, 256, 6)):
+        _check_decode(_decode(q, pool, ptr, idx, *args, variant), q, pool, at)
 
 
 def test_chunk_unwritten_slot_zero_and_tail_rows_untouched():
