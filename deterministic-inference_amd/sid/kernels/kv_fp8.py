@@ -56,5 +56,6 @@ def gather_cache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: to
     n, hkv, d = slots.numel(), shape[1], shape[2]
     # one allocation for both (an eager call of a few rows is bound by the host)
     k, v = torch.empty((2, n, hkv, d), dtype=torch.bfloat16, device=slots.device).unbind(0)
-    load_ext().gather_cache_fp8(k_cache, v_cache, kv_scales, slots.reshape(-1), k, v)
+    flat = slots if slots.dim() == 1 else slots.reshape(-1)
+    load_ext().gather_cache_fp8(k_cache, v_cache, kv_scales, flat, k, v)
     return k, v
