@@ -721,15 +721,14 @@ extern "C" int sid_rmsnorm_qkv_post(const void* src, int src_fp32, const void* n
                          max_positions, slots, q_out, k_cache, v_cache, nullptr, num_slots, stream);
 }
 
-extern "C" int sid_rmsnorm_qkv_post_fp8(const void* src, int src_fp32, const void* norm_w, float eps,
-                                    const void* w_qkv, int64_t m, int64_t hidden,
-                                    int num_q_heads, int num_kv_heads, int head_dim,
-                                    const void* q_norm, const void* k_norm,
-                                    const int64_t* positions, const float* cos_sin,
-                                    int64_t max_positions, const int64_t* slots, void* q_out,
-                                    void* k_cache, void* v_cache, void* kv_scales,
-                                        int64_t num_slots,
-                                    void* stream) {
+extern "C" int sid_rmsnorm_qkv_post_fp8(const void* src, int src_fp32, const void* norm_w,
+                                        float eps, const void* w_qkv, int64_t m, int64_t hidden,
+                                        int num_q_heads, int num_kv_heads, int head_dim,
+                                        const void* q_norm, const void* k_norm,
+                                        const int64_t* positions, const float* cos_sin,
+                                        int64_t max_positions, const int64_t* slots, void* q_out,
+                                        void* k_cache, void* v_cache, void* kv_scales,
+                                        int64_t num_slots, void* stream) {
   SID_REQUIRE(m >= 0 && hidden >= 0, "rmsnorm_qkv_post_fp8: negative size");
   if (m == 0) return SID_OK;
   SID_REQUIRE(kv_scales != nullptr, "rmsnorm_qkv_post_fp8: null pointer");

@@ -153,15 +153,17 @@ WIDE_TOKENS_PER_LONGEST = 170  # the longest workgroup holds <= 1/170 of the bat
 WIDE_MAX_IMBALANCE = 1.3     # busiest CU / mean CU load, once they cover every CU
 
 
-def _busiest_cu(sizes: np.ndarray, cu_count: int) -> int:
+def _busiest_cu(sizes: np.ndarray, cu_count: int, start: int = 0) -> int:
     """The busiest CU's tokens when `sizes` (workgroup tokens) are dealt heaviest first, every
-    other round reversed, as workgroup_order deals them."""
+    other round reversed, as workgroup_order deals them; start: what a CU's second and later
+    workgroups cost beside theirs."""
     w = np.sort(sizes[sizes > 0])[::-1]
     if w.size == 0:
         return 0
     rounds = _cdiv(w.size, cu_count)
     m = np.zeros(rounds * cu_count, dtype=np.int64)
     m[:w.size] = w
+    m[cu_count:w.size] += start
     m = m.reshape(rounds, cu_count)
     m[1::2] = m[1::2, ::-1]
     return int(m.sum(axis=0).max())
@@ -249,18 +251,23 @@ def plan_variant(lengths, max_len: int, num_kv_heads: int, cu_count: int, max_kv
 # the CU's share of the memory's rate, and what decides is how evenly the tokens lie on the CUs
 # and how many workgroups start behind another. With a token's time at that share (2 KiB at a
 # 256th of 6.4 TB/s, 80 ns) as the unit, stage 1 takes about
-#     mean + a (max - mean) + r max(workgroups / CUs - 1, 0) + slots
-# mean and max being a CU's tokens when they are dealt heaviest first: a CU left with tokens
-# when the others are done runs them at 0.57 (8 x 4) or 0.64 (4 x 4) of that time each; an 8 x 4
-# workgroup fills its CU, and the next one's start costs 70 tokens, where 4 x 4 ones start next
-# to each other and cost 30; a partial slot adds a token's time to the merge. Fitted to 24 batches
-# (B = 1-256, uniform and ragged, lengths 20-8192; every segment size and both shapes, graph
-# timed with rotated pools), where the plan of least estimate is 1.5% from the fastest of a
-# batch on average and 5% at worst, and checked on 16 others: 3% and 13%. The 2-byte pool's rules
-# are 8% and up to 26% from the fastest of the 24 (128 requests of 4096 190.8 -> 171.2 us, 64 of
-# 128-4096 73.4 -> 69.2, 8 of 100-8000 31.1 -> 24.7, 256 of 20-300 30.2 -> 24.7).
+#     mean + a (busiest - mean) + r max(workgroups / CUs - 1, 0) + e (empty slots) + merge
+# tokens' times: mean is a CU's tokens, busiest those of the busiest CU when they are dealt heaviest
+# first, with s for each workgroup that starts behind another there. An 8 x 4 workgroup fills its
+# CU, so the next one's whole chain of first loads follows (s = 120, and r = 60 for all); 4 x 4
+# ones start beside each other (15, 20), but a CU that is left with one when the others are done
+# runs it at a = 0.8 of a token's time a token, against 0.5. A slot without tokens costs its
+# workgroup's dispatch, and the merge takes 0.7 of a token's time for each of a request's slots, or,
+# for up to 4 requests, 32 for each 32 slots after the first 32 (1 x 512 with 32 slots 9.5 us, 33
+# 12.1, 64 12.5; 8 x 512 with 16 9.5, 32 10.4, 64 13.4; 128 x 512 with 16 54, 64 71). Fitted to 40
+# batches (B = 1-256, uniform and ragged, lengths 20-9000; every segment size and both shapes,
+# graph timed with rotated pools): the plan of least estimate is 1.3% from the fastest of a batch
+# on average and 11% at worst. Without s it was 2.1%, but chose by a hair between plans 30%
+# apart (32 of 128-4096 38 or 28 us); the 2-byte pool's rules are 8% and up to 26% off (128 requests
+# of 4096 190.8 -> 171.2 us, 64 of 128-4096 73.4 -> 66.1, 8 of 100-8000 31.1 -> 24.7).
 FP8_SEGMENTS = (2048, 1024, 512, 256, 128, 64, 32)
-FP8_SHAPES = ((2, 0.57, 70, 1), (3, 0.64, 30, 0))  # variant, a, r, cost of its own merge
+FP8_SHAPES = ((2, 0.5, 120, 60, 6), (3, 0.8, 15, 20, 0))  # variant, a, s, r, its own merge
+FP8_EMPTY_SLOT = 0.035
 FP8_MAX_PER_CU = 6  # more workgroups than this a CU are never the fastest
 
 
@@ -282,10 +289,12 @@ def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int) -
         sizes = np.concatenate([np.full(int(full.sum()), seg, dtype=np.int64), tail[tail > 0]])
         if best is not None and sizes.size > FP8_MAX_PER_CU * cu_count:
             break
-        longest = _busiest_cu(sizes, cu_count)
         late = max(sizes.size / cu_count - 1.0, 0.0)
-        for variant, a, r, own in FP8_SHAPES:
-            cost = mean + a * (longest - mean) + r * late + slots + own
+        merge = 0.7 * slots if lens.size > 4 else 32 * (_cdiv(slots, 32) - 1) + 0.15 * slots
+        merge += FP8_EMPTY_SLOT * (lens.size * slots - sizes.size)
+        for variant, a, s, r, own in FP8_SHAPES:
+            busiest = _busiest_cu(sizes, cu_count, s)
+            cost = mean + a * (busiest - mean) + r * late + merge + own
             if best is None or cost < best[0]:
                 best = (cost, (1, seg, slots), variant)
     return best[1], best[2]
