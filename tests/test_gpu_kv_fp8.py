@@ -720,6 +720,53 @@ def test_graph_replays_on_another_stream():
         torch.zeros(1 << 20, device="cuda").sum().item()
 
 
+def test_two_graphs_share_the_split_workspace():
+    """Two captured steps of different batches over one pool and one DecodeAttention, replayed in
+    turn with other inputs: each as its eager run."""
+    from sid.kernels.decode_attention import DecodeAttention
+    from sid.kernels.extend_attention import extend_attention_fwd
+    from sid.kernels.ops import qkv_post
+    g = torch.Generator().manual_seed(31)
+    attn = DecodeAttention(5, HQ, HKV, D, 32, 256, 4096, "cuda")
+    pool, ptr, idx, at = _batch([900, 33, 400, 1, 2000], seed=4)
+    kc, vc, sc = pool[:3]
+    norm = (1 + 0.1 * torch.randn(2, D, generator=g)).to(torch.bfloat16).cuda()
+    cos_sin = torch.randn(4096, D, generator=g).cuda()
+
+    def step(pick):
+        lens = [len(at[i]) for i in pick]
+        b = len(pick)
+        p = _i32(np.concatenate([[0], np.cumsum(lens)]).tolist())
+        i = _i32(np.concatenate([at[i] for i in pick]).tolist())
+        slots = torch.tensor([int(at[i][-1]) for i in pick], device="cuda")
+        pos = torch.tensor([n - 1 for n in lens], device="cuda")
+        proj = torch.zeros(b, (HQ + 2 * HKV) * D, dtype=torch.bfloat16, device="cuda")
+        seq, qo, plan = _i32(lens), _i32(list(range(b + 1))), attn.step_plan(lens, kv_fp8=True)
+
+        def run():
+            q = qkv_post(proj, norm[0], norm[1], 1e-6, pos, cos_sin, slots, kc, vc, HQ, kv_scales=sc)
+            o = attn.forward(q, kc, vc, p, i, seq, max(lens), SCALE, False, kv_scales=sc, **plan)
+            c = extend_attention_fwd(q, kc, vc, qo, p, i, 1, SCALE, max_kv_len=max(lens),
+                                     kv_scales=sc)
+            return q, o, c
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        return proj, run, graph, out
+
+    steps = [step([0, 3, 4]), step([4, 2, 1, 0, 3]), step([1])]
+    for _ in range(3):
+        for proj, run, graph, out in steps:
+            proj.copy_(torch.randn(proj.shape, generator=g).to(torch.bfloat16))
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [x.clone() for x in out]
+            for a, b in zip(got, run()):
+                assert torch.equal(a, b)
+
+
 # ---- refusals ---------------------------------------------------------------------------------
 
 def test_refusals():
