@@ -312,8 +312,9 @@ __global__ void __launch_bounds__(NW * 64) decode_stage1_worker_kernel(
 // not needed here); every thread then merges the non-empty slots sequentially in
 // increasing slot order (increasing token order), as in sid/csrc/flash_decode.cu:231-273
 // with segments in place of splits. A request with no used slot gets zeros
-// (flash_decode.cu:246-249). The partial loads of different slots are independent, so they
-// overlap.
+// (flash_decode.cu:246-249); one whose used slots hold no number (a query or keys with a NaN or
+// an infinity: a log-sum-exp of NaN or -inf, which the maximum does not show) gets what its
+// weights give, NaN. The partial loads of different slots are independent, so they overlap.
 __global__ void __launch_bounds__(HEAD_DIM) decode_stage2_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_lse, int grid_slots,
     int part_stride, bf16_t* __restrict__ o) {
@@ -327,8 +328,12 @@ __global__ void __launch_bounds__(HEAD_DIM) decode_stage2_kernel(
   for (int y = d; y < grid_slots; y += HEAD_DIM) s_lse[y] = lse[y];
   __syncthreads();
   float mx = NEG_BIG;
-  for (int y = 0; y < grid_slots; ++y) mx = fmaxf(mx, s_lse[y]);
-  if (mx == NEG_BIG) {
+  bool used = false;
+  for (int y = 0; y < grid_slots; ++y) {
+    mx = fmaxf(mx, s_lse[y]);
+    used |= s_lse[y] != NEG_BIG;
+  }
+  if (!used) {
     o[row * HEAD_DIM + d] = 0;
     return;
   }
@@ -368,10 +373,15 @@ __global__ void __launch_bounds__(HEAD_DIM) decode_stage2_fixed_kernel(
   if (d < grid_slots) s_lse[d] = lse[d];
   __syncthreads();
   float mx = NEG_BIG;
+  bool used = false;
 #pragma unroll
-  for (int y = 0; y < CAP; ++y)
-    if (y < grid_slots) mx = fmaxf(mx, s_lse[y]);
-  if (mx == NEG_BIG) {
+  for (int y = 0; y < CAP; ++y) {
+    if (y < grid_slots) {
+      mx = fmaxf(mx, s_lse[y]);
+      used |= s_lse[y] != NEG_BIG;
+    }
+  }
+  if (!used) {
     o[row * HEAD_DIM + d] = 0;
     return;
   }
@@ -413,6 +423,7 @@ __global__ void __launch_bounds__(HEAD_DIM) decode_stage2_latency_kernel(
   const float* lse = part_lse + row * part_stride;
   const float* po = part_o + row * part_stride * HEAD_DIM;
   float mx = NEG_BIG;
+  bool used = false;
   float num = 0.0f, den = 0.0f;
   // Pass 1 finds the max over the used slots; when the grid fits one chunk (the common
   // case) the chunk's values stay in registers for pass 2.
@@ -423,9 +434,12 @@ __global__ void __launch_bounds__(HEAD_DIM) decode_stage2_latency_kernel(
       lv[j] = c0 + j < grid_slots ? lse[c0 + j] : NEG_BIG;
     }
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) mx = fmaxf(mx, lv[j]);
+    for (int j = 0; j < kChunk; ++j) {
+      mx = fmaxf(mx, lv[j]);
+      used |= lv[j] != NEG_BIG;
+    }
   }
-  if (mx == NEG_BIG) {  // empty request (flash_decode.cu:246-249)
+  if (!used) {  // empty request (flash_decode.cu:246-249)
     o[row * HEAD_DIM + d] = 0;
     return;
   }
