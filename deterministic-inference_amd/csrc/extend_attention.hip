@@ -223,7 +223,11 @@ __global__ void __launch_bounds__(256) extend_fanout_kernel(
   const int kv_start = kv_indptr[b];
   const int kv_len = kv_indptr[b + 1] - kv_start;
   const int prefix = kv_len - extend_len;
-  if (prefix < 0) return;  // malformed batch: the kv range must cover the extend tokens
+  if (prefix < 0) {  // malformed batch: the kv range must cover the extend tokens
+    if (split == 0)
+      skip_rows(part_n, q_start, mtile * BQ, min(extend_len, (mtile + 1) * BQ), num_q_heads, h_kv);
+    return;
+  }
 
   const int hq = h_kv * 2 + (c.wave >> 1);
   const int qr = mtile * BQ + 16 * (c.wave & 1) + c.r;  // extend-local query row of this lane
@@ -472,7 +476,7 @@ constexpr int MERGE_CHUNK = 16;
 __global__ void __launch_bounds__(256) extend_merge_kernel(
     int64_t items, int splits, const float* __restrict__ part_a,
     const float* __restrict__ part_ml, const int32_t* __restrict__ part_n,
-    bf16_t* __restrict__ o) {
+    const int32_t* __restrict__ qo_indptr, int batch, int num_q_heads, bf16_t* __restrict__ o) {
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (item >= items) return;  // whole waves: no barrier below
@@ -481,6 +485,10 @@ __global__ void __launch_bounds__(256) extend_merge_kernel(
   // own hold nothing it reads (measured: verify pass, 4 x 32 rows over 2k keys, 22.1 ->
   // 20.5 us per layer with the fan-out).
   const int nsplits = min(part_n[item], splits);
+  // Rows outside the sequences have no states (the workspace holds whatever it held) and stay.
+  if (item < static_cast<int64_t>(qo_indptr[0]) * num_q_heads ||
+      item >= static_cast<int64_t>(qo_indptr[batch]) * num_q_heads || nsplits <= 0)
+    return;
   float m = NEG_BIG, l = 0.0f;
   float2 acc = make_float2(0.0f, 0.0f);
   for (int c0 = 0; c0 < nsplits; c0 += MERGE_CHUNK) {
@@ -582,9 +590,11 @@ ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, con
   return p;
 }
 
-int extend_merge(const char* name, const ExtendPlan& p, void* o, hipStream_t s) {
+int extend_merge(const char* name, const ExtendPlan& p, const int32_t* qo_indptr, int batch,
+                 int num_q_heads, void* o, hipStream_t s) {
   hipLaunchKernelGGL(extend_merge_kernel, dim3((unsigned)((p.items + 3) / 4)), dim3(256), 0, s,
-                     p.items, p.splits, p.part_a, p.part_ml, p.part_n, (bf16_t*)o);
+                     p.items, p.splits, p.part_a, p.part_ml, p.part_n, qo_indptr, batch, num_q_heads,
+                     (bf16_t*)o);
   return check_launch(name);
 }
 
@@ -632,7 +642,7 @@ extern "C" int sid_extend_attention_fwd(const void* q, const void* k_cache, cons
                        num_kv_heads, num_slots, sm_scale, p.mtiles, total_q, p.part_a, p.part_ml,
                        p.part_n);
     const int rc = check_launch(name);
-    return rc != SID_OK ? rc : extend_merge(name, p, o, s);
+    return rc != SID_OK ? rc : extend_merge(name, p, qo_indptr, batch, num_q_heads, o, s);
   }
   auto prefill = [&](auto kern, int nw) {
     hipLaunchKernelGGL(kern, dim3(p.grid_x, num_kv_heads, p.mtiles), dim3(nw * 64),

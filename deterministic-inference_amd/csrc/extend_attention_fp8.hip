@@ -259,7 +259,11 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   const int kv_start = kv_indptr[b];
   const int kv_len = kv_indptr[b + 1] - kv_start;
   const int prefix = kv_len - extend_len;
-  if (prefix < 0) return;  // malformed batch: the kv range must cover the extend tokens
+  if (prefix < 0) {  // malformed batch: the kv range must cover the extend tokens
+    if (FANOUT && split == 0)
+      skip_rows(part_n, q_start, mtile * ROWS, min(extend_len, (mtile + 1) * ROWS), num_q_heads, h_kv);
+    return;
+  }
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -748,7 +752,7 @@ extern "C" int sid_extend_attention_fp8_fwd(
   if (p.fanout) {
     const int rc = launch(extend_fp8_kernel<4, true>, 4,
                           dim3(batch, num_kv_heads, p.mtiles * p.splits), p.mtiles);
-    return rc != SID_OK ? rc : extend_merge(name, p, o, s);
+    return rc != SID_OK ? rc : extend_merge(name, p, qo_indptr, batch, num_q_heads, o, s);
   }
   const int mtiles = ceil_div(max_extend_len, p.rows);
   const int64_t groups = static_cast<int64_t>(batch) * mtiles * num_kv_heads;

@@ -184,6 +184,15 @@ __device__ __forceinline__ int swz(int key) { return (key & 3) | (((key >> 3) & 
 
 constexpr int kTileBytes = BN * D * 2;  // one K or V tile
 
+// What a fan-out kernel leaves to the merge for each (row, head): how many splits have its state.
+// Rows of a request that is left out get 0, and the merge leaves them as they are, as a kernel that
+// walks the keys does. By the threads of the workgroup that has the split 0 of the rows' tile.
+__device__ __forceinline__ void skip_rows(int32_t* part_n, int q_start, int from, int to,
+                                          int num_q_heads, int h_kv) {
+  for (int i = threadIdx.x; i < 2 * (to - from); i += blockDim.x)
+    part_n[static_cast<int64_t>(q_start + from + (i >> 1)) * num_q_heads + 2 * h_kv + (i & 1)] = 0;
+}
+
 // ---- host side (extend_attention.hip) -----------------------------------------------------
 
 // Query positions (32 or 64) of a workgroup that walks all keys of its rows.
@@ -211,7 +220,9 @@ ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, con
                        int max_extend_len, int max_kv_len, int split_keys, int64_t need,
                        void* workspace, int64_t workspace_bytes);
 
-// The fan-out's second launch: the saved split states of every item folded in order.
-int extend_merge(const char* name, const ExtendPlan& p, void* o, hipStream_t s);
+// The fan-out's second launch: the saved split states of every item of the sequences' rows folded
+// in order.
+int extend_merge(const char* name, const ExtendPlan& p, const int32_t* qo_indptr, int batch,
+                 int num_q_heads, void* o, hipStream_t s);
 
 }  // namespace sid

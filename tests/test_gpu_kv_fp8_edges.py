@@ -1,13 +1,14 @@
-"""The 8-bit KV pool's attention where its inputs are unusual: queries and keys that are not numbers.
-Where a kernel is shared with the bf16 pool, its form is run too."""
+"""The 8-bit KV pool's attention where its inputs are unusual: queries and keys that are not numbers,
+rows that no request covers. Where a kernel is shared with the bf16 pool, its form is run too."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from conftest import HQ, D, SCALE
-from test_gpu_kv_fp8 import _batch, _decode
+from conftest import HKV, HQ, D, SCALE
+from test_gpu_kv_fp8 import _batch, _chunk_batch, _decode, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +31,13 @@ def _decode_bf16(q, kv, ptr, idx, splits, fixed, seg, slots, variant):
     load_ext().flash_decode_fwd(q, *kv, ptr, idx, None, splits, fixed, SCALE, po, pl, o,
                                 segment_size=seg, grid_slots=slots, variant=variant)
     return o
+
+
+def _fan_bytes(q, specs, hq=HQ, hkv=HKV, fp8=True):
+    from sid.kernels.jit import load_ext
+    return load_ext().extend_attention_workspace_bytes(
+        len(specs), q.shape[0], hq, hkv, max(e for _, e in specs), max(p + e for p, e in specs),
+        fp8=fp8)
 
 
 # ---- queries that are not numbers -------------------------------------------------------------
@@ -84,3 +92,50 @@ def test_decode_every_key_nan_gives_nan(args, batch):
     assert torch.equal(o[~hit], clean[~hit])
     if batch > 1:
         assert not o[1].any()
+
+
+# ---- rows that no request covers ------------------------------------------------------------------
+
+@pytest.mark.parametrize("pool8", [True, False], ids=["fp8", "bf16"])
+@pytest.mark.parametrize("fill", [0, 1, 0x3f, 0xff])
+def test_fanned_out_rows_behind_the_last_sequence_stay(pool8, fill):
+    """With the splits fanned out, as without: rows past the last sequence are left as they were,
+    whatever the workspace held."""
+    from sid.kernels.jit import load_ext
+    specs = [(2048, 32), (900, 5)]
+    q, pool, qo, ptr, idx, at, _ = _chunk_batch(specs, seed=18)
+    qq = torch.cat([q, q[:7]])
+    kv, kw = (pool[:2], dict(kv_scales=pool[2])) if pool8 else (_as_bf16(pool), {})
+    need = _fan_bytes(qq, specs, fp8=pool8)
+    assert need > 0
+    ws = torch.full((need,), fill, dtype=torch.uint8, device="cuda")
+    got = []
+    for w in (ws, None):
+        o = torch.full_like(qq, 7.0)
+        load_ext().extend_attention_fwd(qq, *kv, qo, ptr, idx, 32, SCALE, o, 2080, w, **kw)
+        assert (o[q.shape[0]:] == 7.0).all()
+        got.append(o)
+    assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("pool8", [True, False], ids=["fp8", "bf16"])
+@pytest.mark.parametrize("fill", [0, 1])
+def test_fanned_out_rows_of_a_refused_request_stay(pool8, fill):
+    """A request with fewer keys than new tokens is left out (its rows stay), with the fan-out too."""
+    from sid.kernels.jit import load_ext
+    specs = [(2048, 32), (0, 40), (700, 9)]
+    q, pool, qo, ptr, idx, at, qoh = _chunk_batch(specs, seed=19)
+    kv, kw = (pool[:2], dict(kv_scales=pool[2])) if pool8 else (_as_bf16(pool), {})
+    lens = [2080, 39, 709]  # one key short
+    flat = torch.cat([_i32(a[:n].tolist()) for a, n in zip(at, lens)])
+    ptr = _i32(np.concatenate([[0], np.cumsum(lens)]).tolist())
+    need = _fan_bytes(q, specs, fp8=pool8)
+    assert need > 0
+    got = []
+    for w in (torch.full((need,), fill, dtype=torch.uint8, device="cuda"), None):
+        o = torch.full_like(q, 7.0)
+        load_ext().extend_attention_fwd(q, *kv, qo, ptr, flat, 40, SCALE, o, 2080, w, **kw)
+        assert (o[32:72] == 7.0).all()
+        assert not o.isnan().any()
+        got.append(o)
+    assert torch.equal(*got)
