@@ -15,6 +15,7 @@
 #include "extend_tile.h"
 #include "kv_fp8.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace sid {
@@ -233,9 +234,9 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     const uint8_t* __restrict__ v_cache, const uint16_t* __restrict__ kv_scales,
     const int32_t* __restrict__ qo_indptr, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, int batch, int num_q_heads, int num_kv_heads,
-    int64_t num_slots, float sm_scale, int mtiles, int per_round, int ordered, int64_t items,
-    bf16_t* __restrict__ o, float* __restrict__ part_a, float* __restrict__ part_ml,
-    int32_t* __restrict__ part_n) {
+    int64_t num_slots, float sm_scale, int mtiles, int per_round, int ordered, int across,
+    int64_t items, bf16_t* __restrict__ o, float* __restrict__ part_a,
+    float* __restrict__ part_ml, int32_t* __restrict__ part_n) {
   __shared__ __align__(1024) char lds[lds_bytes(NW, FANOUT)];
   constexpr int ROWS = 8 * NW;
   int b, h_kv, mtile, split = 0;
@@ -246,9 +247,11 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
     split = static_cast<int>(blockIdx.z) / mtiles;
   } else {
     // Heads fastest: with 8 of them a head's workgroups, which share its keys, are on one XCD.
+    // A grid's first dimension holds `across` places, its second the rows of them (pick_item has
+    // no tile for those past the last).
     h_kv = blockIdx.x % num_kv_heads;
-    const Item it = pick_item<ROWS>(blockIdx.x / num_kv_heads, ordered != 0, per_round, batch,
-                                    mtiles, qo_indptr, kv_indptr);
+    const Item it = pick_item<ROWS>(blockIdx.x / num_kv_heads + blockIdx.y * across, ordered != 0,
+                                    per_round, batch, mtiles, qo_indptr, kv_indptr);
     if (it.mtile < 0) return;
     b = it.b;
     mtile = it.mtile;
@@ -687,6 +690,10 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp8_kernel(
   }
 }
 
+// Workgroups in a grid's first dimension: 2^21 of 512 work-items are a quarter of what it holds, and
+// at least one place of 65535 heads.
+constexpr int kMaxGridX = 1 << 21;
+
 // Whether a grid of fewer than 512 workgroups fans out. Walking its keys in one workgroup takes about
 // 6 + 1.1 us a tile; fanned out, the launches take 18 us and the saved states of total_q rows in
 // every split 8.5 us a thousand. Walked and fanned out, us: 1 x 512 tokens 14 and 23, 1 x 1024 23 and
@@ -741,22 +748,25 @@ extern "C" int sid_extend_attention_fp8_fwd(
                       (8 * total_q < 7 * static_cast<int64_t>(batch) * max_extend_len ||
                        max_kv_len > max_extend_len);
   const int per_round = p.rows == 32 ? max(1, cu_count() / num_kv_heads) : 0;
-  auto launch = [&](auto kern, int nw, dim3 grid, int mtiles) {
+  auto launch = [&](auto kern, int nw, dim3 grid, int mtiles, int across) {
     hipLaunchKernelGGL(kern, grid, dim3(nw * 64), 0, s, (const bf16_t*)q,
                        (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint16_t*)kv_scales, qo_indptr, kv_indptr, kv_indices, batch,
-                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, per_round, ordered, p.items,
-                       (bf16_t*)o, p.part_a, p.part_ml, p.part_n);
+                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, per_round, ordered, across,
+                       p.items, (bf16_t*)o, p.part_a, p.part_ml, p.part_n);
     return check_launch(name);
   };
   if (p.fanout) {
     const int rc = launch(extend_fp8_kernel<4, true>, 4,
-                          dim3(batch, num_kv_heads, p.mtiles * p.splits), p.mtiles);
+                          dim3(batch, num_kv_heads, p.mtiles * p.splits), p.mtiles, 0);
     return rc != SID_OK ? rc : extend_merge(name, p, qo_indptr, batch, num_q_heads, o, s);
   }
   const int mtiles = ceil_div(max_extend_len, p.rows);
-  const int64_t groups = static_cast<int64_t>(batch) * mtiles * num_kv_heads;
-  SID_REQUIRE(groups < (1ll << 31) / (64 * 8), "%s: grid too large", name);
-  return p.rows == 64 ? launch(extend_fp8_kernel<8, false>, 8, dim3(groups), mtiles)
-                      : launch(extend_fp8_kernel<4, false>, 4, dim3(groups), mtiles);
+  const int64_t places = static_cast<int64_t>(batch) * mtiles;
+  const int across = static_cast<int>(std::min<int64_t>(places, kMaxGridX / num_kv_heads));
+  const int64_t down = (places + across - 1) / across;
+  SID_REQUIRE(places < (1ll << 30) && down <= 65535, "%s: grid too large", name);
+  const dim3 grid(static_cast<unsigned>(across) * num_kv_heads, static_cast<unsigned>(down));
+  return p.rows == 64 ? launch(extend_fp8_kernel<8, false>, 8, grid, mtiles, across)
+                      : launch(extend_fp8_kernel<4, false>, 4, grid, mtiles, across);
 }

@@ -1,5 +1,6 @@
 """The 8-bit KV pool's attention where its inputs are unusual: queries and keys that are not numbers,
-rows that no request covers. Where a kernel is shared with the bf16 pool, its form is run too."""
+rows that no request covers, grids beyond one launch's limits. Where a kernel is shared with the
+bf16 pool, its form is run too."""
 
 from __future__ import annotations
 
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 from conftest import HKV, HQ, D, SCALE
-from test_gpu_kv_fp8 import _batch, _chunk_batch, _decode, _i32
+from test_gpu_kv_fp8 import _batch, _chunk, _chunk_batch, _decode, _i32, _say
 
 pytestmark = pytest.mark.gpu
 
@@ -136,6 +137,42 @@ def test_fanned_out_rows_of_a_refused_request_stay(pool8, fill):
         o = torch.full_like(q, 7.0)
         load_ext().extend_attention_fwd(q, *kv, qo, ptr, flat, 40, SCALE, o, 2080, w, **kw)
         assert (o[32:72] == 7.0).all()
+        assert not o.isnan().any()
+        got.append(o)
+    assert torch.equal(*got)
+
+
+# ---- bounds beyond one launch ----------------------------------------------------------------------
+
+def test_chunk_one_long_prompt_among_thousands():
+    """5000 requests, one of 4000 tokens: 5 million places for workgroups, nearly all of them empty."""
+    rng = np.random.default_rng(1)
+    specs = [(int(rng.integers(0, 4)), 1) for _ in range(5000)]
+    specs[3210] = (0, 4000)
+    q, pool, qo, ptr, idx, at, qoh = _chunk_batch(specs, seed=26)
+    _say("thousands", q.shape[0])
+    o = _chunk(q, pool, qo, ptr, idx, specs, workspace=False)
+    assert not o.isnan().any()
+    for i in (0, 1, 3209, 3210, 3211, 4999, *rng.integers(0, 5000, 6).tolist()):
+        p, e = specs[i]
+        a, b = int(qoh[i]), int(qoh[i + 1])
+        one = _chunk(q[a:b].contiguous(), pool, _i32([0, e]), _i32([0, p + e]),
+                     _i32(at[i].tolist()), [(p, e)], workspace=False)
+        assert torch.equal(one, o[a:b]), i
+
+
+def test_chunk_placed_by_key_count_beyond_one_grid_dimension():
+    """200 ragged requests under a bound of 50000 new tokens: the places of the tiles that there are
+    come first, over 2^18 in all."""
+    from sid.kernels.jit import load_ext
+    rng = np.random.default_rng(3)
+    specs = [(int(rng.integers(0, 60)), int(rng.integers(1, 90))) for _ in range(200)]
+    q, pool, qo, ptr, idx, at, qoh = _chunk_batch(specs, seed=28)
+    got = []
+    for bound in (50000, 89):
+        o = torch.full_like(q, float("nan"))
+        load_ext().extend_attention_fwd(q, pool[0], pool[1], qo, ptr, idx, bound, SCALE, o, 150,
+                                        None, kv_scales=pool[2])
         assert not o.isnan().any()
         got.append(o)
     assert torch.equal(*got)
