@@ -561,14 +561,15 @@ ExtendPlan extend_plan(const char* name, const void* q, const void* k_cache, con
                 num_kv_heads);
     SID_REQUIRE(num_slots > 0, "%s: empty KV pool", name);
     SID_REQUIRE(batch <= 65535 && num_kv_heads <= 65535, "%s: grid too large", name);
-    p.fanout = need > 0 && workspace != nullptr && workspace_bytes >= need;
     p.items = total_q * num_q_heads;
     const int mtiles = ceil_div(max_extend_len, BQ);
+    // (A bound of keys that asks for more splits than the grid's third dimension holds: walked.)
+    p.fanout = need > 0 && workspace != nullptr && workspace_bytes >= need &&
+               static_cast<int64_t>(mtiles) * ceil_div(max_kv_len, split_keys) <= 65535;
     if (p.fanout) {
       p.rows = BQ;
       p.mtiles = mtiles;
       p.splits = ceil_div(max_kv_len, split_keys);
-      SID_REQUIRE(static_cast<int64_t>(mtiles) * p.splits <= 65535, "%s: grid too large", name);
       SID_REQUIRE((p.items + 3) / 4 < (1ll << 31), "%s: too many rows for the merge", name);
       p.part_a = static_cast<float*>(workspace);
       p.part_ml = p.part_a + static_cast<int64_t>(p.splits) * p.items * D;

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from conftest import HKV, HQ, D, SCALE
-from test_gpu_kv_fp8 import _batch, _chunk, _chunk_batch, _decode, _i32, _say
+from test_gpu_kv_fp8 import (_batch, _bounded, _chunk, _chunk_batch, _decode, _i32, _pool, _say)
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +176,24 @@ def test_chunk_placed_by_key_count_beyond_one_grid_dimension():
         assert not o.isnan().any()
         got.append(o)
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("pool8", [True, False], ids=["fp8", "bf16"])
+def test_chunk_bound_of_keys_beyond_a_fanned_out_grid(pool8):
+    """A bound of 17 million keys (no request has them) asks for more splits than a grid's third
+    dimension holds: the keys are walked, with the same bits."""
+    from sid.kernels.jit import load_ext
+    hkv, specs, bound = 1, [(100, 64)], 17_000_000
+    pool = _pool(300, hkv, seed=27)
+    q = _queries(64, 27, 2)
+    at = np.random.default_rng(2).permutation(300)[:164]
+    qo, ptr, idx = _i32([0, 64]), _i32([0, 164]), _i32(at.tolist())
+    kv, kw = (pool[:2], dict(kv_scales=pool[2])) if pool8 else (_as_bf16(pool), {})
+    ext = load_ext()
+    need = ext.extend_attention_workspace_bytes(1, 64, 2, hkv, 64, bound, fp8=pool8)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+    o, want = torch.zeros_like(q), torch.zeros_like(q)
+    ext.extend_attention_fwd(q, *kv, qo, ptr, idx, 64, SCALE, o, bound, ws, **kw)
+    ext.extend_attention_fwd(q, *kv, qo, ptr, idx, 64, SCALE, want, 164, None, **kw)
+    assert torch.equal(o, want)
+    _bounded(o, q, pool[3][at], pool[4][at], first=100, chunk=True)
