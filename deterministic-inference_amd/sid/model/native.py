@@ -92,7 +92,6 @@ class NativeQwen3:
                            model.rope.cos_sin.data_ptr(), w["embed"].data_ptr(),
                            w["norm"].data_ptr(), w["lm_head"].data_ptr(), self.layers)
         self.vocab = cfg.vocab_size
-        self.key = (id(kv_cache), tuple(kv_cache.layer(0)[0].shape))
 
     def forward(self, fb, greedy: bool, sample: bool = False, with_logits: bool = False,
                 sample_tiles: bool = True):

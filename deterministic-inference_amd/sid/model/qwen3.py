@@ -10,6 +10,8 @@ this step's K/V were written by reshape_and_cache.
 
 from __future__ import annotations
 
+import weakref
+
 import torch
 
 from sid.config import ModelConfig, decode_backend_kind
@@ -226,8 +228,10 @@ class Qwen3Model:
     def _native_forward(self, fb: ForwardBatch, kv_cache, greedy: bool, sample: bool = False,
                         with_logits: bool = False):
         from sid.model.native import NativeQwen3
+        # The descriptor holds the pools' addresses, so it is this cache's alone (not that of a
+        # later one with the same id: a dropped cache's reference equals no other).
         pool = kv_cache.layer(0)[0]
-        key = (id(kv_cache), tuple(pool.shape), pool.dtype, self.decode_chain)
+        key = (weakref.ref(kv_cache), tuple(pool.shape), pool.dtype, self.decode_chain)
         if self._native is None or self._native.key != key:
             self._native = NativeQwen3(self, kv_cache, SPLIT_K_MAX_TOKENS,
                                        DECODE_CHAIN_MAX_ROWS if self.decode_chain else 0)
