@@ -12,7 +12,6 @@ import logging
 import weakref
 from collections import OrderedDict
 
-import numpy as np
 import torch
 
 from sid.config import EngineConfig, Mode, ModelConfig
@@ -21,8 +20,7 @@ from sid.engine.batch import (DecodeStatic, ForwardBatch, ForwardMode, batch_buc
 from sid.engine.kv_cache import KVCache
 from sid.engine.sampler import sample as _sample
 from sid.kernels.decode_attention import (INVARIANT_VARIANT, DecodeAttention, length_bucket,
-                                          plan_variant, plan_variant_fp8, segment_tokens,
-                                          stage1_workers, worker_order, workgroup_order)
+                                          placement)
 from sid.kernels.matmul_persistent import linear_sample_supported
 from sid.model.loader import build_model_config, load_weights, random_weights
 from sid.model.qwen3 import Qwen3Model
@@ -183,7 +181,7 @@ class ModelRunner:
             fb = build_decode_batch(reqs, self.kv_cache, self.device, invariant)
             if invariant:
                 fb.decode_variant = INVARIANT_VARIANT
-            geom = None if invariant else self._pick_variant(fb, len(reqs), fb.max_seq_len)
+            geom = None if invariant else self._pick_variant(fb, fb.max_seq_len)
             self._attach_order(fb, len(reqs), invariant, fb.max_seq_len, geom)
             return fb
         static = self.graphs.decode_static
@@ -202,55 +200,40 @@ class ModelRunner:
         if invariant:
             fb.decode_variant = INVARIANT_VARIANT
         else:
-            plan = self._pick_variant(fb, len(reqs), bucket)
+            plan = self._pick_variant(fb, bucket)
         ordered = self._attach_order(fb, pad, invariant, bucket, plan)
         fb.graph_key = ("decode", pad, invariant, bucket, plan, fb.decode_variant, ordered)
         return fb
 
     def _attach_order(self, fb: ForwardBatch, rows: int, invariant: bool, max_len: int,
                       geom: tuple | None) -> int:
-        """The attention's stage-1 placement for this step, from the host-known lengths and
-        the plan the forward will run (fixed splits in batch_invariant mode, else the nondet
-        geometry): the heaviest-first workgroup order (workgroup_order, balanced over the
-        CUs) for the grid, or for a worker launch (stage1_workers) the same dealing over the
-        workers. Grids with fewer non-empty segments than CUs otherwise keep their own order
-        (nothing to balance, and reading the order first costs a small batch 0.2-0.4 us).
-        Placement never changes a result. Returns 0 (grid order), 1 (order attached) or the
-        worker count (fb.decode_workers)."""
+        """The attention's stage-1 placement for this step (placement), from the host-known
+        lengths and the plan the forward will run (fixed splits in batch_invariant mode, else the
+        nondet geometry). Returns 0 (grid order), 1 (order attached) or the worker count
+        (fb.decode_workers)."""
         da = self.decode_attn
         if invariant:
             tile = da.invariant_split_size
             splits, fixed, seg, slots = 0, tile, tile, max(1, -(-max(max_len, 1) // tile))
         else:
             (splits, seg, slots), fixed = geom, 0
-        tokens = segment_tokens(fb.seq_lens_host, rows, splits, fixed, seg, slots)
+        order, fb.decode_workers = placement(fb.seq_lens_host, rows, splits, fixed, seg, slots,
+                                             fb.decode_variant, da.cu_count())
         fb.decode_wg_order = None
-        fb.decode_workers = 0
-        cu = da.cu_count()
-        nonempty = int(np.count_nonzero(tokens))
-        workers = stage1_workers(nonempty, fb.decode_variant, slots, cu)
-        if workers == 0 and nonempty < cu:
+        if order is None:
             return 0
-        order = worker_order(tokens, workers) if workers else workgroup_order(tokens, cu)
         if self.graphs is not None:
             fb.decode_wg_order = self.graphs.decode_static.set_order(order)
         else:
             fb.decode_wg_order = torch.from_numpy(order).to(self.device)
-        fb.decode_workers = workers
-        return workers or 1
+        return fb.decode_workers or 1
 
-    def _pick_variant(self, fb: ForwardBatch, bs: int, max_len: int) -> tuple:
+    def _pick_variant(self, fb: ForwardBatch, max_len: int) -> tuple:
         """The nondet plan's geometry and its stage-1 workgroup shape (fb.decode_variant),
         from the requests' host-known lengths."""
-        cu, splits = self.decode_attn.cu_count(), self.cfg.max_kv_splits
-        if self.kv_cache.kv_scales is not None:
-            geom, fb.decode_variant = plan_variant_fp8(fb.seq_lens_host, max_len, cu, splits)
-        else:
-            geom, fb.decode_variant = plan_variant(fb.seq_lens_host, max_len,
-                                                   self.mcfg.num_kv_heads, cu, splits,
-                                                   invariant=False)
-        fb.decode_geometry = geom
-        return geom
+        fb.decode_geometry, fb.decode_variant = self.decode_attn.pick_plan(
+            fb.seq_lens_host, max_len, self.kv_cache.kv_scales is not None)
+        return fb.decode_geometry
 
     def tag_verify(self, fb: ForwardBatch) -> ForwardBatch:
         """Verify batches always live in the persistent verify buffers: graph them."""

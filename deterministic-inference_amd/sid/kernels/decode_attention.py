@@ -391,6 +391,22 @@ def worker_order(tokens: np.ndarray, workers: int) -> np.ndarray:
     return order
 
 
+def placement(lengths, rows: int, splits: int, fixed_split: int, seg: int, slots: int,
+              variant: int, cu_count: int) -> tuple:
+    """(order, workers) of stage 1 for a plan over requests of these lengths, padded to `rows`:
+    the heaviest-first workgroup order (workgroup_order, balanced over the CUs) for the grid,
+    workers 0, or for a worker launch (stage1_workers) the same dealing over the workers
+    (worker_order). (None, 0), the grid's own order, where fewer segments than CUs hold tokens:
+    there is nothing to balance, and reading the order first costs a small batch 0.2-0.4 us.
+    Placement never changes a result."""
+    tokens = segment_tokens(lengths, rows, splits, fixed_split, seg, slots)
+    nonempty = int(np.count_nonzero(tokens))
+    workers = stage1_workers(nonempty, variant, slots, cu_count)
+    if workers == 0 and nonempty < cu_count:
+        return None, 0
+    return (worker_order(tokens, workers) if workers else workgroup_order(tokens, cu_count)), workers
+
+
 def workspace_slots(max_seq_len: int, max_kv_splits: int, invariant_split_size: int) -> int:
     """Partial slots per request the workspace must hold for any plan."""
     nondet = -(-max_seq_len // SEGMENT_SIZES[-1]) + max_kv_splits
@@ -448,28 +464,28 @@ class DecodeAttention:
         splits, seg, slots = geometry
         return None, splits, 0, seg, slots
 
-    def step_plan(self, lengths, kv_fp8: bool = False, max_len: int | None = None) -> dict:
-        """The nondet/dvr plan of a decode step over requests of these lengths (host-side), as
-        forward's arguments: geometry and workgroup shape (plan_variant; plan_variant_fp8 for
-        an 8-bit pool, kv_fp8) and the placement of the workgroups (workgroup_order,
-        worker_order). One plan serves the step's layers. Its order is copied to the device
-        here: make it outside a graph capture. max_len: the bound that forward is called with,
-        if it is not the longest length."""
-        lens = [int(n) for n in lengths]
-        bound = max(max(lens, default=1) if max_len is None else int(max_len), 1)
+    def pick_plan(self, lengths, max_len: int, kv_fp8: bool) -> tuple:
+        """((grid splits, segment size, grid slots), stage-1 variant) of a nondet/dvr step over
+        requests of these lengths, none longer than max_len: plan_variant, or plan_variant_fp8
+        for an 8-bit pool."""
         cu = self.cu_count()
         if kv_fp8:
-            geom, variant = plan_variant_fp8(lens, bound, cu, self.max_kv_splits)
-        else:
-            geom, variant = plan_variant(lens, bound, self.num_kv_heads, cu, self.max_kv_splits,
-                                         invariant=False)
-        tokens = segment_tokens(lens, len(lens), geom[0], 0, geom[1], geom[2])
-        nonempty = int(np.count_nonzero(tokens))
-        workers = stage1_workers(nonempty, variant, geom[2], cu)
-        order = None
-        if workers or nonempty >= cu:
-            host = worker_order(tokens, workers) if workers else workgroup_order(tokens, cu)
-            order = torch.from_numpy(host).to(self.device)
+            return plan_variant_fp8(lengths, max_len, cu, self.max_kv_splits)
+        return plan_variant(lengths, max_len, self.num_kv_heads, cu, self.max_kv_splits,
+                            invariant=False)
+
+    def step_plan(self, lengths, kv_fp8: bool = False, max_len: int | None = None) -> dict:
+        """The nondet/dvr plan of a decode step over requests of these lengths (host-side), as
+        forward's arguments: geometry and workgroup shape (pick_plan) and the placement of the
+        workgroups (placement). One plan serves the step's layers. Its order is copied to the
+        device here: make it outside a graph capture. max_len: the bound that forward is called
+        with, if it is not the longest length."""
+        lens = [int(n) for n in lengths]
+        bound = max(max(lens, default=1) if max_len is None else int(max_len), 1)
+        geom, variant = self.pick_plan(lens, bound, kv_fp8)
+        host, workers = placement(lens, len(lens), geom[0], 0, geom[1], geom[2], variant,
+                                  self.cu_count())
+        order = None if host is None else torch.from_numpy(host).to(self.device)
         return dict(variant=variant, geometry=geom, wg_order=order, workers=workers)
 
     def forward(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

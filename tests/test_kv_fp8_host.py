@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import types
 
+import numpy as np
+import pytest
 import torch
 
 
@@ -48,3 +50,35 @@ def test_native_executor_goes_by_the_cache_itself(monkeypatch):
     assert model._native_forward(fb, new, True) == "new" and built == ["old", "new"]
     model.decode_chain = False
     assert model._native_forward(fb, new, True) == "new" and built == ["old", "new", "new"]
+
+
+def _host_only_attention(monkeypatch):
+    from sid.kernels.decode_attention import DecodeAttention, workspace_slots
+    da = DecodeAttention.__new__(DecodeAttention)
+    da.num_kv_heads, da.max_kv_splits, da.invariant_split_size = 8, 32, 256
+    da.device = torch.device("cpu")
+    da.ws_splits = workspace_slots(16384, 32, 256)
+    monkeypatch.setattr(DecodeAttention, "cu_count", lambda self: 256)
+    return da
+
+
+@pytest.mark.parametrize("kv_fp8", [False, True])
+@pytest.mark.parametrize("lens", [[1], [1024], [300] * 5, [2000, 64, 7, 900] * 8, [2048] * 64,
+                                  [700 + i for i in range(96)], [40] * 200], ids=lambda s: f"b{len(s)}")
+def test_step_plan_is_the_plan_that_the_engine_runs(monkeypatch, lens, kv_fp8):
+    from sid.engine.model_runner import ModelRunner
+    da = _host_only_attention(monkeypatch)
+    runner = ModelRunner.__new__(ModelRunner)
+    runner.decode_attn, runner.graphs, runner.device = da, None, "cpu"
+    runner.kv_cache = types.SimpleNamespace(kv_scales=[] if kv_fp8 else None)
+    fb = types.SimpleNamespace(seq_lens_host=np.asarray(lens))
+    geom = runner._pick_variant(fb, max(lens))
+    ordered = runner._attach_order(fb, len(lens), False, max(lens), geom)
+    plan = da.step_plan(lens, kv_fp8=kv_fp8)
+    assert plan["geometry"] == geom == fb.decode_geometry and plan["variant"] == fb.decode_variant
+    assert plan["workers"] == fb.decode_workers and geom[2] <= da.ws_splits
+    assert (plan["wg_order"] is None) == (fb.decode_wg_order is None) == (ordered == 0)
+    if ordered:
+        assert torch.equal(plan["wg_order"], fb.decode_wg_order)
+        want = torch.arange(len(lens))[:, None] << 12 | torch.arange(geom[2])
+        assert torch.equal((plan["wg_order"] & ~(1 << 30)).sort()[0], want.reshape(-1).int().sort()[0])
