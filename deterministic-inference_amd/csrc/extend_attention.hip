@@ -55,6 +55,100 @@ __device__ __forceinline__ s16x4_v ld_tr16(const bf16_t* p) {
       (__attribute__((address_space(3))) s16x4_v*)(p));
 }
 
+constexpr int KSPLIT = 256;  // keys per split (4 tiles), anchored at position 0
+
+__device__ __forceinline__ void fresh(RowState& s) {
+  s.m = NEG_BIG;
+  s.l = 0.0f;
+#pragma unroll
+  for (int db = 0; db < 8; ++db) s.acc[db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// run <- fold(run, part): the one merge used by every path.
+__device__ __forceinline__ void fold(RowState& run, float m, float l, const f32x4_v (&a)[8]) {
+  const FoldScale f = fold_scale(run.m, m);
+  run.l = fold_elem(run.l, l, f);
+#pragma unroll
+  for (int db = 0; db < 8; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) run.acc[db][i] = fold_elem(run.acc[db][i], a[db][i], f);
+  run.m = f.mn;
+}
+
+// Softmax of one tile's scores s (in place: s becomes p), in the exp2 domain:
+// p = 2^(s * sc2 - m) with sc2 = sm_scale * log2(e) and m the row's reference maximum in
+// the same units. The reference maximum is lazy: it moves to the tile's maximum only when
+// that exceeds it by more than LAZY_T, so p <= 2^LAZY_T and most tiles leave it (and the
+// accumulator) alone. Every decision is per row (per lane group), so a row's bits depend
+// on its own scores only. MASK: apply causality and row validity (keys beyond the row's
+// position give p = 0). Returns the accumulator's rescale factor (exactly 1 when the
+// reference maximum stays).
+template <bool MASK, class C>
+__device__ __forceinline__ float softmax_tile(float (&s)[16], RowState& st, const C& c, int t0,
+                                              float sc2) {
+  bool vis[16];
+  float tmax = NEG_BIG;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (MASK) {
+      const int key = t0 + 32 * (i >> 3) + 8 * c.g + (i & 7);
+      vis[i] = (key <= c.q_abs) & c.row_ok;
+      tmax = fmaxf(tmax, vis[i] ? s[i] : NEG_BIG);
+    } else {
+      tmax = fmaxf(tmax, s[i]);
+    }
+  }
+  tmax = pair16_max(tmax);
+  tmax = pair32_max(tmax);
+  const float mc = tmax * sc2;
+  const float m_used = mc > st.m + LAZY_T ? mc : st.m;
+  const float rescale = exp2_fast(st.m - m_used);
+  float psum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float p = exp2_fast(__builtin_fmaf(s[i], sc2, -m_used));
+    if constexpr (MASK) s[i] = vis[i] ? p : 0.0f;
+    else s[i] = p;
+    psum += s[i];
+  }
+  psum = pair16_sum(psum);
+  psum = pair32_sum(psum);
+  st.l = __builtin_fmaf(st.l, rescale, psum);
+  st.m = m_used;
+  return rescale;
+}
+
+// p of a tile as the PV product's B operand (p is finite: exp of a finite difference, or 0).
+__device__ __forceinline__ void pack_p(bf16x8_v (&pf)[2], const float (&s)[16]) {
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    uint4 u;
+    u.x = pack_bf16x2(s[8 * kb + 0], s[8 * kb + 1]);
+    u.y = pack_bf16x2(s[8 * kb + 2], s[8 * kb + 3]);
+    u.z = pack_bf16x2(s[8 * kb + 4], s[8 * kb + 5]);
+    u.w = pack_bf16x2(s[8 * kb + 6], s[8 * kb + 7]);
+    pf[kb] = __builtin_bit_cast(bf16x8_v, u);
+  }
+}
+
+// x * 1 == x: the rescale is skipped (same bits) unless some row of the wave moved its
+// reference maximum.
+__device__ __forceinline__ void apply_rescale(RowState& st, float rescale) {
+  if (__builtin_amdgcn_ballot_w64(rescale != 1.0f) != 0) {
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      st.acc[db][0] *= rescale;
+      st.acc[db][1] *= rescale;
+      st.acc[db][2] *= rescale;
+      st.acc[db][3] *= rescale;
+    }
+  }
+}
+
+// LDS tiles are 64 rows of 256 bytes; 16-byte piece p of key's row sits at p ^ swz(key): over
+// the 16 keys of a fragment or transpose read swz takes 16 values.
+__device__ __forceinline__ int swz(int key) { return (key & 3) | (((key >> 3) & 3) << 2); }
+
 struct Ctx {
   const bf16_t* k_cache;
   const bf16_t* v_cache;

@@ -1,9 +1,16 @@
 // Varlen causal "extend" attention over the 8-bit pool (format: kv_fp8.h), gfx950 MFMA.
 //
-// The contract, the splits, the tile arithmetic and the fan-out are extend_attention.hip's
-// (extend_tile.h): a query's result depends only on its position and its sequence's keys. What
-// differs is how the products get their operands: K's codes lie in the LDS as they are and S = K
-// Q^T is taken on them, with q as two e4m3 vectors; V's become bf16 on their way into the LDS.
+// The contract is extend_attention.hip's (a query's result depends only on its position and its
+// sequence's keys), and the fold of the splits and the fan-out's merge are shared with it
+// (extend_tile.h). The tile arithmetic is this kernel's: K's codes lie in the LDS as they are and S
+// = K Q^T is taken on them, with q as two e4m3 vectors; V's become bf16 on their way into the LDS;
+// splits are of 512 keys.
+//
+// Rounded to fewer than 32 bits: p, to bf16 before the product with V (half a step, 2^-8 of p, as
+// over the bf16 pool: both operands of the product are bf16, and P in two parts would double the
+// products), while l sums the unrounded p; and the small elements of a q row that holds far larger
+// ones (QRow). Against 64 bits the result's error, most of it the rounding of the result itself, is
+// 8% (windows, ragged chunks) to 15% (4 x 2048 tokens) above that of fp32 arithmetic rounded once.
 //
 // Bound: 4 operations for each of a query's keys and dims. 1 x 8192 tokens 323 us, 0.85 PFLOP/s;
 // 4 x 2048 111 us, 0.62, a third of which is the workgroups' first loads and last stores (one of 8
@@ -58,10 +65,13 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
 typedef int i32x8_v __attribute__((ext_vector_type(8)));
 
 // A query row as two e4m3 vectors: q = 2^e (hi + lo / 16), with q's own e of the pool's rule.
-// hi keeps 4 significant bits and lo the other 4 of a bf16 value, so the sum is q exactly down to
-// 2^-13 of 2^e (less than 2^-20 of the row's largest element): two fp8 products give q . k to
-// fp32 accuracy, at the matrix rate of one bf16 product and half its operand reads, and the
-// codes need no conversion. A lane holds dims 16 g .. +15 and 64 + 16 g .. +15 of row r.
+// hi keeps 4 significant bits and lo the other 4 of a bf16 value, so the sum is q exactly for
+// elements of 2^-6 2^e and more, and for smaller ones the nearest multiple of 2^-13 2^e. The row's
+// largest element m is above 224 2^e: elements from 2^-13.8 m up are exact and the others off by at
+// most 2^-21.8 m, which puts a score off by at most 2^-21.8 m sum |k| sm_scale: within what fp32
+// sums of m's own products round away unless the keys are zero where q is large. In return two fp8
+// products, at the matrix rate of one bf16 product and half its operand reads, take the place of a
+// bf16 product with converted codes. A lane holds dims 16 g .. +15 and 64 + 16 g .. +15 of row r.
 struct QRow {
   i32x8_v hi, lo;
   int scale;  // E8M0 bytes: hi's in byte 0, lo's in byte 1

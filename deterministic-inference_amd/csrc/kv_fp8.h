@@ -1,6 +1,6 @@
 // The 8-bit KV cache's number format, shared by the kernels that write it, read it back and
 // attend over it (kv_fp8.hip, norm_rope.hip, decode_chain.hip, decode_attention_fp8.hip,
-// extend_attention.hip).
+// extend_attention_fp8.hip).
 //
 // A K (or V) vector of one token's head (128 elements) is 128 e4m3 codes c and one power of
 // two 2^e, stored as the E8M0 byte e + 127: x ~ c 2^e with the smallest e for which

@@ -300,11 +300,10 @@ __global__ void __launch_bounds__(128) silu_mul_kernel(RowSrc gu, uint2* __restr
 // hidden 128), 8 heads per 128-thread block. q/k heads: per-head RMSNorm, round, RoPE (the
 // rotate-half partner of lane j is lane j ^ 8, one DPP row_ror:8 away), round;
 // v heads: copied. q goes to q_out [T, HQ, 128]; k and v to the pools at slots[t].
-constexpr int QD = 128;
-
-//
 // FP8: the pools hold codes and kv_scales their powers of two (kv_fp8.h); k and v are then
 // quantised from the same bf16 values.
+constexpr int QD = 128;
+
 template <int NCH, bool FP8>
 __global__ void __launch_bounds__(128) qkv_post_kernel(
     RowSrc src, int num_q_heads, int num_kv_heads, const uint4* __restrict__ q_norm,
