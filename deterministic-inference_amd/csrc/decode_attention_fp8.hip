@@ -14,9 +14,9 @@
 // keys 173.2 -> 169.3 us with the rows a step ahead, 64 of 2048 48.9 -> 47.0, 32 ragged ones of
 // 128-4096 31.6 -> 29.2). 4 tokens an iteration: with 8 the wave holds 209 registers and one
 // workgroup fits a CU, with 2 too little is in flight (128 x 4096: 172 us with two workgroups a
-// CU, 203 with a plan of one). 128 x 4096 keys: 171 us, 6.3 TB/s, where a plain read of the
-// same size reaches 6.0-6.5; 1 x 1024: 10.4 us, the chain of launch, slots, rows, merge and
-// stage 2's launch.
+// CU, 203 with a plan of one). 128 x 4096 keys: 166 us, 6.5 TB/s, with the
+// merge, where a plain read of the same size reaches 6.0-6.5; 1 x 1024: 9.9 us in a graph, the chain
+// of launch, slots, rows, merge and stage 2's launch (the bf16 pool's kernel 10.3 in the same run).
 #include "decode_split.h"
 #include "kv_fp8.h"
 

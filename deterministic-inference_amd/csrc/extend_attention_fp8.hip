@@ -12,9 +12,11 @@
 // ones (QRow). Against 64 bits the result's error, most of it the rounding of the result itself, is
 // 8% (windows, ragged chunks) to 15% (4 x 2048 tokens) above that of fp32 arithmetic rounded once.
 //
-// Bound: 4 operations for each of a query's keys and dims. 1 x 8192 tokens 323 us, 0.85 PFLOP/s;
-// 4 x 2048 111 us, 0.62, a third of which is the workgroups' first loads and last stores (one of 8
-// waves fills a CU); the 2-byte pool's kernel 420 and 133 us. The matrix products are 1024 of a
+// Bound: 4 operations for each of a query's keys and dims. Calls in a row take, for 1 x 8192 tokens,
+// 319 us, 0.86 PFLOP/s; for 4 x 2048 102 us, 0.67, a third of which is the workgroups' first loads
+// and last stores (one of 8 waves fills a CU; a launch alone takes 120). The 2-byte pool's kernel
+// takes 1.19 and 1.08 times as long, 1.5 times on ragged chunks over long prefixes, and 0.93 on
+// 16 x 512 tokens and on windows of 32. The matrix products are 1024 of a
 // tile's 2800 cycles on a SIMD (two waves, 24 products each); the rest is a wave's own chain, V's
 // conversion, the softmax and the loads' addresses, which two waves that start a tile at the same
 // barrier overlap only in part. It is not the LDS (896 cycles a tile of 8 waves, no bank

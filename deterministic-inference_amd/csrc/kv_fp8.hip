@@ -2,8 +2,8 @@
 // read back as bf16 (format: kv_fp8.h). Both only move bytes: 16 lanes hold a vector of 128
 // (16 bytes of bf16 or 8 of codes a lane), K and V of a token's head side by side in a thread
 // so that both loads are in flight, the maximum over the 16 lanes by DPP. Both run at the rate of a
-// large copy (4.5 TB/s): 8192 rows are written in 10.7 us, 4.7 TB/s, and 65536 read back in 76 us,
-// 5.3; one row takes 1.9 us, the latency of a slot, a row and its maximum.
+// large copy (4.5 TB/s): 8192 rows are written in 10.2 us, 5.0 TB/s, and 65536 read back in 77 us,
+// 5.2; one row takes 1.9 us, the latency of a slot, a row and its maximum.
 #include "kv_fp8.h"
 
 namespace sid {

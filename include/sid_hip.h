@@ -181,7 +181,8 @@ int64_t sid_flash_decode_noalloc_scratch_bytes(void);
  * batch-slot invariant, bit for bit). workspace (optional, any alignment of
  * 16 bytes, sid_extend_attention_workspace_bytes(...) bytes) lets small
  * grids give each split its own workgroup; the result is bitwise the same
- * with or without it.
+ * with or without it. Rows of q outside the sequences, and those of a request
+ * with fewer keys than new tokens, are left as they are in o.
  * Replaces extend_attention_fwd, sid/kernels/extend_attention.py:115-144.
  */
 int sid_extend_attention_fwd(const void* q, const void* k_cache, const void* v_cache,
@@ -634,7 +635,8 @@ int sid_flash_decode_fp8_fwd(const void* q, const void* k_cache, const void* v_c
 /*
  * sid_extend_attention_fwd over an 8-bit pool, with its invariances: a query's result depends
  * only on its position and its sequence's keys (reduced in 512-position splits here). A NaN
- * vector reaches the queries that see its key and no others. workspace as there, of
+ * vector reaches the queries that see its key and no others. q enters the products as two e4m3
+ * vectors: elements below 2^-13.8 of their row's largest, m, are off by up to 2^-21.8 m. workspace as there, of
  * sid_extend_attention_fp8_workspace_bytes(...) bytes (never more than
  * sid_extend_attention_workspace_bytes of the same arguments; 0 = no fan-out).
  */
