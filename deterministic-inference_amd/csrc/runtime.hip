@@ -41,3 +41,5 @@ int cu_count() {
 extern "C" const char* sid_last_error(void) { return sid::g_last_error; }
 
 extern "C" int sid_abi_version(void) { return 22; }
+
+extern "C" int sid_abi_revision(void) { return 1; }

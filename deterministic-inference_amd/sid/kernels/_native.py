@@ -69,13 +69,15 @@ _SIGNATURES = {
     "sid_extend_attention_fp8_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
                                      _i32, _i64, _i32, _i32, _f32, _vp, _i64, _vp, _vp],
 }
-EXPORTED = ("sid_last_error", "sid_abi_version", "sid_extend_attention_workspace_bytes",
+EXPORTED = ("sid_last_error", "sid_abi_version", "sid_abi_revision",
+            "sid_extend_attention_workspace_bytes",
             "sid_linear_argmax_workspace_bytes", "sid_sample_workspace_bytes",
             "sid_qwen3_extend_workspace_bytes", "sid_qwen3_extend_forward",
             "sid_qwen3_extend_forward_fp8", "sid_extend_attention_fp8_workspace_bytes",
             "sid_flash_decode_noalloc_scratch_bytes", "sid_linear_sample_workspace_bytes",
             "sid_extend_attention_query_rows", "sid_linear_tile", *_SIGNATURES)
 ABI_VERSION = 22
+ABI_REVISION = 1  # entry points added under that version (1: the 8-bit KV pool)
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -182,6 +184,11 @@ class NativeLib:
         self.lib.sid_last_error.argtypes = []
         self.lib.sid_abi_version.restype = ctypes.c_int
         self.lib.sid_abi_version.argtypes = []
+        ver = self.lib.sid_abi_version()
+        _check(ver == ABI_VERSION, f"libsid_hip.so ABI {ver} != expected {ABI_VERSION}; rebuild")
+        rev = self.lib.sid_abi_revision() if hasattr(self.lib, "sid_abi_revision") else 0
+        _check(rev >= ABI_REVISION,
+               f"libsid_hip.so ABI {ver} revision {rev} < expected {ABI_REVISION}; rebuild")
         self.lib.sid_extend_attention_workspace_bytes.restype = ctypes.c_int64
         self.lib.sid_extend_attention_workspace_bytes.argtypes = [_i32, _i64, _i32, _i32, _i32, _i32]
         self.lib.sid_extend_attention_fp8_workspace_bytes.restype = ctypes.c_int64
@@ -203,8 +210,6 @@ class NativeLib:
             fn = getattr(self.lib, name)
             fn.argtypes = argtypes
             fn.restype = ctypes.c_int
-        ver = self.lib.sid_abi_version()
-        _check(ver == ABI_VERSION, f"libsid_hip.so ABI {ver} != expected {ABI_VERSION}; rebuild")
 
     def _call(self, name: str, *args) -> None:
         rc = getattr(self.lib, name)(*args)

@@ -38,6 +38,12 @@ const char* sid_last_error(void);
 int sid_abi_version(void);
 
 /*
+ * Additions under that version, whose entry points a library of a lower revision (or one without
+ * this function: 0) lacks. 1: the 8-bit KV pool.
+ */
+int sid_abi_revision(void);
+
+/*
  * Scatter new K/V rows into the paged KV pool: k_cache[slot[t]] = k[t],
  * v_cache[slot[t]] = v[t]. k, v: bf16 [T, HKV, D]; k_cache, v_cache: bf16
  * [S, HKV, D]; slot_mapping: int64 [T]. Slots < 0 are skipped (padding);

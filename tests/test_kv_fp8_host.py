@@ -82,3 +82,25 @@ def test_step_plan_is_the_plan_that_the_engine_runs(monkeypatch, lens, kv_fp8):
         assert torch.equal(plan["wg_order"], fb.decode_wg_order)
         want = torch.arange(len(lens))[:, None] << 12 | torch.arange(geom[2])
         assert torch.equal((plan["wg_order"] & ~(1 << 30)).sort()[0], want.reshape(-1).int().sort()[0])
+
+
+def test_a_library_from_before_the_8bit_pool_is_refused(tmp_path):
+    """A library of the same ABI version that lacks the entry points added since is named as such."""
+    import subprocess
+
+    from sid.kernels._native import ABI_REVISION, ABI_VERSION, NativeLib
+    for rev, text in ((None, "revision 0"), (ABI_REVISION - 1, f"revision {ABI_REVISION - 1}")):
+        src = tmp_path / f"old{rev}.c"
+        src.write_text('const char* sid_last_error(void) { return ""; }\n'
+                       f"int sid_abi_version(void) {{ return {ABI_VERSION}; }}\n"
+                       + ("" if rev is None else f"int sid_abi_revision(void) {{ return {rev}; }}\n"))
+        lib = tmp_path / f"libold{rev}.so"
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(lib), str(src)], check=True)
+        with pytest.raises(RuntimeError, match=text):
+            NativeLib(lib)
+
+
+def test_library_reports_its_revision():
+    from sid.kernels._native import ABI_REVISION
+    from sid.kernels.jit import load_ext
+    assert load_ext().lib.sid_abi_revision() == ABI_REVISION == 1
