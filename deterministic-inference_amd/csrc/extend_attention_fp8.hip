@@ -7,8 +7,8 @@
 // splits are of 512 keys.
 //
 // Rounded to fewer than 32 bits: p, to bf16 before the product with V (half a step, 2^-8 of p, as
-// over the bf16 pool: both operands of the product are bf16, and P in two parts would double the
-// products), while l sums the unrounded p; and the small elements of a q row that holds far larger
+// over the bf16 pool and in sid/kernels/extend_attention.py:106: both operands of the product are
+// bf16, and P in two parts would double the products), while l sums the unrounded p; and the small elements of a q row that holds far larger
 // ones (QRow). Against 64 bits the result's error, most of it the rounding of the result itself, is
 // 8% (windows, ragged chunks) to 15% (4 x 2048 tokens) above that of fp32 arithmetic rounded once.
 //

@@ -20,7 +20,7 @@ from sid.engine.batch import (DecodeStatic, ForwardBatch, ForwardMode, batch_buc
 from sid.engine.kv_cache import KVCache
 from sid.engine.sampler import sample as _sample
 from sid.kernels.decode_attention import (INVARIANT_VARIANT, DecodeAttention, length_bucket,
-                                          placement)
+                                          placement, stage1_workers)
 from sid.kernels.matmul_persistent import linear_sample_supported
 from sid.model.loader import build_model_config, load_weights, random_weights
 from sid.model.qwen3 import Qwen3Model
@@ -218,7 +218,8 @@ class ModelRunner:
         else:
             (splits, seg, slots), fixed = geom, 0
         order, fb.decode_workers = placement(fb.seq_lens_host, rows, splits, fixed, seg, slots,
-                                             fb.decode_variant, da.cu_count())
+                                             fb.decode_variant, da.cu_count(),
+                                             workers_of=stage1_workers)
         fb.decode_wg_order = None
         if order is None:
             return 0

@@ -392,16 +392,16 @@ def worker_order(tokens: np.ndarray, workers: int) -> np.ndarray:
 
 
 def placement(lengths, rows: int, splits: int, fixed_split: int, seg: int, slots: int,
-              variant: int, cu_count: int) -> tuple:
+              variant: int, cu_count: int, workers_of=stage1_workers) -> tuple:
     """(order, workers) of stage 1 for a plan over requests of these lengths, padded to `rows`:
     the heaviest-first workgroup order (workgroup_order, balanced over the CUs) for the grid,
-    workers 0, or for a worker launch (stage1_workers) the same dealing over the workers
+    workers 0, or for a worker launch (workers_of's rule) the same dealing over the workers
     (worker_order). (None, 0), the grid's own order, where fewer segments than CUs hold tokens:
     there is nothing to balance, and reading the order first costs a small batch 0.2-0.4 us.
     Placement never changes a result."""
     tokens = segment_tokens(lengths, rows, splits, fixed_split, seg, slots)
     nonempty = int(np.count_nonzero(tokens))
-    workers = stage1_workers(nonempty, variant, slots, cu_count)
+    workers = workers_of(nonempty, variant, slots, cu_count)
     if workers == 0 and nonempty < cu_count:
         return None, 0
     return (worker_order(tokens, workers) if workers else workgroup_order(tokens, cu_count)), workers
@@ -503,7 +503,9 @@ class DecodeAttention:
         max_seq_len alone); wg_order: workgroup_order of this plan, on the device (None: the
         grid's own order); workers > 0: stage 1 by that many workgroups, each computing the
         items of wg_order dealt to it (then a permutation of every (request, slot) item; see
-        worker_order); kv_scales: the caches are an 8-bit pool (sid.kernels.kv_fp8)."""
+        worker_order); kv_scales: the caches are an 8-bit pool (sid.kernels.kv_fp8): pass
+        step_plan's arguments there, as the plan made here from the sizes alone is the bf16
+        pool's, up to a quarter slower."""
         if variant is None:
             variant = INVARIANT_VARIANT if invariant else 0
         assert not invariant or variant == INVARIANT_VARIANT, \
