@@ -8,19 +8,20 @@
 //
 // Rounded to fewer than 32 bits: p, to bf16 before the product with V (half a step, 2^-8 of p, as
 // over the bf16 pool and in sid/kernels/extend_attention.py:106: both operands of the product are
-// bf16, and P in two parts would double the products), while l sums the unrounded p; and the small elements of a q row that holds far larger
-// ones (QRow). Against 64 bits the result's error, most of it the rounding of the result itself, is
-// 8% (windows, ragged chunks) to 15% (4 x 2048 tokens) above that of fp32 arithmetic rounded once.
+// bf16, and P in two parts would double the products), while l sums the unrounded p; and the small
+// elements of a q row that holds far larger ones (QRow). Against 64 bits the result's error, most of
+// it the rounding of the result itself, is 8% (ragged chunks) to 15% (4 x 2048 tokens) above that of
+// fp32 arithmetic rounded once.
 //
 // Bound: 4 operations for each of a query's keys and dims. Calls in a row take, for 1 x 8192 tokens,
 // 319 us, 0.86 PFLOP/s; for 4 x 2048 102 us, 0.67, a third of which is the workgroups' first loads
 // and last stores (one of 8 waves fills a CU; a launch alone takes 120). The 2-byte pool's kernel
 // takes 1.19 and 1.08 times as long, 1.5 times on ragged chunks over long prefixes, and 0.93 on
-// 16 x 512 tokens and on windows of 32. The matrix products are 1024 of a
-// tile's 2800 cycles on a SIMD (two waves, 24 products each); the rest is a wave's own chain, V's
-// conversion, the softmax and the loads' addresses, which two waves that start a tile at the same
-// barrier overlap only in part. It is not the LDS (896 cycles a tile of 8 waves, no bank
-// conflicts) nor the count of vector operations (a third fewer: 2%).
+// 16 x 512 tokens and on windows of 32. The matrix products are 1024 of a tile's 2800 cycles on a
+// SIMD (two waves, 24 products each); the rest is a wave's own chain, V's conversion, the softmax and
+// the loads' addresses, which two waves that start a tile at the same barrier overlap only in part.
+// It is not the LDS (896 cycles a tile of 8 waves, no bank conflicts) nor the count of vector
+// operations (a third fewer: 2%).
 #include "extend_tile.h"
 #include "kv_fp8.h"
 
@@ -764,8 +765,8 @@ extern "C" int sid_extend_attention_fp8_fwd(
     hipLaunchKernelGGL(kern, grid, dim3(nw * 64), 0, s, (const bf16_t*)q,
                        (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint16_t*)kv_scales, qo_indptr, kv_indptr, kv_indices, batch,
-                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, per_round, ordered, across,
-                       p.items, (bf16_t*)o, p.part_a, p.part_ml, p.part_n);
+                       num_q_heads, num_kv_heads, num_slots, sm_scale, mtiles, per_round, ordered,
+                       across, p.items, (bf16_t*)o, p.part_a, p.part_ml, p.part_n);
     return check_launch(name);
   };
   if (p.fanout) {
