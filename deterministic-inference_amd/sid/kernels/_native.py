@@ -68,6 +68,11 @@ _SIGNATURES = {
                                  _vp, _i32, _vp],
     "sid_extend_attention_fp8_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
                                      _i32, _i64, _i32, _i32, _f32, _vp, _i64, _vp, _vp],
+    "sid_reshape_and_cache_fp4": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32,
+                                  _i64, _vp],
+    "sid_gather_cache_fp4": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _vp],
+    "sid_rope_rotate": [_vp, _i64, _vp, _i64, _vp, _vp, _f32, _i32, _i32, _i64, _i32, _i32, _i32,
+                        _i64, _vp, _i64, _vp, _i64, _vp],
 }
 EXPORTED = ("sid_last_error", "sid_abi_version", "sid_abi_revision",
             "sid_extend_attention_workspace_bytes",
@@ -97,7 +102,7 @@ def _gpu(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> None:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
 
 
-_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_E4M3, _E8M0, _E2M1 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float4_e2m1fn_x2
 _BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 
@@ -164,6 +169,30 @@ def _pool8(k_cache, v_cache, kv_scales, head_dim: int, device: int) -> tuple:
     raise AssertionError("unreachable")
 
 
+def _pool4(k_cache, v_cache, kv_scales, head_dim: int, device: int) -> tuple:
+    """_pool8 for a 4-bit KV pool; the shape [S, HKV, D] of what it stands for."""
+    try:
+        ks = k_cache.shape
+        if (k_cache.dtype is _E2M1 and v_cache.dtype is _E2M1 and kv_scales.dtype is _E8M0
+                and k_cache.get_device() == v_cache.get_device() == kv_scales.get_device() == device
+                and k_cache.is_contiguous() and v_cache.is_contiguous()
+                and kv_scales.is_contiguous() and len(ks) == 3 and 2 * ks[2] == head_dim
+                and v_cache.shape == ks and kv_scales.shape == (ks[0], ks[1], 2, head_dim // 32)):
+            return ks[0], ks[1], head_dim
+    except AttributeError:
+        pass
+    _gpu(k_cache, "k_cache", _E2M1)
+    _gpu(v_cache, "v_cache", _E2M1)
+    _gpu(kv_scales, "kv_scales", _E8M0)
+    if k_cache.dim() != 3 or 2 * ks[2] != head_dim or v_cache.shape != ks:
+        raise RuntimeError(f"k_cache and v_cache must both be [S, HKV, {head_dim} / 2]")
+    if tuple(kv_scales.shape) != (ks[0], ks[1], 2, head_dim // 32):
+        raise RuntimeError(f"kv_scales must be [S, HKV, 2, {head_dim // 32}] = [{ks[0]}, {ks[1]}, 2, "
+                           f"{head_dim // 32}], got {list(kv_scales.shape)}")
+    _same_device(device, k_cache, v_cache, kv_scales)
+    raise AssertionError("unreachable")
+
+
 def _ptr(t) -> int:
     """Device address of an optional tensor (0 for None)."""
     return 0 if t is None else t.data_ptr()
@@ -207,7 +236,8 @@ class NativeLib:
         self.lib.sid_flash_decode_noalloc_scratch_bytes.restype = ctypes.c_int64
         self.lib.sid_flash_decode_noalloc_scratch_bytes.argtypes = []
         for name, argtypes in _SIGNATURES.items():
-            fn = getattr(self.lib, name)
+            fn = getattr(self.lib, name, None)
+            _check(fn is not None, f"libsid_hip.so has no {name}; rebuild")
             fn.argtypes = argtypes
             fn.restype = ctypes.c_int
 
@@ -345,17 +375,31 @@ class NativeLib:
                    v_cache.data_ptr(), slot_mapping.data_ptr(), ks[0], cs[1], cs[2],
                    cs[0], _stream(k))
 
-    # ---- 8-bit pool ----------------------------------------------------------------------
+    # ---- 8-bit and 4-bit pools -----------------------------------------------------------
 
     def reshape_and_cache_fp8(self, k, v, k_cache, v_cache, kv_scales, slot_mapping) -> None:
-        for name, x in (("k", k), ("v", v)):
+        self._store_rows("sid_reshape_and_cache_fp8", _pool8, k, v, k_cache, v_cache, kv_scales,
+                         slot_mapping)
+
+    def reshape_and_cache_fp4(self, k, v, k_cache, v_cache, kv_scales, slot_mapping) -> None:
+        self._store_rows("sid_reshape_and_cache_fp4", _pool4, k, v, k_cache, v_cache, kv_scales,
+                         slot_mapping)
+
+    def gather_cache_fp8(self, k_cache, v_cache, kv_scales, slots, k, v) -> None:
+        self._load_rows("sid_gather_cache_fp8", _pool8, k_cache, v_cache, kv_scales, slots, k, v)
+
+    def gather_cache_fp4(self, k_cache, v_cache, kv_scales, slots, k, v) -> None:
+        self._load_rows("sid_gather_cache_fp4", _pool4, k_cache, v_cache, kv_scales, slots, k, v)
+
+    def _store_rows(self, name, pool, k, v, k_cache, v_cache, kv_scales, slot_mapping) -> None:
+        for what, x in (("k", k), ("v", v)):
             if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype is torch.bfloat16):
-                raise RuntimeError(f"{name} must be a bf16 GPU tensor")
+                raise RuntimeError(f"{what} must be a bf16 GPU tensor")
         xs, device = k.shape, k.get_device()
         if len(xs) != 3 or v.shape != xs:
             raise RuntimeError("k must be [T, HKV, D], and v must have k's shape")
         t, hkv, d = xs
-        cs = _pool8(k_cache, v_cache, kv_scales, d, device)
+        cs = pool(k_cache, v_cache, kv_scales, d, device)
         if hkv != cs[1]:
             raise RuntimeError("k must be [T, HKV, D] matching the cache")
         _gpu(slot_mapping, "slot_mapping", torch.int64)
@@ -366,29 +410,29 @@ class NativeLib:
         if t == 0:
             return
         sk, sv = k.stride(), v.stride()
-        for name, s in (("k", sk), ("v", sv)):  # heads and dims dense, any token stride
+        for what, s in (("k", sk), ("v", sv)):  # heads and dims dense, any token stride
             if s[2] != 1 or (s[1] != d and hkv > 1):
-                raise RuntimeError(f"{name}'s heads and dims must be contiguous")
+                raise RuntimeError(f"{what}'s heads and dims must be contiguous")
         one = t == 1
-        self._launch(device, "sid_reshape_and_cache_fp8", k.data_ptr(), hkv * d if one else sk[0],
+        self._launch(device, name, k.data_ptr(), hkv * d if one else sk[0],
                      v.data_ptr(), hkv * d if one else sv[0], k_cache.data_ptr(),
                      v_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(), t, hkv, d,
                      cs[0])
 
-    def gather_cache_fp8(self, k_cache, v_cache, kv_scales, slots, k, v) -> None:
+    def _load_rows(self, name, pool, k_cache, v_cache, kv_scales, slots, k, v) -> None:
         _gpu(slots, "slots", torch.int64)
         _gpu(k, "k", torch.bfloat16)
         _gpu(v, "v", torch.bfloat16)
         xs, device = k.shape, slots.get_device()
         if len(xs) != 3 or v.shape != xs:
             raise RuntimeError("k and v must both be [N, HKV, D]")
-        cs = _pool8(k_cache, v_cache, kv_scales, xs[2], device)
+        cs = pool(k_cache, v_cache, kv_scales, xs[2], device)
         if xs[0] != slots.numel() or xs[1] != cs[1]:
             raise RuntimeError("k must be [N, HKV, D] matching the slots and the cache")
         _same_device(device, k, v)
         if xs[0] == 0:
             return
-        self._launch(device, "sid_gather_cache_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
+        self._launch(device, name, k_cache.data_ptr(), v_cache.data_ptr(),
                      kv_scales.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), *xs,
                      cs[0])
 
@@ -464,6 +508,36 @@ class NativeLib:
         _check(cos_sin.dim() == 2 and cos_sin.shape[1] == d, "cos_sin must be [max_pos, D]")
         self._call("sid_rope_apply", q.data_ptr(), k.data_ptr(), positions.data_ptr(),
                    cos_sin.data_ptr(), t, hq, k.shape[1], d, cos_sin.shape[0], _stream(q))
+
+    def rope_rotate(self, q, k, positions, turns, gain: float, rotary_dim: int,
+                    interleaved: bool, max_positions: int, q_out, k_out) -> None:
+        """q_out, k_out <- q, k rotated (sid_rope_rotate); they may be q and k."""
+        device = q.get_device()
+        for name, x in (("q", q), ("k", k), ("q_out", q_out), ("k_out", k_out)):
+            if not (x.is_cuda and x.dtype is _BF16 and x.dim() == 3):
+                raise RuntimeError(f"{name} must be a bf16 GPU tensor [T, heads, D]")
+        t, hq, d = q.shape
+        if k.shape[0] != t or k.shape[2] != d:
+            raise RuntimeError("k must be [T, HKV, D] matching q")
+        _check(q_out.shape == q.shape and k_out.shape == k.shape, "outputs must have the inputs' shapes")
+        _gpu(positions, "positions", _I64)
+        _gpu(turns, "turns", _I64)
+        _check(positions.numel() == t, "positions must have T entries")
+        _check(turns.numel() == rotary_dim // 2, "turns must have rotary_dim / 2 entries")
+        _same_device(device, k, positions, turns, q_out, k_out)
+        if t == 0:
+            return
+
+        def row(x, name):  # heads and dims dense, any token stride
+            s, heads = x.stride(), x.shape[1]
+            if heads and (s[2] != 1 and d > 1 or s[1] != d and heads > 1):
+                raise RuntimeError(f"{name}'s heads and dims must be contiguous")
+            return heads * d if t == 1 else s[0]
+
+        self._launch(device, "sid_rope_rotate", q.data_ptr(), row(q, "q"), k.data_ptr(), row(k, "k"),
+                     positions.data_ptr(), turns.data_ptr(), float(gain), int(rotary_dim),
+                     int(interleaved), t, hq, k.shape[1], d, int(max_positions), q_out.data_ptr(),
+                     row(q_out, "q_out"), k_out.data_ptr(), row(k_out, "k_out"))
 
     def linear(self, x, w, bias, y, out_fp32: bool) -> None:
         m, k, n = self._linear_check(x, w)

@@ -39,7 +39,8 @@ int sid_abi_version(void);
 
 /*
  * Additions under that version, whose entry points a library of a lower revision (or one without
- * this function: 0) lacks. 1: the 8-bit KV pool.
+ * this function: 0) lacks. 1: the 8-bit KV pool. (The 4-bit KV pool and sid_rope_rotate came later
+ * without a number of their own: a library that has them exports their symbols.)
  */
 int sid_abi_revision(void);
 
@@ -665,6 +666,42 @@ int sid_qwen3_extend_forward_fp8(const sid_qwen3_model* m, const sid_extend_batc
                                  void* const* kv_scales, void* workspace,
                                  int64_t workspace_bytes, float* logits, int64_t* tokens,
                                  void* stream);
+
+/*
+ * ---- 4-bit KV pool -------------------------------------------------------------------
+ *
+ * k_cache, v_cache: e2m1 codes [S, HKV, 64] (two a byte, the even element in the low half);
+ * kv_scales: E8M0 bytes [S, HKV, 2, 4], K's four blocks', then V's. A vector of 128 elements (one
+ * slot's head) is four blocks of 32 consecutive ones, each stored as codes c and 2^e with the
+ * smallest e for which max |x| <= 6 2^e, clamped to [-125, 125]; c = e2m1(x 2^-e) (+-0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6), round to nearest even, saturating; byte e + 127. c 2^e is exact in bf16. A
+ * vector that holds an infinity or a NaN is NaN as a whole (byte 255 in its four blocks). These
+ * entry points are the 4-bit forms of the 8-bit pool's, with the same arguments and semantics
+ * otherwise. All operands 16-byte aligned; head_dim 128.
+ */
+int sid_reshape_and_cache_fp4(const void* k, int64_t ldk, const void* v, int64_t ldv,
+                              void* k_cache, void* v_cache, void* kv_scales,
+                              const int64_t* slot_mapping, int64_t num_tokens, int num_kv_heads,
+                              int head_dim, int64_t num_slots, void* stream);
+int sid_gather_cache_fp4(const void* k_cache, const void* v_cache, const void* kv_scales,
+                         const int64_t* slots, void* k, void* v, int64_t n, int num_kv_heads,
+                         int head_dim, int64_t num_slots, void* stream);
+
+/*
+ * Rotary positions from frequencies: q [T, HQ, D], k [T, HKV, D] bf16 with token strides ldq, ldk
+ * (elements, at least a row: they may be columns of a projection) into q_out, k_out with their own.
+ * The first rotary_dim (even) elements of a head turn, as pairs (2i, 2i + 1) if `interleaved`, else
+ * (i, i + rotary_dim / 2); the others are copied. Pair i of token t turns by positions[t] times
+ * turns[i] 2^-64 of a whole turn (uint64 [rotary_dim / 2]), its sine and cosine multiplied with
+ * `gain`. A token whose position is outside [0, max_positions) is copied. q_out may be q (with the
+ * same stride) and k_out k; no other output may overlap an input. head_dim at most 1024. No
+ * counterpart in the reference, whose sid/kernels/rope.py:50-61 rotates halves of whole heads.
+ */
+int sid_rope_rotate(const void* q, int64_t ldq, const void* k, int64_t ldk,
+                    const int64_t* positions, const uint64_t* turns, float gain, int rotary_dim,
+                    int interleaved, int64_t num_tokens, int num_q_heads, int num_kv_heads,
+                    int head_dim, int64_t max_positions, void* q_out, int64_t ldq_out,
+                    void* k_out, int64_t ldk_out, void* stream);
 
 #ifdef __cplusplus
 }

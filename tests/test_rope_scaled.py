@@ -1,0 +1,107 @@
+"""Rotary frequencies of the scaled layouts against their formulas, and refusals (no GPU)."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from sid.kernels.rope import _turn_fractions, scaled_frequencies
+
+YARN = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768)
+
+
+def test_default_and_linear():
+    f, g = scaled_frequencies(128, 1e6)
+    want = torch.tensor([1e6 ** (-2 * i / 128) for i in range(64)], dtype=torch.float64)
+    assert g == 1.0 and torch.allclose(f, want, rtol=1e-15, atol=0)
+    f2, g2 = scaled_frequencies(128, 1e6, dict(type="linear", factor=2.5))
+    assert g2 == 1.0 and torch.allclose(f2 * 2.5, f, rtol=1e-15, atol=0)
+
+
+def test_ntk_keeps_the_first_pair_and_divides_the_last():
+    f, _ = scaled_frequencies(64, 1e4)
+    s, g = scaled_frequencies(64, 1e4, dict(rope_type="ntk", factor=4.0))
+    assert g == 1.0 and s[0] == 1.0
+    assert math.isclose(float(s[-1]) * 4.0, float(f[-1]), rel_tol=1e-12)
+
+
+def test_yarn_by_hand():
+    """128 dims, base 1e6, 32768 positions: 32768 / (2 pi 32) = 163.0 and 32768 / (2 pi) = 5215.2,
+    whose logarithms over ln(1e6) times 64 are 23.6 and 39.6: pairs up to 23 are kept, those from
+    40 on divided by 4."""
+    f, _ = scaled_frequencies(128, 1e6)
+    s, g = scaled_frequencies(128, 1e6, YARN)
+    assert math.isclose(g, 0.1 * math.log(4.0) + 1.0)
+    assert torch.allclose(s[:24], f[:24], rtol=1e-15, atol=0)
+    assert torch.allclose(s[40:], f[40:] / 4.0, rtol=1e-15, atol=0)
+    r = (30 - 23) / (40 - 23)
+    assert math.isclose(float(s[30]), float(f[30]) * (r / 4 + 1 - r), rel_tol=1e-14)
+    assert scaled_frequencies(128, 1e6, dict(YARN, attention_factor=1.0))[1] == 1.0
+    kept = scaled_frequencies(128, 1e6, dict(YARN, beta_fast=2.0))[0]
+    assert torch.allclose(kept[:36], f[:36], rtol=1e-15, atol=0)
+
+
+@pytest.mark.parametrize("scaling,text", [
+    (dict(rope_type="other", factor=2.0), "unknown rope_type"), (dict(rope_type="linear"), "factor"),
+    (dict(rope_type="ntk", factor=0.5), "factor"), (dict(rope_type="yarn", factor=2.0), "original"),
+    (dict(rope_type="linear", factor=float("inf")), "factor"),
+    (dict(YARN, beta_fast=1.0, beta_slow=2.0), "beta_fast"),
+])
+def test_bad_scalings(scaling, text):
+    with pytest.raises(ValueError, match=text):
+        scaled_frequencies(64, 1e4, scaling)
+
+
+def test_bad_layouts():
+    from sid.kernels.rope import RotaryEmbedding
+    for n in (0, 3, 66):
+        with pytest.raises(ValueError, match="rotary_dim"):
+            RotaryEmbedding(64, 16, 1e4, "cpu", rotary_dim=n)
+    with pytest.raises(ValueError, match="theta"):
+        scaled_frequencies(64, 1.0)
+
+
+def test_turn_fractions():
+    """Fractions of a turn to 2^-65: pos times one, modulo 2^64, is the angle in turns."""
+    f, _ = scaled_frequencies(128, 1e6, YARN)
+    t = _turn_fractions(f, "cpu")
+    assert t.dtype == torch.int64 and int(t.min()) > 0
+    for i in (0, 13, 40, 63):
+        got = (int(t[i]) * 131071) % (1 << 64) / 2.0 ** 64
+        want = math.fmod(float(f[i]) * 131071 / (2 * math.pi), 1.0)
+        assert abs(got - want) < 1e-11
+
+
+def test_tables_of_the_whole_head():
+    from sid.kernels.rope import RotaryEmbedding, rope_table
+    plain = RotaryEmbedding(64, 50, 1e4, "cpu", scaling=dict(rope_type="default"))
+    assert torch.equal(plain.cos_sin, rope_table(64, 50, 1e4, "cpu"))
+    r = RotaryEmbedding(64, 50, 1e4, "cpu", scaling=dict(YARN, original_max_position_embeddings=16))
+    f, g = scaled_frequencies(64, 1e4, dict(YARN, original_max_position_embeddings=16))
+    angle = 49 * f
+    want = torch.cat([angle.cos(), angle.sin()]) * g
+    assert torch.allclose(r.cos_sin[49].double(), want, rtol=0, atol=2.0 ** -23)
+    assert RotaryEmbedding(64, 50, 1e4, "cpu", interleaved=True).cos_sin is None
+    assert RotaryEmbedding(64, 50, 1e4, "cpu", rotary_dim=32).cos_sin is None
+
+
+def test_entry_point_refuses_bad_arguments():
+    from sid.kernels.jit import load_ext
+    lib = load_ext().lib
+
+    def call(q=16, ldq=512, k=16, ldk=256, pos=16, rot=64, t=1, hq=4, hkv=2, d=128, qo=32, ldqo=512,
+             ko=32, ldko=256):
+        return lib.sid_rope_rotate(q, ldq, k, ldk, pos, 16, ctypes.c_float(1.0), rot, 0, t, hq, hkv,
+                                   d, 100, qo, ldqo, ko, ldko, None)
+
+    for bad, text in ((dict(t=-1), b"negative"), (dict(q=0), b"null"), (dict(ko=0), b"null"),
+                      (dict(pos=0), b"null"), (dict(rot=63), b"rotary_dim"), (dict(rot=0), b"rotary_dim"),
+                      (dict(rot=130), b"rotary_dim"), (dict(d=2048, ldq=1 << 20), b"head_dim"),
+                      (dict(ldq=500), b"stride"), (dict(ldko=255), b"stride"),
+                      (dict(qo=16, ldqo=1024), b"in place"), (dict(hq=-1), b"head counts"),
+                      (dict(hq=0, hkv=0), b"head counts"), (dict(t=1 << 31), b"too many")):
+        assert call(**bad) == 1 and text in lib.sid_last_error(), bad
+    assert call(t=0) == 0
