@@ -71,6 +71,11 @@ _SIGNATURES = {
     "sid_reshape_and_cache_fp4": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32,
                                   _i64, _vp],
     "sid_gather_cache_fp4": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _vp],
+    "sid_flash_decode_fp4_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64,
+                                 _i32, _i32, _i32, _i32, _i32, _vp, _f32, _vp, _vp, _i32, _i32,
+                                 _vp, _i32, _vp],
+    "sid_extend_attention_fp4_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
+                                     _i32, _i64, _i32, _i32, _f32, _vp, _i64, _vp, _vp],
     "sid_rope_rotate": [_vp, _i64, _vp, _i64, _vp, _vp, _f32, _i32, _i32, _i64, _i32, _i32, _i32,
                         _i64, _vp, _i64, _vp, _i64, _vp],
 }
@@ -79,6 +84,7 @@ EXPORTED = ("sid_last_error", "sid_abi_version", "sid_abi_revision",
             "sid_linear_argmax_workspace_bytes", "sid_sample_workspace_bytes",
             "sid_qwen3_extend_workspace_bytes", "sid_qwen3_extend_forward",
             "sid_qwen3_extend_forward_fp8", "sid_extend_attention_fp8_workspace_bytes",
+            "sid_extend_attention_fp4_workspace_bytes",
             "sid_flash_decode_noalloc_scratch_bytes", "sid_linear_sample_workspace_bytes",
             "sid_extend_attention_query_rows", "sid_linear_tile", *_SIGNATURES)
 ABI_VERSION = 22
@@ -193,6 +199,13 @@ def _pool4(k_cache, v_cache, kv_scales, head_dim: int, device: int) -> tuple:
     raise AssertionError("unreachable")
 
 
+def _code_pool(k_cache, v_cache, kv_scales, head_dim: int, device: int) -> tuple:
+    """Checks a KV pool of codes by its type; ("fp8" or "fp4", its shape [S, HKV, D])."""
+    if getattr(k_cache, "dtype", None) is _E2M1:
+        return "fp4", _pool4(k_cache, v_cache, kv_scales, head_dim, device)
+    return "fp8", _pool8(k_cache, v_cache, kv_scales, head_dim, device)
+
+
 def _ptr(t) -> int:
     """Device address of an optional tensor (0 for None)."""
     return 0 if t is None else t.data_ptr()
@@ -220,9 +233,12 @@ class NativeLib:
                f"libsid_hip.so ABI {ver} revision {rev} < expected {ABI_REVISION}; rebuild")
         self.lib.sid_extend_attention_workspace_bytes.restype = ctypes.c_int64
         self.lib.sid_extend_attention_workspace_bytes.argtypes = [_i32, _i64, _i32, _i32, _i32, _i32]
-        self.lib.sid_extend_attention_fp8_workspace_bytes.restype = ctypes.c_int64
-        self.lib.sid_extend_attention_fp8_workspace_bytes.argtypes = [_i32, _i64, _i32, _i32, _i32,
-                                                                      _i32]
+        for name in ("sid_extend_attention_fp8_workspace_bytes",
+                     "sid_extend_attention_fp4_workspace_bytes"):
+            fn = getattr(self.lib, name, None)
+            _check(fn is not None, f"libsid_hip.so has no {name}; rebuild")
+            fn.restype = ctypes.c_int64
+            fn.argtypes = [_i32, _i64, _i32, _i32, _i32, _i32]
         self.lib.sid_extend_attention_query_rows.restype = ctypes.c_int
         self.lib.sid_extend_attention_query_rows.argtypes = [_i32, _i64, _i32, _i32]
         self.lib.sid_linear_tile.restype = ctypes.c_int
@@ -268,14 +284,14 @@ class NativeLib:
         partition, the default workgroup shape, the grid's own order); workers > 0: stage 1
         by that many workgroups over the items of wg_order (sid_flash_decode_workers_fwd; entries
         flagged ORDER_EMPTY hold no tokens); kv_scales: the caches are an 8-bit pool
-        (sid_flash_decode_fp8_fwd)."""
+        (sid_flash_decode_fp8_fwd) or, of that type, a 4-bit one (sid_flash_decode_fp4_fwd)."""
         usual = kv_scales is not None and _usual_decode(q, kv_indptr, kv_indices, part_o, part_lse, o)
         if not usual:
             _gpu(q, "q", torch.bfloat16)
         _check(q.dim() == 3, "q must be [B, HQ, D]")
         b, hq, d = qs = q.shape  # (each .shape builds a new object: taken once)
         if kv_scales is not None:
-            ks = _pool8(k_cache, v_cache, kv_scales, d, q.get_device())
+            kind, ks = _code_pool(k_cache, v_cache, kv_scales, d, q.get_device())
             if usual:
                 _same_device(q.get_device(), num_splits, wg_order)
             else:
@@ -314,7 +330,7 @@ class NativeLib:
                 int(variant), order, float(sm_scale), part_o.data_ptr(), part_lse.data_ptr(),
                 po[0], po[2], o.data_ptr(), int(workers))
         if kv_scales is not None:
-            self._launch(q.get_device(), "sid_flash_decode_fp8_fwd", q.data_ptr(), k_cache.data_ptr(),
+            self._launch(q.get_device(), f"sid_flash_decode_{kind}_fwd", q.data_ptr(), k_cache.data_ptr(),
                          v_cache.data_ptr(), kv_scales.data_ptr(), *plan)
             return
         self._call("sid_flash_decode_workers_fwd", q.data_ptr(), k_cache.data_ptr(),
@@ -439,19 +455,21 @@ class NativeLib:
     # ---- the rest of the decode path ----------------------------------------------------
 
     def extend_attention_workspace_bytes(self, batch, total_q, hq, hkv, max_extend_len,
-                                         max_kv_len, fp8: bool = False) -> int:
+                                         max_kv_len, fp8: bool = False, fp4: bool = False) -> int:
         fn = (self.lib.sid_extend_attention_fp8_workspace_bytes if fp8
+              else self.lib.sid_extend_attention_fp4_workspace_bytes if fp4
               else self.lib.sid_extend_attention_workspace_bytes)
         return int(fn(batch, total_q, hq, hkv, max_extend_len, max_kv_len))
 
     def extend_attention_fwd(self, q, k_buffer, v_buffer, qo_indptr, kv_indptr, kv_indices,
                              max_extend_len: int, sm_scale: float, o, max_kv_len: int,
                              workspace=None, kv_scales=None) -> None:
-        """kv_scales: the buffers are an 8-bit pool (sid_extend_attention_fp8_fwd)."""
+        """kv_scales: the buffers are an 8-bit pool (sid_extend_attention_fp8_fwd) or, of that type, a
+        4-bit one (sid_extend_attention_fp4_fwd)."""
         _gpu(q, "q_extend", torch.bfloat16)
         _check(q.dim() == 3, "q_extend must be [Text, HQ, D]")
         if kv_scales is not None:
-            _pool8(k_buffer, v_buffer, kv_scales, q.shape[2], q.get_device())
+            kind, _ = _code_pool(k_buffer, v_buffer, kv_scales, q.shape[2], q.get_device())
             _same_device(q.get_device(), qo_indptr, kv_indptr, kv_indices, o, workspace)
         else:
             _gpu(k_buffer, "k_buffer", torch.bfloat16)
@@ -473,7 +491,7 @@ class NativeLib:
                 k_buffer.shape[0], int(max_extend_len), int(max_kv_len), float(sm_scale), ws_ptr,
                 ws_bytes, o.data_ptr())
         if kv_scales is not None:
-            self._launch(q.get_device(), "sid_extend_attention_fp8_fwd", q.data_ptr(), k_buffer.data_ptr(),
+            self._launch(q.get_device(), f"sid_extend_attention_{kind}_fwd", q.data_ptr(), k_buffer.data_ptr(),
                          v_buffer.data_ptr(), kv_scales.data_ptr(), *rest)
             return
         self._call("sid_extend_attention_fwd", q.data_ptr(), k_buffer.data_ptr(),

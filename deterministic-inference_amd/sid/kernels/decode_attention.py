@@ -300,6 +300,11 @@ def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int) -
     return best[1], best[2]
 
 
+def plan_variant_fp4(lengths, max_len: int, cu_count: int, max_kv_splits: int) -> tuple:
+    """plan_variant_fp8 for a 4-bit pool (sid_flash_decode_fp4_fwd)."""
+    return plan_variant_fp8(lengths, max_len, cu_count, max_kv_splits)
+
+
 ORDER_SLOT_BITS = 12  # sid_flash_decode_segments_fwd wg_order entries: request << 12 | slot
 ORDER_EMPTY = 1 << 30  # wg_order entry flag of a worker launch: the item holds no tokens
 
@@ -464,17 +469,20 @@ class DecodeAttention:
         splits, seg, slots = geometry
         return None, splits, 0, seg, slots
 
-    def pick_plan(self, lengths, max_len: int, kv_fp8: bool) -> tuple:
+    def pick_plan(self, lengths, max_len: int, kv_fp8: bool, kv_fp4: bool = False) -> tuple:
         """((grid splits, segment size, grid slots), stage-1 variant) of a nondet/dvr step over
         requests of these lengths, none longer than max_len: plan_variant, or plan_variant_fp8
-        for an 8-bit pool."""
+        for an 8-bit pool, plan_variant_fp4 for a 4-bit one."""
         cu = self.cu_count()
+        if kv_fp4:
+            return plan_variant_fp4(lengths, max_len, cu, self.max_kv_splits)
         if kv_fp8:
             return plan_variant_fp8(lengths, max_len, cu, self.max_kv_splits)
         return plan_variant(lengths, max_len, self.num_kv_heads, cu, self.max_kv_splits,
                             invariant=False)
 
-    def step_plan(self, lengths, kv_fp8: bool = False, max_len: int | None = None) -> dict:
+    def step_plan(self, lengths, kv_fp8: bool = False, max_len: int | None = None,
+                  kv_fp4: bool = False) -> dict:
         """The nondet/dvr plan of a decode step over requests of these lengths (host-side), as
         forward's arguments: geometry and workgroup shape (pick_plan) and the placement of the
         workgroups (placement). One plan serves the step's layers. Its order is copied to the
@@ -482,7 +490,7 @@ class DecodeAttention:
         with, if it is not the longest length."""
         lens = [int(n) for n in lengths]
         bound = max(max(lens, default=1) if max_len is None else int(max_len), 1)
-        geom, variant = self.pick_plan(lens, bound, kv_fp8)
+        geom, variant = self.pick_plan(lens, bound, kv_fp8, kv_fp4)
         host, workers = placement(lens, len(lens), geom[0], 0, geom[1], geom[2], variant,
                                   self.cu_count())
         order = None if host is None else torch.from_numpy(host).to(self.device)

@@ -40,6 +40,7 @@ _ext = None
 SOURCE_FLAGS = {
     "extend_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "extend_attention_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "extend_attention_fp4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

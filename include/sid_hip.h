@@ -688,6 +688,35 @@ int sid_gather_cache_fp4(const void* k_cache, const void* v_cache, const void* k
                          int head_dim, int64_t num_slots, void* stream);
 
 /*
+ * sid_flash_decode_fp8_fwd over a 4-bit pool. The workgroup shapes that `variant` picks are this
+ * kernel's own (part of the reduction order): 2 = 8 waves x 8 tokens per wave iteration, 0, 1 and
+ * 3 = 4 x 8.
+ */
+int sid_flash_decode_fp4_fwd(const void* q, const void* k_cache, const void* v_cache,
+                             const void* kv_scales, const int32_t* kv_indptr,
+                             const int32_t* kv_indices, const int32_t* num_splits, int batch,
+                             int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
+                             int max_splits, int fixed_split_size, int segment_size,
+                             int grid_slots, int variant, const int32_t* wg_order,
+                             float sm_scale, float* part_o, float* part_lse, int part_batch,
+                             int part_stride, void* o, int workers, void* stream);
+
+/*
+ * sid_extend_attention_fp8_fwd over a 4-bit pool, with its invariances, its treatment of q and of
+ * NaN vectors, and its workspace (of sid_extend_attention_fp4_workspace_bytes(...) bytes).
+ */
+int64_t sid_extend_attention_fp4_workspace_bytes(int batch, int64_t total_q, int num_q_heads,
+                                                 int num_kv_heads, int max_extend_len,
+                                                 int max_kv_len);
+int sid_extend_attention_fp4_fwd(const void* q, const void* k_cache, const void* v_cache,
+                                 const void* kv_scales, const int32_t* qo_indptr,
+                                 const int32_t* kv_indptr, const int32_t* kv_indices, int batch,
+                                 int64_t total_q, int num_q_heads, int num_kv_heads,
+                                 int head_dim, int64_t num_slots, int max_extend_len,
+                                 int max_kv_len, float sm_scale, void* workspace,
+                                 int64_t workspace_bytes, void* o, void* stream);
+
+/*
  * Rotary positions from frequencies: q [T, HQ, D], k [T, HKV, D] bf16 with token strides ldq, ldk
  * (elements, at least a row: they may be columns of a projection) into q_out, k_out with their own.
  * The first rotary_dim (even) elements of a head turn, as pairs (2i, 2i + 1) if `interleaved`, else
