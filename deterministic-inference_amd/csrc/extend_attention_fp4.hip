@@ -32,7 +32,10 @@ constexpr int kSplitTiles = kSplit / BN;
 constexpr int kKTile = BN * D / 2;
 constexpr int kVAt = 2 * kKTile;  // [2] K tiles, [2] V tiles, [2] K scale words
 constexpr int kScalesAt = kVAt + 2 * kTileBytes;
-constexpr int kLdsBytes = kScalesAt + 2 * 256;
+constexpr int kParkedAt = kScalesAt + 2 * 256;
+// The rows' folded state stays in the LDS between two folds, 8 tiles apart: 8 accumulator vectors a
+// lane and row set (the registers hold the state of the split in work).
+constexpr int lds_bytes(int sets, bool fanout) { return kParkedAt + (fanout ? 0 : 8 * sets * NW * 1024); }
 
 __device__ __forceinline__ int swk(int key) { return (key >> 3) & 3; }
 
@@ -49,7 +52,7 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     int64_t num_slots, float sm_scale, int mtiles, int per_round, int ordered, int across,
     int64_t items, bf16_t* __restrict__ o, float* __restrict__ part_a,
     float* __restrict__ part_ml, int32_t* __restrict__ part_n) {
-  __shared__ __align__(1024) char lds[kLdsBytes];
+  __shared__ __align__(1024) char lds[lds_bytes(SETS, FANOUT)];
   constexpr int ROWS = 8 * NW * SETS;
   int b, h_kv, mtile, split = 0;
   if constexpr (FANOUT) {
@@ -199,26 +202,31 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
 
   // A step takes the softmax of its tile t between the products of two others: S of tile t + 1 (qk)
   // and the output of tile t - 1 (pv), so that no product waits for this tile's exponentials nor
-  // they for it. The softmax is dealt over 8 slices of 2 elements a row set; with them go qk n: key
-  // block n / 2, q's hi part, then its lo part, and pv n: key half n / 4, dim blocks 2 (n % 4) and the
-  // next.
+  // they for it. The softmax is dealt over 8 slices of 2 elements a row set; with them go pv n: key
+  // half n / 4, dim blocks 2 (n % 4) and the next; and two slices behind the key block's softmax, as its
+  // results take the place of the scores that are used up, qk n: key block n / 2, q's hi part, then
+  // its lo part.
   typedef __attribute__((address_space(3))) const u32x4_v* lds_u4_t;
   typedef __attribute__((address_space(3))) s16x4_v* tr_ptr_t;
   u32x4_v kf[2];
-  s16x4_v vw[2][2][2];
-  f32x4_v next[SETS][4];  // S of the next tile
-  float s[SETS][16];      // S of this one: key 8 g + i, or 32 + 8 g + i - 8
-  uint4 pn[SETS][2];      // P of this tile, and of the one before
+  s16x4_v vw[3][2][2];
+  f32x4_v s[SETS][4];  // S: row 4 g + i of key block j at [j][i]
+  uint4 pn[SETS][2];   // P of this tile, and of the one before
   bf16x8_v pf[SETS][2];
   float m[SETS], l[SETS];  // (l: this lane's 16 keys of every tile)
   f32x4_v acc[SETS][8];
-  RowState run[SETS];
+  float run_m[SETS], run_l[SETS];
+  typedef __attribute__((address_space(3))) f32x4_v* park_t;
+  const park_t parked = (park_t)(lds0 + kParkedAt + 16 * tid);  // vector db of set e: + 64 NW (8 e + db)
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
-    m[e] = run[e].m = NEG_BIG;
-    l[e] = run[e].l = 0.0f;
+    m[e] = run_m[e] = NEG_BIG;
+    l[e] = run_l[e] = 0.0f;
 #pragma unroll
-    for (int db = 0; db < 8; ++db) acc[e][db] = run[e].acc[db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int db = 0; db < 8; ++db) {
+      acc[e][db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (!FANOUT) parked[64 * NW * (8 * e + db)] = acc[e][db];
+    }
     pf[e][0] = pf[e][1] = bf16x8_v{};
   }
   auto read_k = [&](auto j_, int buf) {
@@ -226,51 +234,36 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     kf[j & 1] = *(lds_u4_t)(ka + buf * kKTile + (32 * (j >> 1) + 4 * (j & 1)) * (D / 2));
   };
   // V fragments: A = V^T rows 16 db + r (dims), columns 32 kb + 8 g .. +7 (keys), by two
-  // transpose reads (extend_attention.hip): slice n's, before the products of the slice before it.
+  // transpose reads (extend_attention.hip): slice n's, two slices ahead.
   auto read_v = [&](auto n_, int buf) {
     constexpr int n = decltype(n_)::value;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t at = va[2 * (n & 3) + i] + buf * kTileBytes + 8192 * (n >> 2);
-      vw[n & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
-      vw[n & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 1024));
+      vw[n % 3][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
+      vw[n % 3][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 1024));
     }
   };
-  auto qk = [&](auto n_, int ks) {
+  auto qk = [&](auto n_, int e, int ks) {
     constexpr int n = decltype(n_)::value, j = n >> 1;
     constexpr bool lo = (n & 1) != 0;
     const u32x4_v kk = kf[j & 1];
     const i32x8_v a{(int)kk.x, (int)kk.y, (int)kk.z, (int)kk.w, 0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < SETS; ++e) {
-      // (formats 4 and 0: e2m1 and e4m3; the scale operands' byte is an immediate: key block j of ks,
-      // hi or lo of the row's scale)
-      if constexpr (lo)
-        next[e][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[e].lo, next[e][j], 4, 0, j, ks, 1, qf[e].scale);
-      else
-        next[e][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            a, qf[e].hi, f32x4_v{0.0f, 0.0f, 0.0f, 0.0f}, 4, 0, j, ks, 0, qf[e].scale);
-    }
+    // (formats 4 and 0: e2m1 and e4m3; the scale operands' byte is an immediate: key block j of ks,
+    // hi or lo of the row's scale)
+    if constexpr (lo)
+      s[e][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[e].lo, s[e][j], 4, 0, j, ks, 1, qf[e].scale);
+    else
+      s[e][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          a, qf[e].hi, f32x4_v{0.0f, 0.0f, 0.0f, 0.0f}, 4, 0, j, ks, 0, qf[e].scale);
   };
-  auto pv = [&](auto n_) {
+  auto pv = [&](auto n_, int i, int e) {
     constexpr int n = decltype(n_)::value;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bf16x8_v vf = __builtin_bit_cast(
-          bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(vw[n & 1][i][0], vw[n & 1][i][1], 0,
-                                                                 1, 2, 3, 4, 5, 6, 7)));
-#pragma unroll
-      for (int e = 0; e < SETS; ++e) {
-        f32x4_v& a = acc[e][2 * (n & 3) + i];
-        a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[e][n >> 2], a, 0, 0, 0);
-      }
-    }
-  };
-  auto take_scores = [&] {
-#pragma unroll
-    for (int e = 0; e < SETS; ++e)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[e][i] = next[e][i >> 2][i & 3];
+    const bf16x8_v vf = __builtin_bit_cast(
+        bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(vw[n % 3][i][0], vw[n % 3][i][1], 0, 1, 2,
+                                                               3, 4, 5, 6, 7)));
+    f32x4_v& a = acc[e][2 * (n & 3) + i];
+    a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[e][n >> 2], a, 0, 0, 0);
   };
   auto each = [](auto f) {  // f(0) .. f(7), as constants
     f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{});
@@ -279,55 +272,66 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     f(std::integral_constant<int, 6>{}); f(std::integral_constant<int, 7>{});
   };
   typedef std::integral_constant<int, 0> c0;
-  auto barrier = [&] {
-    // Every load has landed (they had a whole tile's time) and every wave is done with the buffers
-    // that are written next.
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-  };
+  auto point = [] { __builtin_amdgcn_sched_barrier(0); };
   // The state (om, ol) and acc of a split that is complete, into the rows'.
   auto fold_split = [&](const float (&om)[SETS], const float (&ol)[SETS]) {
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
-      const FoldScale f = fold_scale(run[e].m, om[e]);
-      run[e].l = fold_elem(run[e].l, pair32_sum(pair16_sum(ol[e])), f);
-      run[e].m = f.mn;
+      const FoldScale f = fold_scale(run_m[e], om[e]);
+      run_l[e] = fold_elem(run_l[e], pair32_sum(pair16_sum(ol[e])), f);
+      run_m[e] = f.mn;
 #pragma unroll
-      for (int db = 0; db < 8; ++db)
+      for (int db = 0; db < 8; ++db) {
+        f32x4_v a = parked[64 * NW * (8 * e + db)];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) run[e].acc[db][i] = fold_elem(run[e].acc[db][i], acc[e][db][i], f);
+        for (int i = 0; i < 4; ++i) a[i] = fold_elem(a[i], acc[e][db][i], f);
+        parked[64 * NW * (8 * e + db)] = a;
+      }
     }
   };
 
   // Tile t's step. MASK: some key of it may be hidden from some row. FIRST: of a split.
   auto step = [&](auto mask, auto first, int t, auto buf) {
     constexpr bool kMask = decltype(mask)::value, kFirst = decltype(first)::value;
-    barrier();
+    // Every wave is done with the buffers that are written next, and every load has landed (they had a
+    // whole tile's time) but V's, the last that went out, which the step's end waits for.
+    point();
+    asm volatile("s_waitcnt vmcnt(1) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    point();
     const bool mine = !kMask || t <= w_tiles;  // (at w_tiles the tile before is still to be added)
     int ks = 0;
     if (mine) {
+      read_v(c0{}, other(buf));
+      read_v(std::integral_constant<int, 1>{}, other(buf));
       ks = *(__attribute__((address_space(3))) const int*)(sa + 256 * other(buf));
       read_k(c0{}, other(buf));
-      read_v(c0{}, other(buf));
     }
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" : "+v"(raw), "+v"(sc0), "+v"(scales_in.x), "+v"(scales_in.y));  // (not ahead of the barrier)
-    store_v(sc0, buf);
-    sc0 = sc1;
-    sc1 = my_scales(scales_in);
-    store_scales(sc1, buf);
-    load_v(sl1);
+    point();
+    asm volatile("" : "+v"(scales_in.x), "+v"(scales_in.y));  // (not looked at ahead of the barrier)
+    const uint32_t sc2nd = my_scales(scales_in);
+    store_scales(sc2nd, buf);
     check(sl3);
     scales_in = load_scales(sl3);
-    const uint32_t k_at = sl2;
+    const uint32_t k_at = sl2, v_at = sl1;
     sl1 = sl2;
     sl2 = sl3;
     sl3 = load_slot(t + 4);
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 2 < t_end) load_k(k_at, buf);  // last: a wait for an earlier load would include the DMA
-    __builtin_amdgcn_sched_barrier(0);
-    if (!mine) return;
+    point();
+    if (t + 2 < t_end) load_k(k_at, buf);
+    point();
+    auto stage_v = [&] {
+      asm volatile("" : "+v"(raw));
+      store_v(sc0, buf);
+      sc0 = sc1;
+      sc1 = sc2nd;
+      point();
+      load_v(v_at);  // last
+      point();
+    };
+    if (!mine) {
+      stage_v();
+      return;
+    }
     float om[SETS], ol[SETS];
     bool vis[16];
     if constexpr (kMask) {
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
       }
       tmax[e] = NEG_BIG;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) tmax[e] = fmaxf(tmax[e], !kMask || vis[i] ? s[e][i] : NEG_BIG);
+      for (int i = 0; i < 16; ++i) tmax[e] = fmaxf(tmax[e], !kMask || vis[i] ? s[e][i >> 2][i & 3] : NEG_BIG);
       high |= tmax[e] * sc2 > m[e] + LAZY_T;
     }
     // Each lane looks at its own scores: only where one of them is LAZY_T above its row's
@@ -366,30 +370,63 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
         if constexpr (!kFirst) l[e] *= rescale[e];
       }
     }
+    // (One wave has a SIMD to itself: while a product runs, only what follows it in program order can
+    // issue, and a second product behind it waits for the first. So between two products stands about
+    // as much of the softmax as the first one takes: 34 cycles a qk, 16 a pv, 16 an exponential.)
     each([&](auto n_) {
-      constexpr int n = decltype(n_)::value;
-      __builtin_amdgcn_sched_barrier(0);
-      qk(n_, ks);
-      if constexpr (n % 2 == 0 && n < 6) read_k(std::integral_constant<int, n / 2 + 1>{}, other(buf));
-      if constexpr (n < 7) read_v(std::integral_constant<int, n + 1>{}, other(buf));
+      constexpr int n = decltype(n_)::value, j = n >> 1, i0 = 2 * (n & 1);
+      typedef std::integral_constant<int, n < 2 ? 0 : n - 2> nq;
+      float x[SETS][2], p[SETS][2];
+      point();
+      if constexpr (n < 6) read_v(std::integral_constant<int, n + 2>{}, other(buf));
+      if constexpr (n % 2 == 0 && n > 0) read_k(std::integral_constant<int, n / 2>{}, other(buf));
+#pragma unroll
+      for (int e = 0; e < SETS; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[e][i] = __builtin_fmaf(s[e][j][i0 + i], sc2, -m[e]);
+      point();
+      if constexpr (n >= 2) qk(nq{}, 0, ks);
+      point();
+      p[0][0] = exp2_fast(x[0][0]);
+      p[0][1] = exp2_fast(x[0][1]);
+      point();
+      if constexpr (n >= 2 && SETS == 2) qk(nq{}, 1, ks);
+      point();
+      if constexpr (SETS == 2) {
+        p[1][0] = exp2_fast(x[1][0]);
+        p[1][1] = exp2_fast(x[1][1]);
+      }
 #pragma unroll
       for (int e = 0; e < SETS; ++e) {
-        float p[2];
+        point();
+        pv(n_, 0, e);
+        point();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          p[i] = exp2_fast(__builtin_fmaf(s[e][2 * n + i], sc2, -m[e]));
-          if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
-          l[e] += p[i];
+          if constexpr (kMask) p[e][i] = vis[2 * n + i] ? p[e][i] : 0.0f;
+          l[e] += p[e][i];
         }
-        reinterpret_cast<uint32_t*>(&pn[e][n >> 2])[n & 3] = pack_bf16x2(p[0], p[1]);
+        reinterpret_cast<uint32_t*>(&pn[e][n >> 2])[n & 3] = pack_bf16x2(p[e][0], p[e][1]);
       }
-      pv(n_);
+#pragma unroll
+      for (int e = 0; e < SETS; ++e) {
+        point();
+        pv(n_, 1, e);
+      }
+      point();
     });
-    __builtin_amdgcn_sched_barrier(0);
+    // The last key block's products, with V's conversion between them.
+    qk(std::integral_constant<int, 6>{}, 0, ks);
+    if constexpr (SETS == 2) qk(std::integral_constant<int, 6>{}, 1, ks);
+    point();
+    stage_v();
+    qk(std::integral_constant<int, 7>{}, 0, ks);
+    if constexpr (SETS == 2) qk(std::integral_constant<int, 7>{}, 1, ks);
+    point();
     // (here, not where the next step uses them: past the branches below they would move there)
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
-      asm volatile("" : "+v"(next[e][0]), "+v"(next[e][1]), "+v"(next[e][2]), "+v"(next[e][3]));
+      asm volatile("" : "+v"(s[e][0]), "+v"(s[e][1]), "+v"(s[e][2]), "+v"(s[e][3]));
       asm volatile("" : "+v"(l[e]), "+v"(pn[e][0].x), "+v"(pn[e][0].y), "+v"(pn[e][0].z), "+v"(pn[e][0].w),
                    "+v"(pn[e][1].x), "+v"(pn[e][1].y), "+v"(pn[e][1].z), "+v"(pn[e][1].w));
     }
@@ -411,10 +448,14 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     for (int e = 0; e < SETS; ++e)
 #pragma unroll
       for (int i = 0; i < 2; ++i) pf[e][i] = __builtin_bit_cast(bf16x8_v, pn[e][i]);
-    take_scores();
   };
 
   // S of the first tile.
+  auto barrier = [&] {
+    point();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    point();
+  };
   barrier();
   {
     const int ks = *(__attribute__((address_space(3))) const int*)sa;
@@ -422,9 +463,9 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     each([&](auto n_) {
       constexpr int n = decltype(n_)::value;
       if constexpr (n < 6 && n % 2 == 0) read_k(std::integral_constant<int, n / 2 + 1>{}, 0);
-      qk(n_, ks);
+#pragma unroll
+      for (int e = 0; e < SETS; ++e) qk(n_, e, ks);
     });
-    take_scores();
   }
   // Tiles that every row of the workgroup sees whole, in pairs (their buffers' addresses are
   // immediates), then the others with the mask: one loop each, split by split (a branch between
@@ -455,7 +496,10 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
       constexpr int n = decltype(n_)::value;
       if constexpr (n < 7) read_v(std::integral_constant<int, n + 1>{}, buf);
       __builtin_amdgcn_sched_barrier(0);
-      pv(n_);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < SETS; ++e) pv(n_, i, e);
     });
   }
   if constexpr (FANOUT) {
@@ -477,7 +521,12 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     fold_split(m, l);
 #pragma unroll
     for (int e = 0; e < SETS; ++e)
-      if (row_ok) store_row(o + (prow + e) * D, run[e], g);
+    {
+      RowState run{run_m[e], run_l[e], {}};
+#pragma unroll
+      for (int db = 0; db < 8; ++db) run.acc[db] = parked[64 * NW * (8 * e + db)];
+      if (row_ok) store_row(o + (prow + e) * D, run, g);
+    }
   }
 }
 
