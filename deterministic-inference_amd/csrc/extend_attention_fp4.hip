@@ -22,20 +22,26 @@ namespace {
 constexpr int NW = 4;  // waves of a workgroup
 constexpr int kSplit = 512;  // keys per split: the unit in which a row's state is folded
 constexpr int kSplitTiles = kSplit / BN;
+// How far above its row's reference maximum a score may be, in log2 units.
+constexpr float kLazy = 24.0f;
 
 // ---- LDS ---------------------------------------------------------------------------------
 //
-// A tile is 64 keys. K stays in codes, 64 bytes a key: 16-byte unit u of a key's row holds block
-// u ^ swk(key), so that the 16 rows of a fragment read fall on all 64 banks. V is bf16 (swv). Beside
-// them K's scale bytes as the matrix instruction takes them: word l holds lane l's for the tile's
-// four key blocks.
-constexpr int kKTile = BN * D / 2;
-constexpr int kVAt = 2 * kKTile;  // [2] K tiles, [2] V tiles, [2] K scale words
-constexpr int kScalesAt = kVAt + 2 * kTileBytes;
-constexpr int kParkedAt = kScalesAt + 2 * 256;
-// The rows' folded state stays in the LDS between two folds, 8 tiles apart: 8 accumulator vectors a
-// lane and row set (the registers hold the state of the split in work).
-constexpr int lds_bytes(int sets, bool fanout) { return kParkedAt + (fanout ? 0 : 8 * sets * NW * 1024); }
+// Two tiles of 64 keys, as four sub-tiles of 32. K stays in codes, 64 bytes a key: 16-byte unit u of a
+// key's row holds block u ^ swk(key), so that the 16 rows of a fragment read fall on all 64 banks. V
+// is bf16 (swv). Beside them K's scale bytes as the matrix instruction takes them: half-word l of a
+// sub-tile holds lane l's for its two key blocks.
+constexpr int BS = 32;  // keys of a sub-tile
+constexpr int kKSub = BS * D / 2, kVSub = BS * D * 2, kScaleSub = 128;
+constexpr int kVAt = 4 * kKSub;
+constexpr int kScalesAt = kVAt + 4 * kVSub;
+// The rows' folded state stays in the LDS between two folds, 512 keys apart (the registers hold the
+// state of the split in work): a lane's 8 accumulator vectors a row set, and the rows' m and l.
+constexpr int kSpareAt = kScalesAt + 4 * kScaleSub;  // a vector of each thread
+constexpr int kRunAt = kSpareAt + NW * 1024;
+constexpr int lds_bytes(int sets, bool fanout) {
+  return kRunAt + (fanout ? 0 : sets * NW * (8 * 1024 + 128));
+}
 
 __device__ __forceinline__ int swk(int key) { return (key >> 3) & 3; }
 
@@ -103,11 +109,12 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   const int w_tiles =
       w_row < extend_len ? (prefix + min(extend_len, w_row + 16) - 1) / BN + 1 : 0;
 
-  // ---- staging. Thread t's piece of 32 codes: key t / 4 of a tile, block t % 4. K's go to the LDS by
-  // DMA; V's through registers, where they become bf16 with their scale (once for all waves).
-  // During tile t's step K of t + 2 and V of t + 1 load, the scales of t + 3 and the slots of t + 4.
-  // No branch guards a load with a register result (past the sequence's end its last key is read
-  // again): such a load is waited for where the branch ends, and the tile's DMA with it.
+  // ---- staging. A step works on a tile of 64 keys, as two sub-tiles 2 t and 2 t + 1, and stages K of
+  // tile t + 2 and V of t + 1. A thread's piece is 32 codes: key t / 4 of a tile, block t % 4. K's go to
+  // the LDS by DMA during the step; V's through registers, where they become bf16 with their scale (once
+  // for all waves) at the step's end, when those of t + 2 go out. No branch that differs between steps
+  // guards a load with a register result (past the sequence's end its last key is read again): such a
+  // load is waited for where the branch ends.
   const int32_t* idx = kv_indices + kv_start;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char_t)lds));
   const uint32_t max_slots = static_cast<uint32_t>(min<int64_t>(num_slots, 0x7fffffff));
@@ -115,82 +122,72 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   auto load_slot = [&](int tile) -> uint32_t { return idx[min(tile * BN + my_key, kv_len - 1)]; };
   // Out of range: slot 0. (Looked at where a slot is used first: at its load, it would be waited
   // for.)
-  auto check = [&](uint32_t& slot) { slot = slot < max_slots ? slot : 0; };
+  auto checked = [&](uint32_t slot) { return slot < max_slots ? slot : 0u; };
   const uint32_t row_bytes = static_cast<uint32_t>(num_kv_heads) * (D / 2);
   const uint8_t* ksrc = k_cache + h_kv * (D / 2) + 16 * (my_blk ^ swk(my_key));
   const uint8_t* vsrc = v_cache + h_kv * (D / 2) + 16 * my_blk;
   const uint2* sbase = kv_scales + h_kv;
   auto load_k = [&](uint32_t slot, int buf) {
-    dma16(ksrc + static_cast<uint64_t>(slot) * row_bytes, lds0 + buf * kKTile + 1024u * wave);
+    dma16(ksrc + static_cast<uint64_t>(slot) * row_bytes, lds0 + 2 * buf * kKSub + 1024u * wave);
   };
-  u32x4_v raw;
   auto load_v = [&](uint32_t slot) {
-    raw = *reinterpret_cast<const u32x4_v*>(vsrc + static_cast<uint64_t>(slot) * row_bytes);
+    return *reinterpret_cast<const u32x4_v*>(vsrc + static_cast<uint64_t>(slot) * row_bytes);
   };
   auto load_scales = [&](uint32_t slot) {
     return sbase[static_cast<uint64_t>(slot) * static_cast<uint32_t>(num_kv_heads)];
   };
-  // This thread's bytes of a head's scales: K | V << 8. A NaN vector must reach the queries that see
-  // its key and no others, but a hidden key's value is multiplied by p = 0, which leaves a NaN. So a
-  // key whose V is NaN gets a NaN scale for K (E8M0's 255: NaN scores, and a hidden key's scores are
-  // never used) and values 0.
-  auto my_scales = [&](uint2 s) -> uint32_t {
-    const uint32_t k = (s.x >> (8 * my_blk)) & 255u, v = (s.y >> (8 * my_blk)) & 255u;
-    return v == kFp4ScaleNaN ? 127u << 8 | kFp4ScaleNaN : v << 8 | k;
+  // A NaN vector must reach the queries that see its key and no others, but a hidden key's value is
+  // multiplied by p = 0, which leaves a NaN. So a key whose V is NaN gets a NaN scale for K (E8M0's
+  // 255: NaN scores, and a hidden key's scores are never used) and values 0.
+  const uint32_t sdst = kScalesAt + (my_key >> 5) * kScaleSub +
+                        2 * (16 * my_blk + 4 * ((my_key >> 3) & 3) + (my_key & 3)) + ((my_key >> 2) & 1);
+  auto store_scales = [&](uint2 sc, int buf) {
+    const uint32_t k = sc.x >> (8 * my_blk), v = (sc.y >> (8 * my_blk)) & 255u;
+    reinterpret_cast<uint8_t*>(lds)[sdst + 2 * buf * kScaleSub] = static_cast<uint8_t>(v == kFp4ScaleNaN ? v : k);
   };
-  const uint32_t sdst = kScalesAt + 4 * (16 * my_blk + 4 * ((my_key >> 3) & 3) + (my_key & 3)) +
-                        2 * (my_key >> 5) + ((my_key >> 2) & 1);
-  auto store_scales = [&](uint32_t sc, int buf) {
-    reinterpret_cast<uint8_t*>(lds)[sdst + 256 * buf] = static_cast<uint8_t>(sc);
-  };
-  uint32_t vdst = lds0 + kVAt + 256 * my_key + 16 * ((4 * my_blk) ^ swv(my_key));
-  asm volatile("" : "+v"(vdst));
-  auto store_v = [&](uint32_t sc, int buf) {
-    const bool nan = (sc & 255u) == kFp4ScaleNaN;
-    const float s = fp4_scale(sc >> 8);
+  const uint32_t vdst = lds0 + kVAt + 256 * my_key + 16 * ((4 * my_blk) ^ swv(my_key));
+  auto store_v = [&](const u32x4_v& codes, uint32_t scales, int buf) {
+    const uint32_t byte = (scales >> (8 * my_blk)) & 255u;
+    const bool nan = byte == kFp4ScaleNaN;
+    const float s = fp4_scale(nan ? 127 : byte);
     typedef __attribute__((address_space(3))) u32x4_v* lds_w_t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 x = fp4_to_bf16x8(nan ? 0u : raw[i], s);
-      *(lds_w_t)((vdst ^ (16u * i)) + buf * kTileBytes) = u32x4_v{x.x, x.y, x.z, x.w};
+      const uint4 x = fp4_to_bf16x8(nan ? 0u : codes[i], s);
+      *(lds_w_t)((vdst ^ (16u * i)) + 2 * buf * kVSub) = u32x4_v{x.x, x.y, x.z, x.w};
     }
   };
 
   // The first loads, in the order of their latencies: slots and q, then what the slots name; q is
-  // split while those are under way.
-  uint32_t sl1 = load_slot(t_begin), sl2 = load_slot(t_begin + 1), sl3 = load_slot(t_begin + 2),
-           sl4 = load_slot(t_begin + 3);
+  // split while those are under way. (t_begin is a split's first tile: even.)
+  const uint32_t slot0 = load_slot(t_begin), slot1 = load_slot(t_begin + 1);
+  uint32_t k_slot = load_slot(t_begin + 2);
   QRaw q_raw[SETS];
 #pragma unroll
   for (int s = 0; s < SETS; ++s) q_raw[s] = load_q(q + (prow + s) * D, g);
   __builtin_amdgcn_sched_barrier(0);
-  check(sl1);
-  check(sl2);
-  check(sl3);
-  const uint2 s0 = load_scales(sl1), s1 = load_scales(sl2);
-  uint2 scales_in = load_scales(sl3);
-  load_v(sl1);
+  const uint2 s0 = load_scales(checked(slot0)), s1 = load_scales(checked(slot1));
+  const u32x4_v raw0 = load_v(checked(slot0));
+  u32x4_v raw = load_v(checked(slot1));
   __builtin_amdgcn_sched_barrier(0);
-  load_k(sl1, 0);  // (t_begin is a split's first tile: even)
-  load_k(sl2, 1);
+  load_k(checked(slot0), 0);
+  load_k(checked(slot1), 1);
   __builtin_amdgcn_sched_barrier(0);
   QRow qf[SETS];
 #pragma unroll
   for (int s = 0; s < SETS; ++s) qf[s] = split_q(q_raw[s], row_ok);
   __builtin_amdgcn_sched_barrier(0);
-  uint32_t sc0 = my_scales(s0), sc1 = my_scales(s1);
-  store_scales(sc0, 0);
-  store_scales(sc1, 1);
-  sl1 = sl2;
-  sl2 = sl3;
-  sl3 = sl4;
+  store_scales(s0, 0);
+  store_scales(s1, 1);
+  store_v(raw0, s0.y, 0);
+  uint32_t v_scales = s1.y;
   __builtin_amdgcn_sched_barrier(0);
 
-  // LDS addresses of a lane's fragments in buffer 0, kept in registers.
-  // S^T = K Q^T: row m of key block j is key 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4, so a lane
-  // ends with the scores of keys 8 g .. +7 and 32 + 8 g .. +7 of its queries.
+  // LDS addresses of a lane's fragments in sub-tile 0, kept in registers.
+  // S^T = K Q^T: row m of a sub-tile's key block j is key 8 (m / 4) + 4 j + m % 4, so a lane ends with
+  // the scores of keys 8 g .. +7 of its queries.
   const int key_a0 = 8 * (r >> 2) + (r & 3);
-  uint32_t ka = lds0 + key_a0 * (D / 2) + 16 * (g ^ swk(key_a0)), sa = lds0 + kScalesAt + 4 * lane;
+  uint32_t ka = lds0 + key_a0 * (D / 2) + 16 * (g ^ swk(key_a0)), sa = lds0 + kScalesAt + 2 * lane;
   const int key_v = 8 * g + (r >> 2);
   uint32_t va[8];
 #pragma unroll
@@ -200,86 +197,89 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   }
   asm volatile("" : "+v"(ka), "+v"(sa));
 
-  // A step takes the softmax of its tile t between the products of two others: S of tile t + 1 (qk)
-  // and the output of tile t - 1 (pv), so that no product waits for this tile's exponentials nor
-  // they for it. The softmax is dealt over 8 slices of 2 elements a row set; with them go pv n: key
-  // half n / 4, dim blocks 2 (n % 4) and the next; and two slices behind the key block's softmax, as its
-  // results take the place of the scores that are used up, qk n: key block n / 2, q's hi part, then
-  // its lo part.
+  // Sub-tile u takes its softmax between the products of two others: S of u + 1 (qk) and the output
+  // of u - 1 (pv), so that no product waits for its exponentials nor they for it. The softmax is dealt
+  // over 4 slices of 2 elements a row set; with slice n go qk n: key block n / 2, q's hi part, then its
+  // lo part, and pv n + 1: dim blocks 2 n + 2 and the next (pv 0 with the maxima before them). The
+  // fragments are in registers when a sub-tile begins: they are read during the one before, each as
+  // soon as its predecessor is used up, so that neither a barrier nor the LDS is waited for.
   typedef __attribute__((address_space(3))) const u32x4_v* lds_u4_t;
   typedef __attribute__((address_space(3))) s16x4_v* tr_ptr_t;
   u32x4_v kf[2];
-  s16x4_v vw[3][2][2];
-  f32x4_v s[SETS][4];  // S: row 4 g + i of key block j at [j][i]
-  uint4 pn[SETS][2];   // P of this tile, and of the one before
-  bf16x8_v pf[SETS][2];
-  float m[SETS], l[SETS];  // (l: this lane's 16 keys of every tile)
+  int ks;  // kf's scales
+  s16x8_v vw[4][2];
+  f32x4_v s[2][SETS][2];  // [u % 2]: S of this sub-tile and of the next
+  uint4 p4[2][SETS];      // [u % 2]: P of this sub-tile and of the one before
+  float m[SETS], l[SETS];  // (l: this lane's 8 keys of every sub-tile)
   f32x4_v acc[SETS][8];
-  float run_m[SETS], run_l[SETS];
   typedef __attribute__((address_space(3))) f32x4_v* park_t;
-  const park_t parked = (park_t)(lds0 + kParkedAt + 16 * tid);  // vector db of set e: + 64 NW (8 e + db)
+  const park_t parked = (park_t)(lds0 + kRunAt + 16 * tid);  // vector db of set e: + 64 NW (8 e + db)
+  typedef __attribute__((address_space(3))) volatile f32x4_v* spare_t;
+  const spare_t spare = (spare_t)(lds0 + kSpareAt + 16 * tid);
+  typedef __attribute__((address_space(3))) f32x2_fp4* row_t;  // a row's m and l
+  const row_t run_ml = (row_t)(lds0 + kRunAt + 8 * SETS * NW * 1024 + 8 * (16 * SETS * wave + r));
 #pragma unroll
   for (int e = 0; e < SETS; ++e) {
-    m[e] = run_m[e] = NEG_BIG;
-    l[e] = run_l[e] = 0.0f;
+    m[e] = NEG_BIG;
+    l[e] = 0.0f;
+    if constexpr (!FANOUT) run_ml[16 * e] = f32x2_fp4{NEG_BIG, 0.0f};
 #pragma unroll
     for (int db = 0; db < 8; ++db) {
       acc[e][db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (!FANOUT) parked[64 * NW * (8 * e + db)] = acc[e][db];
     }
-    pf[e][0] = pf[e][1] = bf16x8_v{};
+    p4[0][e] = p4[1][e] = make_uint4(0, 0, 0, 0);
   }
-  auto read_k = [&](auto j_, int buf) {
-    constexpr int j = decltype(j_)::value;
-    kf[j & 1] = *(lds_u4_t)(ka + buf * kKTile + (32 * (j >> 1) + 4 * (j & 1)) * (D / 2));
+  auto read_k = [&](int at) {
+    ks = *(__attribute__((address_space(3))) const uint16_t*)(sa + at * kScaleSub);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) kf[j] = *(lds_u4_t)(ka + at * kKSub + 4 * j * (D / 2));
   };
-  // V fragments: A = V^T rows 16 db + r (dims), columns 32 kb + 8 g .. +7 (keys), by two
-  // transpose reads (extend_attention.hip): slice n's, two slices ahead.
-  auto read_v = [&](auto n_, int buf) {
-    constexpr int n = decltype(n_)::value;
+  // V fragments: A = V^T rows 16 db + r (dims), columns 8 g .. +7 (keys), by two transpose reads
+  // (extend_attention.hip): those of pv n.
+  auto read_v = [&](int n, int at) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t at = va[2 * (n & 3) + i] + buf * kTileBytes + 8192 * (n >> 2);
-      vw[n % 3][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
-      vw[n % 3][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 1024));
+      const uint32_t a = va[2 * n + i] + at * kVSub;
+      vw[n][i] = __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)a),
+                                         __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(a + 1024)), 0,
+                                         1, 2, 3, 4, 5, 6, 7);
     }
   };
-  auto qk = [&](auto n_, int e, int ks) {
+  auto qk = [&](auto n_, int e, f32x4_v (&to)[2]) {
     constexpr int n = decltype(n_)::value, j = n >> 1;
     constexpr bool lo = (n & 1) != 0;
-    const u32x4_v kk = kf[j & 1];
+    const u32x4_v kk = kf[j];
     const i32x8_v a{(int)kk.x, (int)kk.y, (int)kk.z, (int)kk.w, 0, 0, 0, 0};
     // (formats 4 and 0: e2m1 and e4m3; the scale operands' byte is an immediate: key block j of ks,
     // hi or lo of the row's scale)
     if constexpr (lo)
-      s[e][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[e].lo, s[e][j], 4, 0, j, ks, 1, qf[e].scale);
+      to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[e].lo, to[j], 4, 0, j, ks, 1, qf[e].scale);
     else
-      s[e][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
           a, qf[e].hi, f32x4_v{0.0f, 0.0f, 0.0f, 0.0f}, 4, 0, j, ks, 0, qf[e].scale);
   };
-  auto pv = [&](auto n_, int i, int e) {
-    constexpr int n = decltype(n_)::value;
-    const bf16x8_v vf = __builtin_bit_cast(
-        bf16x8_v, static_cast<s16x8_v>(__builtin_shufflevector(vw[n % 3][i][0], vw[n % 3][i][1], 0, 1, 2,
-                                                               3, 4, 5, 6, 7)));
-    f32x4_v& a = acc[e][2 * (n & 3) + i];
-    a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[e][n >> 2], a, 0, 0, 0);
+  auto pv = [&](int n, int i, int e, const uint4& p) {
+    f32x4_v& a = acc[e][2 * n + i];
+    a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, vw[n][i]),
+                                                __builtin_bit_cast(bf16x8_v, p), a, 0, 0, 0);
   };
-  auto each = [](auto f) {  // f(0) .. f(7), as constants
+  auto each = [](auto f) {  // f(0) .. f(3), as constants
     f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{});
     f(std::integral_constant<int, 2>{}); f(std::integral_constant<int, 3>{});
-    f(std::integral_constant<int, 4>{}); f(std::integral_constant<int, 5>{});
-    f(std::integral_constant<int, 6>{}); f(std::integral_constant<int, 7>{});
   };
   typedef std::integral_constant<int, 0> c0;
+  typedef std::integral_constant<int, 1> c1;
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
   auto point = [] { __builtin_amdgcn_sched_barrier(0); };
   // The state (om, ol) and acc of a split that is complete, into the rows'.
   auto fold_split = [&](const float (&om)[SETS], const float (&ol)[SETS]) {
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
-      const FoldScale f = fold_scale(run_m[e], om[e]);
-      run_l[e] = fold_elem(run_l[e], pair32_sum(pair16_sum(ol[e])), f);
-      run_m[e] = f.mn;
+      const f32x2_fp4 ml = run_ml[16 * e];
+      const FoldScale f = fold_scale(ml.x, om[e]);
+      run_ml[16 * e] = f32x2_fp4{f.mn, fold_elem(ml.y, pair32_sum(pair16_sum(ol[e])), f)};  // (4 lanes, the same bits)
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
         f32x4_v a = parked[64 * NW * (8 * e + db)];
@@ -290,190 +290,193 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     }
   };
 
-  // Tile t's step. MASK: some key of it may be hidden from some row. FIRST: of a split.
-  auto step = [&](auto mask, auto first, int t, auto buf) {
+  // Half h of tile t: sub-tile u = 2 t + h. MASK: some key of it may be hidden from some row. FIRST: of a
+  // split.
+  auto half = [&](auto mask, auto first, auto h_, int t, auto buf, auto tail) {
     constexpr bool kMask = decltype(mask)::value, kFirst = decltype(first)::value;
-    // Every wave is done with the buffers that are written next, and every load has landed (they had a
-    // whole tile's time) but V's, the last that went out, which the step's end waits for.
-    point();
-    asm volatile("s_waitcnt vmcnt(1) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    point();
-    const bool mine = !kMask || t <= w_tiles;  // (at w_tiles the tile before is still to be added)
-    int ks = 0;
-    if (mine) {
-      read_v(c0{}, other(buf));
-      read_v(std::integral_constant<int, 1>{}, other(buf));
-      ks = *(__attribute__((address_space(3))) const int*)(sa + 256 * other(buf));
-      read_k(c0{}, other(buf));
-    }
-    point();
-    asm volatile("" : "+v"(scales_in.x), "+v"(scales_in.y));  // (not looked at ahead of the barrier)
-    const uint32_t sc2nd = my_scales(scales_in);
-    store_scales(sc2nd, buf);
-    check(sl3);
-    scales_in = load_scales(sl3);
-    const uint32_t k_at = sl2, v_at = sl1;
-    sl1 = sl2;
-    sl2 = sl3;
-    sl3 = load_slot(t + 4);
-    point();
-    if (t + 2 < t_end) load_k(k_at, buf);
-    point();
-    auto stage_v = [&] {
-      asm volatile("" : "+v"(raw));
-      store_v(sc0, buf);
-      sc0 = sc1;
-      sc1 = sc2nd;
-      point();
-      load_v(v_at);  // last
-      point();
-    };
-    if (!mine) {
-      stage_v();
-      return;
-    }
-    float om[SETS], ol[SETS];
-    bool vis[16];
+    constexpr int h = decltype(h_)::value;
+    const int v_at = 2 * buf + h, k_at = 2 * other(buf) + h;  // what is read here: V of u, K of u + 2
+    f32x4_v (&sc)[SETS][2] = s[h];
+    bool vis[8];
     if constexpr (kMask) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        vis[i] = (t * BN + 32 * (i >> 3) + 8 * g + (i & 7) <= q_abs) & row_ok;
+      for (int i = 0; i < 8; ++i) vis[i] = (t * BN + BS * h + 8 * g + i <= q_abs) & row_ok;
     }
-    float tmax[SETS];
-    bool high = kFirst;
+    auto seen = [&](int e, int i) { return !kMask || vis[i] ? sc[e][i >> 2][i & 3] : NEG_BIG; };
+    float om[SETS], ol[SETS];
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
+      point();
+      pv(0, 0, e, p4[1 - h][e]);
+      pv(0, 1, e, p4[1 - h][e]);
+      point();
       om[e] = m[e];
       ol[e] = l[e];
       if constexpr (kFirst) {
-        m[e] = NEG_BIG;
+        float top = NEG_BIG;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, seen(e, i));
+        m[e] = pair32_max(pair16_max(top)) * sc2;
         l[e] = 0.0f;
       }
-      tmax[e] = NEG_BIG;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) tmax[e] = fmaxf(tmax[e], !kMask || vis[i] ? s[e][i >> 2][i & 3] : NEG_BIG);
-      high |= tmax[e] * sc2 > m[e] + LAZY_T;
     }
-    // Each lane looks at its own scores: only where one of them is LAZY_T above its row's
-    // reference maximum (seldom, but for a split's first tile) are the rows' maxima taken.
-    const bool moved = kFirst || __builtin_amdgcn_ballot_w64(high) != 0;
-    float rescale[SETS];
+    float tmax[SETS];
 #pragma unroll
-    for (int e = 0; e < SETS; ++e) rescale[e] = 1.0f;
-    if (moved) {
-#pragma unroll
-      for (int e = 0; e < SETS; ++e) {
-        const float mc = pair32_max(pair16_max(tmax[e])) * sc2;
-        const float m_used = mc > m[e] + LAZY_T ? mc : m[e];
-        rescale[e] = exp2_fast(m[e] - m_used);
-        m[e] = m_used;
-        if constexpr (!kFirst) l[e] *= rescale[e];
-      }
-    }
-    // (One wave has a SIMD to itself: while a product runs, only what follows it in program order can
-    // issue, and a second product behind it waits for the first. So between two products stands about
-    // as much of the softmax as the first one takes: 34 cycles a qk, 16 a pv, 16 an exponential.)
+    for (int e = 0; e < SETS; ++e) tmax[e] = NEG_BIG;
+    // (While a product runs, a wave can issue only what follows it in program order, and a second
+    // product behind it waits for the first. So between two products stands about as much of the
+    // softmax as the first one takes: 34 cycles a qk, 16 a pv, 16 an exponential.)
     each([&](auto n_) {
       constexpr int n = decltype(n_)::value, j = n >> 1, i0 = 2 * (n & 1);
-      typedef std::integral_constant<int, n < 2 ? 0 : n - 2> nq;
       float x[SETS][2], p[SETS][2];
       point();
-      if constexpr (n < 6) read_v(std::integral_constant<int, n + 2>{}, other(buf));
-      if constexpr (n % 2 == 0 && n > 0) read_k(std::integral_constant<int, n / 2>{}, other(buf));
+      read_v(n, v_at);
 #pragma unroll
       for (int e = 0; e < SETS; ++e)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[e][i] = __builtin_fmaf(s[e][j][i0 + i], sc2, -m[e]);
+        for (int i = 0; i < 2; ++i) x[e][i] = __builtin_fmaf(sc[e][j][i0 + i], sc2, -m[e]);
       point();
-      if constexpr (n >= 2) qk(nq{}, 0, ks);
+      qk(n_, 0, s[1 - h][0]);
       point();
       p[0][0] = exp2_fast(x[0][0]);
       p[0][1] = exp2_fast(x[0][1]);
       point();
-      if constexpr (n >= 2 && SETS == 2) qk(nq{}, 1, ks);
-      point();
       if constexpr (SETS == 2) {
+        qk(n_, 1, s[1 - h][1]);
+        point();
         p[1][0] = exp2_fast(x[1][0]);
         p[1][1] = exp2_fast(x[1][1]);
+        point();
       }
+      if constexpr (n == 3) read_k(k_at);
 #pragma unroll
       for (int e = 0; e < SETS; ++e) {
-        point();
-        pv(n_, 0, e);
-        point();
+        if constexpr (n < 3) {
+          point();
+          pv(n + 1, 0, e, p4[1 - h][e]);
+          point();
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if constexpr (kMask) p[e][i] = vis[2 * n + i] ? p[e][i] : 0.0f;
           l[e] += p[e][i];
         }
-        reinterpret_cast<uint32_t*>(&pn[e][n >> 2])[n & 3] = pack_bf16x2(p[e][0], p[e][1]);
-      }
-#pragma unroll
-      for (int e = 0; e < SETS; ++e) {
-        point();
-        pv(n_, 1, e);
+        if constexpr (!kFirst) tmax[e] = fmaxf(fmaxf(tmax[e], seen(e, 2 * n)), seen(e, 2 * n + 1));
+        reinterpret_cast<uint32_t*>(&p4[h][e])[n] = pack_bf16x2(p[e][0], p[e][1]);
+        if constexpr (n < 3) {
+          point();
+          pv(n + 1, 1, e, p4[1 - h][e]);
+        }
       }
       point();
     });
-    // The last key block's products, with V's conversion between them.
-    qk(std::integral_constant<int, 6>{}, 0, ks);
-    if constexpr (SETS == 2) qk(std::integral_constant<int, 6>{}, 1, ks);
-    point();
-    stage_v();
-    qk(std::integral_constant<int, 7>{}, 0, ks);
-    if constexpr (SETS == 2) qk(std::integral_constant<int, 7>{}, 1, ks);
-    point();
-    // (here, not where the next step uses them: past the branches below they would move there)
+    // (here, not where they are used: past the branches below they would move there)
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
-      asm volatile("" : "+v"(s[e][0]), "+v"(s[e][1]), "+v"(s[e][2]), "+v"(s[e][3]));
-      asm volatile("" : "+v"(l[e]), "+v"(pn[e][0].x), "+v"(pn[e][0].y), "+v"(pn[e][0].z), "+v"(pn[e][0].w),
-                   "+v"(pn[e][1].x), "+v"(pn[e][1].y), "+v"(pn[e][1].z), "+v"(pn[e][1].w));
+      asm volatile("" : "+v"(s[1 - h][e][0]), "+v"(s[1 - h][e][1]));
+      asm volatile("" : "+v"(l[e]), "+v"(p4[h][e].x), "+v"(p4[h][e].y), "+v"(p4[h][e].z), "+v"(p4[h][e].w));
     }
+    tail();
     if constexpr (kFirst) {
+      // (before the first split: zeros)
       if (!FANOUT && t > t_begin) fold_split(om, ol);
 #pragma unroll
       for (int e = 0; e < SETS; ++e)
 #pragma unroll
         for (int db = 0; db < 8; ++db) acc[e][db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
-    } else if (moved) {  // (x * 1 == x for the rows that did not)
+    } else {
+      // A row's reference maximum is that of its split's first sub-tile as long as no score is kLazy above
+      // it: P's precision does not depend on its size. Each lane looks at its own scores; only where one
+      // is too high (hardly ever) are the rows' maxima taken, their state brought to them and P worked out
+      // again. That is looked at here, after the products, as nothing before has to wait for it.
+      float above = tmax[0] * sc2 - m[0];
+      if constexpr (SETS == 2) above = fmaxf(above, tmax[1] * sc2 - m[1]);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(above > kLazy) != 0, false)) {
 #pragma unroll
-      for (int e = 0; e < SETS; ++e)
+        for (int e = 0; e < SETS; ++e) {
+          const float mc = pair32_max(pair16_max(tmax[e])) * sc2;
+          const float m_used = mc > m[e] + kLazy ? mc : m[e];
+          const float rescale = exp2_fast(m[e] - m_used);  // (x * 1 == x for the rows that stay)
+          m[e] = m_used;
+          l[e] = ol[e] * rescale;
+          // (By way of the LDS: elements of the vectors changed in a branch would be copied, all of
+          // them, on the way past it.)
+          uint4 x;
 #pragma unroll
-        for (int db = 0; db < 8; ++db)
+          for (int n = 0; n < 4; ++n) {
+            float p[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[e][db][i] *= rescale[e];
+            for (int i = 0; i < 2; ++i) {
+              p[i] = exp2_fast(__builtin_fmaf(sc[e][n >> 1][2 * (n & 1) + i], sc2, -m[e]));
+              if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
+              l[e] += p[i];
+            }
+            reinterpret_cast<uint32_t*>(&x)[n] = pack_bf16x2(p[0], p[1]);
+          }
+          *spare = __builtin_bit_cast(f32x4_v, x);
+          p4[h][e] = __builtin_bit_cast(uint4, (f32x4_v)*spare);
+#pragma unroll
+          for (int db = 0; db < 8; ++db) {
+            *spare = acc[e][db];
+            const f32x4_v a = *spare;
+            *spare = f32x4_v{a[0] * rescale, a[1] * rescale, a[2] * rescale, a[3] * rescale};
+            acc[e][db] = *spare;
+          }
+        }
+      }
     }
-#pragma unroll
-    for (int e = 0; e < SETS; ++e)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) pf[e][i] = __builtin_bit_cast(bf16x8_v, pn[e][i]);
   };
 
-  // S of the first tile.
+  auto step = [&](auto mask, auto first, int t, auto buf) {
+    constexpr bool kMask = decltype(mask)::value;
+    // Every wave is done with the tiles that are written over next, and K has landed (it had a whole
+    // tile's time). V and its scale are still under way, the last two loads that went out.
+    point();
+    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    point();
+    const uint32_t v_slot = load_slot(t + 2), slot = checked(k_slot);
+    const uint2 k_scales = load_scales(slot);
+    k_slot = load_slot(t + 3);
+    point();
+    load_k(slot, buf);  // last: a wait for an earlier load would include the DMA
+    point();
+    auto stage = [&] {  // at the step's end
+      store_v(raw, v_scales, other(buf));
+      point();
+      const uint32_t slot = checked(v_slot);
+      raw = load_v(slot);
+      v_scales = load_scales(slot).y;
+      point();
+      store_scales(k_scales, buf);
+      point();
+    };
+    if (!kMask || t <= w_tiles) {  // (at w_tiles the sub-tile before is still to be added)
+      half(mask, first, c0{}, t, buf, [] {});
+      half(mask, no, c1{}, t, buf, stage);
+    } else {
+      stage();
+    }
+  };
+
+  // S of the first sub-tile.
   auto barrier = [&] {
     point();
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     point();
   };
   barrier();
-  {
-    const int ks = *(__attribute__((address_space(3))) const int*)sa;
-    read_k(c0{}, 0);
-    each([&](auto n_) {
-      constexpr int n = decltype(n_)::value;
-      if constexpr (n < 6 && n % 2 == 0) read_k(std::integral_constant<int, n / 2 + 1>{}, 0);
+  read_k(0);
 #pragma unroll
-      for (int e = 0; e < SETS; ++e) qk(n_, e, ks);
-    });
-  }
-  // Tiles that every row of the workgroup sees whole, in pairs (their buffers' addresses are
+  for (int n = 0; n < 4; ++n) vw[n][0] = vw[n][1] = s16x8_v{};
+  each([&](auto n_) {
+#pragma unroll
+    for (int e = 0; e < SETS; ++e) qk(n_, e, s[0][e]);
+  });
+  read_k(1);
+  // Tiles that every row of the workgroup sees whole, in pairs (their places in the rings are
   // immediates), then the others with the mask: one loop each, split by split (a branch between
   // the kinds in one loop, or the fold in it, costs a copy of the accumulators each turn).
   const int t_full = (prefix + mtile * ROWS + 1) / BN;
-  constexpr std::true_type yes;
-  constexpr std::false_type no;
-  typedef std::integral_constant<int, 1> c1;
   for (int s0 = t_begin; s0 < t_end; s0 += kSplitTiles) {
     const int s_end = min(s0 + kSplitTiles, t_end), e = min(s_end, t_full);
     int t = s0;
@@ -487,21 +490,14 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     if (t < e) step(no, no, t++, c1{});
     for (; t < s_end; ++t) step(yes, no, t, t & 1);
   }
-  // The last tile's output. (Its wave skips no P: a wave without that tile has P = 0.)
-  barrier();
-  {
-    const int buf = (t_end - 1) & 1;
-    read_v(c0{}, buf);
-    each([&](auto n_) {
-      constexpr int n = decltype(n_)::value;
-      if constexpr (n < 7) read_v(std::integral_constant<int, n + 1>{}, buf);
-      __builtin_amdgcn_sched_barrier(0);
+  // The last sub-tile's output. (A wave that left out the last tiles has P = 0 and finite values.)
+  each([&](auto n_) {
+    constexpr int n = decltype(n_)::value;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < SETS; ++e) pv(n_, i, e);
-    });
-  }
+      for (int e = 0; e < SETS; ++e) pv(n, i, e, p4[1][e]);
+  });
   if constexpr (FANOUT) {
 #pragma unroll
     for (int e = 0; e < SETS; ++e) {
@@ -522,7 +518,8 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
 #pragma unroll
     for (int e = 0; e < SETS; ++e)
     {
-      RowState run{run_m[e], run_l[e], {}};
+      const f32x2_fp4 ml = run_ml[16 * e];
+      RowState run{ml.x, ml.y, {}};
 #pragma unroll
       for (int db = 0; db < 8; ++db) run.acc[db] = parked[64 * NW * (8 * e + db)];
       if (row_ok) store_row(o + (prow + e) * D, run, g);
