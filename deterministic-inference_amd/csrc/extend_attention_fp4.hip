@@ -11,6 +11,13 @@
 // over the other pools: both operands of the product are bf16, and P in two parts would double the
 // products), while l sums the unrounded p; and the small elements of a q row that holds far larger
 // ones (QRow).
+//
+// Workgroups are of 4 waves and 32 query positions, two to a CU, as an independent workgroup fills the
+// waits of the other best: 8 waves of 64 positions, and 4 waves with two row sets that share each fragment,
+// took 3 to 40 % longer. Over 8 kv heads of 2 query heads: 1 x 8192 328 us
+// (838 TFLOP/s), 4 x 2048 103, 1 x 2048 32, 4 x 32 at 2048 keys 17. Of those 328 the vector ALU (softmax,
+// V to bf16) is busy for 55 % and the matrix units for 38 %, in each other's shadow; what bounds it is the
+// issue of both by two waves a SIMD.
 #include "extend_codes.h"
 #include "kv_fp4.h"
 
@@ -20,7 +27,9 @@ namespace sid {
 namespace {
 
 constexpr int NW = 4;  // waves of a workgroup
-constexpr int kSplit = 512;  // keys per split: the unit in which a row's state is folded
+// Keys per split: the unit in which a row's state is folded. (With 1024 a prompt of 8192 takes 5 % less,
+// but 4 x 32 queries at 2048 keys, which fan out by splits, 20.7 us instead of 17.)
+constexpr int kSplit = 512;
 constexpr int kSplitTiles = kSplit / BN;
 // How far above its row's reference maximum a score may be, in log2 units.
 constexpr float kLazy = 24.0f;
@@ -36,21 +45,17 @@ constexpr int kKSub = BS * D / 2, kVSub = BS * D * 2, kScaleSub = 128;
 constexpr int kVAt = 4 * kKSub;
 constexpr int kScalesAt = kVAt + 4 * kVSub;
 // The rows' folded state stays in the LDS between two folds, 512 keys apart (the registers hold the
-// state of the split in work): a lane's 8 accumulator vectors a row set, and the rows' m and l.
-constexpr int kSpareAt = kScalesAt + 4 * kScaleSub;  // a vector of each thread
-constexpr int kRunAt = kSpareAt + NW * 1024;
-constexpr int lds_bytes(int sets, bool fanout) {
-  return kRunAt + (fanout ? 0 : sets * NW * (8 * 1024 + 128));
-}
+// state of the split in work): a lane's 8 accumulator vectors, and the rows' m and l.
+constexpr int kRunAt = kScalesAt + 4 * kScaleSub;
+constexpr int lds_bytes(bool fanout) { return kRunAt + (fanout ? 0 : NW * (8 * 1024 + 128)); }
 
 __device__ __forceinline__ int swk(int key) { return (key >> 3) & 3; }
 
-// Workgroup = (request, kv head, 8 NW SETS query positions), NW waves. A wave has SETS sets of 16
-// rows: with 2, the two query heads at its 16 positions, which share every K and V fragment that it
-// reads; with 1, one head (w / (NW / 2)). FANOUT: the workgroup computes one split and saves its
-// state for the fold; else it walks the splits in order.
-template <int SETS, bool FANOUT>
-__global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
+// Workgroup = (request, kv head, 8 NW query positions), NW waves; wave w: 16 positions of query head
+// w / (NW / 2). FANOUT: the workgroup computes one split and saves its state for the fold; else it
+// walks the splits in order.
+template <bool FANOUT>
+__global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ k_cache,
     const uint8_t* __restrict__ v_cache, const uint2* __restrict__ kv_scales,
     const int32_t* __restrict__ qo_indptr, const int32_t* __restrict__ kv_indptr,
@@ -58,8 +63,8 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     int64_t num_slots, float sm_scale, int mtiles, int per_round, int ordered, int across,
     int64_t items, bf16_t* __restrict__ o, float* __restrict__ part_a,
     float* __restrict__ part_ml, int32_t* __restrict__ part_n) {
-  __shared__ __align__(1024) char lds[lds_bytes(SETS, FANOUT)];
-  constexpr int ROWS = 8 * NW * SETS;
+  __shared__ __align__(1024) char lds[lds_bytes(FANOUT)];
+  constexpr int ROWS = 8 * NW;
   int b, h_kv, mtile, split = 0;
   if constexpr (FANOUT) {
     b = blockIdx.x;
@@ -90,8 +95,8 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
-  const int hq = h_kv * 2 + (SETS == 2 ? 0 : wave / (NW / 2));  // of set 0
-  const int w_row = mtile * ROWS + 16 * (SETS == 2 ? wave : wave % (NW / 2));  // the wave's first query row
+  const int hq = h_kv * 2 + wave / (NW / 2);
+  const int w_row = mtile * ROWS + 16 * (wave % (NW / 2));  // the wave's first query row
   const int r = lane & 15, g = lane >> 4;
   const bool row_ok = w_row + r < extend_len;
   const int64_t prow = static_cast<int64_t>(q_start + (row_ok ? w_row + r : 0)) * num_q_heads + hq;
@@ -162,9 +167,7 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   // split while those are under way. (t_begin is a split's first tile: even.)
   const uint32_t slot0 = load_slot(t_begin), slot1 = load_slot(t_begin + 1);
   uint32_t k_slot = load_slot(t_begin + 2);
-  QRaw q_raw[SETS];
-#pragma unroll
-  for (int s = 0; s < SETS; ++s) q_raw[s] = load_q(q + (prow + s) * D, g);
+  const QRaw q_raw = load_q(q + prow * D, g);
   __builtin_amdgcn_sched_barrier(0);
   const uint2 s0 = load_scales(checked(slot0)), s1 = load_scales(checked(slot1));
   const u32x4_v raw0 = load_v(checked(slot0));
@@ -173,9 +176,7 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   load_k(checked(slot0), 0);
   load_k(checked(slot1), 1);
   __builtin_amdgcn_sched_barrier(0);
-  QRow qf[SETS];
-#pragma unroll
-  for (int s = 0; s < SETS; ++s) qf[s] = split_q(q_raw[s], row_ok);
+  const QRow qf = split_q(q_raw, row_ok);
   __builtin_amdgcn_sched_barrier(0);
   store_scales(s0, 0);
   store_scales(s1, 1);
@@ -208,28 +209,22 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   u32x4_v kf[2];
   int ks;  // kf's scales
   s16x8_v vw[4][2];
-  f32x4_v s[2][SETS][2];  // [u % 2]: S of this sub-tile and of the next
-  uint4 p4[2][SETS];      // [u % 2]: P of this sub-tile and of the one before
-  float m[SETS], l[SETS];  // (l: this lane's 8 keys of every sub-tile)
-  f32x4_v acc[SETS][8];
+  f32x4_v s[2][2];  // [u % 2]: S of this sub-tile and of the next
+  uint4 p4[2];      // [u % 2]: P of this sub-tile and of the one before
+  float m = NEG_BIG, l = 0.0f;  // (l: this lane's 8 keys of every sub-tile)
+  f32x4_v acc[8];
   typedef __attribute__((address_space(3))) f32x4_v* park_t;
-  const park_t parked = (park_t)(lds0 + kRunAt + 16 * tid);  // vector db of set e: + 64 NW (8 e + db)
-  typedef __attribute__((address_space(3))) volatile f32x4_v* spare_t;
-  const spare_t spare = (spare_t)(lds0 + kSpareAt + 16 * tid);
-  typedef __attribute__((address_space(3))) f32x2_fp4* row_t;  // a row's m and l
-  const row_t run_ml = (row_t)(lds0 + kRunAt + 8 * SETS * NW * 1024 + 8 * (16 * SETS * wave + r));
+  const park_t parked = (park_t)(lds0 + kRunAt + 16 * tid);  // vector db: + 64 NW db
+  typedef __attribute__((address_space(3))) f32x2_fp4* row_t;
+  const row_t run_ml = (row_t)(lds0 + kRunAt + NW * 8 * 1024 + 8 * (16 * wave + r));  // the row's m and l
+  constexpr f32x4_v zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int e = 0; e < SETS; ++e) {
-    m[e] = NEG_BIG;
-    l[e] = 0.0f;
-    if constexpr (!FANOUT) run_ml[16 * e] = f32x2_fp4{NEG_BIG, 0.0f};
-#pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      acc[e][db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (!FANOUT) parked[64 * NW * (8 * e + db)] = acc[e][db];
-    }
-    p4[0][e] = p4[1][e] = make_uint4(0, 0, 0, 0);
+  for (int db = 0; db < 8; ++db) {
+    acc[db] = zero4;
+    if constexpr (!FANOUT) parked[64 * NW * db] = zero4;
   }
+  if constexpr (!FANOUT) *run_ml = f32x2_fp4{NEG_BIG, 0.0f};
+  p4[0] = p4[1] = make_uint4(0, 0, 0, 0);
   auto read_k = [&](int at) {
     ks = *(__attribute__((address_space(3))) const uint16_t*)(sa + at * kScaleSub);
 #pragma unroll
@@ -246,23 +241,22 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
                                          1, 2, 3, 4, 5, 6, 7);
     }
   };
-  auto qk = [&](auto n_, int e, f32x4_v (&to)[2]) {
+  auto qk = [&](auto n_, f32x4_v (&to)[2]) {
     constexpr int n = decltype(n_)::value, j = n >> 1;
-    constexpr bool lo = (n & 1) != 0;
     const u32x4_v kk = kf[j];
     const i32x8_v a{(int)kk.x, (int)kk.y, (int)kk.z, (int)kk.w, 0, 0, 0, 0};
     // (formats 4 and 0: e2m1 and e4m3; the scale operands' byte is an immediate: key block j of ks,
     // hi or lo of the row's scale)
-    if constexpr (lo)
-      to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[e].lo, to[j], 4, 0, j, ks, 1, qf[e].scale);
+    if constexpr ((n & 1) != 0)
+      to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf.lo, to[j], 4, 0, j, ks, 1, qf.scale);
     else
-      to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          a, qf[e].hi, f32x4_v{0.0f, 0.0f, 0.0f, 0.0f}, 4, 0, j, ks, 0, qf[e].scale);
+      to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf.hi, zero4, 4, 0, j, ks, 0, qf.scale);
   };
-  auto pv = [&](int n, int i, int e, const uint4& p) {
-    f32x4_v& a = acc[e][2 * n + i];
+  auto pv = [&](int n, int i, const uint4& p) {
+    f32x4_v& a = acc[2 * n + i];
     a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, vw[n][i]),
-                                                __builtin_bit_cast(bf16x8_v, p), a, 0, 0, 0);
+                                                __builtin_bit_cast(bf16x8_v, p),
+                                                a, 0, 0, 0);
   };
   auto each = [](auto f) {  // f(0) .. f(3), as constants
     f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{});
@@ -273,20 +267,18 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   constexpr std::true_type yes;
   constexpr std::false_type no;
   auto point = [] { __builtin_amdgcn_sched_barrier(0); };
-  // The state (om, ol) and acc of a split that is complete, into the rows'.
-  auto fold_split = [&](const float (&om)[SETS], const float (&ol)[SETS]) {
+  // The state (om, ol) and acc of a split that is complete, into the row's.
+  auto fold_split = [&](float om, float ol) {
+    const f32x2_fp4 ml = *run_ml;
+    const FoldScale f = fold_scale(ml.x, om);
+    *run_ml = f32x2_fp4{f.mn, fold_elem(ml.y, pair32_sum(pair16_sum(ol)), f)};  // (4 lanes, the same bits)
 #pragma unroll
-    for (int e = 0; e < SETS; ++e) {
-      const f32x2_fp4 ml = run_ml[16 * e];
-      const FoldScale f = fold_scale(ml.x, om[e]);
-      run_ml[16 * e] = f32x2_fp4{f.mn, fold_elem(ml.y, pair32_sum(pair16_sum(ol[e])), f)};  // (4 lanes, the same bits)
+    for (int db = 0; db < 8; ++db) {
+      f32x4_v a = parked[64 * NW * db];
 #pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        f32x4_v a = parked[64 * NW * (8 * e + db)];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = fold_elem(a[i], acc[e][db][i], f);
-        parked[64 * NW * (8 * e + db)] = a;
-      }
+      for (int i = 0; i < 4; ++i) a[i] = fold_elem(a[i], acc[db][i], f);
+      parked[64 * NW * db] = a;
+      acc[db] = zero4;
     }
   };
 
@@ -296,132 +288,96 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
     constexpr bool kMask = decltype(mask)::value, kFirst = decltype(first)::value;
     constexpr int h = decltype(h_)::value;
     const int v_at = 2 * buf + h, k_at = 2 * other(buf) + h;  // what is read here: V of u, K of u + 2
-    f32x4_v (&sc)[SETS][2] = s[h];
+    const f32x4_v (&sc)[2] = s[h];
     bool vis[8];
     if constexpr (kMask) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) vis[i] = (t * BN + BS * h + 8 * g + i <= q_abs) & row_ok;
     }
-    auto seen = [&](int e, int i) { return !kMask || vis[i] ? sc[e][i >> 2][i & 3] : NEG_BIG; };
-    float om[SETS], ol[SETS];
+    auto seen = [&](int i) { return !kMask || vis[i] ? sc[i >> 2][i & 3] : NEG_BIG; };
+    point();
+    __builtin_amdgcn_s_setprio(1);
+    pv(0, 0, p4[1 - h]);
+    pv(0, 1, p4[1 - h]);
+    point();
+    const float om = m, ol = l;
+    float tmax = NEG_BIG;
+    if constexpr (kFirst) {
 #pragma unroll
-    for (int e = 0; e < SETS; ++e) {
-      point();
-      pv(0, 0, e, p4[1 - h][e]);
-      pv(0, 1, e, p4[1 - h][e]);
-      point();
-      om[e] = m[e];
-      ol[e] = l[e];
-      if constexpr (kFirst) {
-        float top = NEG_BIG;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, seen(e, i));
-        m[e] = pair32_max(pair16_max(top)) * sc2;
-        l[e] = 0.0f;
-      }
+      for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, seen(i));
+      m = pair32_max(pair16_max(tmax)) * sc2;
+      l = 0.0f;
     }
-    float tmax[SETS];
-#pragma unroll
-    for (int e = 0; e < SETS; ++e) tmax[e] = NEG_BIG;
     // (While a product runs, a wave can issue only what follows it in program order, and a second
     // product behind it waits for the first. So between two products stands about as much of the
-    // softmax as the first one takes: 34 cycles a qk, 16 a pv, 16 an exponential.)
+    // softmax as the first one takes: 34 cycles a qk, 16 a pv. The priority lets the other workgroup's wave
+    // of the SIMD stage while this one keeps the matrix unit fed: 1.5 % of 1 x 8192.)
     each([&](auto n_) {
       constexpr int n = decltype(n_)::value, j = n >> 1, i0 = 2 * (n & 1);
-      float x[SETS][2], p[SETS][2];
+      float x[2], p[2];
       point();
       read_v(n, v_at);
 #pragma unroll
-      for (int e = 0; e < SETS; ++e)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) x[e][i] = __builtin_fmaf(sc[e][j][i0 + i], sc2, -m[e]);
+      for (int i = 0; i < 2; ++i) x[i] = __builtin_fmaf(sc[j][i0 + i], sc2, -m);
       point();
-      qk(n_, 0, s[1 - h][0]);
+      qk(n_, s[1 - h]);
       point();
-      p[0][0] = exp2_fast(x[0][0]);
-      p[0][1] = exp2_fast(x[0][1]);
+      p[0] = exp2_fast(x[0]);
+      p[1] = exp2_fast(x[1]);
       point();
-      if constexpr (SETS == 2) {
-        qk(n_, 1, s[1 - h][1]);
-        point();
-        p[1][0] = exp2_fast(x[1][0]);
-        p[1][1] = exp2_fast(x[1][1]);
-        point();
-      }
       if constexpr (n == 3) read_k(k_at);
+      if constexpr (n < 3) pv(n + 1, 0, p4[1 - h]);
+      point();
 #pragma unroll
-      for (int e = 0; e < SETS; ++e) {
-        if constexpr (n < 3) {
-          point();
-          pv(n + 1, 0, e, p4[1 - h][e]);
-          point();
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if constexpr (kMask) p[e][i] = vis[2 * n + i] ? p[e][i] : 0.0f;
-          l[e] += p[e][i];
-        }
-        if constexpr (!kFirst) tmax[e] = fmaxf(fmaxf(tmax[e], seen(e, 2 * n)), seen(e, 2 * n + 1));
-        reinterpret_cast<uint32_t*>(&p4[h][e])[n] = pack_bf16x2(p[e][0], p[e][1]);
-        if constexpr (n < 3) {
-          point();
-          pv(n + 1, 1, e, p4[1 - h][e]);
-        }
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
+        l += p[i];
       }
+      if constexpr (!kFirst) tmax = fmaxf(fmaxf(tmax, seen(2 * n)), seen(2 * n + 1));
+      reinterpret_cast<uint32_t*>(&p4[h])[n] = pack_bf16x2(p[0], p[1]);
+      point();
+      if constexpr (n < 3) pv(n + 1, 1, p4[1 - h]);
       point();
     });
     // (here, not where they are used: past the branches below they would move there)
-#pragma unroll
-    for (int e = 0; e < SETS; ++e) {
-      asm volatile("" : "+v"(s[1 - h][e][0]), "+v"(s[1 - h][e][1]));
-      asm volatile("" : "+v"(l[e]), "+v"(p4[h][e].x), "+v"(p4[h][e].y), "+v"(p4[h][e].z), "+v"(p4[h][e].w));
-    }
+    asm volatile("" : "+v"(s[1 - h][0]), "+v"(s[1 - h][1]));
+    asm volatile("" : "+v"(l), "+v"(p4[h].x), "+v"(p4[h].y), "+v"(p4[h].z), "+v"(p4[h].w));
+    __builtin_amdgcn_s_setprio(0);
     tail();
     if constexpr (kFirst) {
-      // (before the first split: zeros)
       if (!FANOUT && t > t_begin) fold_split(om, ol);
-#pragma unroll
-      for (int e = 0; e < SETS; ++e)
-#pragma unroll
-        for (int db = 0; db < 8; ++db) acc[e][db] = f32x4_v{0.0f, 0.0f, 0.0f, 0.0f};
     } else {
       // A row's reference maximum is that of its split's first sub-tile as long as no score is kLazy above
       // it: P's precision does not depend on its size. Each lane looks at its own scores; only where one
       // is too high (hardly ever) are the rows' maxima taken, their state brought to them and P worked out
       // again. That is looked at here, after the products, as nothing before has to wait for it.
-      float above = tmax[0] * sc2 - m[0];
-      if constexpr (SETS == 2) above = fmaxf(above, tmax[1] * sc2 - m[1]);
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(above > kLazy) != 0, false)) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(tmax * sc2 > m + kLazy) != 0, false)) {
+        const float mc = pair32_max(pair16_max(tmax)) * sc2;
+        const float m_used = mc > m + kLazy ? mc : m;
+        const float rescale = exp2_fast(m - m_used);  // (x * 1 == x for the rows that stay)
+        m = m_used;
+        l = ol * rescale;
+        uint4 w;
 #pragma unroll
-        for (int e = 0; e < SETS; ++e) {
-          const float mc = pair32_max(pair16_max(tmax[e])) * sc2;
-          const float m_used = mc > m[e] + kLazy ? mc : m[e];
-          const float rescale = exp2_fast(m[e] - m_used);  // (x * 1 == x for the rows that stay)
-          m[e] = m_used;
-          l[e] = ol[e] * rescale;
-          // (By way of the LDS: elements of the vectors changed in a branch would be copied, all of
-          // them, on the way past it.)
-          uint4 x;
+        for (int n = 0; n < 4; ++n) {
+          float p[2];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            float p[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              p[i] = exp2_fast(__builtin_fmaf(sc[e][n >> 1][2 * (n & 1) + i], sc2, -m[e]));
-              if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
-              l[e] += p[i];
-            }
-            reinterpret_cast<uint32_t*>(&x)[n] = pack_bf16x2(p[0], p[1]);
+          for (int i = 0; i < 2; ++i) {
+            p[i] = exp2_fast(__builtin_fmaf(sc[n >> 1][2 * (n & 1) + i], sc2, -m));
+            if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
+            l += p[i];
           }
-          *spare = __builtin_bit_cast(f32x4_v, x);
-          p4[h][e] = __builtin_bit_cast(uint4, (f32x4_v)*spare);
+          reinterpret_cast<uint32_t*>(&w)[n] = pack_bf16x2(p[0], p[1]);
+        }
+        p4[h] = w;
+        // (Out of a product with zeros: vectors whose elements change in a branch would be copied, all of
+        // them, on the way past it.)
 #pragma unroll
-          for (int db = 0; db < 8; ++db) {
-            *spare = acc[e][db];
-            const f32x4_v a = *spare;
-            *spare = f32x4_v{a[0] * rescale, a[1] * rescale, a[2] * rescale, a[3] * rescale};
-            acc[e][db] = *spare;
-          }
+        for (int db = 0; db < 8; ++db) {
+          const f32x4_v a = acc[db];
+          acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              bf16x8_v{}, bf16x8_v{}, f32x4_v{a[0] * rescale, a[1] * rescale, a[2] * rescale, a[3] * rescale},
+              0, 0, 0);
         }
       }
     }
@@ -468,10 +424,7 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   read_k(0);
 #pragma unroll
   for (int n = 0; n < 4; ++n) vw[n][0] = vw[n][1] = s16x8_v{};
-  each([&](auto n_) {
-#pragma unroll
-    for (int e = 0; e < SETS; ++e) qk(n_, e, s[0][e]);
-  });
+  each([&](auto n_) { qk(n_, s[0]); });
   read_k(1);
   // Tiles that every row of the workgroup sees whole, in pairs (their places in the rings are
   // immediates), then the others with the mask: one loop each, split by split (a branch between
@@ -493,46 +446,41 @@ __global__ void __launch_bounds__(NW * 64, SETS == 1 ? 2 : 1) extend_fp4_kernel(
   // The last sub-tile's output. (A wave that left out the last tiles has P = 0 and finite values.)
   each([&](auto n_) {
     constexpr int n = decltype(n_)::value;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int e = 0; e < SETS; ++e) pv(n, i, e, p4[1][e]);
+    pv(n, 0, p4[1]);
+    pv(n, 1, p4[1]);
   });
   if constexpr (FANOUT) {
+    l = pair32_sum(pair16_sum(l));
+    if (!row_ok) return;
+    const int64_t pr = split * items + prow;
 #pragma unroll
-    for (int e = 0; e < SETS; ++e) {
-      const float sum = pair32_sum(pair16_sum(l[e]));
-      if (!row_ok) continue;
-      const int64_t pr = split * items + prow + e;
-#pragma unroll
-      for (int db = 0; db < 8; ++db)
-        *reinterpret_cast<f32x4_v*>(part_a + pr * D + 16 * db + 4 * g) = acc[e][db];
-      if (g == 0) {
-        part_ml[2 * pr] = m[e];
-        part_ml[2 * pr + 1] = sum;
-        if (split == 0) part_n[prow + e] = nsplits;
-      }
+    for (int db = 0; db < 8; ++db)
+      *reinterpret_cast<f32x4_v*>(part_a + pr * D + 16 * db + 4 * g) = acc[db];
+    if (g == 0) {
+      part_ml[2 * pr] = m;
+      part_ml[2 * pr + 1] = l;
+      if (split == 0) part_n[prow] = nsplits;
     }
   } else {
     fold_split(m, l);
+    const f32x2_fp4 ml = *run_ml;
+    RowState run{ml.x, ml.y, {}};
 #pragma unroll
-    for (int e = 0; e < SETS; ++e)
-    {
-      const f32x2_fp4 ml = run_ml[16 * e];
-      RowState run{ml.x, ml.y, {}};
-#pragma unroll
-      for (int db = 0; db < 8; ++db) run.acc[db] = parked[64 * NW * (8 * e + db)];
-      if (row_ok) store_row(o + (prow + e) * D, run, g);
-    }
+    for (int db = 0; db < 8; ++db) run.acc[db] = parked[64 * NW * db];
+    if (row_ok) store_row(o + prow * D, run, g);
   }
 }
 
-// Whether a grid of fewer than 512 workgroups fans out: where walking its keys in one workgroup takes
-// longer than the launches and the saved states of total_q rows in every split.
+// Whether a grid of fewer than 512 workgroups fans out: where walking its keys in one workgroup (about
+// a microsecond a tile) takes longer than the launches (10) and the saved states of total_q rows in every
+// split. Walked and fanned out, us: 1 x 32 queries at 700 keys 15.8 and 14.0, 4 x 32 at 2048 32 and 18, 1 x 64 at
+// 16384 227 and 34, 16 x 32 at 2048 38 and 34; 1 x 512 12 and 21, 1 x 700 at 4000 63 and 70 (the line's
+// wrong side, as 1 x 512 at 2048, 37 and 41), 16 x 32 at 1024 24 and 26, 32 x 32 at 2048 41 and 59,
+// 64 x 8 at 1024 35 and 44.
 bool fans_out(int batch, int64_t total_q, int num_kv_heads, int max_extend_len, int max_kv_len) {
   const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * ceil_div(max_extend_len, BQ);
   const int64_t states = total_q * ceil_div(max_kv_len, kSplit);
-  return groups < 512 && 110 * static_cast<int64_t>(ceil_div(max_kv_len, BN)) > 1200 + states * 85 / 100;
+  return groups < 512 && 105 * static_cast<int64_t>(ceil_div(max_kv_len, BN)) > 1000 + states * 95 / 100;
 }
 
 }  // namespace
@@ -576,7 +524,7 @@ extern "C" int sid_extend_attention_fp4_fwd(
   const int ordered = batch > 1 && batch <= 64 * kOrderSteps &&
                       (8 * total_q < 7 * static_cast<int64_t>(batch) * max_extend_len ||
                        max_kv_len > max_extend_len);
-  const int per_round = p.rows == 32 ? max(1, cu_count() / num_kv_heads) : 0;
+  const int per_round = max(1, cu_count() / num_kv_heads);
   auto launch = [&](auto kern, dim3 grid, int mtiles, int across) {
     hipLaunchKernelGGL(kern, grid, dim3(NW * 64), 0, s, (const bf16_t*)q, (const uint8_t*)k_cache,
                        (const uint8_t*)v_cache, (const uint2*)kv_scales, qo_indptr, kv_indptr,
@@ -585,16 +533,15 @@ extern "C" int sid_extend_attention_fp4_fwd(
     return check_launch(name);
   };
   if (p.fanout) {
-    const int rc = launch(extend_fp4_kernel<1, true>, dim3(batch, num_kv_heads, p.mtiles * p.splits),
+    const int rc = launch(extend_fp4_kernel<true>, dim3(batch, num_kv_heads, p.mtiles * p.splits),
                           p.mtiles, 0);
     return rc != SID_OK ? rc : extend_merge(name, p, qo_indptr, batch, num_q_heads, o, s);
   }
-  const int mtiles = ceil_div(max_extend_len, p.rows);
+  const int mtiles = ceil_div(max_extend_len, 8 * NW);
   const int64_t places = static_cast<int64_t>(batch) * mtiles;
   const int across = static_cast<int>(std::min<int64_t>(places, kMaxGridX / num_kv_heads));
   const int64_t down = (places + across - 1) / across;
   SID_REQUIRE(places < (1ll << 30) && down <= 65535, "%s: grid too large", name);
   const dim3 grid(static_cast<unsigned>(across) * num_kv_heads, static_cast<unsigned>(down));
-  return p.rows == 64 ? launch(extend_fp4_kernel<2, false>, grid, mtiles, across)
-                      : launch(extend_fp4_kernel<1, false>, grid, mtiles, across);
+  return launch(extend_fp4_kernel<false>, grid, mtiles, across);
 }
