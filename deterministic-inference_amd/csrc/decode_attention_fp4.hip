@@ -10,40 +10,66 @@
 // The halves' softmax states are merged once, before the waves'.
 #include "decode_split.h"
 #include "kv_fp4.h"
+#include "q_codes.h"
+
+#include <type_traits>
 
 namespace sid {
 namespace {
 
-__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, a),
-                                         __builtin_bit_cast(bf16x2_v, b), c, false);
-}
+typedef float f32x4_v __attribute__((ext_vector_type(4)));
 
-constexpr int TPL = 4;  // tokens of a lane per wave iteration (a wave: 8)
+constexpr int WT = 16;            // tokens of a wave iteration
+constexpr int PT = WT / 2;        // those of a half-wave's V rows
+constexpr int kPRow = WT + 4;     // floats between two heads' weights (16-byte pieces, spread over the banks)
+constexpr int kScaleRow = 64 + 16;  // bytes between two tokens' scales
 
-struct TileRegs {
-  u32x4_v k[TPL];
-  u32x4_v v[TPL];
-  uint2 sc[TPL];
+// A wave's own corner of the LDS: no other wave reads it.
+struct alignas(16) WaveLds {
+  float p[HQ][kPRow];
+  float rs[HQ];
+  uint8_t sc[WT * kScaleRow];
 };
 
+__device__ __forceinline__ float pair_sum(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float pair_max(float v) {
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
+// What a wave wrote to its corner is there for its other lanes (the LDS serves a wave in order; this
+// holds the compiler to it).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The partial attention of request b over partial slot y (a segment of one split), by one
-// workgroup of NW waves taking 2 TPL tokens per wave iteration. Every exit is workgroup-uniform.
+// workgroup of NW waves taking WT tokens per wave iteration. Every exit is workgroup-uniform.
 template <int NW>
 __device__ __forceinline__ void stage1_item(
-    Stage1Lds<NW>& sh, int b, int y, const bf16_t* __restrict__ q,
+    Stage1Lds<NW>& sh, WaveLds (&own)[NW], int b, int y, const bf16_t* __restrict__ q,
     const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
-    const uint2* __restrict__ kv_scales, const int32_t* __restrict__ kv_indptr,
+    const uint8_t* __restrict__ kv_scales, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ num_splits,
     int max_splits, int fixed_split, int seg, float sm_scale, int64_t num_slots, int part_stride,
     float* __restrict__ part_o, float* __restrict__ part_lse, bf16_t* __restrict__ o_direct) {
-  constexpr int IT = NW * 2 * TPL;  // tokens per workgroup iteration
+  constexpr int IT = NW * WT;  // tokens per workgroup iteration
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
-  const int half = lane >> 5;
-  const int grp = (lane >> 2) & 7;  // kv head
-  const int blk = lane & 3;         // block of 32 dims
+  const int r = lane & 15, g = lane >> 4;  // K: token and block; S: query head, tokens 4 g .. +3
+  const int half = lane >> 5;              // V: tokens PT half .. +PT-1,
+  const int grp = (lane >> 2) & 7;         // kv head
+  const int blk = lane & 3;                // and block of 32 dims
 
   const int kv_base = kv_indptr[b];
   const int seq_len = kv_indptr[b + 1] - kv_base;
@@ -65,159 +91,160 @@ __device__ __forceinline__ void stage1_item(
     return;
   }
 
-  // Query heads 2 grp and 2 grp + 1: the lane's 32 dims, packed bf16.
-  u32x4_v qv[QPK][4];
+  WaveLds& mine = own[wave];
+  const int32_t* idx = kv_indices + kv_base;
+  int t0 = start + wave * WT;
+  // Positions past the segment's end load its last token again and get weight 0.
+  auto slot_of = [&](int t) { return idx[min(t, end - 1)]; };
+  auto checked = [&](int32_t raw) -> int64_t {
+    return raw < 0 || raw >= num_slots ? 0 : static_cast<int64_t>(raw);
+  };
+  int32_t k_raw, s_raw, v_raw[PT];  // slots of this lane's K row, scales and V rows
+  u32x4_v k[HKV], v[PT], sc;
+  auto load_idx = [&](int t) {
+    s_raw = slot_of(t + (lane >> 2));
+    k_raw = slot_of(t + r);
 #pragma unroll
-  for (int h = 0; h < QPK; ++h) {
-    const u32x4_v* qb =
-        reinterpret_cast<const u32x4_v*>(q + (out_row + QPK * grp + h) * HEAD_DIM + 32 * blk);
+    for (int i = 0; i < PT; ++i) v_raw[i] = slot_of(t + PT * half + i);
+  };
+  auto load_k = [&] {
+    sc = ld16<true>(reinterpret_cast<const u32x4_v*>(kv_scales + checked(s_raw) * (8 * HKV)) + (lane & 3));
+    const u32x4_v* row = reinterpret_cast<const u32x4_v*>(k_cache + checked(k_raw) * (HKV * HEAD_DIM / 2)) + g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qv[h][i] = qb[i];
-  }
-  float m[QPK], l[QPK], acc[QPK][32];
+    for (int h = 0; h < HKV; ++h) k[h] = ld16<true>(row + 4 * h);
+  };
+  // V's rows, behind the slots of the tokens at t: those are waited for while V is under way.
+  auto load_v = [&](int t) {
+    int32_t raw[PT];
 #pragma unroll
-  for (int h = 0; h < QPK; ++h) {
-    m[h] = NEG_BIG;
-    l[h] = 0.0f;
+    for (int i = 0; i < PT; ++i) raw[i] = v_raw[i];
+    load_idx(t);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < PT; ++i)
+      v[i] = ld16<true>(reinterpret_cast<const u32x4_v*>(v_cache + checked(raw[i]) * (HKV * HEAD_DIM / 2)) +
+                        (lane & 31));
+  };
+  load_idx(t0);
+  const QRaw q_raw = load_q(q + (out_row + r) * HEAD_DIM, g);
+  __builtin_amdgcn_sched_barrier(0);
+  load_k();
+  load_v(t0 + IT);
+  __builtin_amdgcn_sched_barrier(0);
+  const QRow qf = split_q(q_raw, true);
+
+  float m = NEG_BIG, l = 0.0f;  // of query head r (l: over the lane's tokens)
+  float acc[QPK][32];           // query heads 2 grp and 2 grp + 1, over the half's tokens
+#pragma unroll
+  for (int h = 0; h < QPK; ++h)
 #pragma unroll
     for (int d = 0; d < 32; ++d) acc[h][d] = 0.0f;
-  }
 
-  const int32_t* idx = kv_indices + kv_base;
-  auto load_idx = [&](int t0, int32_t (&raw)[TPL]) {
+  // MORE: the next iteration's rows are loaded, K's once this one's are used up, V's likewise.
+  auto iterate = [&](auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    *reinterpret_cast<u32x4_v*>(mine.sc + (lane >> 2) * kScaleRow + 16 * (lane & 3)) = sc;
+    wave_sync();
+    f32x4_v s;
 #pragma unroll
-    for (int t = 0; t < TPL; ++t) raw[t] = idx[min(t0 + 2 * t + half, end - 1)];
-  };
-  // Positions past the segment's end load its last token again and get weight 0.
-  auto load_tile = [&](int t0, const int32_t (&raw)[TPL], bool (&ok)[TPL], TileRegs& r) {
+    for (int h = 0; h < HKV; ++h) {
+      const i32x8_v a{(int)k[h].x, (int)k[h].y, (int)k[h].z, (int)k[h].w, 0, 0, 0, 0};
+      const int ks = mine.sc[r * kScaleRow + 8 * h + g];
+      // (formats 4 and 0: e2m1 and e4m3; the last operands name the scales' bytes)
+      f32x4_v d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf.hi, f32x4_v{}, 4, 0, 0, ks, 0, qf.scale);
+      d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf.lo, d, 4, 0, 0, ks, 1, qf.scale);
 #pragma unroll
-    for (int t = 0; t < TPL; ++t) {
-      int64_t sv = static_cast<int64_t>(raw[t]);
-      if (sv < 0 || sv >= num_slots) sv = 0;
-      ok[t] = t0 + 2 * t + half < end;
-      r.k[t] = ld16<true>(reinterpret_cast<const u32x4_v*>(k_cache + sv * (HKV * HEAD_DIM / 2)) +
-                          (lane & 31));
-      r.v[t] = ld16<true>(reinterpret_cast<const u32x4_v*>(v_cache + sv * (HKV * HEAD_DIM / 2)) +
-                          (lane & 31));
-      r.sc[t] = kv_scales[sv * HKV + grp];
+      for (int i = 0; i < 4; ++i) s[i] = h == 0 || (r >> 1) == h ? d[i] : s[i];
     }
-    __builtin_amdgcn_sched_barrier(0);  // (as in decode_attention.hip: all loads go out first)
-  };
-  auto compute = [&](const bool (&ok)[TPL], const TileRegs& r) {
-    float sc[QPK][TPL];
+    float vs[PT];
 #pragma unroll
-    for (int t = 0; t < TPL; ++t) {
-      const float ks = fp4_scale((r.sc[t].x >> (8 * blk)) & 255u);
-      float s[QPK] = {};
+    for (int i = 0; i < PT; ++i)
+      vs[i] = fp4_scale(mine.sc[(PT * half + i) * kScaleRow + 8 * grp + 4 + blk]);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kMore) load_k();
+    __builtin_amdgcn_sched_barrier(0);
+    float tmax = NEG_BIG;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 kc = fp4_to_bf16x8(r.k[t][i], ks);
-#pragma unroll
-        for (int h = 0; h < QPK; ++h) {
-          s[h] = dot2(qv[h][i].x, kc.x, s[h]);
-          s[h] = dot2(qv[h][i].y, kc.y, s[h]);
-          s[h] = dot2(qv[h][i].z, kc.z, s[h]);
-          s[h] = dot2(qv[h][i].w, kc.w, s[h]);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < QPK; ++h) {  // over the head's 4 lanes
-        s[h] += dpp<DPP_QUAD_XOR1>(s[h]);
-        s[h] += dpp<DPP_QUAD_XOR2>(s[h]);
-        sc[h][t] = s[h] * sm_scale;
-      }
+    for (int i = 0; i < 4; ++i) {
+      s[i] = s[i] * sm_scale;
+      tmax = t0 + 4 * g + i < end ? fmaxf(tmax, s[i]) : tmax;
     }
+    const float mn = fmaxf(m, pair_max(tmax));
+    const float rs = __expf(m - mn);
+    f32x4_v p;
+    float psum = 0.0f;
 #pragma unroll
-    for (int h = 0; h < QPK; ++h) {
-      float tmax = NEG_BIG;
+    for (int i = 0; i < 4; ++i) {
+      p[i] = t0 + 4 * g + i < end ? __expf(s[i] - mn) : 0.0f;
+      psum += p[i];
+    }
+    l = l * rs + psum;
+    m = mn;
+    *reinterpret_cast<f32x4_v*>(&mine.p[r][4 * g]) = p;
+    const bool moved = __builtin_amdgcn_ballot_w64(rs != 1.0f) != 0;
+    if (moved) {
+      if (g == 0) mine.rs[r] = rs;
+      wave_sync();
 #pragma unroll
-      for (int t = 0; t < TPL; ++t)
-        if (ok[t]) tmax = fmaxf(tmax, sc[h][t]);
-      const float mn = fmaxf(m[h], tmax);
-      const float rs = __expf(m[h] - mn);
-      float psum = 0.0f;
+      for (int h = 0; h < QPK; ++h) {
+        const float x = mine.rs[QPK * grp + h];
 #pragma unroll
-      for (int t = 0; t < TPL; ++t) {
-        sc[h][t] = ok[t] ? __expf(sc[h][t] - mn) : 0.0f;
-        psum += sc[h][t];
-      }
-      l[h] = l[h] * rs + psum;
-      m[h] = mn;
-      if (__builtin_amdgcn_ballot_w64(rs != 1.0f) != 0) {
-#pragma unroll
-        for (int d = 0; d < 32; ++d) acc[h][d] *= rs;
+        for (int d = 0; d < 32; ++d) acc[h][d] *= x;
       }
     }
+    wave_sync();
+    f32x4_v w[QPK][PT / 4];
 #pragma unroll
-    for (int t = 0; t < TPL; ++t) {
-      const float vs = fp4_scale((r.sc[t].y >> (8 * blk)) & 255u);
+    for (int h = 0; h < QPK; ++h)
+#pragma unroll
+      for (int i = 0; i < PT / 4; ++i)
+        w[h][i] = *reinterpret_cast<const f32x4_v*>(&mine.p[QPK * grp + h][PT * half + 4 * i]);
+#pragma unroll
+    for (int t = 0; t < PT; ++t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         f32x2_fp4 x[4];
-        x[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.v[t][i], vs, 0);
-        x[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.v[t][i], vs, 1);
-        x[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.v[t][i], vs, 2);
-        x[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.v[t][i], vs, 3);
+        x[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[t][i], vs[t], 0);
+        x[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[t][i], vs[t], 1);
+        x[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[t][i], vs[t], 2);
+        x[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[t][i], vs[t], 3);
 #pragma unroll
         for (int h = 0; h < QPK; ++h) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            acc[h][8 * i + 2 * e] += sc[h][t] * x[e].x;
-            acc[h][8 * i + 2 * e + 1] += sc[h][t] * x[e].y;
+            acc[h][8 * i + 2 * e] += w[h][t / 4][t % 4] * x[e].x;
+            acc[h][8 * i + 2 * e + 1] += w[h][t / 4][t % 4] * x[e].y;
           }
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kMore) load_v(t0 + 2 * IT);
+    wave_sync();
   };
+  // (a wave whose first token is past the segment's end adds nothing)
+  for (; t0 + IT < end; t0 += IT) iterate(std::true_type{});
+  if (t0 < end) iterate(std::false_type{});
 
-  // Rows are loaded one iteration ahead of their math, their slots two.
-  int32_t raw[TPL];
-  TileRegs r;
-  bool ok[TPL];
-  int t0 = start + wave * 2 * TPL;
-  load_idx(t0, raw);
-  load_tile(t0, raw, ok, r);
-  load_idx(t0 + IT, raw);
-  for (; t0 + IT < end; t0 += IT) {
-    TileRegs next;
-    bool next_ok[TPL];
-    load_tile(t0 + IT, raw, next_ok, next);
-    load_idx(t0 + 2 * IT, raw);
-    compute(ok, r);
-    r = next;
-#pragma unroll
-    for (int t = 0; t < TPL; ++t) ok[t] = next_ok[t];
+  l = pair_sum(l);
+  if (g == 0) {
+    sh.m[wave][r] = m;
+    sh.l[wave][r] = l;
   }
-  if (t0 < end) compute(ok, r);
-
-  // The halves' states into one: both lanes of a pair compute it on the same operands.
 #pragma unroll
   for (int h = 0; h < QPK; ++h) {
-    auto pair = [](float v) {
-      return __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    };
-    const auto pm = pair(m[h]), pl = pair(l[h]);
-    const float m0 = __uint_as_float(pm[0]), m1 = __uint_as_float(pm[1]);
-    const float mn = fmaxf(m0, m1);
-    const float a0 = __expf(m0 - mn), a1 = __expf(m1 - mn);
-    m[h] = mn;
-    l[h] = __uint_as_float(pl[0]) * a0 + __uint_as_float(pl[1]) * a1;
 #pragma unroll
     for (int d = 0; d < 32; ++d) {
-      const auto p = pair(acc[h][d]);
-      acc[h][d] = __uint_as_float(p[0]) * a0 + __uint_as_float(p[1]) * a1;
+      const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[h][d]), __float_as_uint(acc[h][d]),
+                                                      false, false);
+      acc[h][d] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
     }
     // half h writes query head h of the pair
     if (half == h) {
-      const int hq = QPK * grp + h;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<float4*>(&sh.acc[wave][hq][32 * blk + 4 * j]) =
+        *reinterpret_cast<float4*>(&sh.acc[wave][QPK * grp + h][32 * blk + 4 * j]) =
             make_float4(acc[h][4 * j], acc[h][4 * j + 1], acc[h][4 * j + 2], acc[h][4 * j + 3]);
-      if (blk == 0) {
-        sh.m[wave][hq] = m[h];
-        sh.l[wave][hq] = l[h];
-      }
     }
   }
   __syncthreads();
@@ -228,17 +255,18 @@ __device__ __forceinline__ void stage1_item(
 // wg_order at its linear id; or the items that wg_order deals to each of `gridDim.x` workers
 // (order entries i, i + workers, ...; from the first one flagged empty on, all are).
 template <int NW, bool WORKER>
-__global__ void __launch_bounds__(NW * 64) decode_fp4_stage1_kernel(
+__global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ k_cache,
-    const uint8_t* __restrict__ v_cache, const uint2* __restrict__ kv_scales,
+    const uint8_t* __restrict__ v_cache, const uint8_t* __restrict__ kv_scales,
     const int32_t* __restrict__ kv_indptr, const int32_t* __restrict__ kv_indices,
     const int32_t* __restrict__ num_splits, int max_splits, int fixed_split, int seg,
     float sm_scale, int64_t num_slots, int part_stride, float* __restrict__ part_o,
     float* __restrict__ part_lse, bf16_t* __restrict__ o_direct,
     const int32_t* __restrict__ wg_order, int batch, int grid_slots) {
   __shared__ Stage1Lds<NW> sh;
+  __shared__ WaveLds own[NW];
   auto item = [&](int b, int y) {
-    stage1_item<NW>(sh, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, num_splits,
+    stage1_item<NW>(sh, own, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, num_splits,
                     max_splits, fixed_split, seg, sm_scale, num_slots, part_stride, part_o, part_lse,
                     o_direct);
   };
@@ -312,7 +340,7 @@ extern "C" int sid_flash_decode_fp4_fwd(
   auto stage1 = [&](auto kern, int nw) {
     hipLaunchKernelGGL(kern, worker ? dim3(workers) : dim3(batch, grid_slots), dim3(nw * 64), 0, s,
                        (const bf16_t*)q, (const uint8_t*)k_cache, (const uint8_t*)v_cache,
-                       (const uint2*)kv_scales, kv_indptr, kv_indices, num_splits, max_splits,
+                       (const uint8_t*)kv_scales, kv_indptr, kv_indices, num_splits, max_splits,
                        fixed_split_size, segment_size, sm_scale, num_slots, part_stride, part_o,
                        part_lse, direct ? (bf16_t*)o : nullptr, wg_order, batch, grid_slots);
   };
