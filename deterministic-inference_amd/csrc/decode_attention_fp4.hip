@@ -56,7 +56,7 @@ __device__ __forceinline__ void wave_sync() {
 // workgroup of NW waves taking WT tokens per wave iteration. Every exit is workgroup-uniform.
 template <int NW>
 __device__ __forceinline__ void stage1_item(
-    Stage1Lds<NW>& sh, WaveLds (&own)[NW], int b, int y, const bf16_t* __restrict__ q,
+    Stage1Lds<NW>& sh, WaveLds (&own)[NW], char* q_rows, int b, int y, const bf16_t* __restrict__ q,
     const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
     const uint8_t* __restrict__ kv_scales, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ num_splits,
@@ -67,7 +67,7 @@ __device__ __forceinline__ void stage1_item(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;  // K: token and block; S: query head, tokens 4 g .. +3
-  const int half = lane >> 5;              // V: tokens PT half .. +PT-1,
+  const int half = lane >> 5;              // V: tokens half, 2 + half, ..,
   const int grp = (lane >> 2) & 7;         // kv head
   const int blk = lane & 3;                // and block of 32 dims
 
@@ -91,47 +91,57 @@ __device__ __forceinline__ void stage1_item(
     return;
   }
 
+  // q as codes, by the first 256 threads for all waves.
+  uint4 q_raw;
+  if (tid < 256) q_raw = *reinterpret_cast<const uint4*>(q + out_row * HEAD_DIM + 8 * tid);
+
   WaveLds& mine = own[wave];
   const int32_t* idx = kv_indices + kv_base;
-  int t0 = start + wave * WT;
-  // Positions past the segment's end load its last token again and get weight 0.
-  auto slot_of = [&](int t) { return idx[min(t, end - 1)]; };
-  auto checked = [&](int32_t raw) -> int64_t {
-    return raw < 0 || raw >= num_slots ? 0 : static_cast<int64_t>(raw);
-  };
-  int32_t k_raw, s_raw, v_raw[PT];  // slots of this lane's K row, scales and V rows
+  // Fewer tokens than an iteration takes: an even number for each wave, as a wave's time goes with its
+  // tokens.
+  if (end - start < IT) {
+    const int n = ceil_div(end - start, 2 * NW) * 2;
+    start += wave * n;
+    end = min(start + n, end);
+  } else {
+    start += wave * WT;
+  }
+  int t0 = start;
+  const uint32_t max_slots = static_cast<uint32_t>(min<int64_t>(num_slots, 0x7fffffff));
+  uint32_t raw, v_slot[PT];  // slots of token r of the next iteration and of this lane's V rows
   u32x4_v k[HKV], v[PT], sc;
-  auto load_idx = [&](int t) {
-    s_raw = slot_of(t + (lane >> 2));
-    k_raw = slot_of(t + r);
-#pragma unroll
-    for (int i = 0; i < PT; ++i) v_raw[i] = slot_of(t + PT * half + i);
+  // Positions past the segment's end load its last token again and get weight 0.
+  auto load_idx = [&](int t) { raw = idx[min(t + r, end - 1)]; };
+  auto from_lane = [](uint32_t x, int l) -> uint32_t { return __builtin_amdgcn_ds_bpermute(4 * l, x); };
+  auto row_at = [](const uint8_t* base, uint32_t slot) {  // 512 bytes a slot
+    return reinterpret_cast<const u32x4_v*>(base + (static_cast<uint64_t>(slot >> 23) << 32 | slot << 9));
   };
+  const uint8_t* k_base = k_cache + 16 * g;
+  const uint8_t* v_base = v_cache + 16 * (lane & 31);
+  const uint8_t* s_base = kv_scales + 16 * (lane & 3);
   auto load_k = [&] {
-    sc = ld16<true>(reinterpret_cast<const u32x4_v*>(kv_scales + checked(s_raw) * (8 * HKV)) + (lane & 3));
-    const u32x4_v* row = reinterpret_cast<const u32x4_v*>(k_cache + checked(k_raw) * (HKV * HEAD_DIM / 2)) + g;
+    const uint32_t slot = raw < max_slots ? raw : 0u;
+    sc = ld16<true>(reinterpret_cast<const u32x4_v*>(s_base + static_cast<uint64_t>(from_lane(slot, lane >> 2)) * 64u));
+    const u32x4_v* row = row_at(k_base, slot);
 #pragma unroll
     for (int h = 0; h < HKV; ++h) k[h] = ld16<true>(row + 4 * h);
+#pragma unroll
+    for (int i = 0; i < PT; ++i) v_slot[i] = from_lane(slot, 2 * i + half);
   };
   // V's rows, behind the slots of the tokens at t: those are waited for while V is under way.
   auto load_v = [&](int t) {
-    int32_t raw[PT];
-#pragma unroll
-    for (int i = 0; i < PT; ++i) raw[i] = v_raw[i];
     load_idx(t);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < PT; ++i)
-      v[i] = ld16<true>(reinterpret_cast<const u32x4_v*>(v_cache + checked(raw[i]) * (HKV * HEAD_DIM / 2)) +
-                        (lane & 31));
+    for (int i = 0; i < PT; ++i) v[i] = ld16<true>(row_at(v_base, v_slot[i]));
   };
   load_idx(t0);
-  const QRaw q_raw = load_q(q + (out_row + r) * HEAD_DIM, g);
-  __builtin_amdgcn_sched_barrier(0);
   load_k();
   load_v(t0 + IT);
   __builtin_amdgcn_sched_barrier(0);
-  const QRow qf = split_q(q_raw, true);
+  if (tid < 256) split_q_row(q_raw, tid & 15, q_rows + (tid >> 4) * kQRow);
+  __syncthreads();
+  const QRow qf = read_q_row(q_rows + r * kQRow, g);
 
   float m = NEG_BIG, l = 0.0f;  // of query head r (l: over the lane's tokens)
   float acc[QPK][32];           // query heads 2 grp and 2 grp + 1, over the half's tokens
@@ -159,7 +169,7 @@ __device__ __forceinline__ void stage1_item(
     float vs[PT];
 #pragma unroll
     for (int i = 0; i < PT; ++i)
-      vs[i] = fp4_scale(mine.sc[(PT * half + i) * kScaleRow + 8 * grp + 4 + blk]);
+      vs[i] = fp4_scale(mine.sc[(2 * i + half) * kScaleRow + 8 * grp + 4 + blk]);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (kMore) load_k();
     __builtin_amdgcn_sched_barrier(0);
@@ -180,7 +190,9 @@ __device__ __forceinline__ void stage1_item(
     }
     l = l * rs + psum;
     m = mn;
-    *reinterpret_cast<f32x4_v*>(&mine.p[r][4 * g]) = p;
+    // (tokens 0, 2, .., 1, 3, ..: a half's weights in two pieces)
+    *reinterpret_cast<f32x2_fp4*>(&mine.p[r][2 * g]) = f32x2_fp4{p[0], p[2]};
+    *reinterpret_cast<f32x2_fp4*>(&mine.p[r][PT + 2 * g]) = f32x2_fp4{p[1], p[3]};
     const bool moved = __builtin_amdgcn_ballot_w64(rs != 1.0f) != 0;
     if (moved) {
       if (g == 0) mine.rs[r] = rs;
@@ -201,6 +213,7 @@ __device__ __forceinline__ void stage1_item(
         w[h][i] = *reinterpret_cast<const f32x4_v*>(&mine.p[QPK * grp + h][PT * half + 4 * i]);
 #pragma unroll
     for (int t = 0; t < PT; ++t) {
+      if (!kMore && t0 + 2 * t >= end) break;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         f32x2_fp4 x[4];
@@ -231,22 +244,17 @@ __device__ __forceinline__ void stage1_item(
     sh.m[wave][r] = m;
     sh.l[wave][r] = l;
   }
+  // The halves' sums; half h gets and writes query head h of the pair.
 #pragma unroll
-  for (int h = 0; h < QPK; ++h) {
-#pragma unroll
-    for (int d = 0; d < 32; ++d) {
-      const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[h][d]), __float_as_uint(acc[h][d]),
-                                                      false, false);
-      acc[h][d] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-    }
-    // half h writes query head h of the pair
-    if (half == h) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<float4*>(&sh.acc[wave][QPK * grp + h][32 * blk + 4 * j]) =
-            make_float4(acc[h][4 * j], acc[h][4 * j + 1], acc[h][4 * j + 2], acc[h][4 * j + 3]);
-    }
+  for (int d = 0; d < 32; ++d) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[0][d]), __float_as_uint(acc[1][d]),
+                                                    false, false);
+    acc[0][d] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(&sh.acc[wave][QPK * grp + half][32 * blk + 4 * j]) =
+        make_float4(acc[0][4 * j], acc[0][4 * j + 1], acc[0][4 * j + 2], acc[0][4 * j + 3]);
   __syncthreads();
   stage1_merge<NW>(sh, tid, out_row, y, part_stride, part_o, part_lse, o_direct);
 }
@@ -265,8 +273,9 @@ __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
     const int32_t* __restrict__ wg_order, int batch, int grid_slots) {
   __shared__ Stage1Lds<NW> sh;
   __shared__ WaveLds own[NW];
+  __shared__ __align__(16) char q_rows[HQ * kQRow];
   auto item = [&](int b, int y) {
-    stage1_item<NW>(sh, own, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, num_splits,
+    stage1_item<NW>(sh, own, q_rows, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, num_splits,
                     max_splits, fixed_split, seg, sm_scale, num_slots, part_stride, part_o, part_lse,
                     o_direct);
   };
