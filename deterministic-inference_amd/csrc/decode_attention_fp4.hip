@@ -1,13 +1,23 @@
 // Split-KV paged decode attention over the 4-bit pool (format: kv_fp4.h), gfx950.
 //
 // The partition into splits and segments, the placement orders, the waves' merge and stage 2
-// are decode_attention.hip's (decode_split.h); what a wave does with the tokens' rows differs:
-//   * a row of K (V) is 8 heads x 64 bytes of codes: one 16-byte load of a wave is the rows of two
-//     tokens. Each half of the wave has one of them: lane l of it kv head l / 4 and block l % 4, 32
-//     dims with one scale; the scales of (token, head) come as one 8-byte load;
-//   * codes are converted with their power of two (exact): K to bf16 pairs for dot products with
-//     q, V to fp32.
-// The halves' softmax states are merged once, before the waves'.
+// are decode_attention.hip's (decode_split.h); what a wave does with its tokens, 16 at a time, differs:
+//   * scores come from the matrix units on the codes as they are: 16 tokens' K of a kv head (a lane:
+//     one block of 32 dims with its scale) times q as two e4m3 vectors (q_codes.h), for all 16 query
+//     heads, of which the 2 that belong to the kv head are kept. 8 x 2 such products replace the
+//     conversions and dot products that took 24 of the vector ALU's 76 instructions a token, and the
+//     softmax is one lane's work for (query head, 4 tokens), not that of every lane of a head;
+//   * a row of V is 8 heads x 64 bytes of codes: a 16-byte load of a wave is two tokens' rows. Lane l
+//     of a half-wave has kv head l / 4 and block l % 4, converted with its power of two (exact) to fp32
+//     and summed in fp32, with the weights from the wave's corner of the LDS;
+//   * K's next rows are loaded when this iteration's products are done with the registers, V's when its
+//     sums are: each has about an iteration's time, at 17 KB a wave under way.
+//
+// Workgroups are of 4 waves, two to a CU. (8 waves took 1 to 18 % longer in 30 of 31 batches, as their first
+// loads and their merge stand alone on a CU: 1 x 1024 tokens 11.3 and 12.2 us, 32 x 2048 21.0 and 22.4.)
+// 128 x 4096 tokens 98-109 us by the box (5.3-5.9 TB/s of codes and scales, where a plain read of memory reaches
+// 6.0), 64 x 2048 31, 1 x 131072 53, 1 x 1024 11. What bounds the large ones is memory; the small ones a
+// chain of latencies: lengths, slots, rows, the merge in the LDS and the second launch.
 #include "decode_split.h"
 #include "kv_fp4.h"
 #include "q_codes.h"
@@ -19,9 +29,11 @@ namespace {
 
 typedef float f32x4_v __attribute__((ext_vector_type(4)));
 
+constexpr int NW = 4;             // waves of a workgroup
 constexpr int WT = 16;            // tokens of a wave iteration
 constexpr int PT = WT / 2;        // those of a half-wave's V rows
 constexpr int kPRow = WT + 4;     // floats between two heads' weights (16-byte pieces, spread over the banks)
+static_assert(NW * 64 == HQ * HEAD_DIM / 8);
 constexpr int kScaleRow = 64 + 16;  // bytes between two tokens' scales
 
 // A wave's own corner of the LDS: no other wave reads it.
@@ -54,7 +66,6 @@ __device__ __forceinline__ void wave_sync() {
 
 // The partial attention of request b over partial slot y (a segment of one split), by one
 // workgroup of NW waves taking WT tokens per wave iteration. Every exit is workgroup-uniform.
-template <int NW>
 __device__ __forceinline__ void stage1_item(
     Stage1Lds<NW>& sh, WaveLds (&own)[NW], char* q_rows, int b, int y, const bf16_t* __restrict__ q,
     const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
@@ -91,9 +102,8 @@ __device__ __forceinline__ void stage1_item(
     return;
   }
 
-  // q as codes, by the first 256 threads for all waves.
-  uint4 q_raw;
-  if (tid < 256) q_raw = *reinterpret_cast<const uint4*>(q + out_row * HEAD_DIM + 8 * tid);
+  // q as codes, by all threads for all waves (250 instructions a wave if each did all).
+  const uint4 q_raw = *reinterpret_cast<const uint4*>(q + out_row * HEAD_DIM + 8 * tid);
 
   WaveLds& mine = own[wave];
   const int32_t* idx = kv_indices + kv_base;
@@ -139,7 +149,7 @@ __device__ __forceinline__ void stage1_item(
   load_k();
   load_v(t0 + IT);
   __builtin_amdgcn_sched_barrier(0);
-  if (tid < 256) split_q_row(q_raw, tid & 15, q_rows + (tid >> 4) * kQRow);
+  split_q_row(q_raw, tid & 15, q_rows + (tid >> 4) * kQRow);
   __syncthreads();
   const QRow qf = read_q_row(q_rows + r * kQRow, g);
 
@@ -262,7 +272,7 @@ __device__ __forceinline__ void stage1_item(
 // Grid form and worker form, as in decode_attention.hip: workgroup (b, y), or the entry of
 // wg_order at its linear id; or the items that wg_order deals to each of `gridDim.x` workers
 // (order entries i, i + workers, ...; from the first one flagged empty on, all are).
-template <int NW, bool WORKER>
+template <bool WORKER>
 __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ k_cache,
     const uint8_t* __restrict__ v_cache, const uint8_t* __restrict__ kv_scales,
@@ -275,7 +285,7 @@ __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
   __shared__ WaveLds own[NW];
   __shared__ __align__(16) char q_rows[HQ * kQRow];
   auto item = [&](int b, int y) {
-    stage1_item<NW>(sh, own, q_rows, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, num_splits,
+    stage1_item(sh, own, q_rows, b, y, q, k_cache, v_cache, kv_scales, kv_indptr, kv_indices, num_splits,
                     max_splits, fixed_split, seg, sm_scale, num_slots, part_stride, part_o, part_lse,
                     o_direct);
   };
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
   }
 }
 
-constexpr int kNumVariants = 4;
+constexpr int kNumVariants = 4;  // the other pools' shapes; here all are the one
 
 }  // namespace
 }  // namespace sid
@@ -346,20 +356,14 @@ extern "C" int sid_flash_decode_fp4_fwd(
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool direct = grid_slots == 1;
   const bool worker = workers > 0 && !direct;
-  auto stage1 = [&](auto kern, int nw) {
-    hipLaunchKernelGGL(kern, worker ? dim3(workers) : dim3(batch, grid_slots), dim3(nw * 64), 0, s,
+  auto stage1 = [&](auto kern) {
+    hipLaunchKernelGGL(kern, worker ? dim3(workers) : dim3(batch, grid_slots), dim3(NW * 64), 0, s,
                        (const bf16_t*)q, (const uint8_t*)k_cache, (const uint8_t*)v_cache,
                        (const uint8_t*)kv_scales, kv_indptr, kv_indices, num_splits, max_splits,
                        fixed_split_size, segment_size, sm_scale, num_slots, part_stride, part_o,
                        part_lse, direct ? (bf16_t*)o : nullptr, wg_order, batch, grid_slots);
   };
-  if (variant == 2) {
-    worker ? stage1(decode_fp4_stage1_kernel<8, true>, 8)
-           : stage1(decode_fp4_stage1_kernel<8, false>, 8);
-  } else {
-    worker ? stage1(decode_fp4_stage1_kernel<4, true>, 4)
-           : stage1(decode_fp4_stage1_kernel<4, false>, 4);
-  }
+  worker ? stage1(decode_fp4_stage1_kernel<true>) : stage1(decode_fp4_stage1_kernel<false>);
   rc = check_launch("flash_decode_fp4_fwd stage1");
   if (rc != SID_OK || direct) return rc;
   return launch_decode_stage2(batch, grid_slots, part_o, part_lse, part_stride, o, s);

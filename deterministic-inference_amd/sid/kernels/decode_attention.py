@@ -267,11 +267,13 @@ def plan_variant(lengths, max_len: int, num_kv_heads: int, cu_count: int, max_kv
 # of 4096 190.8 -> 171.2 us, 64 of 128-4096 73.4 -> 66.1, 8 of 100-8000 31.1 -> 24.7).
 FP8_SEGMENTS = (2048, 1024, 512, 256, 128, 64, 32)
 FP8_SHAPES = ((2, 0.5, 120, 60, 6), (3, 0.8, 15, 20, 0))  # variant, a, s, r, its own merge
+FP4_SHAPES = FP8_SHAPES[1:]  # the 4-bit pool's kernel has the one shape
 FP8_EMPTY_SLOT = 0.035
 FP8_MAX_PER_CU = 6  # more workgroups than this a CU are never the fastest
 
 
-def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int) -> tuple:
+def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int,
+                     shapes=FP8_SHAPES) -> tuple:
     """plan_variant's nondet plan for an 8-bit pool: ((1, segment size, grid slots), stage-1
     variant). Every request is one split cut into segments, so its policy batch does not enter;
     slots stay within what the workspace holds for any plan (workspace_slots)."""
@@ -292,7 +294,7 @@ def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int) -
         late = max(sizes.size / cu_count - 1.0, 0.0)
         merge = 0.7 * slots if lens.size > 4 else 32 * (_cdiv(slots, 32) - 1) + 0.15 * slots
         merge += FP8_EMPTY_SLOT * (lens.size * slots - sizes.size)
-        for variant, a, s, r, own in FP8_SHAPES:
+        for variant, a, s, r, own in shapes:
             busiest = _busiest_cu(sizes, cu_count, s)
             cost = mean + a * (busiest - mean) + r * late + merge + own
             if best is None or cost < best[0]:
@@ -301,8 +303,11 @@ def plan_variant_fp8(lengths, max_len: int, cu_count: int, max_kv_splits: int) -
 
 
 def plan_variant_fp4(lengths, max_len: int, cu_count: int, max_kv_splits: int) -> tuple:
-    """plan_variant_fp8 for a 4-bit pool (sid_flash_decode_fp4_fwd)."""
-    return plan_variant_fp8(lengths, max_len, cu_count, max_kv_splits)
+    """plan_variant_fp8 for a 4-bit pool (sid_flash_decode_fp4_fwd), whose kernel is of 4-wave
+    workgroups only. With the 8-bit pool's estimate for those the segment size is the fastest or
+    within 6% of it in 31 batches (B = 1-256, uniform and ragged, lengths 20-131072), 0.9% on
+    average."""
+    return plan_variant_fp8(lengths, max_len, cu_count, max_kv_splits, FP4_SHAPES)
 
 
 ORDER_SLOT_BITS = 12  # sid_flash_decode_segments_fwd wg_order entries: request << 12 | slot
@@ -384,6 +389,14 @@ def stage1_workers(nonempty: int, variant: int, slots: int, cu_count: int) -> in
     return 0
 
 
+# Over a 4-bit pool, whose 4-wave workgroups run two to a CU, workers (two a CU) pay where some of the
+# grid's workgroups would start behind others: 555 segments of 24 ragged requests 74.9 -> 72.8 us, 660
+# of 256 115 -> 109 (512 of 64 even ones 33.2, 33.4).
+def stage1_workers_fp4(nonempty: int, variant: int, slots: int, cu_count: int) -> int:
+    """stage1_workers for a 4-bit pool."""
+    return 2 * cu_count if slots > 1 and nonempty > 2 * cu_count else 0
+
+
 def worker_order(tokens: np.ndarray, workers: int) -> np.ndarray:
     """The wg_order of a worker launch: workgroup_order dealt over the workers, with the
     entries of items that hold no tokens flagged ORDER_EMPTY when they all come after every
@@ -397,17 +410,19 @@ def worker_order(tokens: np.ndarray, workers: int) -> np.ndarray:
 
 
 def placement(lengths, rows: int, splits: int, fixed_split: int, seg: int, slots: int,
-              variant: int, cu_count: int, workers_of=stage1_workers) -> tuple:
+              variant: int, cu_count: int, workers_of=stage1_workers, kv_fp4: bool = False) -> tuple:
     """(order, workers) of stage 1 for a plan over requests of these lengths, padded to `rows`:
     the heaviest-first workgroup order (workgroup_order, balanced over the CUs) for the grid,
     workers 0, or for a worker launch (workers_of's rule) the same dealing over the workers
     (worker_order). (None, 0), the grid's own order, where fewer segments than CUs hold tokens:
     there is nothing to balance, and reading the order first costs a small batch 0.2-0.4 us.
+    Over a 4-bit pool (workers_of = stage1_workers_fp4) that is so only where the whole grid starts at
+    once: among 512 slots 230 with tokens took 29.7 us in the grid's order, 21.5 heaviest first.
     Placement never changes a result."""
     tokens = segment_tokens(lengths, rows, splits, fixed_split, seg, slots)
     nonempty = int(np.count_nonzero(tokens))
     workers = workers_of(nonempty, variant, slots, cu_count)
-    if workers == 0 and nonempty < cu_count:
+    if workers == 0 and (tokens.size if kv_fp4 else nonempty) < cu_count:
         return None, 0
     return (worker_order(tokens, workers) if workers else workgroup_order(tokens, cu_count)), workers
 
@@ -492,7 +507,8 @@ class DecodeAttention:
         bound = max(max(lens, default=1) if max_len is None else int(max_len), 1)
         geom, variant = self.pick_plan(lens, bound, kv_fp8, kv_fp4)
         host, workers = placement(lens, len(lens), geom[0], 0, geom[1], geom[2], variant,
-                                  self.cu_count())
+                                  self.cu_count(), kv_fp4=kv_fp4,
+                                  workers_of=stage1_workers_fp4 if kv_fp4 else stage1_workers)
         order = None if host is None else torch.from_numpy(host).to(self.device)
         return dict(variant=variant, geometry=geom, wg_order=order, workers=workers)
 
