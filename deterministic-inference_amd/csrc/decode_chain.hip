@@ -29,7 +29,7 @@
 // numbered so they land on the same XCD (workgroups are dealt round-robin over the 8 XCDs
 // in id order) and share its L2.
 #include "common.h"
-#include "kv_fp8.h"
+#include "kv_codes.h"
 
 namespace sid {
 namespace {
@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(2 * PL * (NB / NBW) * 64) norm_silu_kernel(
 constexpr int QD = 128;
 
 // MBS = 2: 32-row workgroups (each weight fragment used for two row blocks), for batches
-// whose 16-row grid would not fit the CUs in one round. FP8: 8-bit pools (kv_fp8.h), k and v
-// quantised from the same bf16 values.
-template <int PL, bool F32, int MBS, bool FP8>
+// whose 16-row grid would not fit the CUs in one round. POOL: of codes (kv_fp8.h, kv_fp4.h), k
+// and v quantised from the same bf16 values.
+template <int PL, bool F32, int MBS, int POOL>
 __global__ void __launch_bounds__(512) norm_qkv_kernel(
     const void* __restrict__ src, const uint4* __restrict__ norm_w, float eps,
     const bf16_t* __restrict__ w, int M, int num_q_heads, int num_kv_heads, int R,
@@ -497,9 +497,9 @@ __global__ void __launch_bounds__(512) norm_qkv_kernel(
   const int kv_row = 16 * num_kv_heads;  // uint4 per pool row
   if (is_v) {
     const int h = head - num_q_heads - num_kv_heads;
-    if constexpr (FP8) {
-      fp8_store_vector(y, j, slot_ok, static_cast<uint2*>(v_cache), kv_scales,
-                       slot * num_kv_heads + h, 1);
+    if constexpr (POOL != kPoolBf16) {
+      code_store_vector<POOL>(y, j, slot_ok, v_cache, kv_scales,
+                               slot * num_kv_heads + h, 1);
     } else if (slot_ok) {
       static_cast<uint4*>(v_cache)[slot * kv_row + h * 16 + j] = store8(y);
     }
@@ -509,9 +509,9 @@ __global__ void __launch_bounds__(512) norm_qkv_kernel(
   qk_head_norm_rope(y, j, in, eps, o);
   if (is_q) {
     if (valid) q_out[(t * num_q_heads + head) * 16 + j] = store8(o);
-  } else if constexpr (FP8) {
-    fp8_store_vector(o, j, slot_ok, static_cast<uint2*>(k_cache), kv_scales,
-                     slot * num_kv_heads + head - num_q_heads, 0);
+  } else if constexpr (POOL != kPoolBf16) {
+    code_store_vector<POOL>(o, j, slot_ok, k_cache, kv_scales,
+                               slot * num_kv_heads + head - num_q_heads, 0);
   } else if (slot_ok) {
     static_cast<uint4*>(k_cache)[slot * kv_row + (head - num_q_heads) * 16 + j] = store8(o);
   }
@@ -659,8 +659,8 @@ extern "C" int sid_rmsnorm_linear_silu_mul(const void* src, int src_fp32, const 
   return check_launch("rmsnorm_linear_silu_mul");
 }
 
-// sid_rmsnorm_qkv_post (kv_scales NULL: bf16 pools) and sid_rmsnorm_qkv_post_fp8.
-static int launch_norm_qkv(const char* name, const void* src, int src_fp32, const void* norm_w,
+// sid_rmsnorm_qkv_post (kv_scales NULL), sid_rmsnorm_qkv_post_fp8 and sid_rmsnorm_qkv_post_fp4.
+static int launch_norm_qkv(const char* name, Pool pool, const void* src, int src_fp32, const void* norm_w,
                            float eps, const void* w_qkv, int64_t m, int64_t hidden,
                            int num_q_heads, int num_kv_heads, int head_dim, const void* q_norm,
                            const void* k_norm, const int64_t* positions, const float* cos_sin,
@@ -692,17 +692,19 @@ static int launch_norm_qkv(const char* name, const void* src, int src_fp32, cons
                        max_positions, slots, (uint4*)q_out, k_cache, v_cache,
                        (uint8_t*)kv_scales, num_slots);
   };
-#define SID_NQ(PL, F)                                                                         \
-  (kv_scales ? (mbs == 1 ? go(norm_qkv_kernel<PL, F, 1, true>)                                \
-                         : go(norm_qkv_kernel<PL, F, 2, true>))                               \
-             : (mbs == 1 ? go(norm_qkv_kernel<PL, F, 1, false>)                               \
-                         : go(norm_qkv_kernel<PL, F, 2, false>)))
+#define SID_NQP(PL, F, P) \
+  (mbs == 1 ? go(norm_qkv_kernel<PL, F, 1, P>) : go(norm_qkv_kernel<PL, F, 2, P>))
+#define SID_NQ(PL, F)                                  \
+  (pool == kPoolFp4   ? SID_NQP(PL, F, kPoolFp4)       \
+   : pool == kPoolFp8 ? SID_NQP(PL, F, kPoolFp8)       \
+                      : SID_NQP(PL, F, kPoolBf16))
   if (hidden == 512) {
     if (src_fp32) SID_NQ(1, true); else SID_NQ(1, false);
   } else {
     if (src_fp32) SID_NQ(2, true); else SID_NQ(2, false);
   }
 #undef SID_NQ
+#undef SID_NQP
   return check_launch(name);
 }
 
@@ -716,7 +718,7 @@ extern "C" int sid_rmsnorm_qkv_post(const void* src, int src_fp32, const void* n
                                     void* stream) {
   SID_REQUIRE(m >= 0 && hidden >= 0, "rmsnorm_qkv_post: negative size");
   if (m == 0) return SID_OK;
-  return launch_norm_qkv("rmsnorm_qkv_post", src, src_fp32, norm_w, eps, w_qkv, m, hidden,
+  return launch_norm_qkv("rmsnorm_qkv_post", kPoolBf16, src, src_fp32, norm_w, eps, w_qkv, m, hidden,
                          num_q_heads, num_kv_heads, head_dim, q_norm, k_norm, positions, cos_sin,
                          max_positions, slots, q_out, k_cache, v_cache, nullptr, num_slots, stream);
 }
@@ -732,7 +734,23 @@ extern "C" int sid_rmsnorm_qkv_post_fp8(const void* src, int src_fp32, const voi
   SID_REQUIRE(m >= 0 && hidden >= 0, "rmsnorm_qkv_post_fp8: negative size");
   if (m == 0) return SID_OK;
   SID_REQUIRE(kv_scales != nullptr, "rmsnorm_qkv_post_fp8: null pointer");
-  return launch_norm_qkv("rmsnorm_qkv_post_fp8", src, src_fp32, norm_w, eps, w_qkv, m, hidden,
+  return launch_norm_qkv("rmsnorm_qkv_post_fp8", kPoolFp8, src, src_fp32, norm_w, eps, w_qkv, m, hidden,
+                         num_q_heads, num_kv_heads, head_dim, q_norm, k_norm, positions, cos_sin,
+                         max_positions, slots, q_out, k_cache, v_cache, kv_scales, num_slots, stream);
+}
+
+extern "C" int sid_rmsnorm_qkv_post_fp4(const void* src, int src_fp32, const void* norm_w,
+                                        float eps, const void* w_qkv, int64_t m, int64_t hidden,
+                                        int num_q_heads, int num_kv_heads, int head_dim,
+                                        const void* q_norm, const void* k_norm,
+                                        const int64_t* positions, const float* cos_sin,
+                                        int64_t max_positions, const int64_t* slots, void* q_out,
+                                        void* k_cache, void* v_cache, void* kv_scales,
+                                        int64_t num_slots, void* stream) {
+  SID_REQUIRE(m >= 0 && hidden >= 0, "rmsnorm_qkv_post_fp4: negative size");
+  if (m == 0) return SID_OK;
+  SID_REQUIRE(kv_scales != nullptr, "rmsnorm_qkv_post_fp4: null pointer");
+  return launch_norm_qkv("rmsnorm_qkv_post_fp4", kPoolFp4, src, src_fp32, norm_w, eps, w_qkv, m, hidden,
                          num_q_heads, num_kv_heads, head_dim, q_norm, k_norm, positions, cos_sin,
                          max_positions, slots, q_out, k_cache, v_cache, kv_scales, num_slots, stream);
 }

@@ -80,10 +80,13 @@ Layout plan(const sid_qwen3_model* m, const sid_extend_batch* b, void* ws) {
   l.attn = c.take(t * ao * 2);
   l.act = c.take(t * inter * 2);
   const int64_t kvmax = b->max_kv_len > 0 ? b->max_kv_len : b->num_kv_indices;
-  l.ext_ws_bytes = sid_extend_attention_workspace_bytes(b->batch, t, m->num_q_heads,
-                                                        m->num_kv_heads,
-                                                        std::max(b->max_extend_len, 1),
-                                                        static_cast<int>(kvmax));
+  // (the pool's type is not known here: what any asks for. 4-bit pools split the keys of some batches
+  // that bf16 ones walk; 8-bit ones never ask for more than bf16 ones.)
+  const int longest = std::max(b->max_extend_len, 1), keys = static_cast<int>(kvmax);
+  l.ext_ws_bytes = std::max(
+      sid_extend_attention_workspace_bytes(b->batch, t, m->num_q_heads, m->num_kv_heads, longest, keys),
+      sid_extend_attention_fp4_workspace_bytes(b->batch, t, m->num_q_heads, m->num_kv_heads, longest,
+                                               keys));
   l.ext_ws = l.ext_ws_bytes > 0 ? c.take(l.ext_ws_bytes) : nullptr;
   l.rows = b->sample_indices ? c.take(r * h * 2) : nullptr;
   l.argmax_ws_bytes = b->temperatures ? sid_linear_sample_workspace_bytes(r)
@@ -149,9 +152,10 @@ extern "C" int64_t sid_qwen3_extend_workspace_bytes(const sid_qwen3_model* m,
   return plan(m, b, nullptr).total;
 }
 
-// kv_scales NULL: the layers' pools are bf16; else their scales' addresses, layer by layer.
+// kv_scales NULL: the layers' pools are bf16; else of 8-bit (fp4: 4-bit) codes, and these their scales'
+// addresses, layer by layer.
 static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
-                          void* const* kv_scales, void* workspace, int64_t workspace_bytes,
+                          void* const* kv_scales, bool fp4, void* workspace, int64_t workspace_bytes,
                           float* logits, int64_t* greedy_tokens, void* stream) {
   SID_REQUIRE(m && b, "qwen3_extend_forward: null descriptor");
   SID_REQUIRE(b->num_tokens >= 0 && b->batch >= 0, "qwen3_extend_forward: negative size");
@@ -189,10 +193,10 @@ static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
   auto norm_qkv_post = [&](int i, const void* src, int f32) {
     const sid_qwen3_layer& lw = m->layers[i];
     if (scales(i)) {
-      return sid_rmsnorm_qkv_post_fp8(src, f32, lw.input_ln, eps, lw.qkv_packed, t, h, hq, hkv, d,
-                                      lw.q_norm, lw.k_norm, b->positions, m->cos_sin,
-                                      m->max_positions, b->out_slots, l.q, lw.k_cache, lw.v_cache,
-                                      scales(i), m->num_slots, stream);
+      return (fp4 ? sid_rmsnorm_qkv_post_fp4 : sid_rmsnorm_qkv_post_fp8)(
+          src, f32, lw.input_ln, eps, lw.qkv_packed, t, h, hq, hkv, d, lw.q_norm, lw.k_norm,
+          b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q, lw.k_cache, lw.v_cache,
+          scales(i), m->num_slots, stream);
     }
     return sid_rmsnorm_qkv_post(src, f32, lw.input_ln, eps, lw.qkv_packed, t, h, hq, hkv, d,
                                 lw.q_norm, lw.k_norm, b->positions, m->cos_sin, m->max_positions,
@@ -201,9 +205,10 @@ static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
   auto qkv_post = [&](int i, const void* qkv, const float* partials, int nch) {
     const sid_qwen3_layer& lw = m->layers[i];
     if (scales(i)) {
-      return sid_qkv_post_fp8(qkv, partials, nch, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps,
-                              b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q,
-                              lw.k_cache, lw.v_cache, scales(i), m->num_slots, stream);
+      return (fp4 ? sid_qkv_post_fp4 : sid_qkv_post_fp8)(
+          qkv, partials, nch, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps, b->positions, m->cos_sin,
+          m->max_positions, b->out_slots, l.q, lw.k_cache, lw.v_cache, scales(i), m->num_slots,
+          stream);
     }
     return sid_qkv_post(qkv, partials, nch, t, hq, hkv, d, lw.q_norm, lw.k_norm, eps,
                         b->positions, m->cos_sin, m->max_positions, b->out_slots, l.q, lw.k_cache,
@@ -213,10 +218,10 @@ static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
     const sid_qwen3_layer& lw = m->layers[i];
     const int longest = std::max(b->max_extend_len, 1);
     if (scales(i)) {
-      return sid_extend_attention_fp8_fwd(l.q, lw.k_cache, lw.v_cache, scales(i), b->qo_indptr,
-                                          b->kv_indptr, b->kv_indices, b->batch, t, hq, hkv, d,
-                                          m->num_slots, longest, kvmax, m->sm_scale, l.ext_ws,
-                                          l.ext_ws_bytes, l.attn, stream);
+      return (fp4 ? sid_extend_attention_fp4_fwd : sid_extend_attention_fp8_fwd)(
+          l.q, lw.k_cache, lw.v_cache, scales(i), b->qo_indptr, b->kv_indptr, b->kv_indices, b->batch,
+          t, hq, hkv, d, m->num_slots, longest, kvmax, m->sm_scale, l.ext_ws, l.ext_ws_bytes, l.attn,
+          stream);
     }
     return sid_extend_attention_fwd(l.q, lw.k_cache, lw.v_cache, b->qo_indptr, b->kv_indptr,
                                     b->kv_indices, b->batch, t, hq, hkv, d, m->num_slots, longest,
@@ -290,7 +295,7 @@ static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
 extern "C" int sid_qwen3_extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
                                         void* workspace, int64_t workspace_bytes, float* logits,
                                         int64_t* greedy_tokens, void* stream) {
-  return extend_forward(m, b, nullptr, workspace, workspace_bytes, logits, greedy_tokens, stream);
+  return extend_forward(m, b, nullptr, false, workspace, workspace_bytes, logits, greedy_tokens, stream);
 }
 
 extern "C" int sid_qwen3_extend_forward_fp8(const sid_qwen3_model* m, const sid_extend_batch* b,
@@ -300,5 +305,15 @@ extern "C" int sid_qwen3_extend_forward_fp8(const sid_qwen3_model* m, const sid_
   SID_REQUIRE(m && kv_scales, "qwen3_extend_forward_fp8: null descriptor");
   for (int i = 0; i < m->num_layers; ++i)
     SID_REQUIRE(kv_scales[i] != nullptr, "qwen3_extend_forward_fp8: layer %d has no scales", i);
-  return extend_forward(m, b, kv_scales, workspace, workspace_bytes, logits, greedy_tokens, stream);
+  return extend_forward(m, b, kv_scales, false, workspace, workspace_bytes, logits, greedy_tokens, stream);
+}
+
+extern "C" int sid_qwen3_extend_forward_fp4(const sid_qwen3_model* m, const sid_extend_batch* b,
+                                            void* const* kv_scales, void* workspace,
+                                            int64_t workspace_bytes, float* logits,
+                                            int64_t* greedy_tokens, void* stream) {
+  SID_REQUIRE(m && kv_scales, "qwen3_extend_forward_fp4: null descriptor");
+  for (int i = 0; i < m->num_layers; ++i)
+    SID_REQUIRE(kv_scales[i] != nullptr, "qwen3_extend_forward_fp4: layer %d has no scales", i);
+  return extend_forward(m, b, kv_scales, true, workspace, workspace_bytes, logits, greedy_tokens, stream);
 }

@@ -13,7 +13,7 @@
 // kernels share goes through the same helpers with explicit fmaf, so the
 // fused and unfused paths also agree bit for bit after the first rounding.
 #include "common.h"
-#include "kv_fp8.h"
+#include "kv_codes.h"
 
 #include <cmath>
 
@@ -300,11 +300,11 @@ __global__ void __launch_bounds__(128) silu_mul_kernel(RowSrc gu, uint2* __restr
 // hidden 128), 8 heads per 128-thread block. q/k heads: per-head RMSNorm, round, RoPE (the
 // rotate-half partner of lane j is lane j ^ 8, one DPP row_ror:8 away), round;
 // v heads: copied. q goes to q_out [T, HQ, 128]; k and v to the pools at slots[t].
-// FP8: the pools hold codes and kv_scales their powers of two (kv_fp8.h); k and v are then
+// POOL: of codes, with their powers of two in kv_scales (kv_fp8.h, kv_fp4.h); k and v are then
 // quantised from the same bf16 values.
 constexpr int QD = 128;
 
-template <int NCH, bool FP8>
+template <int NCH, int POOL>
 __global__ void __launch_bounds__(128) qkv_post_kernel(
     RowSrc src, int num_q_heads, int num_kv_heads, const uint4* __restrict__ q_norm,
     const uint4* __restrict__ k_norm, float eps, const int64_t* __restrict__ positions,
@@ -328,9 +328,9 @@ __global__ void __launch_bounds__(128) qkv_post_kernel(
   const int kv_row = 16 * num_kv_heads;  // uint4 per pool row
   if (is_v) {
     const int h = hh - num_q_heads - num_kv_heads;
-    if constexpr (FP8) {
-      fp8_store_vector(v, j, valid && slot_ok, static_cast<uint2*>(v_cache), kv_scales,
-                       slot * num_kv_heads + h, 1);
+    if constexpr (POOL != kPoolBf16) {
+      code_store_vector<POOL>(v, j, valid && slot_ok, v_cache, kv_scales,
+                               slot * num_kv_heads + h, 1);
     } else if (valid && slot_ok) {
       static_cast<uint4*>(v_cache)[slot * kv_row + h * 16 + j] = store8(v);
     }
@@ -344,9 +344,9 @@ __global__ void __launch_bounds__(128) qkv_post_kernel(
   if (!valid) return;
   if (is_q) {
     q_out[(t * num_q_heads + hh) * 16 + j] = store8(o);
-  } else if constexpr (FP8) {
-    fp8_store_vector(o, j, slot_ok, static_cast<uint2*>(k_cache), kv_scales,
-                     slot * num_kv_heads + hh - num_q_heads, 0);
+  } else if constexpr (POOL != kPoolBf16) {
+    code_store_vector<POOL>(o, j, slot_ok, k_cache, kv_scales,
+                               slot * num_kv_heads + hh - num_q_heads, 0);
   } else if (slot_ok) {
     static_cast<uint4*>(k_cache)[slot * kv_row + (hh - num_q_heads) * 16 + j] = store8(o);
   }
@@ -473,8 +473,8 @@ extern "C" int sid_silu_mul_partials(const float* partials, int nchunks, void* o
                      stream, "silu_mul_partials");
 }
 
-// sid_qkv_post (kv_scales NULL: bf16 pools) and sid_qkv_post_fp8.
-static int launch_qkv_post(const char* name, const void* qkv, const float* partials, int nchunks,
+// sid_qkv_post (kv_scales NULL), sid_qkv_post_fp8 and sid_qkv_post_fp4.
+static int launch_qkv_post(const char* name, Pool pool, const void* qkv, const float* partials, int nchunks,
                            int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
                            const void* q_norm, const void* k_norm, float eps,
                            const int64_t* positions, const float* cos_sin, int64_t max_positions,
@@ -500,7 +500,9 @@ static int launch_qkv_post(const char* name, const void* qkv, const float* parti
                          eps, positions, cos_sin, max_positions, slots, (uint4*)q_out, k_cache,
                          v_cache, (uint8_t*)kv_scales, num_slots);
     };
-    if (kv_scales) go(qkv_post_kernel<NCH, true>); else go(qkv_post_kernel<NCH, false>);
+    if (pool == kPoolFp4) go(qkv_post_kernel<NCH, kPoolFp4>);
+    else if (pool == kPoolFp8) go(qkv_post_kernel<NCH, kPoolFp8>);
+    else go(qkv_post_kernel<NCH, kPoolBf16>);
   });
   return check_launch(name);
 }
@@ -513,7 +515,7 @@ extern "C" int sid_qkv_post(const void* qkv, const float* partials, int nchunks,
                             void* k_cache, void* v_cache, int64_t num_slots, void* stream) {
   SID_REQUIRE(num_tokens >= 0, "qkv_post: negative token count");
   if (num_tokens == 0) return SID_OK;
-  return launch_qkv_post("qkv_post", qkv, partials, nchunks, num_tokens, num_q_heads,
+  return launch_qkv_post("qkv_post", kPoolBf16, qkv, partials, nchunks, num_tokens, num_q_heads,
                          num_kv_heads, head_dim, q_norm, k_norm, eps, positions, cos_sin,
                          max_positions, slots, q_out, k_cache, v_cache, nullptr, num_slots,
                          stream);
@@ -529,7 +531,23 @@ extern "C" int sid_qkv_post_fp8(const void* qkv, const float* partials, int nchu
   SID_REQUIRE(num_tokens >= 0, "qkv_post_fp8: negative token count");
   if (num_tokens == 0) return SID_OK;
   SID_REQUIRE(kv_scales != nullptr, "qkv_post_fp8: null pointer");
-  return launch_qkv_post("qkv_post_fp8", qkv, partials, nchunks, num_tokens, num_q_heads,
+  return launch_qkv_post("qkv_post_fp8", kPoolFp8, qkv, partials, nchunks, num_tokens, num_q_heads,
+                         num_kv_heads, head_dim, q_norm, k_norm, eps, positions, cos_sin,
+                         max_positions, slots, q_out, k_cache, v_cache, kv_scales, num_slots,
+                         stream);
+}
+
+extern "C" int sid_qkv_post_fp4(const void* qkv, const float* partials, int nchunks,
+                                int64_t num_tokens, int num_q_heads, int num_kv_heads,
+                                int head_dim, const void* q_norm, const void* k_norm, float eps,
+                                const int64_t* positions, const float* cos_sin,
+                                int64_t max_positions, const int64_t* slots, void* q_out,
+                                void* k_cache, void* v_cache, void* kv_scales, int64_t num_slots,
+                                void* stream) {
+  SID_REQUIRE(num_tokens >= 0, "qkv_post_fp4: negative token count");
+  if (num_tokens == 0) return SID_OK;
+  SID_REQUIRE(kv_scales != nullptr, "qkv_post_fp4: null pointer");
+  return launch_qkv_post("qkv_post_fp4", kPoolFp4, qkv, partials, nchunks, num_tokens, num_q_heads,
                          num_kv_heads, head_dim, q_norm, k_norm, eps, positions, cos_sin,
                          max_positions, slots, q_out, k_cache, v_cache, kv_scales, num_slots,
                          stream);

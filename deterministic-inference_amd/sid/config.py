@@ -38,6 +38,8 @@ class ModelConfig:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 1e6
     max_position_embeddings: int = 40960
+    # Scaled rotary positions, as a checkpoint's config.json gives them (sid.kernels.rope)
+    rope_scaling: Optional[dict] = None
     tie_word_embeddings: bool = True
     eos_token_ids: tuple = (151645, 151643)
 
@@ -66,6 +68,9 @@ class EngineConfig:
     # instead of 4096 (Qwen3-0.6B), so twice the tokens fit, and decode attention reads half as
     # much. Tokens differ from a bf16 pool's (each K/V value is rounded to 4 significant bits);
     # the modes' guarantees are the same, since every path reads the same stored values.
+    # "fp4_e2m1": a 4-bit pool, e2m1 codes with a power of two for each 32 of them
+    # (sid.kernels.kv_fp4), 1088 bytes a token and layer: each value is rounded to 2 significant
+    # bits.
     kv_cache_dtype: str = "bfloat16"
     # KV pages: a request holds whole pages of this many consecutive pool slots (a power of
     # two; 1 = the reference's token-granular pool). Slot numbering, and so every kernel's
@@ -143,7 +148,7 @@ class EngineConfig:
 # Rows one lm_head-fused sampling pass takes with 128-column tiles (sid_linear_sample).
 MAX_SAMPLED_ROWS = 4096
 
-KV_CACHE_DTYPES = ("bfloat16", "fp8_e4m3")
+KV_CACHE_DTYPES = ("bfloat16", "fp8_e4m3", "fp4_e2m1")
 
 _DECODE_BACKENDS = {"cuda": "hip", "hip": "hip", "triton": "extend", "extend": "extend"}
 

@@ -3,8 +3,8 @@
 Replaces sid/engine/kv_cache.py of the reference, whose pool is token-granular (a GPU free
 stack of single slots and an int32 request -> token table [max_reqs, max_seq_len]). Here:
 
-  * pools: per layer, K and V bf16 [num_pages * page_size, HKV, D] (kv_cache_dtype "fp8_e4m3":
-    codes of that shape, and their scales; sid.kernels.kv_fp8). Slot numbering is
+  * pools: per layer, K and V bf16 [num_pages * page_size, HKV, D] (kv_cache_dtype "fp8_e4m3"
+    or "fp4_e2m1": codes, and their scales; sid.kernels.kv_fp8, sid.kernels.kv_fp4). Slot numbering is
     unchanged (slot = page * page_size + offset), so every kernel that takes slots
     (reshape_and_cache, attention through kv_indices) sees the reference's pool format;
   * block tables: int32 [max_reqs, max_pages] page ids per request row. The host copy is
@@ -30,6 +30,7 @@ import torch
 
 from sid.config import EngineConfig, ModelConfig
 from sid.kernels.jit import load_ext
+from sid.kernels.kv_fp4 import alloc_cache_fp4, gather_cache_fp4
 from sid.kernels.kv_fp8 import HEAD_DIM, alloc_cache_fp8, gather_cache_fp8
 from sid.kernels.ops import gather_rows
 
@@ -55,10 +56,13 @@ class KVCache:
         self.device = device
         self.ext = load_ext()
         self.kv_scales = None
-        if cfg.kv_cache_dtype == "fp8_e4m3":
+        self.dtype = cfg.kv_cache_dtype
+        if self.dtype != "bfloat16":
+            kind, alloc = (("an 8-bit", alloc_cache_fp8) if self.dtype == "fp8_e4m3"
+                           else ("a 4-bit", alloc_cache_fp4))
             if mcfg.head_dim != HEAD_DIM:
-                raise ValueError(f"an 8-bit KV pool needs head_dim {HEAD_DIM}, got {mcfg.head_dim}")
-            layers = [alloc_cache_fp8(self.num_slots, mcfg.num_kv_heads, device)
+                raise ValueError(f"{kind} KV pool needs head_dim {HEAD_DIM}, got {mcfg.head_dim}")
+            layers = [alloc(self.num_slots, mcfg.num_kv_heads, device)
                       for _ in range(mcfg.num_layers)]
             self.k_pools, self.v_pools, self.kv_scales = (list(x) for x in zip(*layers))
         else:
@@ -85,7 +89,7 @@ class KVCache:
         return self.k_pools[i], self.v_pools[i]
 
     def scales(self, i: int):
-        """The scales of layer i's 8-bit pools (sid.kernels.kv_fp8); None for bf16 pools."""
+        """The scales of layer i's pools of codes (sid.kernels.kv_fp8, kv_fp4); None for bf16 pools."""
         return None if self.kv_scales is None else self.kv_scales[i]
 
     def read(self, i: int, row: int, start: int, end: int) -> tuple:
@@ -94,7 +98,8 @@ class KVCache:
         slots = torch.from_numpy(self.slot_range(row, start, end)).to(self.device)
         k, v = self.layer(i)
         if self.kv_scales is not None:
-            return gather_cache_fp8(k, v, self.kv_scales[i], slots)
+            gather = gather_cache_fp8 if self.dtype == "fp8_e4m3" else gather_cache_fp4
+            return gather(k, v, self.kv_scales[i], slots)
         return tuple(gather_rows(x.view(self.num_slots, -1), slots).view(-1, *x.shape[1:])
                      for x in (k, v))
 

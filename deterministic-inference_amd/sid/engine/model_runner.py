@@ -20,7 +20,7 @@ from sid.engine.batch import (DecodeStatic, ForwardBatch, ForwardMode, batch_buc
 from sid.engine.kv_cache import KVCache
 from sid.engine.sampler import sample as _sample
 from sid.kernels.decode_attention import (INVARIANT_VARIANT, DecodeAttention, length_bucket,
-                                          placement, stage1_workers)
+                                          placement, stage1_workers, stage1_workers_fp4)
 from sid.kernels.matmul_persistent import linear_sample_supported
 from sid.model.loader import build_model_config, load_weights, random_weights
 from sid.model.qwen3 import Qwen3Model
@@ -217,9 +217,11 @@ class ModelRunner:
             splits, fixed, seg, slots = 0, tile, tile, max(1, -(-max(max_len, 1) // tile))
         else:
             (splits, seg, slots), fixed = geom, 0
+        kv_fp4 = self._kv_fp4()
         order, fb.decode_workers = placement(fb.seq_lens_host, rows, splits, fixed, seg, slots,
-                                             fb.decode_variant, da.cu_count(),
-                                             workers_of=stage1_workers)
+                                             fb.decode_variant, da.cu_count(), kv_fp4=kv_fp4,
+                                             workers_of=stage1_workers_fp4 if kv_fp4
+                                             else stage1_workers)
         fb.decode_wg_order = None
         if order is None:
             return 0
@@ -229,11 +231,14 @@ class ModelRunner:
             fb.decode_wg_order = torch.from_numpy(order).to(self.device)
         return fb.decode_workers or 1
 
+    def _kv_fp4(self) -> bool:
+        return getattr(self.kv_cache, "dtype", None) == "fp4_e2m1"
+
     def _pick_variant(self, fb: ForwardBatch, max_len: int) -> tuple:
         """The nondet plan's geometry and its stage-1 workgroup shape (fb.decode_variant),
         from the requests' host-known lengths."""
         fb.decode_geometry, fb.decode_variant = self.decode_attn.pick_plan(
-            fb.seq_lens_host, max_len, self.kv_cache.kv_scales is not None)
+            fb.seq_lens_host, max_len, self.kv_cache.kv_scales is not None, self._kv_fp4())
         return fb.decode_geometry
 
     def tag_verify(self, fb: ForwardBatch) -> ForwardBatch:

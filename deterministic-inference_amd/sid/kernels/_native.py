@@ -71,6 +71,10 @@ _SIGNATURES = {
     "sid_reshape_and_cache_fp4": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32,
                                   _i64, _vp],
     "sid_gather_cache_fp4": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _vp],
+    "sid_qkv_post_fp4": [_vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _vp, _vp, _i64,
+                         _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "sid_rmsnorm_qkv_post_fp4": [_vp, _i32, _vp, _f32, _vp, _i64, _i64, _i32, _i32, _i32, _vp,
+                                 _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "sid_flash_decode_fp4_fwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64,
                                  _i32, _i32, _i32, _i32, _i32, _vp, _f32, _vp, _vp, _i32, _i32,
                                  _vp, _i32, _vp],
@@ -84,7 +88,7 @@ EXPORTED = ("sid_last_error", "sid_abi_version", "sid_abi_revision",
             "sid_linear_argmax_workspace_bytes", "sid_sample_workspace_bytes",
             "sid_qwen3_extend_workspace_bytes", "sid_qwen3_extend_forward",
             "sid_qwen3_extend_forward_fp8", "sid_extend_attention_fp8_workspace_bytes",
-            "sid_extend_attention_fp4_workspace_bytes",
+            "sid_qwen3_extend_forward_fp4", "sid_extend_attention_fp4_workspace_bytes",
             "sid_flash_decode_noalloc_scratch_bytes", "sid_linear_sample_workspace_bytes",
             "sid_extend_attention_query_rows", "sid_linear_tile", *_SIGNATURES)
 ABI_VERSION = 22
@@ -648,7 +652,7 @@ class NativeLib:
 
     def qkv_post(self, qkv, partials, q_norm, k_norm, eps: float, positions, cos_sin, slots,
                  q_out, k_cache, v_cache, kv_scales=None) -> None:
-        """kv_scales: the caches are an 8-bit pool (sid_qkv_post_fp8)."""
+        """kv_scales: the caches are a pool of codes (sid_qkv_post_fp8, sid_qkv_post_fp4)."""
         _check((qkv is None) != (partials is None), "give exactly one of qkv and partials")
         if qkv is not None:
             _gpu(qkv, "qkv", torch.bfloat16)
@@ -661,7 +665,7 @@ class NativeLib:
             _gpu(q_out, "q_out", torch.bfloat16)
         _check(q_out.dim() == 3 and q_out.shape[0] == t, "q_out must be [T, HQ, D]")
         hq, d = q_out.shape[1], q_out.shape[2]
-        self._cache_operands(k_cache, v_cache, kv_scales, d, q_out)
+        kind = self._cache_operands(k_cache, v_cache, kv_scales, d, q_out)
         hkv = k_cache.shape[1]
         _check(width == (hq + 2 * hkv) * d, "projection width != (HQ + 2*HKV) * D")
         if not usual:
@@ -681,15 +685,15 @@ class NativeLib:
             else:
                 _same_device(q_out.get_device(), qkv, partials, q_norm, k_norm, positions, cos_sin,
                              slots)
-            self._launch(q_out.get_device(), "sid_qkv_post_fp8", *args, kv_scales.data_ptr(), k_cache.shape[0])
+            self._launch(q_out.get_device(), f"sid_qkv_post_{kind}", *args, kv_scales.data_ptr(), k_cache.shape[0])
             return
         self._call("sid_qkv_post", *args, k_cache.shape[0], _stream(q_out))
 
     @staticmethod
-    def _cache_operands(k_cache, v_cache, kv_scales, d: int, q) -> None:
+    def _cache_operands(k_cache, v_cache, kv_scales, d: int, q) -> str | None:
+        """Checks a pool; a pool of codes' kind."""
         if kv_scales is not None:
-            _pool8(k_cache, v_cache, kv_scales, d, q.get_device())
-            return
+            return _code_pool(k_cache, v_cache, kv_scales, d, q.get_device())[0]
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             _gpu(c, name, torch.bfloat16)
             _check(c.dim() == 3 and c.shape[2] == d, f"{name} must be [S, HKV, D]")
@@ -728,7 +732,7 @@ class NativeLib:
     def rmsnorm_qkv_post(self, src, norm_w, eps: float, w, q_norm, k_norm, positions, cos_sin,
                          slots, q_out, k_cache, v_cache, kv_scales=None) -> None:
         """qkv_post over bf16(rmsnorm(src) * norm_w) @ w^T (one launch); kv_scales: the caches
-        are an 8-bit pool (sid_rmsnorm_qkv_post_fp8)."""
+        are a pool of codes (sid_rmsnorm_qkv_post_fp8, sid_rmsnorm_qkv_post_fp4)."""
         f32 = self._norm_src(src)
         m, hidden = src.shape
         _gpu(norm_w, "norm weight", torch.bfloat16)
@@ -736,7 +740,7 @@ class NativeLib:
         _gpu(q_out, "q_out", torch.bfloat16)
         _check(q_out.dim() == 3 and q_out.shape[0] == m, "q_out must be [M, HQ, D]")
         hq, d = q_out.shape[1], q_out.shape[2]
-        self._cache_operands(k_cache, v_cache, kv_scales, d, q_out)
+        kind = self._cache_operands(k_cache, v_cache, kv_scales, d, q_out)
         hkv = k_cache.shape[1]
         _check(w.dim() == 2 and w.shape[0] == (hq + 2 * hkv) * d and w.shape[1] == hidden
                and norm_w.numel() == hidden, "qkv weight must be [(HQ + 2*HKV) * D, hidden]")
@@ -752,7 +756,7 @@ class NativeLib:
                 k_cache.data_ptr(), v_cache.data_ptr())
         if kv_scales is not None:
             _same_device(q_out.get_device(), src, norm_w, w, q_norm, k_norm, positions, cos_sin, slots)
-            self._launch(q_out.get_device(), "sid_rmsnorm_qkv_post_fp8", *args, kv_scales.data_ptr(),
+            self._launch(q_out.get_device(), f"sid_rmsnorm_qkv_post_{kind}", *args, kv_scales.data_ptr(),
                          k_cache.shape[0])
             return
         self._call("sid_rmsnorm_qkv_post", *args, k_cache.shape[0], _stream(q_out))

@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from sid.kernels.jit import load_ext
+from sid.kernels.kv_fp4 import FP4
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
@@ -62,16 +63,22 @@ def fused_add_rmsnorm_partials(partials: torch.Tensor, residual: torch.Tensor,
     return out, residual
 
 
+def _head_dim(k_cache: torch.Tensor) -> int:
+    d = k_cache.shape[2]
+    return 2 * d if k_cache.dtype == FP4 else d  # (two codes a byte)
+
+
 def qkv_post(qkv_or_partials: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
              positions: torch.Tensor, cos_sin: torch.Tensor, slots: torch.Tensor,
              k_cache: torch.Tensor, v_cache: torch.Tensor, num_q_heads: int,
              kv_scales: torch.Tensor | None = None) -> torch.Tensor:
     """Fused q/k-norm + RoPE + KV-cache write of a QKV projection (bf16 [T, W] or chunk
-    partials [C, T, W]); returns q [T, HQ, D]. kv_scales: the caches are an 8-bit pool, which
-    gets what reshape_and_cache_fp8 of the same rows would store (sid.kernels.kv_fp8)."""
+    partials [C, T, W]); returns q [T, HQ, D]. kv_scales: the caches are an 8-bit or a 4-bit
+    pool, which gets what reshape_and_cache_fp8 (reshape_and_cache_fp4) of the same rows would
+    store (sid.kernels.kv_fp8, sid.kernels.kv_fp4)."""
     partial = qkv_or_partials.dtype == torch.float32
     t = qkv_or_partials.shape[1] if partial else qkv_or_partials.shape[0]
-    d = k_cache.shape[2]
+    d = _head_dim(k_cache)
     q = torch.empty(t, num_q_heads, d, dtype=torch.bfloat16, device=k_cache.device)
     load_ext().qkv_post(None if partial else qkv_or_partials, qkv_or_partials if partial else None,
                         q_norm, k_norm, eps, positions, cos_sin, slots, q, k_cache, v_cache,
@@ -123,7 +130,7 @@ def rmsnorm_qkv_post(src: torch.Tensor, norm_w: torch.Tensor, eps: float, weight
                      kv_scales: torch.Tensor | None = None) -> torch.Tensor:
     """qkv_post of the qkv projection of bf16(rmsnorm(src) * norm_w); returns q [T, HQ, D].
     weight = pack_decode_weight(qkv); kv_scales as in qkv_post."""
-    d = k_cache.shape[2]
+    d = _head_dim(k_cache)
     q = torch.empty(src.shape[0], num_q_heads, d, dtype=torch.bfloat16, device=src.device)
     load_ext().rmsnorm_qkv_post(src, norm_w, eps, weight, q_norm, k_norm, positions, cos_sin,
                                 slots, q, k_cache, v_cache, kv_scales=kv_scales)

@@ -15,6 +15,7 @@ from pathlib import Path
 import torch
 
 from sid.config import ModelConfig
+from sid.kernels.rope import rope_type, scaled_frequencies
 
 
 def random_weights(mcfg: ModelConfig, device, seed: int = 0, std: float = 0.02,
@@ -59,6 +60,15 @@ def _read_json(path: Path) -> dict:
     return json.loads(path.read_text()) if path.exists() else {}
 
 
+def _rope_scaling(hf: dict) -> dict | None:
+    """config.json's rope_scaling, checked: positions that the model was not made for are an error."""
+    scaling = hf.get("rope_scaling")
+    if not scaling or rope_type(scaling) == "default":
+        return None
+    scaled_frequencies(hf["head_dim"], hf["rope_theta"], scaling)
+    return dict(scaling)
+
+
 def load_model_config(model_dir: Path, model_path: str) -> ModelConfig:
     """ModelConfig of a local Qwen3 checkpoint directory (config.json, and the stop ids of
     generation_config.json when present, as sid/model/loader.py:30-50 reads them)."""
@@ -72,6 +82,7 @@ def load_model_config(model_dir: Path, model_path: str) -> ModelConfig:
         "eos_token_id", hf.get("eos_token_id", 151645))
     return ModelConfig(model_path=model_path,
                        tie_word_embeddings=bool(hf.get("tie_word_embeddings", False)),
+                       rope_scaling=_rope_scaling(hf),
                        eos_token_ids=tuple(stop) if isinstance(stop, list) else (stop,),
                        **{field: hf[key] for field, key in _CONFIG_FIELDS})
 

@@ -58,7 +58,7 @@ class Qwen3Model:
         self.w = weights
         self.device = device
         self.rope = RotaryEmbedding(mcfg.head_dim, mcfg.max_position_embeddings,
-                                    mcfg.rope_theta, device)
+                                    mcfg.rope_theta, device, scaling=mcfg.rope_scaling)
         self.sm_scale = mcfg.head_dim ** -0.5
         self.invariant_gemm = False
         # Prefill / verify batches go through the native executor (one library call per

@@ -687,10 +687,25 @@ int sid_gather_cache_fp4(const void* k_cache, const void* v_cache, const void* k
                          const int64_t* slots, void* k, void* v, int64_t n, int num_kv_heads,
                          int head_dim, int64_t num_slots, void* stream);
 
+/* sid_qkv_post_fp8 / sid_rmsnorm_qkv_post_fp8 into a 4-bit pool. */
+int sid_qkv_post_fp4(const void* qkv, const float* partials, int nchunks, int64_t num_tokens,
+                     int num_q_heads, int num_kv_heads, int head_dim, const void* q_norm,
+                     const void* k_norm, float eps, const int64_t* positions,
+                     const float* cos_sin, int64_t max_positions, const int64_t* slots,
+                     void* q_out, void* k_cache, void* v_cache, void* kv_scales,
+                     int64_t num_slots, void* stream);
+int sid_rmsnorm_qkv_post_fp4(const void* src, int src_fp32, const void* norm_w, float eps,
+                             const void* w_qkv, int64_t m, int64_t hidden, int num_q_heads,
+                             int num_kv_heads, int head_dim, const void* q_norm,
+                             const void* k_norm, const int64_t* positions, const float* cos_sin,
+                             int64_t max_positions, const int64_t* slots, void* q_out,
+                             void* k_cache, void* v_cache, void* kv_scales, int64_t num_slots,
+                             void* stream);
+
 /*
- * sid_flash_decode_fp8_fwd over a 4-bit pool. The workgroup shapes that `variant` picks are this
- * kernel's own (part of the reduction order): 2 = 8 waves x 8 tokens per wave iteration, 0, 1 and
- * 3 = 4 x 8.
+ * sid_flash_decode_fp8_fwd over a 4-bit pool. The kernel has one workgroup shape, 4 waves x 16 tokens
+ * per wave iteration: any `variant` that the others take (0 .. 3) gives it. q enters the products
+ * as two e4m3 vectors (sid_extend_attention_fp8_fwd).
  */
 int sid_flash_decode_fp4_fwd(const void* q, const void* k_cache, const void* v_cache,
                              const void* kv_scales, const int32_t* kv_indptr,
@@ -715,6 +730,12 @@ int sid_extend_attention_fp4_fwd(const void* q, const void* k_cache, const void*
                                  int head_dim, int64_t num_slots, int max_extend_len,
                                  int max_kv_len, float sm_scale, void* workspace,
                                  int64_t workspace_bytes, void* o, void* stream);
+
+/* sid_qwen3_extend_forward_fp8 with 4-bit pools. Same workspace. */
+int sid_qwen3_extend_forward_fp4(const sid_qwen3_model* m, const sid_extend_batch* b,
+                                 void* const* kv_scales, void* workspace,
+                                 int64_t workspace_bytes, float* logits, int64_t* tokens,
+                                 void* stream);
 
 /*
  * Rotary positions from frequencies: q [T, HQ, D], k [T, HKV, D] bf16 with token strides ldq, ldk
