@@ -146,6 +146,32 @@ def _usual_qkv(q_out, q_norm, k_norm, positions, cos_sin, slots) -> bool:
         return False
 
 
+def _usual_load(slots, k, v) -> bool:
+    try:
+        return (-1 < slots.get_device() == k.get_device() == v.get_device() and slots.dtype is _I64
+                and k.dtype is _BF16 and v.dtype is _BF16 and slots.is_contiguous()
+                and k.is_contiguous() and v.is_contiguous())
+    except AttributeError:
+        return False
+
+
+def _usual_rope(turns, positions, q, k, q_out, k_out, rotary_dim: int) -> bool:
+    try:
+        (t, _, d), (tk, _, dk) = q.shape, k.shape
+        dense = (d, 1)
+        return (-1 < q.get_device() == k.get_device() == positions.get_device()
+                == turns.get_device() == q_out.get_device() == k_out.get_device()
+                and q.dtype is _BF16 and k.dtype is _BF16 and q_out.dtype is _BF16
+                and k_out.dtype is _BF16 and positions.dtype is _I64 and turns.dtype is _I64
+                and tk == t and dk == d and q_out.shape == q.shape and k_out.shape == k.shape
+                and positions.numel() == t and 2 * turns.numel() == rotary_dim
+                and positions.is_contiguous() and turns.is_contiguous()
+                and q.stride()[1:] == dense and k.stride()[1:] == dense
+                and q_out.stride()[1:] == dense and k_out.stride()[1:] == dense)
+    except (AttributeError, ValueError):
+        return False
+
+
 def _same_device(device: int, *tensors) -> None:
     """Every tensor (None: absent) is on GPU `device` (an index)."""
     for t in tensors:
@@ -440,16 +466,17 @@ class NativeLib:
                      cs[0])
 
     def _load_rows(self, name, pool, k_cache, v_cache, kv_scales, slots, k, v) -> None:
-        _gpu(slots, "slots", torch.int64)
-        _gpu(k, "k", torch.bfloat16)
-        _gpu(v, "v", torch.bfloat16)
+        if not _usual_load(slots, k, v):
+            _gpu(slots, "slots", torch.int64)
+            _gpu(k, "k", torch.bfloat16)
+            _gpu(v, "v", torch.bfloat16)
+            _same_device(slots.get_device(), k, v)
         xs, device = k.shape, slots.get_device()
         if len(xs) != 3 or v.shape != xs:
             raise RuntimeError("k and v must both be [N, HKV, D]")
         cs = pool(k_cache, v_cache, kv_scales, xs[2], device)
         if xs[0] != slots.numel() or xs[1] != cs[1]:
             raise RuntimeError("k must be [N, HKV, D] matching the slots and the cache")
-        _same_device(device, k, v)
         if xs[0] == 0:
             return
         self._launch(device, name, k_cache.data_ptr(), v_cache.data_ptr(),
@@ -534,11 +561,25 @@ class NativeLib:
     def rope_rotate(self, q, k, positions, turns, gain: float, rotary_dim: int,
                     interleaved: bool, max_positions: int, q_out, k_out) -> None:
         """q_out, k_out <- q, k rotated (sid_rope_rotate); they may be q and k."""
-        device = q.get_device()
+        args = (turns, positions, q, k, q_out, k_out)
+        if not _usual_rope(*args, rotary_dim):
+            self._rope_checks(*args, rotary_dim)
+        (t, hq, d), hkv = q.shape, k.shape[1]
+        if t == 0:
+            return
+        one = t == 1
+        self._launch(q.get_device(), "sid_rope_rotate", q.data_ptr(), hq * d if one else q.stride(0),
+                     k.data_ptr(), hkv * d if one else k.stride(0), positions.data_ptr(),
+                     turns.data_ptr(), gain, rotary_dim, interleaved, t, hq, hkv, d, max_positions,
+                     q_out.data_ptr(), hq * d if one else q_out.stride(0), k_out.data_ptr(),
+                     hkv * d if one else k_out.stride(0))
+
+    @staticmethod
+    def _rope_checks(turns, positions, q, k, q_out, k_out, rotary_dim: int) -> None:
         for name, x in (("q", q), ("k", k), ("q_out", q_out), ("k_out", k_out)):
             if not (x.is_cuda and x.dtype is _BF16 and x.dim() == 3):
                 raise RuntimeError(f"{name} must be a bf16 GPU tensor [T, heads, D]")
-        t, hq, d = q.shape
+        t, _, d = q.shape
         if k.shape[0] != t or k.shape[2] != d:
             raise RuntimeError("k must be [T, HKV, D] matching q")
         _check(q_out.shape == q.shape and k_out.shape == k.shape, "outputs must have the inputs' shapes")
@@ -546,20 +587,11 @@ class NativeLib:
         _gpu(turns, "turns", _I64)
         _check(positions.numel() == t, "positions must have T entries")
         _check(turns.numel() == rotary_dim // 2, "turns must have rotary_dim / 2 entries")
-        _same_device(device, k, positions, turns, q_out, k_out)
-        if t == 0:
-            return
-
-        def row(x, name):  # heads and dims dense, any token stride
-            s, heads = x.stride(), x.shape[1]
-            if heads and (s[2] != 1 and d > 1 or s[1] != d and heads > 1):
+        _same_device(q.get_device(), k, positions, turns, q_out, k_out)
+        for name, x in (("q", q), ("k", k), ("q_out", q_out), ("k_out", k_out)):
+            s, heads = x.stride(), x.shape[1]  # heads and dims dense, any token stride
+            if t and heads and (s[2] != 1 and d > 1 or s[1] != d and heads > 1):
                 raise RuntimeError(f"{name}'s heads and dims must be contiguous")
-            return heads * d if t == 1 else s[0]
-
-        self._launch(device, "sid_rope_rotate", q.data_ptr(), row(q, "q"), k.data_ptr(), row(k, "k"),
-                     positions.data_ptr(), turns.data_ptr(), float(gain), int(rotary_dim),
-                     int(interleaved), t, hq, k.shape[1], d, int(max_positions), q_out.data_ptr(),
-                     row(q_out, "q_out"), k_out.data_ptr(), row(k_out, "k_out"))
 
     def linear(self, x, w, bias, y, out_fp32: bool) -> None:
         m, k, n = self._linear_check(x, w)

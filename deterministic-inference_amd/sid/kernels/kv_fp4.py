@@ -54,7 +54,7 @@ def gather_cache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: to
         raise RuntimeError("k_cache must be [S, HKV, D / 2]")
     n, hkv = slots.numel(), shape[1]
     # one allocation for both (an eager call of a few rows is bound by the host)
-    k, v = torch.empty((2, n, hkv, HEAD_DIM), dtype=torch.bfloat16, device=slots.device).unbind(0)
+    k, v = slots.new_empty((2, n, hkv, HEAD_DIM), dtype=torch.bfloat16).unbind(0)
     flat = slots if slots.dim() == 1 else slots.reshape(-1)
     load_ext().gather_cache_fp4(k_cache, v_cache, kv_scales, flat, k, v)
     return k, v
