@@ -14,10 +14,10 @@
 //
 // Workgroups are of 4 waves and 32 query positions, two to a CU, as an independent workgroup fills the
 // waits of the other best: 8 waves of 64 positions, and 4 waves with two row sets that share each fragment,
-// took 3 to 40 % longer. Over 8 kv heads of 2 query heads: 1 x 8192 328 us
-// (838 TFLOP/s), 4 x 2048 103, 1 x 2048 32, 4 x 32 at 2048 keys 17. Of those 328 the vector ALU (softmax,
-// V to bf16) is busy for 55 % and the matrix units for 38 %, in each other's shadow; what bounds it is the
-// issue of both by two waves a SIMD.
+// took 3 to 40 % longer. Over 8 kv heads of 2 query heads, us by the card: 1 x 8192 306-336 (898-818
+// TFLOP/s; the 8-bit pool's kernel 349 beside 336), 4 x 2048 97-102, 1 x 2048 31-33, 4 x 32 at 2048 keys 17.
+// Of 4 x 2048 the vector ALU (softmax, V to bf16) issues for 58 % and the matrix units and the LDS (each wave reads all of V for its 16 rows) are
+// busy for 32 % and 46 %, in each other's shadow: what bounds it is each wave's own chain, two a SIMD.
 #include "extend_codes.h"
 #include "kv_fp4.h"
 
@@ -32,7 +32,7 @@ constexpr int NW = 4;  // waves of a workgroup
 constexpr int kSplit = 512;
 constexpr int kSplitTiles = kSplit / BN;
 // How far above its row's reference maximum a score may be, in log2 units.
-constexpr float kLazy = 24.0f;
+constexpr float kLazy = 24.0f, kLazySum = 16777216.0f;
 
 // ---- LDS ---------------------------------------------------------------------------------
 //
@@ -129,21 +129,18 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
   // for.)
   auto checked = [&](uint32_t slot) { return slot < max_slots ? slot : 0u; };
   const uint32_t row_bytes = static_cast<uint32_t>(num_kv_heads) * (D / 2);
+  // Of the row in a pool of codes; the scales' are an eighth of it.
+  auto offset = [&](uint32_t slot) { return static_cast<uint64_t>(slot) * row_bytes; };
   const uint8_t* ksrc = k_cache + h_kv * (D / 2) + 16 * (my_blk ^ swk(my_key));
   const uint8_t* vsrc = v_cache + h_kv * (D / 2) + 16 * my_blk;
-  const uint2* sbase = kv_scales + h_kv;
-  auto load_k = [&](uint32_t slot, int buf) {
-    dma16(ksrc + static_cast<uint64_t>(slot) * row_bytes, lds0 + 2 * buf * kKSub + 1024u * wave);
-  };
-  auto load_v = [&](uint32_t slot) {
-    return *reinterpret_cast<const u32x4_v*>(vsrc + static_cast<uint64_t>(slot) * row_bytes);
-  };
-  auto load_scales = [&](uint32_t slot) {
-    return sbase[static_cast<uint64_t>(slot) * static_cast<uint32_t>(num_kv_heads)];
-  };
+  const uint8_t* sbase = reinterpret_cast<const uint8_t*>(kv_scales + h_kv);
+  auto load_k = [&](uint64_t off, int buf) { dma16(ksrc + off, lds0 + 2 * buf * kKSub + 1024u * wave); };
+  auto load_v = [&](uint64_t off) { return *reinterpret_cast<const u32x4_v*>(vsrc + off); };
+  auto load_scales = [&](uint64_t off) { return *reinterpret_cast<const uint2*>(sbase + (off >> 3)); };
   // A NaN vector must reach the queries that see its key and no others, but a hidden key's value is
   // multiplied by p = 0, which leaves a NaN. So a key whose V is NaN gets a NaN scale for K (E8M0's
-  // 255: NaN scores, and a hidden key's scores are never used) and values 0.
+  // 255: NaN scores, and a hidden key's scores are never used) and values of next to nothing (scale
+  // byte 0).
   const uint32_t sdst = kScalesAt + (my_key >> 5) * kScaleSub +
                         2 * (16 * my_blk + 4 * ((my_key >> 3) & 3) + (my_key & 3)) + ((my_key >> 2) & 1);
   auto store_scales = [&](uint2 sc, int buf) {
@@ -153,12 +150,11 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
   const uint32_t vdst = lds0 + kVAt + 256 * my_key + 16 * ((4 * my_blk) ^ swv(my_key));
   auto store_v = [&](const u32x4_v& codes, uint32_t scales, int buf) {
     const uint32_t byte = (scales >> (8 * my_blk)) & 255u;
-    const bool nan = byte == kFp4ScaleNaN;
-    const float s = fp4_scale(nan ? 127 : byte);
+    const float s = fp4_scale(byte == kFp4ScaleNaN ? 0u : byte);
     typedef __attribute__((address_space(3))) u32x4_v* lds_w_t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 x = fp4_to_bf16x8(nan ? 0u : codes[i], s);
+      const uint4 x = fp4_to_bf16x8(codes[i], s);
       *(lds_w_t)((vdst ^ (16u * i)) + 2 * buf * kVSub) = u32x4_v{x.x, x.y, x.z, x.w};
     }
   };
@@ -166,15 +162,16 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
   // The first loads, in the order of their latencies: slots and q, then what the slots name; q is
   // split while those are under way. (t_begin is a split's first tile: even.)
   const uint32_t slot0 = load_slot(t_begin), slot1 = load_slot(t_begin + 1);
-  uint32_t k_slot = load_slot(t_begin + 2);
+  uint32_t next_slot = load_slot(t_begin + 2);
   const QRaw q_raw = load_q(q + prow * D, g);
   __builtin_amdgcn_sched_barrier(0);
-  const uint2 s0 = load_scales(checked(slot0)), s1 = load_scales(checked(slot1));
-  const u32x4_v raw0 = load_v(checked(slot0));
-  u32x4_v raw = load_v(checked(slot1));
+  const uint64_t off0 = offset(checked(slot0)), off1 = offset(checked(slot1));
+  const uint2 s0 = load_scales(off0), s1 = load_scales(off1);
+  const u32x4_v raw0 = load_v(off0);
+  u32x4_v raw = load_v(off1);
   __builtin_amdgcn_sched_barrier(0);
-  load_k(checked(slot0), 0);
-  load_k(checked(slot1), 1);
+  load_k(off0, 0);
+  load_k(off1, 1);
   __builtin_amdgcn_sched_barrier(0);
   const QRow qf = split_q(q_raw, row_ok);
   __builtin_amdgcn_sched_barrier(0);
@@ -301,11 +298,14 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
     pv(0, 1, p4[1 - h]);
     point();
     const float om = m, ol = l;
-    float tmax = NEG_BIG;
-    if constexpr (kFirst) {
+    auto row_max = [&] {
+      float tmax = NEG_BIG;
 #pragma unroll
       for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, seen(i));
-      m = pair32_max(pair16_max(tmax)) * sc2;
+      return pair32_max(pair16_max(tmax)) * sc2;
+    };
+    if constexpr (kFirst) {
+      m = row_max();
       l = 0.0f;
     }
     // (While a product runs, a wave can issue only what follows it in program order, and a second
@@ -333,7 +333,6 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
         if constexpr (kMask) p[i] = vis[2 * n + i] ? p[i] : 0.0f;
         l += p[i];
       }
-      if constexpr (!kFirst) tmax = fmaxf(fmaxf(tmax, seen(2 * n)), seen(2 * n + 1));
       reinterpret_cast<uint32_t*>(&p4[h])[n] = pack_bf16x2(p[0], p[1]);
       point();
       if constexpr (n < 3) pv(n + 1, 1, p4[1 - h]);
@@ -348,11 +347,13 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
       if (!FANOUT && t > t_begin) fold_split(om, ol);
     } else {
       // A row's reference maximum is that of its split's first sub-tile as long as no score is kLazy above
-      // it: P's precision does not depend on its size. Each lane looks at its own scores; only where one
-      // is too high (hardly ever) are the rows' maxima taken, their state brought to them and P worked out
-      // again. That is looked at here, after the products, as nothing before has to wait for it.
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(tmax * sc2 > m + kLazy) != 0, false)) {
-        const float mc = pair32_max(pair16_max(tmax)) * sc2;
+      // it: P's precision does not depend on its size. A score that is makes its lane's sum grow by 2^kLazy
+      // or more; only where one does (hardly ever) are the rows' maxima taken, their state brought to
+      // them and P worked out again. That is looked at here, after the products, as nothing before has to
+      // wait for it. (By the sums, not by the scores' maximum: 5 operations fewer of some 50, 2 % of
+      // 1 x 8192.)
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(l - ol > kLazySum) != 0, false)) {
+        const float mc = row_max();
         const float m_used = mc > m + kLazy ? mc : m;
         const float rescale = exp2_fast(m - m_used);  // (x * 1 == x for the rows that stay)
         m = m_used;
@@ -386,24 +387,23 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
   auto step = [&](auto mask, auto first, int t, auto buf) {
     constexpr bool kMask = decltype(mask)::value;
     // Every wave is done with the tiles that are written over next, and K has landed (it had a whole
-    // tile's time). V and its scale are still under way, the last two loads that went out.
+    // tile's time). V is still under way, the last load that went out.
     point();
-    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(1) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     point();
-    const uint32_t v_slot = load_slot(t + 2), slot = checked(k_slot);
-    const uint2 k_scales = load_scales(slot);
-    k_slot = load_slot(t + 3);
+    const uint64_t off = offset(checked(next_slot));  // of tile t + 2
+    const uint2 scales = load_scales(off);
+    next_slot = load_slot(t + 3);
     point();
-    load_k(slot, buf);  // last: a wait for an earlier load would include the DMA
+    load_k(off, buf);  // last: a wait for an earlier load would include the DMA
     point();
     auto stage = [&] {  // at the step's end
       store_v(raw, v_scales, other(buf));
       point();
-      const uint32_t slot = checked(v_slot);
-      raw = load_v(slot);
-      v_scales = load_scales(slot).y;
+      raw = load_v(off);
+      v_scales = scales.y;
       point();
-      store_scales(k_scales, buf);
+      store_scales(scales, buf);
       point();
     };
     if (!kMask || t <= w_tiles) {  // (at w_tiles the sub-tile before is still to be added)
