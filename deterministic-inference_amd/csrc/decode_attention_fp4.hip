@@ -246,7 +246,7 @@ __device__ __forceinline__ void stage1_item(
     wave_sync();
   };
   // (a wave whose first token is past the segment's end adds nothing)
-  for (; t0 + IT < end; t0 += IT) iterate(std::true_type{});
+  for (; t0 < end - IT; t0 += IT) iterate(std::true_type{});
   if (t0 < end) iterate(std::false_type{});
 
   l = pair_sum(l);

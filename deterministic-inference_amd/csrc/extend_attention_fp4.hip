@@ -514,6 +514,8 @@ extern "C" int sid_extend_attention_fp4_fwd(
                                    workspace, workspace_bytes);
   if (p.rc != SID_OK || p.empty) return p.rc;
   SID_REQUIRE(kv_scales != nullptr, "%s: null pointer", name);
+  SID_REQUIRE(sm_scale >= 0.0f && sm_scale < INFINITY,
+              "%s: sm_scale must be finite and not negative (the scores' maxima are taken before it)", name);
   auto misaligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) != 0; };
   SID_REQUIRE(!misaligned(q) && !misaligned(k_cache) && !misaligned(v_cache) &&
                   !misaligned(kv_scales) && !misaligned(o) && !misaligned(workspace),

@@ -54,7 +54,9 @@ struct Layout {
   int64_t total;
 };
 
-Layout plan(const sid_qwen3_model* m, const sid_extend_batch* b, void* ws) {
+// fp4: 4-bit pools, whose attention splits other batches than bf16 ones (8-bit ones ask for no more
+// than those).
+Layout plan(const sid_qwen3_model* m, const sid_extend_batch* b, void* ws, bool fp4) {
   const int64_t t = b->num_tokens;
   const int64_t h = m->hidden;
   const int64_t wq = static_cast<int64_t>(m->num_q_heads + 2 * m->num_kv_heads) * m->head_dim;
@@ -80,13 +82,10 @@ Layout plan(const sid_qwen3_model* m, const sid_extend_batch* b, void* ws) {
   l.attn = c.take(t * ao * 2);
   l.act = c.take(t * inter * 2);
   const int64_t kvmax = b->max_kv_len > 0 ? b->max_kv_len : b->num_kv_indices;
-  // (the pool's type is not known here: what any asks for. 4-bit pools split the keys of some batches
-  // that bf16 ones walk; 8-bit ones never ask for more than bf16 ones.)
-  const int longest = std::max(b->max_extend_len, 1), keys = static_cast<int>(kvmax);
-  l.ext_ws_bytes = std::max(
-      sid_extend_attention_workspace_bytes(b->batch, t, m->num_q_heads, m->num_kv_heads, longest, keys),
-      sid_extend_attention_fp4_workspace_bytes(b->batch, t, m->num_q_heads, m->num_kv_heads, longest,
-                                               keys));
+  l.ext_ws_bytes = (fp4 ? sid_extend_attention_fp4_workspace_bytes
+                        : sid_extend_attention_workspace_bytes)(
+      b->batch, t, m->num_q_heads, m->num_kv_heads, std::max(b->max_extend_len, 1),
+      static_cast<int>(kvmax));
   l.ext_ws = l.ext_ws_bytes > 0 ? c.take(l.ext_ws_bytes) : nullptr;
   l.rows = b->sample_indices ? c.take(r * h * 2) : nullptr;
   l.argmax_ws_bytes = b->temperatures ? sid_linear_sample_workspace_bytes(r)
@@ -149,7 +148,13 @@ using namespace sid;
 extern "C" int64_t sid_qwen3_extend_workspace_bytes(const sid_qwen3_model* m,
                                                     const sid_extend_batch* b) {
   if (m == nullptr || b == nullptr || b->num_tokens <= 0) return 0;
-  return plan(m, b, nullptr).total;
+  return plan(m, b, nullptr, false).total;
+}
+
+extern "C" int64_t sid_qwen3_extend_fp4_workspace_bytes(const sid_qwen3_model* m,
+                                                        const sid_extend_batch* b) {
+  if (m == nullptr || b == nullptr || b->num_tokens <= 0) return 0;
+  return plan(m, b, nullptr, true).total;
 }
 
 // kv_scales NULL: the layers' pools are bf16; else of 8-bit (fp4: 4-bit) codes, and these their scales'
@@ -171,7 +176,7 @@ static int extend_forward(const sid_qwen3_model* m, const sid_extend_batch* b,
   const int64_t t = b->num_tokens;
   const int64_t r = b->sample_indices ? b->num_samples : t;
   SID_REQUIRE(r > 0, "qwen3_extend_forward: no sampled rows");
-  const Layout l = plan(m, b, workspace);
+  const Layout l = plan(m, b, workspace, fp4);
   SID_REQUIRE(workspace && workspace_bytes >= l.total,
               "qwen3_extend_forward: workspace %lld bytes, need %lld",
               (long long)workspace_bytes, (long long)l.total);

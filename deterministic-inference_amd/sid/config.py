@@ -38,7 +38,7 @@ class ModelConfig:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 1e6
     max_position_embeddings: int = 40960
-    # Scaled rotary positions, as a checkpoint's config.json gives them (sid.kernels.rope)
+    # Scaled rotary positions (sid.kernels.rope)
     rope_scaling: Optional[dict] = None
     tie_word_embeddings: bool = True
     eos_token_ids: tuple = (151645, 151643)
@@ -76,6 +76,11 @@ class EngineConfig:
     # two; 1 = the reference's token-granular pool). Slot numbering, and so every kernel's
     # view of the pool, is the same for any page size.
     kv_page_size: int = 16
+    # Rotary positions scaled for contexts beyond the trained ones: a dict as checkpoints give it
+    # (rope_type "linear", "ntk" or "yarn", factor, ...; sid.kernels.rope), or "checkpoint" for the
+    # one in the checkpoint's own config.json. None: unscaled, whatever that file says, as the
+    # reference (sid/model/loader.py:30-50 does not read it).
+    rope_scaling: Optional[dict | str] = None
     max_reqs: int = 256
     max_seq_len: int = 32768
     max_prompt_len: int = 16384
@@ -132,6 +137,8 @@ class EngineConfig:
         if self.kv_cache_dtype not in KV_CACHE_DTYPES:
             raise ValueError(f"unknown kv_cache_dtype {self.kv_cache_dtype!r}: use one of "
                              f"{', '.join(KV_CACHE_DTYPES)}")
+        if isinstance(self.rope_scaling, str) and self.rope_scaling != "checkpoint":
+            raise ValueError(f"rope_scaling must be a dict or 'checkpoint', got {self.rope_scaling!r}")
         # Prefill batches (at most max_decode_batch sequences) and verify passes (G x W
         # rows) draw their untruncated rows inside the lm_head with one fixed grouping,
         # which takes up to MAX_SAMPLED_ROWS rows per pass; larger passes would switch those

@@ -42,7 +42,7 @@ class ModelRunner:
         self.device = device
         self.mcfg: ModelConfig
         self.mcfg, self.model_dir = build_model_config(cfg.model_path, cfg.num_layers,
-                                                       cfg.vocab_size)
+                                                       cfg.vocab_size, cfg.rope_scaling)
         logger.info("model %s: %d layers, %d/%d heads, head_dim %d", cfg.model_path,
                     self.mcfg.num_layers, self.mcfg.num_q_heads, self.mcfg.num_kv_heads,
                     self.mcfg.head_dim)

@@ -88,7 +88,8 @@ EXPORTED = ("sid_last_error", "sid_abi_version", "sid_abi_revision",
             "sid_linear_argmax_workspace_bytes", "sid_sample_workspace_bytes",
             "sid_qwen3_extend_workspace_bytes", "sid_qwen3_extend_forward",
             "sid_qwen3_extend_forward_fp8", "sid_extend_attention_fp8_workspace_bytes",
-            "sid_qwen3_extend_forward_fp4", "sid_extend_attention_fp4_workspace_bytes",
+            "sid_qwen3_extend_forward_fp4", "sid_qwen3_extend_fp4_workspace_bytes",
+            "sid_extend_attention_fp4_workspace_bytes",
             "sid_flash_decode_noalloc_scratch_bytes", "sid_linear_sample_workspace_bytes",
             "sid_extend_attention_query_rows", "sid_linear_tile", *_SIGNATURES)
 ABI_VERSION = 22

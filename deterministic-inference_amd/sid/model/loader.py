@@ -60,15 +60,6 @@ def _read_json(path: Path) -> dict:
     return json.loads(path.read_text()) if path.exists() else {}
 
 
-def _rope_scaling(hf: dict) -> dict | None:
-    """config.json's rope_scaling, checked: positions that the model was not made for are an error."""
-    scaling = hf.get("rope_scaling")
-    if not scaling or rope_type(scaling) == "default":
-        return None
-    scaled_frequencies(hf["head_dim"], hf["rope_theta"], scaling)
-    return dict(scaling)
-
-
 def load_model_config(model_dir: Path, model_path: str) -> ModelConfig:
     """ModelConfig of a local Qwen3 checkpoint directory (config.json, and the stop ids of
     generation_config.json when present, as sid/model/loader.py:30-50 reads them)."""
@@ -82,7 +73,6 @@ def load_model_config(model_dir: Path, model_path: str) -> ModelConfig:
         "eos_token_id", hf.get("eos_token_id", 151645))
     return ModelConfig(model_path=model_path,
                        tie_word_embeddings=bool(hf.get("tie_word_embeddings", False)),
-                       rope_scaling=_rope_scaling(hf),
                        eos_token_ids=tuple(stop) if isinstance(stop, list) else (stop,),
                        **{field: hf[key] for field, key in _CONFIG_FIELDS})
 
@@ -143,8 +133,22 @@ def load_weights(model_dir: Path, mcfg: ModelConfig, device,
     return w
 
 
-def build_model_config(model_path: str, num_layers=None, vocab_size=None) -> tuple[ModelConfig, Path | None]:
-    """-> (ModelConfig, model_dir or None for a random-init model)."""
+def scale_positions(mcfg: ModelConfig, scaling: dict) -> None:
+    """Scaled rotary positions (sid.kernels.rope) for a model, and the positions that they reach:
+    factor times the trained ones, if config.json does not say more."""
+    if rope_type(scaling) == "default":
+        return
+    scaled_frequencies(mcfg.head_dim, mcfg.rope_theta, scaling)  # (raises where it is incomplete)
+    trained = scaling.get("original_max_position_embeddings", mcfg.max_position_embeddings)
+    mcfg.max_position_embeddings = max(mcfg.max_position_embeddings,
+                                       int(trained * float(scaling["factor"])))
+    mcfg.rope_scaling = dict(scaling)
+
+
+def build_model_config(model_path: str, num_layers=None, vocab_size=None,
+                       rope_scaling: dict | str | None = None) -> tuple[ModelConfig, Path | None]:
+    """-> (ModelConfig, model_dir or None for a random-init model). rope_scaling:
+    EngineConfig.rope_scaling."""
     if model_path.startswith("random:"):
         mcfg = ModelConfig(model_path=model_path)
         model_dir = None
@@ -155,6 +159,10 @@ def build_model_config(model_path: str, num_layers=None, vocab_size=None) -> tup
                 f"model directory {model_path!r} not found (no network downloads; use "
                 "'random:qwen3-0.6b' for a random-init model)")
         mcfg = load_model_config(model_dir, model_path)
+    if rope_scaling == "checkpoint":
+        rope_scaling = _read_json(model_dir / "config.json").get("rope_scaling") if model_dir else None
+    if rope_scaling:
+        scale_positions(mcfg, rope_scaling)
     if num_layers is not None:
         mcfg.num_layers = num_layers
     if vocab_size is not None:

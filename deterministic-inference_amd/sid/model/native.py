@@ -56,6 +56,8 @@ def _bind(lib) -> None:
     lib.sid_qwen3_extend_forward_fp8.restype = _i32
     lib.sid_qwen3_extend_forward_fp8.argtypes = [ctypes.POINTER(Model), ctypes.POINTER(Batch),
                                                  ctypes.POINTER(_vp), _vp, _i64, _vp, _vp, _vp]
+    lib.sid_qwen3_extend_fp4_workspace_bytes.restype = _i64
+    lib.sid_qwen3_extend_fp4_workspace_bytes.argtypes = lib.sid_qwen3_extend_workspace_bytes.argtypes
     lib.sid_qwen3_extend_forward_fp4.restype = _i32
     lib.sid_qwen3_extend_forward_fp4.argtypes = lib.sid_qwen3_extend_forward_fp8.argtypes
     lib._sid_native_forward_bound = True
@@ -87,9 +89,11 @@ class NativeQwen3:
         scales = [layer_scales(kv_cache, i) for i in range(cfg.num_layers)]
         self.kv_scales = None if scales[0] is None else (_vp * cfg.num_layers)(
             *(s.data_ptr() for s in scales))
-        self.code_forward = (self.ext.lib.sid_qwen3_extend_forward_fp4
-                             if kv_cache.layer(0)[0].dtype == FP4
+        fp4 = kv_cache.layer(0)[0].dtype == FP4
+        self.code_forward = (self.ext.lib.sid_qwen3_extend_forward_fp4 if fp4
                              else self.ext.lib.sid_qwen3_extend_forward_fp8)
+        self.workspace_bytes = (self.ext.lib.sid_qwen3_extend_fp4_workspace_bytes if fp4
+                                else self.ext.lib.sid_qwen3_extend_workspace_bytes)
         kp0, _ = kv_cache.layer(0)
         self.model = Model(cfg.num_layers, cfg.hidden_size, cfg.num_q_heads, cfg.num_kv_heads,
                            cfg.head_dim, cfg.intermediate_size, cfg.vocab_size,
@@ -118,7 +122,7 @@ class NativeQwen3:
                   fb.sample_indices.data_ptr() if fb.sample_indices is not None else None, r,
                   *samp)
         lib = self.ext.lib
-        need = int(lib.sid_qwen3_extend_workspace_bytes(ctypes.byref(self.model), ctypes.byref(b)))
+        need = int(self.workspace_bytes(ctypes.byref(self.model), ctypes.byref(b)))
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
         logits: Optional[torch.Tensor] = None
         tokens: Optional[torch.Tensor] = None

@@ -731,7 +731,11 @@ int sid_extend_attention_fp4_fwd(const void* q, const void* k_cache, const void*
                                  int max_kv_len, float sm_scale, void* workspace,
                                  int64_t workspace_bytes, void* o, void* stream);
 
-/* sid_qwen3_extend_forward_fp8 with 4-bit pools. Same workspace. */
+/*
+ * sid_qwen3_extend_forward_fp8 with 4-bit pools, and a workspace of
+ * sid_qwen3_extend_fp4_workspace_bytes(m, b) bytes.
+ */
+int64_t sid_qwen3_extend_fp4_workspace_bytes(const sid_qwen3_model* m, const sid_extend_batch* b);
 int sid_qwen3_extend_forward_fp4(const sid_qwen3_model* m, const sid_extend_batch* b,
                                  void* const* kv_scales, void* workspace,
                                  int64_t workspace_bytes, float* logits, int64_t* tokens,

@@ -749,3 +749,33 @@ def test_refusals():
     q4 = torch.zeros(2, 8, D, dtype=torch.bfloat16, device="cuda")
     refused("workspace|q heads", attn.forward, q4, kc, vc, ptr, idx, seq, 2, SCALE, False, kv_scales=sc)
     refused("q heads", extend_attention_fwd, q4, kc, vc, qo, ptr, idx, 1, SCALE, kv_scales=sc)
+
+
+def test_chunk_scale_that_is_refused():
+    q, pool, qo, ptr, idx, at, qoh = _chunk_batch([(10, 5)], seed=1)
+    from sid.kernels.extend_attention import extend_attention_fwd
+    for bad in (-0.1, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="sm_scale"):
+            extend_attention_fwd(q, *pool[:2], qo, ptr, idx, 5, bad, max_kv_len=15, kv_scales=pool[2])
+
+
+def test_decode_two_workers_a_cu_keep_bits():
+    """More segments than two a CU: the placement deals them to workers."""
+    from sid.kernels.decode_attention import DecodeAttention, placement, stage1_workers_fp4
+    lens = [9000 - 150 * i for i in range(40)]
+    pool, ptr, idx, at = _batch(lens, seed=23, page=16)
+    q = _queries(len(lens), 23)
+    attn = DecodeAttention(len(lens), HQ, HKV, D, 32, 256, max(lens), "cuda")
+    order, workers = placement(lens, len(lens), 1, 0, 256, 36, 3, attn.cu_count(),
+                               workers_of=stage1_workers_fp4, kv_fp4=True)
+    assert workers == 2 * attn.cu_count()
+    plan = dict(geometry=(1, 256, 36), variant=3, wg_order=torch.from_numpy(order).cuda(),
+                workers=workers)
+    run = lambda **kw: attn.forward(q, *pool[:2], ptr, idx, _i32(lens), max(lens), SCALE, False,  # noqa: E731
+                                    kv_scales=pool[2], **{**plan, **kw})
+    attn.part_o.fill_(float("nan"))
+    attn.part_lse.fill_(float("nan"))
+    o = run()
+    assert torch.equal(o, run(wg_order=None, workers=0))
+    for i in (0, 17, 39):
+        _check_decode(o[i:i + 1], q[i:i + 1], pool, [at[i]])

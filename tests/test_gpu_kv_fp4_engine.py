@@ -183,6 +183,12 @@ def test_scaled_positions_reach_the_models_pool():
     # half a bf16 step of each stored value, the table's fp32 angles' sines
     assert (np.abs(yarn - want) <= 2.0 ** -8 * (mag + np.abs(want)) + 2.0 ** -20 * mag).all()
     assert np.abs(yarn - plain).max() > 0.1
+    # the engine's own setting is that model
+    runner = ModelRunner(_cfg(kv_cache_dtype="bfloat16", use_graphs=False, rope_scaling=YARN), "cuda")
+    assert runner.mcfg.rope_scaling == YARN
+    _, _, reqs = _run_plain(runner, prompt)
+    assert np.array_equal(runner.kv_cache.read(0, reqs[0].req_row, 0, len(prompt[0]))[0]
+                          .double().cpu().numpy(), yarn)
 
 
 def _run_plain(runner, prompts):

@@ -63,25 +63,62 @@ def _write_config(tmp_path, scaling):
     (tmp_path / "config.json").write_text(json.dumps(hf))
 
 
-@pytest.mark.parametrize("scaling,want", [
-    (None, None), ({}, None), ({"rope_type": "default"}, None),
-    ({"type": "linear", "factor": 2.0}, {"type": "linear", "factor": 2.0}),
-    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768},) * 2,
+YARN = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+
+
+@pytest.mark.parametrize("given", ["checkpoint", "dict"])
+@pytest.mark.parametrize("scaling,want,positions", [
+    (None, None, 40960), ({}, None, 40960), ({"rope_type": "default"}, None, 40960),
+    ({"type": "linear", "factor": 2.0}, {"type": "linear", "factor": 2.0}, 81920),
+    (YARN, YARN, 131072), (dict(YARN, factor=1.0), dict(YARN, factor=1.0), 40960),
 ], ids=str)
-def test_checkpoint_scaling(tmp_path, scaling, want):
-    from sid.model.loader import load_model_config
+def test_scaled_positions_of_a_model(tmp_path, given, scaling, want, positions):
+    from sid.model.loader import build_model_config
     _write_config(tmp_path, scaling)
-    assert load_model_config(tmp_path, str(tmp_path)).rope_scaling == want
+    got, _ = build_model_config(str(tmp_path), rope_scaling="checkpoint" if given == "checkpoint"
+                                else scaling)
+    assert got.rope_scaling == want and got.max_position_embeddings == positions
+    plain, _ = build_model_config(str(tmp_path))
+    assert plain.rope_scaling is None and plain.max_position_embeddings == 40960
+    random, _ = build_model_config("random:qwen3-0.6b", rope_scaling=scaling)
+    assert random.rope_scaling == want and random.max_position_embeddings == positions
 
 
 @pytest.mark.parametrize("scaling", [{"rope_type": "other", "factor": 2.0}, {"rope_type": "linear"},
                                      {"rope_type": "yarn", "factor": 4.0},
                                      {"type": "linear", "factor": 0.5}], ids=str)
-def test_checkpoint_scaling_that_is_refused(tmp_path, scaling):
-    from sid.model.loader import load_model_config
+def test_scaled_positions_that_are_refused(tmp_path, scaling):
+    from sid.config import EngineConfig
+    from sid.model.loader import build_model_config
     _write_config(tmp_path, scaling)
-    with pytest.raises(ValueError):
-        load_model_config(tmp_path, str(tmp_path))
+    for given in ("checkpoint", scaling):
+        with pytest.raises(ValueError):
+            build_model_config(str(tmp_path), rope_scaling=given)
+    build_model_config(str(tmp_path))  # not asked for: not read
+    with pytest.raises(ValueError, match="checkpoint"):
+        EngineConfig(rope_scaling="yarn")
+
+
+def test_executor_workspace_is_its_pools():
+    """The 4-bit pool's attention splits the keys of a window that the bf16 pool's walks, or the
+    other way round: the workspace differs by what each asks for."""
+    import ctypes
+
+    from sid.kernels.jit import load_ext
+    from sid.model.native import Batch, Model, _bind
+    ext = load_ext()
+    _bind(ext.lib)
+    m, b = Model(), Batch()
+    m.num_layers, m.hidden, m.num_q_heads, m.num_kv_heads, m.head_dim = 1, 1024, 16, 8, 128
+    m.intermediate, m.vocab, m.split_k_max_tokens = 2048, 1000, 64
+    args = (ctypes.byref(m), ctypes.byref(b))
+    for batch, e, keys in ((1, 32, 2048), (16, 32, 2048), (1, 512, 512), (4, 256, 2048), (1, 64, 100000)):
+        b.num_tokens, b.batch, b.max_extend_len, b.max_kv_len = batch * e, batch, e, keys
+        plain = ext.lib.sid_qwen3_extend_workspace_bytes(*args)
+        four = ext.lib.sid_qwen3_extend_fp4_workspace_bytes(*args)
+        own = [ext.extend_attention_workspace_bytes(batch, batch * e, 16, 8, e, keys, fp4=x)
+               for x in (False, True)]
+        assert abs((plain - own[0]) - (four - own[1])) <= 512  # (each piece starts on 256 bytes)
 
 
 def test_executor_refuses_missing_scales():
