@@ -9,15 +9,18 @@
 // their Taylor sums (terms to x^9 and x^8: the first left out is 2e-9 and 2.5e-8). q and k are
 // rounded once, to bf16.
 //
-// Bound: q and k read and written. The angles are worked out once a workgroup, each of its tokens'
-// rotary / 2 for all heads, into the LDS, while the first elements are on their way.
+// Bound: q and k read and written. A workgroup takes one token and works its rotary / 2 angles out once for
+// all heads, into the LDS. (Two or four tokens a workgroup: 64 tokens 2.7 us with one, 3.2 and 3.7; 8192 of
+// 24 heads of 128 16.5, 16.9 and 17.3; with half of a head turned 18.1, 17.5 and 18.1, and 32768 of those 85, 78
+// and 78, the one case that gains.) 8192 tokens in 16.5 us move 100 MB at 6.1 TB/s, half of it out of the
+// last level cache.
 #include "rowmath.h"
 
 namespace sid {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxPairs = 512;  // of the tokens of a workgroup: 4 KiB of the LDS
+constexpr int kMaxPairs = 512;  // of a head: 4 KiB of the LDS
 
 // (sin, cos) of a 64-bit fraction of a turn.
 __device__ __forceinline__ float2 sincos_turns(uint64_t turns) {
@@ -42,7 +45,7 @@ struct RopeArgs {
   int64_t ldq, ldk, ldqo, ldko;  // elements between tokens
   const int64_t* positions;
   const uint64_t* turns;
-  int64_t tokens, max_positions;
+  int64_t max_positions;
   float gain;
   int rotary, head_dim, q_heads, heads;  // heads: of q and k
 };
@@ -59,34 +62,32 @@ __device__ __forceinline__ void head_at(const RopeArgs& a, int64_t t, int h, con
   }
 }
 
-// A workgroup takes `per` consecutive tokens. A unit is 8 pairs of halves (two 16-byte words), 4
-// pairs of neighbours or 8 elements behind the rotated ones (one word); with VEC false, one pair or
-// one element. COPY: the elements behind the rotated ones are written too (not where a call rotates
-// in place). A token whose position is outside [0, max_positions) is copied.
+// A workgroup takes a token. A unit is 8 pairs of halves (two 16-byte words), 4 pairs of neighbours or 8
+// elements behind the rotated ones (one word); with VEC false, for heads that do not start on words, one
+// pair or one element (8192 tokens 38 us instead of 17). `copy`: the elements behind the rotated ones are
+// written too (not where a call rotates in place). A token whose position is outside [0, max_positions) is
+// copied.
 template <bool INTER, bool VEC>
-__global__ void __launch_bounds__(kThreads) rope_angles_kernel(RopeArgs a, int per, int copy) {
+__global__ void __launch_bounds__(kThreads) rope_angles_kernel(RopeArgs a, int copy) {
   __shared__ float2 angle[kMaxPairs];  // (cos, sin) times the gain
   constexpr int W = VEC ? 8 : 1;       // elements of a word
   const int pairs = a.rotary / 2;
   const int rot_units = VEC ? (INTER ? a.rotary / 8 : pairs / 8) : pairs;
   const int units = rot_units + (copy ? (a.head_dim - a.rotary) / W : 0);  // of a head
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * per;
-  const int tokens = static_cast<int>(min(static_cast<int64_t>(per), a.tokens - t0));
-  for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
-    const int64_t pos = a.positions[t0 + i / pairs];
-    const float2 sc = sincos_turns(static_cast<uint64_t>(pos) * a.turns[i % pairs]);
-    const bool in = pos >= 0 && pos < a.max_positions;
+  const int64_t t = blockIdx.x;
+  const int64_t pos = a.positions[t];
+  const bool in = pos >= 0 && pos < a.max_positions;
+  for (int i = threadIdx.x; i < pairs; i += kThreads) {
+    const float2 sc = sincos_turns(static_cast<uint64_t>(pos) * a.turns[i]);
     angle[i] = in ? make_float2(sc.y * a.gain, sc.x * a.gain) : make_float2(1.0f, 0.0f);
   }
   __syncthreads();
-  const int total = tokens * a.heads * units;
+  const int total = a.heads * units;
   for (int u = threadIdx.x; u < total; u += kThreads) {
     const int head = u / units, i = u % units;
-    const int tok = head / a.heads;
     const bf16_t* src;
     bf16_t* dst;
-    head_at(a, t0 + tok, head % a.heads, src, dst);
-    const float2* ang = angle + tok * pairs;
+    head_at(a, t, head, src, dst);
     if (i >= rot_units) {
       const int at = a.rotary + (i - rot_units) * W;
       if constexpr (VEC) *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(src + at);
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kThreads) rope_angles_kernel(RopeArgs a, int p
     } else if constexpr (!VEC) {
       const int x = INTER ? 2 * i : i, y = INTER ? 2 * i + 1 : pairs + i;
       float o1, o2;
-      rope_pair(bf16_to_f32(src[x]), bf16_to_f32(src[y]), ang[i].x, ang[i].y, o1, o2);
+      rope_pair(bf16_to_f32(src[x]), bf16_to_f32(src[y]), angle[i].x, angle[i].y, o1, o2);
       dst[x] = f32_to_bf16(o1);
       dst[y] = f32_to_bf16(o2);
     } else if constexpr (INTER) {
@@ -102,14 +103,14 @@ __global__ void __launch_bounds__(kThreads) rope_angles_kernel(RopeArgs a, int p
       load8(*reinterpret_cast<const uint4*>(src + 8 * i), x);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        rope_pair(x[2 * e], x[2 * e + 1], ang[4 * i + e].x, ang[4 * i + e].y, o[2 * e], o[2 * e + 1]);
+        rope_pair(x[2 * e], x[2 * e + 1], angle[4 * i + e].x, angle[4 * i + e].y, o[2 * e], o[2 * e + 1]);
       *reinterpret_cast<uint4*>(dst + 8 * i) = store8(o);
     } else {
       float x[8], y[8], o1[8], o2[8];
       load8(*reinterpret_cast<const uint4*>(src + 8 * i), x);
       load8(*reinterpret_cast<const uint4*>(src + pairs + 8 * i), y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rope_pair(x[e], y[e], ang[8 * i + e].x, ang[8 * i + e].y, o1[e], o2[e]);
+      for (int e = 0; e < 8; ++e) rope_pair(x[e], y[e], angle[8 * i + e].x, angle[8 * i + e].y, o1[e], o2[e]);
       *reinterpret_cast<uint4*>(dst + 8 * i) = store8(o1);
       *reinterpret_cast<uint4*>(dst + pairs + 8 * i) = store8(o2);
     }
@@ -146,7 +147,7 @@ extern "C" int sid_rope_rotate(const void* q, int64_t ldq, const void* k, int64_
               "%s: a row stride is less than a row", name);
   SID_REQUIRE((q != q_out || ldq == ldq_out) && (k != k_out || ldk == ldk_out),
               "%s: in place, the row strides must be the same", name);
-  SID_REQUIRE(num_tokens < (1ll << 31), "%s: too many tokens", name);
+  SID_REQUIRE(num_tokens < (1ll << 24), "%s: too many tokens", name);  // (2^32 threads)
   const bool in_place = (num_q_heads == 0 || q == q_out) && (num_kv_heads == 0 || k == k_out);
   // Words of 16 bytes where every piece of a head starts on one.
   auto word = [](const void* p, int64_t ld, int heads) {
@@ -155,14 +156,12 @@ extern "C" int sid_rope_rotate(const void* q, int64_t ldq, const void* k, int64_
   const bool vec = head_dim % 8 == 0 && rotary_dim % (interleaved ? 8 : 16) == 0 &&
                    word(q, ldq, num_q_heads) && word(q_out, ldq_out, num_q_heads) &&
                    word(k, ldk, num_kv_heads) && word(k_out, ldk_out, num_kv_heads);
-  const int most = kMaxPairs / (rotary_dim / 2);
-  const int per = num_tokens < 1024 ? 1 : min(4, most);
   const RopeArgs a{(const bf16_t*)q, (const bf16_t*)k, (bf16_t*)q_out, (bf16_t*)k_out, ldq, ldk,
-                   ldq_out, ldk_out, positions, turns, num_tokens, max_positions, gain, rotary_dim,
+                   ldq_out, ldk_out, positions, turns, max_positions, gain, rotary_dim,
                    head_dim, num_q_heads, num_q_heads + num_kv_heads};
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)((num_tokens + per - 1) / per)), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), a, per, in_place ? 0 : 1);
+    hipLaunchKernelGGL(kern, dim3((unsigned)num_tokens), dim3(kThreads), 0,
+                       static_cast<hipStream_t>(stream), a, in_place ? 0 : 1);
     return check_launch(name);
   };
   if (vec) return interleaved ? go(rope_angles_kernel<true, true>) : go(rope_angles_kernel<false, true>);

@@ -748,7 +748,8 @@ int sid_qwen3_extend_forward_fp4(const sid_qwen3_model* m, const sid_extend_batc
  * (i, i + rotary_dim / 2); the others are copied. Pair i of token t turns by positions[t] times
  * turns[i] 2^-64 of a whole turn (uint64 [rotary_dim / 2]), its sine and cosine multiplied with
  * `gain`. A token whose position is outside [0, max_positions) is copied. q_out may be q (with the
- * same stride) and k_out k; no other output may overlap an input. head_dim at most 1024. No
+ * same stride) and k_out k; no other output may overlap an input. head_dim at most 1024, less than
+ * 2^24 tokens. No
  * counterpart in the reference, whose sid/kernels/rope.py:50-61 rotates halves of whole heads.
  */
 int sid_rope_rotate(const void* q, int64_t ldq, const void* k, int64_t ldk,
