@@ -14,8 +14,8 @@
 //
 // Workgroups are of 4 waves and 32 query positions, two to a CU, as an independent workgroup fills the
 // waits of the other best: 8 waves of 64 positions, and 4 waves with two row sets that share each fragment,
-// took 3 to 40 % longer. Over 8 kv heads of 2 query heads, us by the card: 1 x 8192 306-336 (898-818
-// TFLOP/s; the 8-bit pool's kernel 349 beside 336), 4 x 2048 97-102, 1 x 2048 31-33, 4 x 32 at 2048 keys 17.
+// took 3 to 40 % longer. Over 8 kv heads of 2 query heads, us by the card: 1 x 8192 296-330 (930-833
+// TFLOP/s; the 8-bit pool's kernel 349 beside 336), 4 x 2048 93-101, 1 x 2048 30-33, 4 x 32 at 2048 keys 17.
 // Of 4 x 2048 the vector ALU (softmax, V to bf16) issues for 58 % and the matrix units and the LDS (each wave reads all of V for its 16 rows) are
 // busy for 32 % and 46 %, in each other's shadow: what bounds it is each wave's own chain, two a SIMD.
 #include "extend_codes.h"
@@ -249,11 +249,12 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
     else
       to[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf.hi, zero4, 4, 0, j, ks, 0, qf.scale);
   };
-  auto pv = [&](int n, int i, const uint4& p) {
+  // FRESH: acc holds nothing of this split yet.
+  auto pv = [&](auto fresh, int n, int i, const uint4& p) {
     f32x4_v& a = acc[2 * n + i];
     a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, vw[n][i]),
                                                 __builtin_bit_cast(bf16x8_v, p),
-                                                a, 0, 0, 0);
+                                                decltype(fresh)::value ? zero4 : a, 0, 0, 0);
   };
   auto each = [](auto f) {  // f(0) .. f(3), as constants
     f(std::integral_constant<int, 0>{}); f(std::integral_constant<int, 1>{});
@@ -275,13 +276,12 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = fold_elem(a[i], acc[db][i], f);
       parked[64 * NW * db] = a;
-      acc[db] = zero4;
     }
   };
 
   // Half h of tile t: sub-tile u = 2 t + h. MASK: some key of it may be hidden from some row. FIRST: of a
-  // split.
-  auto half = [&](auto mask, auto first, auto h_, int t, auto buf, auto tail) {
+  // split (it finishes the one before). FRESH: the second of a split.
+  auto half = [&](auto mask, auto first, auto fresh, auto h_, int t, auto buf, auto tail) {
     constexpr bool kMask = decltype(mask)::value, kFirst = decltype(first)::value;
     constexpr int h = decltype(h_)::value;
     const int v_at = 2 * buf + h, k_at = 2 * other(buf) + h;  // what is read here: V of u, K of u + 2
@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
     auto seen = [&](int i) { return !kMask || vis[i] ? sc[i >> 2][i & 3] : NEG_BIG; };
     point();
     __builtin_amdgcn_s_setprio(1);
-    pv(0, 0, p4[1 - h]);
-    pv(0, 1, p4[1 - h]);
+    pv(fresh, 0, 0, p4[1 - h]);
+    pv(fresh, 0, 1, p4[1 - h]);
     point();
     const float om = m, ol = l;
     auto row_max = [&] {
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
       p[1] = exp2_fast(x[1]);
       point();
       if constexpr (n == 3) read_k(k_at);
-      if constexpr (n < 3) pv(n + 1, 0, p4[1 - h]);
+      if constexpr (n < 3) pv(fresh, n + 1, 0, p4[1 - h]);
       point();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
       }
       reinterpret_cast<uint32_t*>(&p4[h])[n] = pack_bf16x2(p[0], p[1]);
       point();
-      if constexpr (n < 3) pv(n + 1, 1, p4[1 - h]);
+      if constexpr (n < 3) pv(fresh, n + 1, 1, p4[1 - h]);
       point();
     });
     // (here, not where they are used: past the branches below they would move there)
@@ -407,8 +407,8 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
       point();
     };
     if (!kMask || t <= w_tiles) {  // (at w_tiles the sub-tile before is still to be added)
-      half(mask, first, c0{}, t, buf, [] {});
-      half(mask, no, c1{}, t, buf, stage);
+      half(mask, first, no, c0{}, t, buf, [] {});
+      half(mask, no, first, c1{}, t, buf, stage);
     } else {
       stage();
     }
@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
   // The last sub-tile's output. (A wave that left out the last tiles has P = 0 and finite values.)
   each([&](auto n_) {
     constexpr int n = decltype(n_)::value;
-    pv(n, 0, p4[1]);
-    pv(n, 1, p4[1]);
+    pv(no, n, 0, p4[1]);
+    pv(no, n, 1, p4[1]);
   });
   if constexpr (FANOUT) {
     l = pair32_sum(pair16_sum(l));
