@@ -16,8 +16,8 @@
 // waits of the other best: 8 waves of 64 positions, and 4 waves with two row sets that share each fragment,
 // took 3 to 40 % longer. Over 8 kv heads of 2 query heads, us by the card: 1 x 8192 296-330 (930-833
 // TFLOP/s; the 8-bit pool's kernel 349 beside 336), 4 x 2048 93-101, 1 x 2048 30-33, 4 x 32 at 2048 keys 17.
-// Of 4 x 2048 the vector ALU (softmax, V to bf16) issues for 58 % and the matrix units and the LDS (each wave reads all of V for its 16 rows) are
-// busy for 32 % and 46 %, in each other's shadow: what bounds it is each wave's own chain, two a SIMD.
+// Of 4 x 2048 the vector ALU (softmax, V to bf16) issues for 56 % and the matrix units and the LDS (each wave reads all of V for its 16 rows) are
+// busy for 34 % and 45 %, in each other's shadow: what bounds it is each wave's own chain, two a SIMD.
 #include "extend_codes.h"
 #include "kv_fp4.h"
 
@@ -37,7 +37,7 @@ constexpr float kLazy = 24.0f, kLazySum = 16777216.0f;
 // ---- LDS ---------------------------------------------------------------------------------
 //
 // Two tiles of 64 keys, as four sub-tiles of 32. K stays in codes, 64 bytes a key: 16-byte unit u of a
-// key's row holds block u ^ swk(key), so that the 16 rows of a fragment read fall on all 64 banks. V
+// key's row holds block u ^ swk(key), which spreads a fragment's 16 rows over the banks. V
 // is bf16 (swv). Beside them K's scale bytes as the matrix instruction takes them: half-word l of a
 // sub-tile holds lane l's for its two key blocks.
 constexpr int BS = 32;  // keys of a sub-tile
@@ -49,7 +49,13 @@ constexpr int kScalesAt = kVAt + 4 * kVSub;
 constexpr int kRunAt = kScalesAt + 4 * kScaleSub;
 constexpr int lds_bytes(bool fanout) { return kRunAt + (fanout ? 0 : NW * (8 * 1024 + 128)); }
 
-__device__ __forceinline__ int swk(int key) { return (key >> 3) & 3; }
+// 0, 2, 3, 1 for the four groups of rows: a read of 16 bytes takes lanes 0-3, 12-15, 20-27 and their like at
+// once, whose blocks are then four different ones. (0, 1, 2, 3: 6.9 M cycles of conflicts in 4 x 2048, and
+// 1 % longer; 4.6 M are left.)
+__device__ __forceinline__ int swk(int key) {
+  const int x = (key >> 3) & 3;
+  return ((x << 1) & 3) ^ 3 * (x >> 1);
+}
 
 // Workgroup = (request, kv head, 8 NW query positions), NW waves; wave w: 16 positions of query head
 // w / (NW / 2). FANOUT: the workgroup computes one split and saves its state for the fold; else it
