@@ -147,6 +147,20 @@ def _usual_qkv(q_out, q_norm, k_norm, positions, cos_sin, slots) -> bool:
         return False
 
 
+def _usual_chunk(q, qo_indptr, kv_indptr, kv_indices, o, workspace) -> bool:
+    try:
+        return (-1 < q.get_device() == qo_indptr.get_device() == kv_indptr.get_device()
+                == kv_indices.get_device() == o.get_device()
+                and q.dtype is _BF16 and o.dtype is _BF16 and qo_indptr.dtype is _I32
+                and kv_indptr.dtype is _I32 and kv_indices.dtype is _I32
+                and q.is_contiguous() and o.is_contiguous() and qo_indptr.is_contiguous()
+                and kv_indptr.is_contiguous() and kv_indices.is_contiguous()
+                and (workspace is None or workspace.get_device() == q.get_device()
+                     and workspace.dtype is torch.uint8 and workspace.is_contiguous()))
+    except AttributeError:
+        return False
+
+
 def _usual_load(slots, k, v) -> bool:
     try:
         return (-1 < slots.get_device() == k.get_device() == v.get_device() and slots.dtype is _I64
@@ -498,25 +512,30 @@ class NativeLib:
                              workspace=None, kv_scales=None) -> None:
         """kv_scales: the buffers are an 8-bit pool (sid_extend_attention_fp8_fwd) or, of that type, a
         4-bit one (sid_extend_attention_fp4_fwd)."""
-        _gpu(q, "q_extend", torch.bfloat16)
+        usual = kv_scales is not None and _usual_chunk(q, qo_indptr, kv_indptr, kv_indices, o, workspace)
+        if not usual:
+            _gpu(q, "q_extend", torch.bfloat16)
         _check(q.dim() == 3, "q_extend must be [Text, HQ, D]")
         if kv_scales is not None:
             kind, _ = _code_pool(k_buffer, v_buffer, kv_scales, q.shape[2], q.get_device())
-            _same_device(q.get_device(), qo_indptr, kv_indptr, kv_indices, o, workspace)
+            if not usual:
+                _same_device(q.get_device(), qo_indptr, kv_indptr, kv_indices, o, workspace)
         else:
             _gpu(k_buffer, "k_buffer", torch.bfloat16)
             _gpu(v_buffer, "v_buffer", torch.bfloat16)
             _check(k_buffer.shape == v_buffer.shape and k_buffer.dim() == 3
                    and k_buffer.shape[2] == q.shape[2], "bad KV buffer shapes")
-        _gpu(qo_indptr, "qo_indptr", torch.int32)
-        _gpu(kv_indptr, "kv_indptr", torch.int32)
-        _gpu(kv_indices, "kv_indices", torch.int32)
+        if not usual:
+            _gpu(qo_indptr, "qo_indptr", torch.int32)
+            _gpu(kv_indptr, "kv_indptr", torch.int32)
+            _gpu(kv_indices, "kv_indices", torch.int32)
+            _gpu(o, "o", torch.bfloat16)
+            if workspace is not None:
+                _gpu(workspace, "workspace", torch.uint8)
         _check(qo_indptr.numel() == kv_indptr.numel(), "qo_indptr/kv_indptr length mismatch")
-        _gpu(o, "o", torch.bfloat16)
         _check(o.shape == q.shape, "o must have q's shape")
         ws_ptr, ws_bytes = None, 0
         if workspace is not None:
-            _gpu(workspace, "workspace", torch.uint8)
             ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
         rest = (qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
                 qo_indptr.numel() - 1, q.shape[0], q.shape[1], k_buffer.shape[1], q.shape[2],

@@ -527,8 +527,8 @@ class DecodeAttention:
         max_seq_len alone); wg_order: workgroup_order of this plan, on the device (None: the
         grid's own order); workers > 0: stage 1 by that many workgroups, each computing the
         items of wg_order dealt to it (then a permutation of every (request, slot) item; see
-        worker_order); kv_scales: the caches are an 8-bit pool (sid.kernels.kv_fp8): pass
-        step_plan's arguments there, as the plan made here from the sizes alone is the bf16
+        worker_order); kv_scales: the caches are an 8-bit pool (sid.kernels.kv_fp8)
+        or, by their type, a 4-bit one (sid.kernels.kv_fp4): pass step_plan's arguments there, as the plan made here from the sizes alone is the bf16
         pool's, up to a quarter slower."""
         if variant is None:
             variant = INVARIANT_VARIANT if invariant else 0
