@@ -15,7 +15,7 @@
 //
 // Workgroups are of 4 waves, two to a CU. (8 waves took 1 to 18 % longer in 30 of 31 batches, as their first
 // loads and their merge stand alone on a CU: 1 x 1024 tokens 11.3 and 12.2 us, 32 x 2048 21.0 and 22.4.)
-// 128 x 4096 tokens 98-109 us by the box (5.3-5.9 TB/s of codes and scales, where a plain read of memory reaches
+// 128 x 4096 tokens 94-109 us by the card (5.3-6.1 TB/s of codes and scales, where a plain read of memory reaches
 // 6.0), 64 x 2048 31, 1 x 131072 53, 1 x 1024 11. What bounds the large ones is memory; the small ones a
 // chain of latencies: lengths, slots, rows, the merge in the LDS and the second launch.
 #include "decode_split.h"
