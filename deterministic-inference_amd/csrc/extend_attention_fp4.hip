@@ -51,7 +51,8 @@ constexpr int lds_bytes(bool fanout) { return kRunAt + (fanout ? 0 : NW * (8 * 1
 
 // 0, 2, 3, 1 for the four groups of rows: a read of 16 bytes takes lanes 0-3, 12-15, 20-27 and their like at
 // once, whose blocks are then four different ones. (0, 1, 2, 3: 6.9 M cycles of conflicts in 4 x 2048, and
-// 1 % longer; 4.6 M are left.)
+// 1 % longer. 4.6 M are left, of V's writes: half of the lanes writing their words in another order ends
+// them, but its selects cost what that gains.)
 __device__ __forceinline__ int swk(int key) {
   const int x = (key >> 3) & 3;
   return ((x << 1) & 3) ^ 3 * (x >> 1);
