@@ -31,8 +31,9 @@ constexpr int NW = 4;  // waves of a workgroup
 // but 4 x 32 queries at 2048 keys, which fan out by splits, 20.7 us instead of 17.)
 constexpr int kSplit = 512;
 constexpr int kSplitTiles = kSplit / BN;
-// How far above its row's reference maximum a score may be, in log2 units.
-constexpr float kLazy = 24.0f, kLazySum = 16777216.0f;
+// How far above its row's reference maximum a score may be: 24 octaves, as p. (A split's sums of p v are
+// then at most 2^33 of its largest |v|: finite below 2^94.)
+constexpr float kLazySum = 16777216.0f;
 
 // ---- LDS ---------------------------------------------------------------------------------
 //
@@ -353,15 +354,19 @@ __global__ void __launch_bounds__(NW * 64, 2) extend_fp4_kernel(
     if constexpr (kFirst) {
       if (!FANOUT && t > t_begin) fold_split(om, ol);
     } else {
-      // A row's reference maximum is that of its split's first sub-tile as long as no score is kLazy above
-      // it: P's precision does not depend on its size. A score that is makes its lane's sum grow by 2^kLazy
-      // or more; only where one does (hardly ever) are the rows' maxima taken, their state brought to
-      // them and P worked out again. That is looked at here, after the products, as nothing before has to
-      // wait for it. (By the sums, not by the scores' maximum: 5 operations fewer of some 50, 2 % of
-      // 1 x 8192.)
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(l - ol > kLazySum) != 0, false)) {
-        const float mc = row_max();
-        const float m_used = mc > m + kLazy ? mc : m;
+      // A row's reference maximum is that of its split's first sub-tile until one of its scores is 24
+      // octaves above it: P's precision does not depend on its size. Such a score makes its lane's sum grow by
+      // more than kLazySum (at the border the roundings decide); only where one does (hardly ever) are the
+      // rows' maxima taken, their state brought to them and P worked out again. Each row goes by the sums
+      // of its own four lanes there, so whether it moves does not depend on who shares its wave. That is
+      // looked at here, after the products, as nothing before has to wait for it. (By the sums, not by the
+      // scores' maximum: 5 operations fewer of some 50, 2 % of 1 x 8192.)
+      uint64_t up = __builtin_amdgcn_ballot_w64(l - ol > kLazySum);
+      if (__builtin_expect(up != 0, false)) {
+        up |= up >> 32 | up << 32;  // a row's four lanes are 16 apart
+        up |= up >> 16 | up << 48;
+        const float mc = row_max();  // (of a row that moves some 20 octaves above m, or more)
+        const float m_used = __builtin_amdgcn_inverse_ballot_w64(up) ? mc : m;
         const float rescale = exp2_fast(m - m_used);  // (x * 1 == x for the rows that stay)
         m = m_used;
         l = ol * rescale;
