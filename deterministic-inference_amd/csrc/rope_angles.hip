@@ -66,7 +66,7 @@ __device__ __forceinline__ void head_at(const RopeArgs& a, int64_t t, int h, con
 // elements behind the rotated ones (one word); with VEC false, for heads that do not start on words, one
 // pair or one element (8192 tokens 38 us instead of 17). `copy`: the elements behind the rotated ones are
 // written too (not where a call rotates in place). A token whose position is outside [0, max_positions) is
-// copied.
+// copied bit by bit, or in place left alone.
 template <bool INTER, bool VEC>
 __global__ void __launch_bounds__(kThreads) rope_angles_kernel(RopeArgs a, int copy) {
   __shared__ float2 angle[kMaxPairs];  // (cos, sin) times the gain
@@ -76,10 +76,21 @@ __global__ void __launch_bounds__(kThreads) rope_angles_kernel(RopeArgs a, int c
   const int units = rot_units + (copy ? (a.head_dim - a.rotary) / W : 0);  // of a head
   const int64_t t = blockIdx.x;
   const int64_t pos = a.positions[t];
-  const bool in = pos >= 0 && pos < a.max_positions;
+  if (pos < 0 || pos >= a.max_positions) {  // (the whole workgroup's)
+    const int words = a.head_dim / W;  // of a head
+    for (int u = threadIdx.x; copy && u < a.heads * words; u += kThreads) {
+      const int at = (u % words) * W;
+      const bf16_t* src;
+      bf16_t* dst;
+      head_at(a, t, u / words, src, dst);
+      if constexpr (VEC) *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(src + at);
+      else dst[at] = src[at];
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < pairs; i += kThreads) {
     const float2 sc = sincos_turns(static_cast<uint64_t>(pos) * a.turns[i]);
-    angle[i] = in ? make_float2(sc.y * a.gain, sc.x * a.gain) : make_float2(1.0f, 0.0f);
+    angle[i] = make_float2(sc.y * a.gain, sc.x * a.gain);
   }
   __syncthreads();
   const int total = a.heads * units;

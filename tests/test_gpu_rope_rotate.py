@@ -167,3 +167,26 @@ def test_rotate_in_a_graph_and_on_another_stream():
         torch.cuda.synchronize()
         eager = rope.rotate(q, k, pos + i)
         assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+
+
+@pytest.mark.parametrize("rotary,interleaved", [(64, False), (64, True), (32, False), (6, True)])
+def test_positions_outside_keep_every_bit(rotary, interleaved):
+    """Infinities, NaNs and zeros of both signs too, out of place and in place, by words and by
+    elements."""
+    from sid.kernels.rope import RotaryEmbedding
+    rope = RotaryEmbedding(64, 100, 1e4, "cuda", rotary_dim=rotary, interleaved=interleaved,
+                           scaling=dict(YARN, factor=2.0))
+    g = torch.Generator().manual_seed(rotary)
+    bits = torch.randint(-(1 << 15), 1 << 15, (6, 3, 64), generator=g).to(torch.int16)
+    for i, special in enumerate((0x7f80, -0x80, 0x7fc0, -0x3f, -0x8000, 0)):  # inf, -inf, NaNs, -0, 0
+        bits[:, :, i::7] = special
+    proj = bits.view(torch.bfloat16).cuda()
+    q, k = proj[:, :2], proj[:, 2:]
+    pos = torch.tensor([-1, 100, 3, 1 << 40, -(1 << 62), 99], device="cuda")
+    out = [0, 1, 3, 4]
+    for got, x in zip(rope.rotate(q, k, pos), (q, k)):
+        assert torch.equal(got[out].view(torch.int16), x[out].contiguous().view(torch.int16))
+    a, b = q.contiguous(), k.contiguous()
+    rope.apply(a, b, pos)
+    for got, x in ((a, q), (b, k)):
+        assert torch.equal(got[out].view(torch.int16), x[out].contiguous().view(torch.int16))
