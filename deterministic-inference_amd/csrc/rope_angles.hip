@@ -5,9 +5,9 @@
 // a 64-bit fraction of a turn, so pos f_i modulo a turn is the low 64 bits of an integer product.
 // That is exact but for f_i's own 2^-65: off by pos 2^-62 radians, whatever the position, where a
 // product in 32 bits is off by pos 2^-25 of its angle. What is left of it after whole quarter turns, at most
-// an eighth of one either way, goes to fp32 (31 bits rounded to 24), and its sine and cosine to
-// their Taylor sums (terms to x^9 and x^8: the first left out is 2e-9 and 2.5e-8). q and k are
-// rounded once, to bf16.
+// an eighth of one either way, goes to fp32 with all its 62 bits (so a small angle's sine is as near, in
+// proportion, as a large one's), and its sine and cosine to their Taylor sums (terms to x^9 and x^8: the
+// first left out is 2e-9 and 2.5e-8). q and k are rounded once, to bf16.
 //
 // Bound: q and k read and written. A workgroup takes one token and works its rotary / 2 angles out once for
 // all heads, into the LDS. (Two or four tokens a workgroup: 64 tokens 2.7 us with one, 3.2 and 3.7; 8192 of
@@ -24,10 +24,9 @@ constexpr int kMaxPairs = 512;  // of a head: 4 KiB of the LDS
 
 // (sin, cos) of a 64-bit fraction of a turn.
 __device__ __forceinline__ float2 sincos_turns(uint64_t turns) {
-  const uint32_t top = static_cast<uint32_t>(turns >> 32);
-  const uint32_t quarter = (top + 0x20000000u) >> 30;
-  // 2 pi 2^-32 radians a unit
-  const float x = static_cast<float>(static_cast<int32_t>(top - (quarter << 30))) * 1.4629180793e-9f;
+  const uint32_t quarter = (static_cast<uint32_t>(turns >> 32) + 0x20000000u) >> 30;
+  const int64_t rest = static_cast<int64_t>(turns - (static_cast<uint64_t>(quarter) << 62));
+  const float x = static_cast<float>(rest) * 3.406121580086e-19f;  // 2 pi 2^-64 radians a unit
   const float y = x * x;
   const float s = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.0f / 362880.0f, -1.0f / 5040.0f), 1.0f / 120.0f),
                                    -1.0f / 6.0f), x);

@@ -190,3 +190,23 @@ def test_positions_outside_keep_every_bit(rotary, interleaved):
     rope.apply(a, b, pos)
     for got, x in ((a, q), (b, k)):
         assert torch.equal(got[out].view(torch.int16), x[out].contiguous().view(torch.int16))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_small_angles_keep_their_sines(interleaved):
+    """Pairs (0, y): out is (-y sin, y cos), to the rounding of bf16 (2^-8) and a few of fp32's, the
+    angle's, the sum's and the product's (2^-20), of each value itself."""
+    from sid.kernels.rope import RotaryEmbedding, scaled_frequencies
+    scaling = dict(rope_type="linear", factor=64.0)
+    rope = RotaryEmbedding(128, 131072, 1e6, "cuda", interleaved=interleaved, scaling=scaling)
+    freq, _ = scaled_frequencies(128, 1e6, scaling)
+    q, k = _inputs(70, 4, 2, 128, strided=False)
+    x, y = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, 64), slice(64, None))
+    q[..., x] = 0.0
+    pos = torch.arange(70, device="cuda")
+    got = rope.rotate(q, k, pos)[0].double().cpu()
+    angle = (pos.double().cpu()[:, None] * freq)[:, None]
+    v = q.double().cpu()[..., y]
+    for part, want in ((x, -v * angle.sin()), (y, v * angle.cos())):
+        over = (got[..., part] - want).abs() - want.abs() * (2.0 ** -8 + 2.0 ** -20)
+        assert float(over.max()) <= 0.0
