@@ -30,23 +30,42 @@ from sid.kernels.jit import load_ext
 
 ROPE_TYPES = ("default", "linear", "ntk", "yarn")
 
+# What a scaling dict may say, yarn's beside the others'.
+_KEYS = ("rope_type", "type", "factor", "original_max_position_embeddings", "rope_theta")
+_YARN_KEYS = ("beta_fast", "beta_slow", "attention_factor", "truncate")
+
 
 def rope_type(scaling: dict | None) -> str:
-    """One of ROPE_TYPES: a scaling dict's rope_type (or type)."""
+    """One of ROPE_TYPES: a scaling dict's rope_type (or type). A key that is not read here would
+    mean other positions than these, so it is refused unless it is None."""
     scaling = scaling or {}
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if not isinstance(scaling, dict):
+        raise ValueError(f"rope scaling must be a dict, got {scaling!r}")
+    said = {key: value for key, value in scaling.items() if value is not None}
+    kind = said.get("rope_type", said.get("type", "default"))
     if kind not in ROPE_TYPES:
         raise ValueError(f"unknown rope_type {kind!r}: use one of {', '.join(ROPE_TYPES)}")
+    if said.get("type", kind) != kind:
+        raise ValueError(f"rope_type {kind!r} and type {said['type']!r} disagree")
+    if said and "rope_type" not in said and "type" not in said:
+        raise ValueError(f"rope scaling names no rope_type: {scaling!r}")
+    other = [key for key in said if key not in _KEYS + (_YARN_KEYS if kind == "yarn" else ())]
+    if said.get("truncate", True) is not True:
+        other.append("truncate other than True")
+    if other:
+        raise ValueError(f"{kind} rope scaling does not take {', '.join(map(str, other))}")
     return kind
 
 
 def scaled_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None) -> tuple:
     """(float64 [rotary_dim / 2] radians a position, the gain of cos and sin) of a scaling dict:
     rope_type (or type), factor, and for yarn original_max_position_embeddings, beta_fast,
-    beta_slow, attention_factor."""
+    beta_slow, attention_factor; any other key that says something is refused (rope_type)."""
     kind, scaling = rope_type(scaling), dict(scaling or {})
     if not theta > 1.0:
         raise ValueError(f"rope theta must be above 1, got {theta}")
+    if scaling.get("rope_theta") not in (None, theta):
+        raise ValueError(f"rope scaling's rope_theta {scaling['rope_theta']!r} is not the model's {theta}")
     n = rotary_dim
     at = torch.arange(0, n, 2, dtype=torch.float64) / n
     if kind == "default":

@@ -136,9 +136,9 @@ def load_weights(model_dir: Path, mcfg: ModelConfig, device,
 def scale_positions(mcfg: ModelConfig, scaling: dict) -> None:
     """Scaled rotary positions (sid.kernels.rope) for a model, and the positions that they reach:
     factor times the trained ones, if config.json does not say more."""
+    scaled_frequencies(mcfg.head_dim, mcfg.rope_theta, scaling)  # (raises where it is incomplete)
     if rope_type(scaling) == "default":
         return
-    scaled_frequencies(mcfg.head_dim, mcfg.rope_theta, scaling)  # (raises where it is incomplete)
     trained = scaling.get("original_max_position_embeddings", mcfg.max_position_embeddings)
     mcfg.max_position_embeddings = max(mcfg.max_position_embeddings,
                                        int(trained * float(scaling["factor"])))

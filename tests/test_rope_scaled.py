@@ -105,3 +105,30 @@ def test_entry_point_refuses_bad_arguments():
                       (dict(hq=0, hkv=0), b"head counts"), (dict(t=1 << 31), b"too many")):
         assert call(**bad) == 1 and text in lib.sid_last_error(), bad
     assert call(t=0) == 0
+
+
+@pytest.mark.parametrize("scaling,text", [
+    (dict(YARN, mscale=1.0, mscale_all_dim=1.0), "mscale, mscale_all_dim"),
+    (dict(YARN, truncate=False), "truncate"), (dict(YARN, mrope_section=[16, 24, 24]), "mrope_section"),
+    (dict(rope_type="linear", factor=2.0, beta_fast=32.0), "beta_fast"),
+    (dict(rope_type="ntk", factor=2.0, attention_factor=1.0), "attention_factor"),
+    (dict(rope_type="default", mrope_section=[16, 24, 24]), "mrope_section"),
+    (dict(factor=4.0), "names no rope_type"), (dict(YARN, type="linear"), "rope_type"),
+    (dict(YARN, rope_theta=5e5), "rope_theta"), (["yarn", 4.0], "dict"),
+], ids=str)
+def test_what_a_scaling_says_is_done_or_refused(scaling, text):
+    """A key that would change positions or gain and is not read; a type that is not clear."""
+    from sid.config import ModelConfig
+    from sid.model.loader import scale_positions
+    with pytest.raises(ValueError, match=text):
+        scaled_frequencies(128, 1e6, scaling)
+    with pytest.raises(ValueError, match=text):
+        scale_positions(ModelConfig(model_path="random:"), scaling)
+
+
+def test_keys_that_say_nothing_more_are_taken():
+    f, g = scaled_frequencies(128, 1e6, YARN)
+    for more in (dict(type="yarn"), dict(truncate=True), dict(mscale=None, truncate=None),
+                 dict(rope_theta=1e6), dict(beta_fast=None, beta_slow=None, attention_factor=None)):
+        f2, g2 = scaled_frequencies(128, 1e6, dict(YARN, **more))
+        assert torch.equal(f, f2) and g == g2
