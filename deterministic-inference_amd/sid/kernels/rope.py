@@ -57,6 +57,19 @@ def rope_type(scaling: dict | None) -> str:
     return kind
 
 
+def scaling_number(scaling: dict, key: str, default: float | None = None, least: float = 0.0) -> float:
+    """A scaling dict's number above 0, finite and at least `least`; None is the default."""
+    value = default if scaling.get(key) is None else scaling[key]
+    try:
+        x = math.nan if isinstance(value, bool) else float(value)
+    except (TypeError, ValueError, OverflowError):
+        x = math.nan
+    if not (0.0 < x < math.inf and x >= least):
+        raise ValueError(f"rope scaling needs a finite {key} "
+                         f"{f'of at least {least:g}' if least else 'above 0'}, got {value!r}")
+    return x
+
+
 def scaled_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None) -> tuple:
     """(float64 [rotary_dim / 2] radians a position, the gain of cos and sin) of a scaling dict:
     rope_type (or type), factor, and for yarn original_max_position_embeddings, beta_fast,
@@ -70,19 +83,15 @@ def scaled_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
     at = torch.arange(0, n, 2, dtype=torch.float64) / n
     if kind == "default":
         return theta ** -at, 1.0
-    factor = float(scaling.get("factor", 0.0))
-    if not (factor >= 1.0 and math.isfinite(factor)):
-        raise ValueError(f"rope scaling needs a factor of at least 1, got {scaling.get('factor')!r}")
+    factor = scaling_number(scaling, "factor", least=1.0)
     if kind == "linear":
         return theta ** -at / factor, 1.0
     if kind == "ntk":
         return (theta * factor ** (n / max(n - 2, 1))) ** -at, 1.0
-    trained = scaling.get("original_max_position_embeddings")
-    if not (isinstance(trained, (int, float)) and trained > 0):
-        raise ValueError("yarn scaling needs original_max_position_embeddings")
-    fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
-    if not fast > slow > 0:
-        raise ValueError(f"yarn scaling needs beta_fast > beta_slow > 0, got {fast}, {slow}")
+    trained = scaling_number(scaling, "original_max_position_embeddings")
+    fast, slow = (scaling_number(scaling, key, x) for key, x in (("beta_fast", 32.0), ("beta_slow", 1.0)))
+    if not fast > slow:
+        raise ValueError(f"yarn scaling needs beta_fast > beta_slow, got {fast}, {slow}")
 
     def pair_of(turns: float) -> float:  # the pair that turns that often in the trained positions
         return n * math.log(trained / (2 * math.pi * turns)) / (2 * math.log(theta))
@@ -90,8 +99,7 @@ def scaled_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
     low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), n - 1)
     ramp = (torch.arange(n // 2, dtype=torch.float64) - low) / (high - low or 0.001)
     ramp = ramp.clamp(0.0, 1.0)
-    gain = scaling.get("attention_factor")
-    gain = 0.1 * math.log(factor) + 1.0 if gain is None else float(gain)
+    gain = scaling_number(scaling, "attention_factor", 0.1 * math.log(factor) + 1.0)
     return theta ** -at * (ramp / factor + (1.0 - ramp)), gain
 
 

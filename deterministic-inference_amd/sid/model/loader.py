@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 from sid.config import ModelConfig
-from sid.kernels.rope import rope_type, scaled_frequencies
+from sid.kernels.rope import rope_type, scaled_frequencies, scaling_number
 
 
 def random_weights(mcfg: ModelConfig, device, seed: int = 0, std: float = 0.02,
@@ -139,9 +139,9 @@ def scale_positions(mcfg: ModelConfig, scaling: dict) -> None:
     scaled_frequencies(mcfg.head_dim, mcfg.rope_theta, scaling)  # (raises where it is incomplete)
     if rope_type(scaling) == "default":
         return
-    trained = scaling.get("original_max_position_embeddings", mcfg.max_position_embeddings)
+    trained = scaling_number(scaling, "original_max_position_embeddings", mcfg.max_position_embeddings)
     mcfg.max_position_embeddings = max(mcfg.max_position_embeddings,
-                                       int(trained * float(scaling["factor"])))
+                                       int(trained * scaling_number(scaling, "factor")))
     mcfg.rope_scaling = dict(scaling)
 
 

@@ -132,3 +132,38 @@ def test_keys_that_say_nothing_more_are_taken():
                  dict(rope_theta=1e6), dict(beta_fast=None, beta_slow=None, attention_factor=None)):
         f2, g2 = scaled_frequencies(128, 1e6, dict(YARN, **more))
         assert torch.equal(f, f2) and g == g2
+
+
+@pytest.mark.parametrize("scaling,text", [
+    (dict(rope_type="linear", factor=None), "factor"), (dict(rope_type="ntk", factor="much"), "factor"),
+    (dict(YARN, factor=float("nan")), "factor"), (dict(YARN, factor=True), "factor"),
+    (dict(YARN, attention_factor=float("nan")), "attention_factor"),
+    (dict(YARN, attention_factor=float("inf")), "attention_factor"),
+    (dict(YARN, attention_factor=0.0), "attention_factor"),
+    (dict(YARN, beta_slow=0), "beta_slow"), (dict(YARN, beta_fast=0.0), "beta_fast"),
+    (dict(YARN, beta_fast=float("inf")), "beta_fast"),
+    (dict(YARN, original_max_position_embeddings=None), "original"),
+    (dict(YARN, original_max_position_embeddings=float("inf")), "original"),
+    (dict(YARN, original_max_position_embeddings=True), "original"),
+    (dict(YARN, original_max_position_embeddings=-5), "original"),
+], ids=str)
+def test_values_that_are_no_numbers_are_refused(scaling, text):
+    from sid.config import ModelConfig
+    from sid.model.loader import scale_positions
+    with pytest.raises(ValueError, match=text):
+        scaled_frequencies(128, 1e6, scaling)
+    with pytest.raises(ValueError, match=text):
+        scale_positions(ModelConfig(model_path="random:"), scaling)
+
+
+@pytest.mark.parametrize("kind", ["linear", "ntk"])
+def test_trained_positions_that_are_null_are_the_models(kind):
+    from sid.config import ModelConfig
+    from sid.model.loader import scale_positions
+    mcfg = ModelConfig(model_path="random:")
+    trained = mcfg.max_position_embeddings
+    scale_positions(mcfg, dict(rope_type=kind, factor=2.0, original_max_position_embeddings=None))
+    assert mcfg.max_position_embeddings == 2 * trained
+    for bad in (float("nan"), float("inf"), 0, "many"):
+        with pytest.raises(ValueError, match="original"):
+            scale_positions(mcfg, dict(rope_type=kind, factor=2.0, original_max_position_embeddings=bad))
