@@ -14,9 +14,9 @@ position p is p f_i):
                          by the factor, the first one's is kept
     rope_type "yarn"     f_i = theta^(-2i/n) (r_i / factor + 1 - r_i), r_i going linearly from 0 at
                          the pair that turns beta_fast (32) times within
-                         original_max_position_embeddings to 1 at the one that turns beta_slow (1)
-                         times; cos and sin are multiplied with attention_factor
-                         (0.1 ln(factor) + 1)
+                         original_max_position_embeddings (rounded down) to 1 at the one that turns
+                         beta_slow (1) times (rounded up); cos and sin are multiplied with
+                         attention_factor (0.1 ln(factor) + 1)
 """
 
 from __future__ import annotations
@@ -99,6 +99,8 @@ def scaled_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
     low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), n - 1)
     ramp = (torch.arange(n // 2, dtype=torch.float64) - low) / (high - low or 0.001)
     ramp = ramp.clamp(0.0, 1.0)
+    if high < low:  # no pair is between the two: all turn less than beta_slow times, or none less than beta_fast
+        ramp.fill_(1.0 if high < 0 else 0.0)
     gain = scaling_number(scaling, "attention_factor", 0.1 * math.log(factor) + 1.0)
     return theta ** -at * (ramp / factor + (1.0 - ramp)), gain
 

@@ -167,3 +167,15 @@ def test_trained_positions_that_are_null_are_the_models(kind):
     for bad in (float("nan"), float("inf"), 0, "many"):
         with pytest.raises(ValueError, match="original"):
             scale_positions(mcfg, dict(rope_type=kind, factor=2.0, original_max_position_embeddings=bad))
+
+
+def test_yarn_where_every_pair_is_on_one_side():
+    """Trained positions of less than a turn of the fastest pair: all pairs are divided; of more than
+    32 turns of the slowest one: none is."""
+    few = dict(YARN, original_max_position_embeddings=2)
+    f, _ = scaled_frequencies(128, 1e6)
+    s, _ = scaled_frequencies(128, 1e6, few)
+    assert torch.allclose(s, f / 4.0, rtol=1e-15, atol=0)
+    f, _ = scaled_frequencies(4, 10.0)
+    s, _ = scaled_frequencies(4, 10.0, dict(YARN, original_max_position_embeddings=1 << 20))
+    assert torch.allclose(s, f, rtol=1e-15, atol=0)
