@@ -143,14 +143,16 @@ class RotaryEmbedding:
         if not (0 < self.rotary_dim <= head_dim and self.rotary_dim % 2 == 0):
             raise ValueError(f"rotary_dim {rotary_dim} must be even and at most head_dim {head_dim}")
         self.interleaved = bool(interleaved)
-        freq, self.gain = scaled_frequencies(self.rotary_dim, theta, scaling)
-        self.turns = _turn_fractions(freq, device)
-        self.cos_sin = None
-        if self.rotary_dim == head_dim and not self.interleaved:
-            if rope_type(scaling) == "default":
-                self.cos_sin = rope_table(head_dim, max_positions, theta, device)
-            else:
-                self.cos_sin = _table(freq.to(device), self.gain, max_positions, device)
+        table = self.rotary_dim == head_dim and not self.interleaved
+        plain = table and rope_type(scaling) == "default"
+        self.gain, self.turns, self.cos_sin = 1.0, None, None
+        if theta > 1.0 or not plain:  # (a plain table takes any base)
+            freq, self.gain = scaled_frequencies(self.rotary_dim, theta, scaling)
+            self.turns = _turn_fractions(freq, device)
+        if plain:
+            self.cos_sin = rope_table(head_dim, max_positions, theta, device)
+        elif table:
+            self.cos_sin = _table(freq.to(device), self.gain, max_positions, device)
 
     def apply(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor) -> None:
         """In place. q: [T, HQ, D] bf16, k: [T, HKV, D] bf16, positions: int64 [T]. A position
@@ -170,6 +172,8 @@ class RotaryEmbedding:
         are columns of a projection (any token stride). Its sines and cosines are those of the
         exact angles to fp32's accuracy, apply's with a table that table's: the two can differ by
         the last bf16 rounding."""
+        if self.turns is None:
+            raise ValueError("rotate needs a rope theta above 1; apply takes any")
         if q.dim() != 3 or q.shape[2] != self.head_dim:
             raise RuntimeError(f"q must be [T, HQ, {self.head_dim}]")
         q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), \

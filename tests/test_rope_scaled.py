@@ -179,3 +179,18 @@ def test_yarn_where_every_pair_is_on_one_side():
     f, _ = scaled_frequencies(4, 10.0)
     s, _ = scaled_frequencies(4, 10.0, dict(YARN, original_max_position_embeddings=1 << 20))
     assert torch.allclose(s, f, rtol=1e-15, atol=0)
+
+
+@pytest.mark.parametrize("theta", [1.0, 0.5])
+def test_a_table_of_any_base(theta):
+    """Unscaled tables of a whole head in halves do not ask for a base above 1; what needs frequencies
+    below half a turn does."""
+    from sid.kernels.rope import RotaryEmbedding, rope_table
+    rope = RotaryEmbedding(64, 50, theta, "cpu")
+    assert torch.equal(rope.cos_sin, rope_table(64, 50, theta, "cpu"))
+    x = torch.zeros(1, 1, 64)
+    with pytest.raises(ValueError, match="theta"):
+        rope.rotate(x, x, torch.zeros(1, dtype=torch.int64))
+    for more in (dict(rotary_dim=32), dict(interleaved=True), dict(scaling=YARN)):
+        with pytest.raises(ValueError, match="theta"):
+            RotaryEmbedding(64, 50, theta, "cpu", **more)
