@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(NW * 64) decode_stage1_kernel(
   int y = blockIdx.y;
   if (wg_order != nullptr) {
     const int packed = wg_order[blockIdx.x + blockIdx.y * gridDim.x] & ~kOrderEmpty;
-    b = packed >> kOrderSlotBits;
+    b = static_cast<int>(static_cast<uint32_t>(packed) >> kOrderSlotBits);
     y = packed & ((1 << kOrderSlotBits) - 1);
     if (b >= static_cast<int>(gridDim.x) || y >= static_cast<int>(gridDim.y)) return;
   }
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(NW * 64) decode_stage1_worker_kernel(
   for (; i < n_items; i += W) {
     const int packed = order[i];  // workgroup-uniform
     if (packed & kOrderEmpty) break;
-    const int b = packed >> kOrderSlotBits;
+    const int b = static_cast<int>(static_cast<uint32_t>(packed) >> kOrderSlotBits);
     const int y = packed & ((1 << kOrderSlotBits) - 1);
     if (b < batch && y < grid_slots) {
       stage1_item<NW, TPL>(sh, b, y, q, k_cache, v_cache, kv_indptr, kv_indices, num_splits,
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(NW * 64) decode_stage1_worker_kernel(
   const int rest = i < n_items ? (n_items - i + W - 1) / W : 0;
   for (int t = threadIdx.x; t < rest * HQ; t += NW * 64) {
     const int packed = order[i + (t / HQ) * W] & ~kOrderEmpty;
-    const int b = packed >> kOrderSlotBits;
+    const int b = static_cast<int>(static_cast<uint32_t>(packed) >> kOrderSlotBits);
     const int y = packed & ((1 << kOrderSlotBits) - 1);
     if (b < batch && y < grid_slots)
       part_lse[(static_cast<int64_t>(b) * HQ + t % HQ) * part_stride + y] = NEG_BIG;

@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
     int y = blockIdx.y;
     if (wg_order != nullptr) {
       const int packed = wg_order[blockIdx.x + blockIdx.y * gridDim.x] & ~kOrderEmpty;
-      b = packed >> kOrderSlotBits;
+      b = static_cast<int>(static_cast<uint32_t>(packed) >> kOrderSlotBits);
       y = packed & kSlotMask;
       if (b >= batch || y >= grid_slots) return;
     }
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
     for (; i < n_items; i += W) {
       const int packed = wg_order[i];  // workgroup-uniform
       if (packed & kOrderEmpty) break;
-      const int b = packed >> kOrderSlotBits;
+      const int b = static_cast<int>(static_cast<uint32_t>(packed) >> kOrderSlotBits);
       const int y = packed & kSlotMask;
       if (b < batch && y < grid_slots) item(b, y);
       __syncthreads();  // the item's merge reads of the LDS are done before the next one's writes
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(NW * 64, 2) decode_fp4_stage1_kernel(
     const int rest = i < n_items ? (n_items - i + W - 1) / W : 0;
     for (int t = threadIdx.x; t < rest * HQ; t += NW * 64) {
       const int packed = wg_order[i + (t / HQ) * W] & ~kOrderEmpty;
-      const int b = packed >> kOrderSlotBits;
+      const int b = static_cast<int>(static_cast<uint32_t>(packed) >> kOrderSlotBits);
       const int y = packed & kSlotMask;
       if (b < batch && y < grid_slots)
         part_lse[(static_cast<int64_t>(b) * HQ + t % HQ) * part_stride + y] = NEG_BIG;
