@@ -1,5 +1,5 @@
-// What the decode attention's two pool formats (decode_attention.hip: bf16,
-// decode_attention_fp8.hip: e4m3 codes) share: the split and segment geometry, the placement
+// What the decode attention's three pool formats (decode_attention.hip: bf16,
+// decode_attention_fp8.hip: e4m3 codes, decode_attention_fp4.hip: e2m1 codes) share: the split and segment geometry, the placement
 // orders, the merge of a workgroup's waves and the launch of stage 2 (the merge of a request's
 // segments, which only sees partials).
 #pragma once

@@ -1,8 +1,8 @@
-// What the extend attention's kernels for the two pool formats (extend_attention.hip: bf16,
-// extend_attention_fp8.hip: e4m3 codes) share: the tile sizes, a row's folded softmax state, its fold
-// and its output, the lane reductions, the host's plan and the merge of a fan-out. The tile
-// arithmetic is each kernel's own, and so are their bits: the 8-bit kernel takes S on e4m3 operands,
-// sums l by lanes and folds every 512 keys instead of 256.
+// What the extend attention's kernels for the three pool formats (extend_attention.hip: bf16,
+// extend_attention_fp8.hip: e4m3 codes, extend_attention_fp4.hip: e2m1 codes) share: the tile sizes, a
+// row's folded softmax state, its fold and its output, the lane reductions, the host's plan and the merge
+// of a fan-out. The tile arithmetic is each kernel's own, and so are their bits: the kernels over codes
+// take S on the codes with q as e4m3, sum l by lanes and fold every 512 keys instead of 256.
 #pragma once
 
 #include "common.h"
@@ -14,12 +14,14 @@ constexpr int BN = 64;          // keys per tile
 constexpr int BQ = 32;          // query positions per workgroup (x 2 heads = 64 rows)
 constexpr float NEG_BIG = -1e30f;
 constexpr float LOG2E = 1.4426950408889634f;
-// Slack of the lazy softmax maximum, in log2 units: scores up to 2^LAZY_T above the row's
-// reference maximum are taken without moving it.
+// Slack of the lazy softmax maximum, in log2 units: scores up to LAZY_T above the row's
+// reference maximum are taken without moving it (the 4-bit pool's kernel has a slack of its own).
 constexpr float LAZY_T = 8.0f;
 
-// 2^x by the hardware instruction (v_exp_f32): the argument is at most LAZY_T, and results
-// that would be denormal may flush to zero.
+// 2^x by the hardware instruction (v_exp_f32): results that would be denormal may flush to zero. The
+// argument is at most LAZY_T over bf16 and 8-bit pools. The 4-bit pool's kernel bounds it only after
+// the fact, by the sum that it grows: there it may be any number, and one that is too large must give a
+// large result or infinity.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Reductions over lanes l and l ^ 16 (l ^ 32): v_permlane16/32_swap hand each lane the
@@ -107,7 +109,7 @@ __device__ __forceinline__ void skip_rows(int32_t* part_n, int q_start, int from
 // Query positions (32 or 64) of a workgroup that walks all keys of its rows.
 int extend_prefill_rows(int batch, int64_t total_q, int num_kv_heads, int max_extend_len);
 
-// The launch of a call, worked out once for both formats: what is checked, whether the splits fan
+// The launch of a call, worked out once for all formats: what is checked, whether the splits fan
 // out over workgroups (the caller's rule asks for `need` bytes and the workspace has them), the
 // grid.
 struct ExtendPlan {
