@@ -25,7 +25,7 @@ def extend_attention_fwd(q_extend: torch.Tensor, k_buffer: torch.Tensor, v_buffe
     """max_kv_len (an extension of the reference signature): an upper bound of every
     request's kv length; defaults to kv_indices.numel(), which needs no device sync.
     kv_scales: the buffers are an 8-bit pool and these its scales (sid.kernels.kv_fp8), or a 4-bit
-    pool (sid.kernels.kv_fp4), by their type."""
+    pool (sid.kernels.kv_fp4), by their type; over that one sm_scale is finite and not negative."""
     assert q_extend.is_contiguous()
     assert k_buffer.is_contiguous() and v_buffer.is_contiguous()
     ext = load_ext()

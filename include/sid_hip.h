@@ -705,7 +705,8 @@ int sid_rmsnorm_qkv_post_fp4(const void* src, int src_fp32, const void* norm_w, 
 /*
  * sid_flash_decode_fp8_fwd over a 4-bit pool. The kernel has one workgroup shape, 4 waves x 16 tokens
  * per wave iteration: any `variant` that the others take (0 .. 3) gives it. q enters the products
- * as two e4m3 vectors (sid_extend_attention_fp8_fwd).
+ * as two e4m3 vectors (sid_extend_attention_fp8_fwd). sm_scale is multiplied with the scores as it is,
+ * of either sign.
  */
 int sid_flash_decode_fp4_fwd(const void* q, const void* k_cache, const void* v_cache,
                              const void* kv_scales, const int32_t* kv_indptr,
@@ -718,7 +719,10 @@ int sid_flash_decode_fp4_fwd(const void* q, const void* k_cache, const void* v_c
 
 /*
  * sid_extend_attention_fp8_fwd over a 4-bit pool, with its invariances, its treatment of q and of
- * NaN vectors, and its workspace (of sid_extend_attention_fp4_workspace_bytes(...) bytes).
+ * NaN vectors, and its workspace (of sid_extend_attention_fp4_workspace_bytes(...) bytes). Unlike
+ * there, an sm_scale that is negative, infinite or NaN is an error: the rows' maxima are taken before
+ * the scores are scaled. Sums of p v are held relative to a maximum that may be 24 octaves low, which
+ * fp32 holds for |v| below 2^94.
  */
 int64_t sid_extend_attention_fp4_workspace_bytes(int batch, int64_t total_q, int num_q_heads,
                                                  int num_kv_heads, int max_extend_len,
