@@ -160,7 +160,8 @@ def build_model_config(model_path: str, num_layers=None, vocab_size=None,
                 "'random:qwen3-0.6b' for a random-init model)")
         mcfg = load_model_config(model_dir, model_path)
     if rope_scaling == "checkpoint":
-        rope_scaling = _read_json(model_dir / "config.json").get("rope_scaling") if model_dir else None
+        hf = _read_json(model_dir / "config.json") if model_dir else {}
+        rope_scaling = hf.get("rope_scaling") or hf.get("rope_parameters")  # (newer files' name for it)
     if rope_scaling:
         scale_positions(mcfg, rope_scaling)
     if num_layers is not None:

@@ -194,3 +194,23 @@ def test_a_table_of_any_base(theta):
     for more in (dict(rotary_dim=32), dict(interleaved=True), dict(scaling=YARN)):
         with pytest.raises(ValueError, match="theta"):
             RotaryEmbedding(64, 50, theta, "cpu", **more)
+
+
+def test_checkpoints_that_name_their_scaling_rope_parameters(tmp_path):
+    import json
+
+    from sid.model.loader import build_model_config
+    hf = dict(model_type="qwen3", num_hidden_layers=2, hidden_size=1024, num_attention_heads=16,
+              num_key_value_heads=8, head_dim=128, intermediate_size=2048, vocab_size=1000,
+              rms_norm_eps=1e-6, rope_theta=1e6, max_position_embeddings=40960)
+
+    def config(**more):
+        (tmp_path / "config.json").write_text(json.dumps(dict(hf, **more)))
+        return build_model_config(str(tmp_path), rope_scaling="checkpoint")[0]
+    said = dict(YARN, rope_theta=1e6)
+    mcfg = config(rope_parameters=said)
+    assert mcfg.rope_scaling == said and mcfg.max_position_embeddings == 131072
+    mcfg = config(rope_parameters=dict(rope_type="default", rope_theta=1e6), rope_scaling=None)
+    assert mcfg.rope_scaling is None and mcfg.max_position_embeddings == 40960
+    with pytest.raises(ValueError, match="rope_theta"):
+        config(rope_parameters=dict(said, rope_theta=5e6))
