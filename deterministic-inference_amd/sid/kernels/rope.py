@@ -178,7 +178,6 @@ class RotaryEmbedding:
             raise RuntimeError(f"q must be [T, HQ, {self.head_dim}]")
         q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), \
             torch.empty_like(k, memory_format=torch.contiguous_format)
-        if q.shape[0]:
-            load_ext().rope_rotate(q, k, positions, self.turns, self.gain, self.rotary_dim,
-                                   self.interleaved, self.max_positions, q_out, k_out)
+        load_ext().rope_rotate(q, k, positions, self.turns, self.gain, self.rotary_dim,
+                               self.interleaved, self.max_positions, q_out, k_out)
         return q_out, k_out

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from conftest import HKV, HQ, D
-from test_gpu_kv_fp4_attention import _chunk, _i32, _of_rows, _ramp, _say
+from test_gpu_kv_fp4_attention import _batch, _chunk, _i32, _of_rows, _queries, _ramp, _say
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,23 @@ def test_rising_scores_keep_bits(size):
             part = _chunk(q[a + lo:a + hi].contiguous(), pool, _i32([0, hi - lo]), _i32([0, p + hi]),
                           _i32(at[i][:p + hi].tolist()), [(p + lo, hi - lo)], workspace=lo % 2 == 0)
             assert torch.equal(part, o[a + lo:a + hi]), (i, lo, hi)
+
+
+def test_decode_scales_of_either_sign():
+    """q at -s is -q at s: the codes' signs alone differ."""
+    from sid.kernels.jit import load_ext
+    lens = [1, 70, 500, 1300]
+    pool, ptr, idx, _ = _batch(lens, seed=4)
+    q = _queries(len(lens), 4)
+
+    def run(q, scale, slots):
+        po = torch.full((len(lens), HQ, slots, D), float("nan"), device="cuda")
+        pl = torch.full((len(lens), HQ, slots), float("nan"), device="cuda")
+        o = torch.full_like(q, float("nan"))
+        load_ext().flash_decode_fwd(q, pool[0], pool[1], ptr, idx, None, 1, 0, scale, po, pl, o,
+                                    segment_size=256 if slots > 1 else 0, grid_slots=slots, variant=3,
+                                    kv_scales=pool[2])
+        return o
+    for slots in (1, 6):
+        o = run(q, 0.09, slots)
+        assert torch.isfinite(o).all() and torch.equal(run(-q, -0.09, slots), o)

@@ -210,3 +210,15 @@ def test_small_angles_keep_their_sines(interleaved):
     for part, want in ((x, -v * angle.sin()), (y, v * angle.cos())):
         over = (got[..., part] - want).abs() - want.abs() * (2.0 ** -8 + 2.0 ** -20)
         assert float(over.max()) <= 0.0
+
+
+def test_no_tokens_of_q_are_none_of_k():
+    from sid.kernels.rope import RotaryEmbedding
+    rope = RotaryEmbedding(64, 100, 1e4, "cuda", rotary_dim=32)
+    q, k = _inputs(3, 2, 1, 64)
+    pos = torch.arange(3, device="cuda")
+    for args in ((q[:0], k, pos[:0]), (q[:0], k, pos), (q[:0], k[:0], pos), (q[:0], k[:0].float(), pos[:0])):
+        with pytest.raises(RuntimeError):
+            rope.rotate(*args)
+    none = rope.rotate(q[:0], k[:0], pos[:0])
+    assert none[0].shape == (0, 2, 64) and none[1].shape == (0, 1, 64)
