@@ -16,7 +16,9 @@
 // Workgroups are of 4 waves, two to a CU. (8 waves took 1 to 18 % longer in 30 of 31 batches, as their first
 // loads and their merge stand alone on a CU: 1 x 1024 tokens 11.3 and 12.2 us, 32 x 2048 21.0 and 22.4.)
 // 128 x 4096 tokens 94-109 us by the card (5.3-6.1 TB/s of codes and scales, where a plain read of memory reaches
-// 6.0), 64 x 2048 31, 1 x 131072 53, 1 x 1024 11. What bounds the large ones is memory; the small ones a
+// 6.0), 64 x 2048 31, 1 x 131072 53, 1 x 1024 11. In fixed splits of 256 tokens (batch_invariant) 128 x 4096
+// 126 (stage 1 119, the merge 6) and 24 requests of 150-20001 tokens 69 instead of 62: a split is four iterations
+// of a workgroup, beside q's codes, the first loads, the waves' merge and one more partial. What bounds the large ones is memory; the small ones a
 // chain of latencies: lengths, slots, rows, the merge in the LDS and the second launch.
 #include "decode_split.h"
 #include "kv_fp4.h"

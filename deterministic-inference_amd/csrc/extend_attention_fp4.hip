@@ -15,9 +15,13 @@
 // Workgroups are of 4 waves and 32 query positions, two to a CU, as an independent workgroup fills the
 // waits of the other best: 8 waves of 64 positions, and 4 waves with two row sets that share each fragment,
 // took 3 to 40 % longer. Over 8 kv heads of 2 query heads, us by the card: 1 x 8192 296-330 (930-833
-// TFLOP/s; the 8-bit pool's kernel 349 beside 336), 4 x 2048 93-101, 1 x 2048 30-33, 4 x 32 at 2048 keys 17.
+// TFLOP/s; the 8-bit pool's kernel 349 beside 336), 4 x 2048 93-101, 1 x 2048 30-33, 4 x 32 at 2048 keys 17-19.
 // Of 4 x 2048 the vector ALU (softmax, V to bf16) issues for 56 % and the matrix units and the LDS (each wave reads all of V for its 16 rows) are
-// busy for 34 % and 45 %, in each other's shadow: what bounds it is each wave's own chain, two a SIMD.
+// busy for 33 % and 44 %, in each other's shadow: what bounds it is each wave's own chain, two a SIMD. 16 x 512 to 1 x 8192
+// (8192 queries each) take 6.7 us a workgroup, its first loads, first S and last fold, and 1.05 us a tile of 64 keys
+// beside it, within 5 %: 27 of 4 x 2048's 96 us, as a CU's places take four workgroups one after the other. A third
+// workgroup a CU has no room: the walking form is compiled to 256 registers, and its LDS is 74752 bytes, 33280
+// of them the parked rows.
 #include "extend_codes.h"
 #include "kv_fp4.h"
 

@@ -1,5 +1,6 @@
 // A K or V vector into a pool of codes, whichever: for the kernels that end in a pool (norm_rope.hip,
-// decode_chain.hip).
+// decode_chain.hip). Over a 4-bit pool qkv_post of 8192 rows takes 28 us (110 MB; bf16 34 us for 135) and of
+// 64 rows of partials 3.4; rmsnorm_qkv_post of 64 rows 8.7 (8.4 MB of weights; latency), both as over bf16.
 #pragma once
 
 #include "kv_fp4.h"

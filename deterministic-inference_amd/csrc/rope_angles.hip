@@ -10,7 +10,7 @@
 // first left out is 2e-9 and 2.5e-8). q and k are rounded once, to bf16.
 //
 // Bound: q and k read and written. A workgroup takes one token and works its rotary / 2 angles out once for
-// all heads, into the LDS. (Two or four tokens a workgroup: 64 tokens 2.7 us with one, 3.2 and 3.7; 8192 of
+// all heads, into the LDS. (Two or four tokens a workgroup, in turn on one card: 64 tokens 2.7 us with one, 3.2 and 3.7; 8192 of
 // 24 heads of 128 16.5, 16.9 and 17.3; with half of a head turned 18.1, 17.5 and 18.1, and 32768 of those 85, 78
 // and 78, the one case that gains.) 8192 tokens in 16.5 us move 100 MB at 6.1 TB/s, half of it out of the
 // last level cache.
@@ -63,7 +63,8 @@ __device__ __forceinline__ void head_at(const RopeArgs& a, int64_t t, int h, con
 
 // A workgroup takes a token. A unit is 8 pairs of halves (two 16-byte words), 4 pairs of neighbours or 8
 // elements behind the rotated ones (one word); with VEC false, for heads that do not start on words, one
-// pair or one element (8192 tokens 38 us instead of 17). `copy`: the elements behind the rotated ones are
+// pair or one element (8192 tokens of 24 heads of 128 at an odd address 26 us instead of 17; of 80, 38 of
+// them turned, 30, where the bytes take 14). `copy`: the elements behind the rotated ones are
 // written too (not where a call rotates in place). A token whose position is outside [0, max_positions) is
 // copied bit by bit, or in place left alone.
 template <bool INTER, bool VEC>

@@ -78,7 +78,7 @@ class EngineConfig:
     kv_page_size: int = 16
     # Rotary positions scaled for contexts beyond the trained ones: a dict as checkpoints give it
     # (rope_type "linear", "ntk" or "yarn", factor, ...; sid.kernels.rope), or "checkpoint" for the
-    # one in the checkpoint's own config.json. None: unscaled, whatever that file says, as the
+    # one in the checkpoint's own config.json (rope_scaling or rope_parameters). None: unscaled, whatever that file says, as the
     # reference (sid/model/loader.py:30-50 does not read it).
     rope_scaling: Optional[dict | str] = None
     max_reqs: int = 256
